@@ -23,7 +23,7 @@ class Results(dict):
     def __getitem__(self, name):
         value = dict.__getitem__(self, name)
         if not isinstance(value, torch.Tensor):
-            value = torch.from_dlpack(value)
+            value = torch.from_dlpack(value.detach())
         return value.long() if name == "chosen" else value
 
 
