@@ -482,6 +482,99 @@ int vc_hip_xent_backward_colsum_pending(const float* logits, const int32_t* targ
                                         const float* grad_loss, float grad_loss_value, size_t rows, size_t classes,
                                         float* grad_logits, float* column_sum, vc_hip_colsum** pending);
 
+/* ---- memory of other libraries ----------------------------------------------------
+ * No counterpart in the reference. A buffer that another library allocated on
+ * the same GPU is passed to the entry points like any other; these three order
+ * the library's stream against the stream that the other library works on. */
+/* The library's stream (a hipStream_t as a number). */
+int vc_hip_stream(uint64_t* stream);
+/* Later work of the library's stream waits for what is enqueued on `stream` (a
+ * hipStream_t as a number, 0 for the default stream) by now. No work is done
+ * for a stream that is idle. */
+int vc_hip_wait_for_stream(uint64_t stream);
+/* Later work of `stream` waits for what is enqueued on the library's stream by now. */
+int vc_hip_release_to_stream(uint64_t stream);
+/* Calls done(context) once the work enqueued on the library's stream by now has
+ * finished, from a later call of this function or of vc_hip_synchronize,
+ * vc_hip_download or vc_hip_alloc, on the calling thread. For buffers of other
+ * libraries that must not be freed before. */
+int vc_hip_when_done(void (*done)(void*), void* context);
+
+/* ---- mixture of experts -------------------------------------------------------------
+ * No counterpart in the reference. */
+/* Scores of a router: softmax over the experts, or a sigmoid of each logit. */
+#define VC_HIP_SCORE_SOFTMAX 0
+#define VC_HIP_SCORE_SIGMOID 1
+/* The top_k experts of each row of logits [tokens, experts]. Experts are
+ * ranked by score + bias[expert] (bias may be NULL), equal ones by the lower
+ * index; of groups > 1 equal groups of neighbouring experts only the top_groups
+ * with the largest sums of their two best ranks take part. weights [tokens,
+ * top_k] are the chosen scores without the bias, divided by their sum if
+ * renormalise; chosen [tokens, top_k] the expert numbers as floats, best first.
+ * A score that is NaN ranks first. experts <= 1024, top_k and groups <= 64. */
+int vc_hip_route_forward(const float* logits, const float* bias, size_t tokens, size_t experts, size_t top_k, int score,
+                         size_t groups, size_t top_groups, int renormalise, float* weights, float* chosen);
+/* Gradient of the weights with respect to the logits, the choice held fixed. */
+int vc_hip_route_backward(const float* logits, const float* chosen, const float* grad_weights, size_t tokens,
+                          size_t experts, size_t top_k, int score, int renormalise, float* grad_logits);
+
+/* The picks of a batch (tokens * top_k entries of `chosen`, numbered row by row)
+ * sorted by expert, equal experts in pick order. An entry that is no expert
+ * number (negative, not whole, too large, NaN) is a dropped pick: it counts to
+ * the group `experts`, whose rows are zero in every result. words holds
+ * vc_hip_expert_plan_words int32 values: offsets [experts + 2] of the groups'
+ * first rows, order [rows] the pick of each row, place [rows] the row of each
+ * pick, with scratch behind them. */
+typedef struct vc_hip_expert_plan {
+    const int32_t* words;
+    size_t tokens, top_k, experts;
+} vc_hip_expert_plan;
+/* experts <= 1024; tokens * top_k < 2^31. */
+int vc_hip_expert_plan_words(size_t tokens, size_t top_k, size_t experts, size_t* words);
+int vc_hip_expert_plan_build(const float* chosen, size_t tokens, size_t top_k, size_t experts, int32_t* words);
+/* Row r of the plan's tokens * top_k rows, of expert e: out[r] = x_r @ w[e], with w [experts, width, columns] and x_r
+ * row r of x (ordered) or the row of x [tokens, width] of its token. */
+int vc_hip_expert_linear_forward(const float* x, const float* w, const vc_hip_expert_plan* plan, size_t width,
+                                 size_t columns, int ordered, float* out);
+/* out[r] = silu(g) * u with g = x_r @ gate[e], u = x_r @ up[e]; g and u are kept in save_gate and save_up
+ * [rows, columns] (both or neither NULL) for the backward pass. */
+int vc_hip_expert_gated_forward(const float* x, const float* gate, const float* up, const vc_hip_expert_plan* plan,
+                                size_t width, size_t columns, int ordered, float* out, float* save_gate, float* save_up);
+/* Gradients of silu(g) * u over count elements. */
+int vc_hip_expert_gated_backward(const float* grad, const float* saved_gate, const float* saved_up, size_t count,
+                                 float* grad_gate, float* grad_up);
+/* grad_rows[r] = grad[r] @ w[e]^T (+ grad2[r] @ w2[e]^T unless both are NULL), [rows, width]. */
+int vc_hip_expert_linear_backward_input(const float* grad, const float* w, const float* grad2, const float* w2,
+                                        const vc_hip_expert_plan* plan, size_t width, size_t columns, float* grad_rows);
+/* grad_w[e] = sum over e's rows of x_r^T grad[r], zero for an expert without rows. */
+int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, const vc_hip_expert_plan* plan, size_t width,
+                                         size_t columns, int ordered, float* grad_w);
+/* out[t] = sum over t's picks of weights[pick] * rows[place], in pick order; weights NULL: all one. Dropped picks add
+ * nothing. */
+int vc_hip_expert_combine_forward(const float* rows, const float* weights, const vc_hip_expert_plan* plan, size_t width,
+                                  float* out);
+/* grad_rows[place] = weights[pick] * grad[t] and grad_weights[pick] = rows[place] . grad[t]; either output may be
+ * NULL, with it the inputs that only it needs. */
+int vc_hip_expert_combine_backward(const float* grad, const float* rows, const float* weights,
+                                   const vc_hip_expert_plan* plan, size_t width, float* grad_rows, float* grad_weights);
+
+/* ---- orthogonalised updates -----------------------------------------------------------
+ * No counterpart in the reference. */
+/* out = the Newton-Schulz iterate of `count` matrices [rows, cols] one after another: X = in / ||in||, then `steps`
+ * times X <- a X + (b G + c G G) X with G = X X^T on the shorter side and (a, b, c) = (3.4445, -4.7750, 2.0315), which
+ * brings every singular value near one. A matrix of zeros stays zero. */
+int vc_hip_orthogonalise(const float* in, size_t count, size_t rows, size_t cols, size_t steps, float* out);
+/* One parameter of vc_hip_muon_step: `count` matrices [rows, cols], all updated in place but grad. */
+typedef struct vc_hip_muon_item {
+    float* param;
+    float* momentum;
+    const float* grad;
+    size_t count, rows, cols;
+} vc_hip_muon_item;
+/* For every item: momentum = mu * momentum + grad; O = orthogonalise(grad + mu * momentum);
+ * param = (1 - rate * decay) * param - rate * sqrt(max(1, cols / rows)) * O. Items must not overlap. */
+int vc_hip_muon_step(const vc_hip_muon_item* items, size_t n_items, float rate, float mu, float decay, size_t steps);
+
 /* ---- measurement ------------------------------------------------------------- */
 /* When enabled, the kernels of each labelled entry-point call carry HIP
  * events as dispatch timestamps on the library stream (no marker packets

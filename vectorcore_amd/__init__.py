@@ -8,9 +8,14 @@ it links) must be built in-tree: ``python vectorcore_amd/build.py``.
 """
 
 from ._vectorcore import (  # noqa: F401
+    ExpertPlan,
     Linear,
     Tensor,
     cross_entropy,
+    expert_combine,
+    expert_gated,
+    expert_linear,
+    from_dlpack,
     hip_available,
     hip_defer_products,
     hip_device_name,
@@ -27,6 +32,9 @@ from ._vectorcore import (  # noqa: F401
     metal_device_name,
     metal_gemm_kernel,
     mse_loss,
+    muon_step,
+    orthogonalise,
+    route,
     sgd_step,
     softmax,
     synchronize,

@@ -49,6 +49,20 @@ class MapMatrix(ctypes.Structure):
                 ("row_sum_slots", ctypes.c_ubyte * MAP_SUMS), ("n_row_sums", _sz)]
 
 
+SOFTMAX, SIGMOID_SCORE = 0, 1
+
+
+class ExpertPlan(ctypes.Structure):
+    _fields_ = [("words", _vp), ("tokens", _sz), ("top_k", _sz), ("experts", _sz)]
+
+
+class MuonItem(ctypes.Structure):
+    _fields_ = [("param", _vp), ("momentum", _vp), ("grad", _vp), ("count", _sz), ("rows", _sz), ("cols", _sz)]
+
+
+WHEN_DONE = ctypes.CFUNCTYPE(None, _vp)
+
+
 def map_word(op: int, a: int, b: int, dst: int) -> int:
     """One instruction of a vc_hip_map program: slot[dst] = slot[a] op slot[b]."""
     return op | a << 8 | b << 16 | dst << 24
@@ -142,6 +156,23 @@ _SIGNATURES = {
     "vc_hip_xent_backward_value": ([_vp, _vp, _vp, _f, _sz, _sz, _vp], _i),
     "vc_hip_xent_backward_colsum": ([_vp, _vp, _vp, _vp, _f, _sz, _sz, _vp, _vp], _i),
     "vc_hip_xent_backward_colsum_pending": ([_vp, _vp, _vp, _vp, _f, _sz, _sz, _vp, _vp, ctypes.POINTER(_vp)], _i),
+    "vc_hip_stream": ([ctypes.POINTER(ctypes.c_uint64)], _i),
+    "vc_hip_wait_for_stream": ([ctypes.c_uint64], _i),
+    "vc_hip_release_to_stream": ([ctypes.c_uint64], _i),
+    "vc_hip_when_done": ([WHEN_DONE, _vp], _i),
+    "vc_hip_route_forward": ([_vp, _vp, _sz, _sz, _sz, _i, _sz, _sz, _i, _vp, _vp], _i),
+    "vc_hip_route_backward": ([_vp, _vp, _vp, _sz, _sz, _sz, _i, _i, _vp], _i),
+    "vc_hip_expert_plan_words": ([_sz, _sz, _sz, _szp], _i),
+    "vc_hip_expert_plan_build": ([_vp, _sz, _sz, _sz, _vp], _i),
+    "vc_hip_expert_linear_forward": ([_vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _sz, _i, _vp], _i),
+    "vc_hip_expert_gated_forward": ([_vp, _vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _sz, _i, _vp, _vp, _vp], _i),
+    "vc_hip_expert_gated_backward": ([_vp, _vp, _vp, _sz, _vp, _vp], _i),
+    "vc_hip_expert_linear_backward_input": ([_vp, _vp, _vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _sz, _vp], _i),
+    "vc_hip_expert_linear_backward_weight": ([_vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _sz, _i, _vp], _i),
+    "vc_hip_expert_combine_forward": ([_vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _vp], _i),
+    "vc_hip_expert_combine_backward": ([_vp, _vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _vp, _vp], _i),
+    "vc_hip_orthogonalise": ([_vp, _sz, _sz, _sz, _sz, _vp], _i),
+    "vc_hip_muon_step": ([ctypes.POINTER(MuonItem), _sz, _f, _f, _f, _sz], _i),
     "vc_hip_profile_enable": ([_i], _i),
     "vc_hip_profile_labels": ([ctypes.c_char_p], _i),
     "vc_hip_profile_reset": ([], _i),

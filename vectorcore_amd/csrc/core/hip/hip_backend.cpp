@@ -119,10 +119,24 @@ public:
     HipStorage(std::size_t elements, MapExpr expr, std::size_t summed, bool row_sums)
         : elements_(elements), sum_of_(std::move(expr)), summed_(summed), row_sums_(row_sums), shadow_valid_(false) {}
 
+    // Another library's memory (HipBackend::adopt).
+    HipStorage(std::size_t elements, float* data, std::function<void()> release)
+        : elements_(elements), ptr_(data), shadow_valid_(false), pinned_(true),
+          release_(std::make_unique<std::function<void()>>(std::move(release))) {}
+
     ~HipStorage() override {
         if (mirror_) (void)vc_hip_mirror_release(mirror_);
         if (pending_sums_) (void)vc_hip_colsum_release(pending_sums_);
-        if (ptr_) (void)vc_hip_release(ptr_);
+        if (release_) {
+            const auto call = [](void* f) {
+                const std::unique_ptr<std::function<void()>> release(static_cast<std::function<void()>*>(f));
+                (*release)();
+            };
+            // The owner's memory must outlive the kernels enqueued on it: where that cannot be seen to, it stays.
+            (void)vc_hip_when_done(call, release_.release());
+        } else if (ptr_) {
+            (void)vc_hip_release(ptr_);
+        }
     }
     HipStorage(const HipStorage&) = delete;
     HipStorage& operator=(const HipStorage&) = delete;
@@ -334,13 +348,15 @@ public:
         }
         void* fresh_buffer = nullptr;
         check(vc_hip_alloc(bytes(), &fresh_buffer), "HIP allocation failed");
-        if (offset != 0 || count != elements_) {
+        if (pinned_ || offset != 0 || count != elements_) {
             const int status = vc_hip_copy(fresh_buffer, ptr_, bytes());
             if (status != VC_HIP_OK) {
                 (void)vc_hip_release(fresh_buffer);
                 throw_status(status, "HIP copy failed");
             }
         }
+        // Another library knows a pinned storage's buffer: the readers get the copy.
+        if (pinned_) std::swap(fresh_buffer, ptr_);
         auto previous = std::make_shared<HipStorage>(elements_, ptr_);  // takes over the current buffer
         ptr_ = fresh_buffer;
         for (const auto& r : waiting) {
@@ -351,6 +367,23 @@ public:
         }
         readers_.clear();
         return previous;
+    }
+
+    // See HipBackend::expose: what is known of the contents here no longer holds
+    // once the other library writes them.
+    float* expose() {
+        std::lock_guard<std::recursive_mutex> lock(state_mutex());
+        (void)ptr();
+        pinned_ = true;
+        shadow_valid_ = false;
+        column_sum_.reset();
+        row_argmax_.reset();
+        relu_bits_.reset();
+        if (mirror_) {
+            (void)vc_hip_mirror_release(mirror_);
+            mirror_ = nullptr;
+        }
+        return static_cast<float*>(ptr_);
     }
 
 private:
@@ -378,6 +411,8 @@ private:
     mutable std::shared_ptr<HipStorage> relu_bits_;  // see relu_bits
     mutable std::size_t relu_bits_rows_ = 0, relu_bits_cols_ = 0;
     bool shadow_valid_;
+    bool pinned_ = false;  // another library holds this buffer's address
+    std::unique_ptr<std::function<void()>> release_;  // of another library's memory
 };
 
 constexpr std::size_t kHostKeptElements = 16;
@@ -1517,6 +1552,184 @@ std::shared_ptr<Storage> HipBackend::cross_entropy_backward(const Storage& logit
     check(status, "HIP cross-entropy backward failed");
     return out;
 }
+
+// ---- a mixture of experts ----------------------------------------------------------
+
+std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> HipBackend::route_forward(
+    const Storage& logits, std::size_t logits_offset, const Storage* bias, std::size_t bias_offset, std::size_t tokens,
+    std::size_t experts, std::size_t top_k, bool sigmoid, std::size_t groups, std::size_t top_groups, bool renormalise) {
+    require(*this);
+    auto weights = fresh(tokens * top_k), chosen = fresh(tokens * top_k);
+    check(vc_hip_route_forward(dptr(logits, logits_offset), bias ? dptr(*bias, bias_offset) : nullptr, tokens, experts, top_k,
+                               sigmoid ? VC_HIP_SCORE_SIGMOID : VC_HIP_SCORE_SOFTMAX, groups, top_groups, renormalise,
+                               weights->ptr(), chosen->ptr()),
+          "HIP route failed");
+    return {weights, chosen};
+}
+
+std::shared_ptr<Storage> HipBackend::route_backward(const Storage& logits, std::size_t logits_offset, const Storage& chosen,
+                                                    std::size_t chosen_offset, const Storage& grad, std::size_t grad_offset,
+                                                    std::size_t tokens, std::size_t experts, std::size_t top_k, bool sigmoid,
+                                                    bool renormalise) {
+    require(*this);
+    auto out = fresh(tokens * experts);
+    check(vc_hip_route_backward(dptr(logits, logits_offset), dptr(chosen, chosen_offset), dptr(grad, grad_offset), tokens,
+                                experts, top_k, sigmoid ? VC_HIP_SCORE_SIGMOID : VC_HIP_SCORE_SOFTMAX, renormalise, out->ptr()),
+          "HIP route backward failed");
+    return out;
+}
+
+std::shared_ptr<Storage> HipBackend::expert_plan(const Storage& chosen, std::size_t offset, std::size_t tokens,
+                                                 std::size_t top_k, std::size_t experts) {
+    require(*this);
+    std::size_t words = 0;
+    check(vc_hip_expert_plan_words(tokens, top_k, experts, &words), "HIP expert plan failed");
+    auto out = fresh(words);
+    check(vc_hip_expert_plan_build(dptr(chosen, offset), tokens, top_k, experts, reinterpret_cast<std::int32_t*>(out->ptr())),
+          "HIP expert plan failed");
+    return out;
+}
+
+namespace {
+vc_hip_expert_plan abi(const HipBackend::ExpertRows& plan) {
+    return {reinterpret_cast<const std::int32_t*>(dptr(*plan.words, 0)), plan.tokens, plan.top_k, plan.experts};
+}
+}  // namespace
+
+std::shared_ptr<Storage> HipBackend::expert_linear_forward(const Storage& x, std::size_t x_offset, const Storage& w,
+                                                           std::size_t w_offset, const ExpertRows& plan, std::size_t width,
+                                                           std::size_t columns, bool ordered) {
+    require(*this);
+    auto out = fresh(plan.tokens * plan.top_k * columns);
+    const auto rows = abi(plan);
+    check(vc_hip_expert_linear_forward(dptr(x, x_offset), dptr(w, w_offset), &rows, width, columns, ordered, out->ptr()),
+          "HIP expert product failed");
+    return out;
+}
+
+std::shared_ptr<Storage> HipBackend::expert_gated_forward(const Storage& x, std::size_t x_offset, const Storage& gate,
+                                                          std::size_t gate_offset, const Storage& up, std::size_t up_offset,
+                                                          const ExpertRows& plan, std::size_t width, std::size_t columns,
+                                                          bool ordered, std::shared_ptr<Storage>* save_gate,
+                                                          std::shared_ptr<Storage>* save_up) {
+    require(*this);
+    const std::size_t count = plan.tokens * plan.top_k * columns;
+    auto out = fresh(count);
+    std::shared_ptr<HipStorage> g, u;
+    if (save_gate && save_up) {
+        g = fresh(count);
+        u = fresh(count);
+    }
+    const auto rows = abi(plan);
+    check(vc_hip_expert_gated_forward(dptr(x, x_offset), dptr(gate, gate_offset), dptr(up, up_offset), &rows, width, columns,
+                                      ordered, out->ptr(), g ? g->ptr() : nullptr, u ? u->ptr() : nullptr),
+          "HIP gated expert product failed");
+    if (g) {
+        *save_gate = std::move(g);
+        *save_up = std::move(u);
+    }
+    return out;
+}
+
+std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> HipBackend::expert_gated_backward(
+    const Storage& grad, std::size_t grad_offset, const Storage& saved_gate, const Storage& saved_up, std::size_t count) {
+    require(*this);
+    auto dg = fresh(count), du = fresh(count);
+    check(vc_hip_expert_gated_backward(dptr(grad, grad_offset), dptr(saved_gate, 0), dptr(saved_up, 0), count, dg->ptr(),
+                                       du->ptr()),
+          "HIP gated expert backward failed");
+    return {dg, du};
+}
+
+std::shared_ptr<Storage> HipBackend::expert_linear_backward_input(const Storage& grad, std::size_t grad_offset,
+                                                                  const Storage& w, std::size_t w_offset,
+                                                                  const Storage* grad2, std::size_t grad2_offset,
+                                                                  const Storage* w2, std::size_t w2_offset,
+                                                                  const ExpertRows& plan, std::size_t width,
+                                                                  std::size_t columns) {
+    require(*this);
+    auto out = fresh(plan.tokens * plan.top_k * width);
+    const auto rows = abi(plan);
+    check(vc_hip_expert_linear_backward_input(dptr(grad, grad_offset), dptr(w, w_offset),
+                                              grad2 ? dptr(*grad2, grad2_offset) : nullptr, w2 ? dptr(*w2, w2_offset) : nullptr,
+                                              &rows, width, columns, out->ptr()),
+          "HIP expert product backward failed");
+    return out;
+}
+
+std::shared_ptr<Storage> HipBackend::expert_linear_backward_weight(const Storage& x, std::size_t x_offset, const Storage& grad,
+                                                                   std::size_t grad_offset, const ExpertRows& plan,
+                                                                   std::size_t width, std::size_t columns, bool ordered) {
+    require(*this);
+    auto out = fresh(plan.experts * width * columns);
+    const auto rows = abi(plan);
+    check(vc_hip_expert_linear_backward_weight(dptr(x, x_offset), dptr(grad, grad_offset), &rows, width, columns, ordered,
+                                               out->ptr()),
+          "HIP expert product backward failed");
+    return out;
+}
+
+std::shared_ptr<Storage> HipBackend::expert_combine_forward(const Storage& rows, std::size_t rows_offset,
+                                                            const Storage* weights, std::size_t weights_offset,
+                                                            const ExpertRows& plan, std::size_t width) {
+    require(*this);
+    auto out = fresh(plan.tokens * width);
+    const auto p = abi(plan);
+    check(vc_hip_expert_combine_forward(dptr(rows, rows_offset), weights ? dptr(*weights, weights_offset) : nullptr, &p, width,
+                                        out->ptr()),
+          "HIP expert combine failed");
+    return out;
+}
+
+std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> HipBackend::expert_combine_backward(
+    const Storage& grad, std::size_t grad_offset, const Storage& rows, std::size_t rows_offset, const Storage& weights,
+    std::size_t weights_offset, const ExpertRows& plan, std::size_t width, bool need_rows, bool need_weights) {
+    require(*this);
+    std::shared_ptr<HipStorage> dr, dw;
+    if (need_rows) dr = fresh(plan.tokens * plan.top_k * width);
+    if (need_weights) dw = fresh(plan.tokens * plan.top_k);
+    const auto p = abi(plan);
+    check(vc_hip_expert_combine_backward(dptr(grad, grad_offset), dptr(rows, rows_offset), dptr(weights, weights_offset), &p,
+                                         width, dr ? dr->ptr() : nullptr, dw ? dw->ptr() : nullptr),
+          "HIP expert combine backward failed");
+    return {dr, dw};
+}
+
+std::shared_ptr<Storage> HipBackend::orthogonalise(const Storage& input, std::size_t offset, std::size_t count,
+                                                   std::size_t rows, std::size_t cols, std::size_t steps) {
+    require(*this);
+    auto out = fresh(count * rows * cols);
+    check(vc_hip_orthogonalise(dptr(input, offset), count, rows, cols, steps, out->ptr()), "HIP orthogonalise failed");
+    return out;
+}
+
+void HipBackend::muon_step(const std::vector<MuonItem>& items, float rate, float mu, float decay, std::size_t steps) {
+    require(*this);
+    std::vector<vc_hip_muon_item> batch;
+    std::vector<std::shared_ptr<const HipStorage>> current;  // kept alive until the launches are enqueued
+    for (const MuonItem& it : items) {
+        const std::size_t n = it.count * it.rows * it.cols;
+        if (it.param_offset + n > it.param->size() || it.momentum_offset + n > it.momentum->size() ||
+            it.grad_offset + n > it.grad->size())
+            throw std::out_of_range("HIP muon step exceeds storage");
+        const float* grad = dptr(*it.grad, it.grad_offset);
+        auto &p = as_hip(*it.param), &m = as_hip(*it.momentum);
+        // The old values are read too: a write of nothing keeps them in the buffer.
+        current.push_back(p.before_write(0, 0));
+        current.push_back(m.before_write(0, 0));
+        batch.push_back({p.ptr() + it.param_offset, m.ptr() + it.momentum_offset, grad, it.count, it.rows, it.cols});
+    }
+    check(vc_hip_muon_step(batch.data(), batch.size(), rate, mu, decay, steps), "HIP muon step failed");
+}
+
+// ---- memory shared with other libraries ----------------------------------------------
+
+std::shared_ptr<Storage> HipBackend::adopt(float* data, std::size_t elements, std::function<void()> release) {
+    require(*this);
+    return std::make_shared<HipStorage>(elements, data, std::move(release));
+}
+
+float* HipBackend::expose(Storage& storage) { return as_hip(storage).expose(); }
 
 std::optional<float> hip_host_scalar(const Storage& storage) {
     const auto* h = dynamic_cast<const HipStorage*>(&storage);

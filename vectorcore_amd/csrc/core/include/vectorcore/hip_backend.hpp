@@ -11,6 +11,7 @@
 #include "vectorcore/storage.hpp"
 
 #include <cstdint>
+#include <functional>
 #include <memory>
 #include <optional>
 #include <string>
@@ -212,6 +213,77 @@ public:
                                                                   const Storage& grad_loss, std::size_t grad_offset,
                                                                   std::size_t rows, std::size_t classes,
                                                                   bool column_sum = false);
+
+    // --- a mixture of experts (the entry points of the same names) ---
+    // {weights, chosen}.
+    [[nodiscard]] std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> route_forward(
+        const Storage& logits, std::size_t logits_offset, const Storage* bias, std::size_t bias_offset, std::size_t tokens,
+        std::size_t experts, std::size_t top_k, bool sigmoid, std::size_t groups, std::size_t top_groups, bool renormalise);
+    [[nodiscard]] std::shared_ptr<Storage> route_backward(const Storage& logits, std::size_t logits_offset,
+                                                          const Storage& chosen, std::size_t chosen_offset,
+                                                          const Storage& grad, std::size_t grad_offset, std::size_t tokens,
+                                                          std::size_t experts, std::size_t top_k, bool sigmoid,
+                                                          bool renormalise);
+    // The plan's words (vc_hip_expert_plan), as int32 bits.
+    [[nodiscard]] std::shared_ptr<Storage> expert_plan(const Storage& chosen, std::size_t offset, std::size_t tokens,
+                                                       std::size_t top_k, std::size_t experts);
+    struct ExpertRows {
+        const Storage* words;
+        std::size_t tokens, top_k, experts;
+    };
+    [[nodiscard]] std::shared_ptr<Storage> expert_linear_forward(const Storage& x, std::size_t x_offset, const Storage& w,
+                                                                 std::size_t w_offset, const ExpertRows& plan,
+                                                                 std::size_t width, std::size_t columns, bool ordered);
+    // save_gate, save_up: receive the two products, or both null.
+    [[nodiscard]] std::shared_ptr<Storage> expert_gated_forward(const Storage& x, std::size_t x_offset, const Storage& gate,
+                                                                std::size_t gate_offset, const Storage& up,
+                                                                std::size_t up_offset, const ExpertRows& plan,
+                                                                std::size_t width, std::size_t columns, bool ordered,
+                                                                std::shared_ptr<Storage>* save_gate,
+                                                                std::shared_ptr<Storage>* save_up);
+    [[nodiscard]] std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> expert_gated_backward(
+        const Storage& grad, std::size_t grad_offset, const Storage& saved_gate, const Storage& saved_up, std::size_t count);
+    // grad2, w2: a second product to add, or both null.
+    [[nodiscard]] std::shared_ptr<Storage> expert_linear_backward_input(const Storage& grad, std::size_t grad_offset,
+                                                                        const Storage& w, std::size_t w_offset,
+                                                                        const Storage* grad2, std::size_t grad2_offset,
+                                                                        const Storage* w2, std::size_t w2_offset,
+                                                                        const ExpertRows& plan, std::size_t width,
+                                                                        std::size_t columns);
+    [[nodiscard]] std::shared_ptr<Storage> expert_linear_backward_weight(const Storage& x, std::size_t x_offset,
+                                                                         const Storage& grad, std::size_t grad_offset,
+                                                                         const ExpertRows& plan, std::size_t width,
+                                                                         std::size_t columns, bool ordered);
+    [[nodiscard]] std::shared_ptr<Storage> expert_combine_forward(const Storage& rows, std::size_t rows_offset,
+                                                                  const Storage* weights, std::size_t weights_offset,
+                                                                  const ExpertRows& plan, std::size_t width);
+    // {gradient of the rows, of the weights}, either may be skipped.
+    [[nodiscard]] std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> expert_combine_backward(
+        const Storage& grad, std::size_t grad_offset, const Storage& rows, std::size_t rows_offset, const Storage& weights,
+        std::size_t weights_offset, const ExpertRows& plan, std::size_t width, bool need_rows, bool need_weights);
+
+    // --- orthogonalised updates ---
+    [[nodiscard]] std::shared_ptr<Storage> orthogonalise(const Storage& input, std::size_t offset, std::size_t count,
+                                                         std::size_t rows, std::size_t cols, std::size_t steps);
+    struct MuonItem {
+        Storage* param;
+        std::size_t param_offset;
+        Storage* momentum;
+        std::size_t momentum_offset;
+        const Storage* grad;
+        std::size_t grad_offset, count, rows, cols;
+    };
+    // Distinct storages but for the gradients. The caller bumps the versions.
+    void muon_step(const std::vector<MuonItem>& items, float rate, float mu, float decay, std::size_t steps);
+
+    // --- memory shared with other libraries ---
+    // A storage over device memory that its owner keeps until `release` is
+    // called, which is once the work enqueued before the storage died is done.
+    // In-place ops write to that memory.
+    [[nodiscard]] std::shared_ptr<Storage> adopt(float* data, std::size_t elements, std::function<void()> release);
+    // The buffer of a storage for another library, computed; it stays the
+    // storage's buffer from now on, also across in-place writes.
+    [[nodiscard]] float* expose(Storage& storage);
 };
 
 // Host-side value of a one-element hip storage created from host data, if it

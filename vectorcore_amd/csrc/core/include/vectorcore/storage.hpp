@@ -4,6 +4,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <functional>
 #include <memory>
 
 namespace vectorcore {
@@ -28,5 +29,7 @@ private:
 
 std::shared_ptr<Storage> make_cpu_storage(std::size_t elements);
 std::shared_ptr<Storage> make_cpu_storage(const float* values, std::size_t elements);
+// A storage over host memory that its owner keeps until `release` is called.
+std::shared_ptr<Storage> adopt_cpu_storage(float* values, std::size_t elements, std::function<void()> release);
 
 }  // namespace vectorcore

@@ -4,6 +4,7 @@
 #include "vectorcore/vectorcore.hpp"
 #include "vectorcore/detail/tensor_impl.hpp"
 
+#include "dlpack.hpp"
 #include "vc_hip.h"
 
 #include <pybind11/numpy.h>
@@ -143,6 +144,14 @@ PYBIND11_MODULE(_vectorcore, m) {
         .def("backward", py::overload_cast<>(&Tensor::backward, py::const_))
         .def("backward", py::overload_cast<const Tensor&>(&Tensor::backward, py::const_))
         .def("zero_grad", &Tensor::zero_grad)
+        .def("__dlpack__",
+             [](const Tensor& t, const py::object& stream, const py::object&, const py::object& device, const py::object& copy) {
+                 return dlpack::export_(t, stream, device, copy);
+             },
+             py::kw_only(), py::arg("stream") = py::none(), py::arg("max_version") = py::none(),
+             py::arg("dl_device") = py::none(), py::arg("copy") = py::none(),
+             "A DLPack capsule of the tensor's memory; the given stream waits for the work enqueued on it.")
+        .def("__dlpack_device__", &dlpack::device_of)
         .def("__repr__", &Tensor::repr)
         .def("__matmul__", &Tensor::matmul, py::is_operator())
         .def("__add__", [](const Tensor& a, const Tensor& b) { return a + b; }, py::is_operator())
@@ -181,6 +190,58 @@ PYBIND11_MODULE(_vectorcore, m) {
         for (auto& p : params) ptrs.push_back(&p);
         nn::sgd_step(ptrs, lr);
     });
+    py::class_<ExpertPlan>(m, "ExpertPlan",
+                           "The picks of `chosen` [tokens, top_k] sorted by expert. An entry that is no expert number is a "
+                           "dropped pick, whose row is zero in every result.")
+        .def(py::init<const Tensor&, std::size_t>(), py::arg("chosen"), py::arg("experts"))
+        .def_property_readonly("tokens", &ExpertPlan::tokens)
+        .def_property_readonly("top_k", &ExpertPlan::top_k)
+        .def_property_readonly("experts", &ExpertPlan::experts)
+        .def_property_readonly("rows", &ExpertPlan::rows);
+    m.def(
+        "route",
+        [](const Tensor& logits, std::size_t top_k, std::optional<Tensor> bias, const std::string& score, std::size_t groups,
+           std::size_t top_groups, bool renormalise) {
+            if (score != "softmax" && score != "sigmoid") throw std::invalid_argument("score must be 'softmax' or 'sigmoid'");
+            Routed r = route(logits, top_k,
+                             {std::move(bias), score == "sigmoid" ? RouterScore::Sigmoid : RouterScore::Softmax, groups,
+                              top_groups, renormalise});
+            return py::make_tuple(std::move(r.weights), std::move(r.chosen));
+        },
+        py::arg("logits"), py::arg("top_k"), py::arg("bias") = py::none(), py::arg("score") = "softmax",
+        py::arg("groups") = 1, py::arg("top_groups") = 1, py::arg("renormalise") = true,
+        "The top_k experts of each row of logits [tokens, experts]: (weights, chosen), both [tokens, top_k], best first. "
+        "Experts are ranked by score + bias, equal ones by the lower index; of `groups` equal groups of neighbouring experts "
+        "the `top_groups` with the largest sums of their two best ranks take part. The weights are the scores, divided by "
+        "their sum if `renormalise`, and carry the gradient to the logits.");
+    m.def("expert_linear", &expert_linear, py::arg("x"), py::arg("weight"), py::arg("plan"), py::arg("ordered") = false,
+          "Each row times the matrix of its expert in weight [experts, width, columns]. x: [tokens, width], or with `ordered` "
+          "[rows, width] in the plan's order.");
+    m.def("expert_gated", &expert_gated, py::arg("x"), py::arg("gate"), py::arg("up"), py::arg("plan"),
+          py::arg("ordered") = false, "silu(x @ gate[expert]) * (x @ up[expert]) for each row of the plan.");
+    m.def("expert_combine", &expert_combine, py::arg("rows"), py::arg("weights"), py::arg("plan"),
+          "[tokens, width]: the sum of each token's rows, times its weights [tokens, top_k].");
+    m.def("orthogonalise", &orthogonalise, py::arg("value"), py::arg("steps") = 5,
+          "Each matrix of value [..., rows, cols] with its singular values brought near one by Newton-Schulz iterations.");
+    m.def(
+        "muon_step",
+        [](std::vector<Tensor> params, std::vector<Tensor> momenta, float lr, float momentum, float weight_decay,
+           std::size_t steps, std::optional<std::vector<Tensor>> grads) {
+            std::vector<Tensor*> p, mo;
+            for (auto& t : params) p.push_back(&t);
+            for (auto& t : momenta) mo.push_back(&t);
+            if (grads && grads->size() != params.size())
+                throw std::invalid_argument("muon_step: " + std::to_string(grads->size()) + " gradients for " +
+                                            std::to_string(params.size()) + " parameters");
+            nn::muon_step(p, mo, lr, momentum, weight_decay, steps, grads ? *grads : std::vector<Tensor>{});
+        },
+        py::arg("params"), py::arg("momenta"), py::arg("lr"), py::arg("momentum") = 0.95F, py::arg("weight_decay") = 0.0F,
+        py::arg("steps") = 5, py::arg("grads") = py::none(),
+        "Orthogonalised momentum update in place: m = momentum * m + g; p = (1 - lr * weight_decay) * p - "
+        "lr * sqrt(max(1, cols / rows)) * orthogonalise(g + momentum * m). g: `grads`, or the parameters' own gradients.");
+    m.def("from_dlpack", &dlpack::import_,
+          "Tensors over the memory of the given objects (__dlpack__): float32, contiguous, on the host or the GPU. Always a "
+          "tuple.");
     m.def("zero_grad", [](std::vector<Tensor> params) {
         for (auto& p : params) p.zero_grad();
     });

@@ -2,6 +2,7 @@
 
 #include <algorithm>
 #include <stdexcept>
+#include <utility>
 
 namespace vectorcore {
 
@@ -23,6 +24,23 @@ private:
     std::size_t n_;
 };
 
+class AdoptedStorage final : public Storage {
+public:
+    AdoptedStorage(float* values, std::size_t n, std::function<void()> release)
+        : values_(values), n_(n), release_(std::move(release)) {}
+    ~AdoptedStorage() override { release_(); }
+    AdoptedStorage(const AdoptedStorage&) = delete;
+    AdoptedStorage& operator=(const AdoptedStorage&) = delete;
+    [[nodiscard]] Device device() const noexcept override { return Device::cpu(); }
+    [[nodiscard]] std::size_t size() const noexcept override { return n_; }
+    [[nodiscard]] const float* data() const override { return values_; }
+    [[nodiscard]] float* mutable_data() override { return values_; }
+private:
+    float* values_;
+    std::size_t n_;
+    std::function<void()> release_;
+};
+
 }  // namespace
 
 std::shared_ptr<Storage> make_cpu_storage(std::size_t elements) { return std::make_shared<HostStorage>(elements); }
@@ -32,6 +50,10 @@ std::shared_ptr<Storage> make_cpu_storage(const float* values, std::size_t eleme
     auto s = std::make_shared<HostStorage>(elements);
     if (elements) std::copy(values, values + elements, s->mutable_data());
     return s;
+}
+
+std::shared_ptr<Storage> adopt_cpu_storage(float* values, std::size_t elements, std::function<void()> release) {
+    return std::make_shared<AdoptedStorage>(values, elements, std::move(release));
 }
 
 }  // namespace vectorcore

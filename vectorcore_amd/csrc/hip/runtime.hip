@@ -65,6 +65,8 @@ void init_device(Device& d) {
     d.ready = true;
 }
 
+void poll_deferred(Device& d);
+
 // ---- pool ---------------------------------------------------------------------
 
 class Pool {
@@ -81,6 +83,8 @@ public:
         return (bytes + kStep - 1) / kStep * kStep;
     }
 
+    // Before the device's own allocator is asked (a miss), callbacks whose work
+    // is done give back what they hold.
     void* alloc(size_t bytes) {
         Device& d = require_device();
         const size_t cls = size_class(bytes);
@@ -97,6 +101,7 @@ public:
                 return p;
             }
         }
+        poll_deferred(d);
         void* p = nullptr;
         hipError_t e = hipMalloc(&p, cls);
         if (e != hipSuccess) {
@@ -154,6 +159,77 @@ private:
 Pool& pool() {
     static Pool p;
     return p;
+}
+
+// ---- what waits for the stream to pass a point (vc_hip_when_done) -----------------
+
+// Callbacks in batches, one event for each: what is added while a batch waits
+// forms the next one, so that releasing many buffers costs one event.
+class Deferred {
+public:
+    void add(Device& d, void (*done)(void*), void* context) {
+        {
+            std::lock_guard<std::mutex> lock(mu_);
+            added_.push_back(Entry{done, context});
+            any_.store(true, std::memory_order_relaxed);
+        }
+        poll(d);
+    }
+
+    // Calls what the stream has passed, in the order it was added; outside the
+    // lock, as a callback may come back here.
+    void poll(Device& d) {
+        if (!any_.load(std::memory_order_relaxed)) return;
+        std::vector<Entry> ready;
+        {
+            std::lock_guard<std::mutex> lock(mu_);
+            if (!waiting_.empty()) {
+                const hipError_t state = hipEventQuery(event_);
+                if (state == hipSuccess) ready.swap(waiting_);
+                else (void)hipGetLastError();
+            }
+            if (waiting_.empty() && !added_.empty()) {
+                if (!event_) check_hip(hipEventCreateWithFlags(&event_, hipEventDisableTiming), "hipEventCreate");
+                check_hip(hipEventRecord(event_, d.stream), "hipEventRecord");
+                waiting_.swap(added_);
+            }
+            any_.store(!waiting_.empty(), std::memory_order_relaxed);
+        }
+        for (const Entry& e : ready) e.done(e.context);
+    }
+
+private:
+    struct Entry {
+        void (*done)(void*);
+        void* context;
+    };
+    std::mutex mu_;
+    hipEvent_t event_ = nullptr;
+    std::vector<Entry> waiting_, added_;
+    std::atomic<bool> any_{false};
+};
+
+Deferred& deferred() {
+    static Deferred d;
+    return d;
+}
+
+void poll_deferred(Device& d) { deferred().poll(d); }
+
+// Work enqueued on `later` from now on waits for what is on `earlier`. An idle
+// stream needs no event and no wait packet, the usual case of a caller that
+// passes finished inputs.
+void stream_after(hipStream_t later, hipStream_t earlier) {
+    if (later == earlier) return;
+    const hipError_t state = hipStreamQuery(earlier);
+    if (state == hipSuccess) return;
+    (void)hipGetLastError();
+    if (state != hipErrorNotReady) check_hip(state, "hipStreamQuery");
+    // A recorded wait keeps its point: the event can be recorded again at once.
+    thread_local hipEvent_t event = nullptr;
+    if (!event) check_hip(hipEventCreateWithFlags(&event, hipEventDisableTiming), "hipEventCreate");
+    check_hip(hipEventRecord(event, earlier), "hipEventRecord");
+    check_hip(hipStreamWaitEvent(later, event, 0), "hipStreamWaitEvent");
 }
 
 // ---- pinned staging ring for uploads --------------------------------------------
@@ -629,6 +705,8 @@ int vc_hip_download(void* dst, const void* src, size_t bytes) {
         }
         check_hip(hipStreamSynchronize(d.stream), "HIP command failed");
         staging().on_synchronized();
+        deferred().poll(d);
+        deferred().poll(d);  // and what was added behind the first batch's event
     });
 }
 
@@ -679,6 +757,38 @@ int vc_hip_synchronize(void) {
         if (!d.ready) return;  // like the reference: a no-op without a device
         check_hip(hipStreamSynchronize(d.stream), "HIP command failed");
         staging().on_synchronized();
+        deferred().poll(d);
+        deferred().poll(d);  // and what was added behind the first batch's event
+    });
+}
+
+int vc_hip_stream(uint64_t* stream) {
+    return guard([&] {
+        Device& d = require_device();
+        if (!stream) fail(VC_HIP_ERR_INVALID_ARGUMENT, "vc_hip_stream: null pointer");
+        *stream = reinterpret_cast<uint64_t>(d.stream);
+    });
+}
+
+int vc_hip_wait_for_stream(uint64_t stream) {
+    return guard([&] {
+        Device& d = require_device();
+        stream_after(d.stream, reinterpret_cast<hipStream_t>(stream));
+    });
+}
+
+int vc_hip_release_to_stream(uint64_t stream) {
+    return guard([&] {
+        Device& d = require_device();
+        stream_after(reinterpret_cast<hipStream_t>(stream), d.stream);
+    });
+}
+
+int vc_hip_when_done(void (*done)(void*), void* context) {
+    return guard([&] {
+        Device& d = require_device();
+        if (!done) fail(VC_HIP_ERR_INVALID_ARGUMENT, "vc_hip_when_done: null callback");
+        deferred().add(d, done, context);
     });
 }
 
