@@ -523,7 +523,7 @@ int vc_hip_route_backward(const float* logits, const float* chosen, const float*
  * number (negative, not whole, too large, NaN) is a dropped pick: it counts to
  * the group `experts`, whose rows are zero in every result. words holds
  * vc_hip_expert_plan_words int32 values: offsets [experts + 2] of the groups'
- * first rows, order [rows] the pick of each row, place [rows] the row of each
+ * first rows, token [rows] the token of each row, place [rows] the row of each
  * pick, with scratch behind them. */
 typedef struct vc_hip_expert_plan {
     const int32_t* words;

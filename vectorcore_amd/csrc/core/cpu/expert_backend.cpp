@@ -47,7 +47,7 @@ const float* group_rows(const float* x, const ExpertRows& plan, std::size_t e, s
     if (ordered) return x + lo * width;
     gathered.resize((hi - lo) * width);
     for (std::size_t r = lo; r < hi; ++r) {
-        const float* row = x + static_cast<std::size_t>(plan.order[r]) / plan.top_k * width;
+        const float* row = x + static_cast<std::size_t>(plan.token[r]) * width;
         std::copy(row, row + width, gathered.data() + (r - lo) * width);
     }
     return gathered.data();
@@ -127,7 +127,7 @@ void route_backward(const float* logits, const float* chosen, const float* grad_
 
 void expert_plan_build(const float* chosen, std::size_t tokens, std::size_t top_k, std::size_t experts, std::int32_t* words) {
     const std::size_t rows = tokens * top_k;
-    std::int32_t *const offsets = words, *const order = words + experts + 2, *const place = order + rows;
+    std::int32_t *const offsets = words, *const token = words + experts + 2, *const place = token + rows;
     std::vector<std::int32_t> group(rows);
     std::fill(offsets, offsets + experts + 2, 0);
     for (std::size_t p = 0; p < rows; ++p) {
@@ -140,7 +140,7 @@ void expert_plan_build(const float* chosen, std::size_t tokens, std::size_t top_
     std::vector<std::int32_t> next(offsets, offsets + experts + 1);
     for (std::size_t p = 0; p < rows; ++p) {
         const std::int32_t r = next[static_cast<std::size_t>(group[p])]++;
-        order[r] = static_cast<std::int32_t>(p);
+        token[r] = static_cast<std::int32_t>(p / top_k);
         place[p] = r;
     }
 }

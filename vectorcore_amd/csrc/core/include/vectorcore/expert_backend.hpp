@@ -14,10 +14,10 @@ void route_backward(const float* logits, const float* chosen, const float* grad_
 
 struct ExpertRows {  // a plan's words
     std::size_t tokens, top_k, experts;
-    const std::int32_t *offsets, *order, *place;
+    const std::int32_t *offsets, *token, *place;
     [[nodiscard]] std::size_t rows() const { return tokens * top_k; }
 };
-// words: offsets [experts + 2], order [rows], place [rows].
+// words: offsets [experts + 2], token [rows], place [rows].
 void expert_plan_build(const float* chosen, std::size_t tokens, std::size_t top_k, std::size_t experts, std::int32_t* words);
 void expert_linear_forward(const float* x, const float* w, const ExpertRows& plan, std::size_t width, std::size_t columns,
                            bool ordered, float* out);

@@ -2,6 +2,7 @@
 // products of each expert's rows with its matrices and their gradients, and
 // the weighted sum of a token's picks.
 #include "reduce_common.hpp"
+#include "split_product.hpp"
 #include "vc_hip_internal.hpp"
 
 #include <algorithm>
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_count_kernel(const float* __r
 // counts: of every chunk, or null for one chunk counted here.
 __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(const float* __restrict__ chosen, int rows, int chunk,
                                                                 int experts, const int* __restrict__ counts,
-                                                                int* __restrict__ offsets, int* __restrict__ order,
+                                                                int top_k, int* __restrict__ offsets, int* __restrict__ token,
                                                                 int* __restrict__ place) {
     extern __shared__ int lds[];
     const int groups = experts + 1, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(const float* __r
         if (p < end) {
             int row = next[e] + rank;
             for (int w = 0; w < wave; ++w) row += found[w * groups + e];
-            order[row] = p;
+            token[row] = p / top_k;
             place[p] = row;
         }
         __syncthreads();
@@ -130,7 +131,7 @@ void check_plan_sizes(size_t tokens, size_t top_k, size_t experts) {
 
 struct Plan {
     size_t tokens, top_k, experts, rows;
-    const int *offsets, *order, *place;
+    const int *offsets, *token, *place;
 };
 
 Plan plan_of(const vc_hip_expert_plan* plan) {
@@ -142,138 +143,270 @@ Plan plan_of(const vc_hip_expert_plan* plan) {
 }
 
 // ---- products -----------------------------------------------------------------------
-// 64 x 64 tiles of C by 256 threads, 4 x 4 each, k through LDS 16 at a time.
+// Tiles of 128 rows of one group by 128 columns (split_product.hpp).
 
-constexpr int kTile = 64, kSlice = 16;
+constexpr int kTile = 128;
+using S = split::Bf16x3;
 
-// A's element (row i of the tile, k) and B's (k, column j) as each kind of product stores them.
 struct ProductArgs {
     const float *a, *b, *a2, *b2;
-    float* c;
-    const int *offsets, *order;
-    int experts, top_k;     // top_k: of a gathered A, 0 where A lies in row order
+    float *c, *c2, *c3;
+    const int *offsets, *token;  // token: of each row of a gathered A, null where A lies in row order
+    int experts;
     int64_t width, columns;  // of each expert's matrix [width, columns]
 };
 
-// Which of the tiles of kTile rows, counted group by group, this is.
-__device__ inline bool find_rows(const int* offsets, int groups, int tile, int& group, int& begin, int& end) {
-    for (int e = 0; e < groups; ++e) {
-        const int lo = offsets[e], hi = offsets[e + 1], tiles = (hi - lo + kTile - 1) / kTile;
-        if (tile < tiles) {
-            group = e;
-            begin = lo + tile * kTile;
-            end = min(hi, begin + kTile);
-            return true;
-        }
-        tile -= tiles;
+struct RowTile {
+    int group, begin, end;  // rows of one group
+    int64_t column;         // tile of columns
+    bool live;
+};
+
+// The tile of this workgroup: tiles are numbered group by group, their columns
+// together, and dealt out so that each of the chip's eight dies (workgroups go
+// to them in turn) works on neighbouring ones, which read the same operands
+// through its cache.
+__device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups, int64_t column_tiles) {
+    const int lane = threadIdx.x % kWave;
+    int all = 0;
+    for (int base = 0; base < groups; base += kWave) {
+        const int e = base + lane;
+        const int n = e < groups ? (offsets[e + 1] - offsets[e] + kTile - 1) / kTile : 0;
+        int sum = n;
+        for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
+        all += sum;
     }
-    return false;
-}
-
-enum class Product { Forward, Input, Weight };
-
-template <Product P>
-__global__ __launch_bounds__(256) void product_kernel(ProductArgs p) {
-    __shared__ float as[kSlice][kTile + 4], bs[kSlice][kTile + 4];
-    const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
-    int group = blockIdx.z, begin = 0, end = 0;
-    int64_t m0 = 0;
-    const int64_t n0 = int64_t(blockIdx.x) * kTile, n = P == Product::Input ? p.width : p.columns;
-    int64_t depth;
-    if constexpr (P == Product::Weight) {
-        begin = p.offsets[group];
-        end = p.offsets[group + 1];
-        m0 = int64_t(blockIdx.y) * kTile;
-        depth = end - begin;
-    } else {
-        if (!find_rows(p.offsets, p.experts + 1, blockIdx.y, group, begin, end)) return;
-        depth = P == Product::Input ? p.columns : p.width;
-    }
-    float acc[4][4] = {};
-    for (int pass = 0; pass < (P == Product::Input && p.a2 ? 2 : 1); ++pass) {
-        const float* const a = pass ? p.a2 : p.a;
-        const float* const w = (pass ? p.b2 : p.b) + (P == Product::Weight ? 0 : int64_t(group) * p.width * p.columns);
-        if (P != Product::Weight && group == p.experts) break;  // dropped picks: zero rows
-        for (int64_t k0 = 0; k0 < depth; k0 += kSlice) {
-            for (int i = tid; i < kSlice * kTile; i += 256) {
-                float av = 0.0f, bv = 0.0f;
-                if constexpr (P == Product::Weight) {
-                    const int kk = i / kTile, x = i % kTile;
-                    const int64_t r = begin + k0 + kk;
-                    if (r < end) {
-                        const int64_t row = p.top_k ? p.order[r] / p.top_k : r;
-                        if (m0 + x < p.width) av = a[row * p.width + m0 + x];
-                        if (n0 + x < n) bv = w[r * p.columns + n0 + x];
-                    }
-                    as[kk][x] = av;
-                    bs[kk][x] = bv;
-                } else {
-                    const int x = i / kSlice, kk = i % kSlice;
-                    const int64_t r = begin + x;
-                    if (r < end && k0 + kk < depth) {
-                        const int64_t row = p.top_k ? p.order[r] / p.top_k : r;
-                        av = a[row * depth + k0 + kk];
-                    }
-                    as[kk][x] = av;
-                    if constexpr (P == Product::Input) {
-                        if (n0 + x < n && k0 + kk < depth) bv = w[(n0 + x) * p.columns + k0 + kk];
-                        bs[kk][x] = bv;
-                    } else {
-                        const int bk = i / kTile, bx = i % kTile;
-                        if (n0 + bx < n && k0 + bk < depth) bv = w[(k0 + bk) * p.columns + n0 + bx];
-                        bs[bk][bx] = bv;
-                    }
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int kk = 0; kk < kSlice; ++kk)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[kk][ty + 16 * i], bs[kk][tx + 16 * j], acc[i][j]);
-            __syncthreads();
+    const int64_t total = all * column_tiles, share = (total + 7) / 8;
+    const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8;
+    RowTile t{0, 0, 0, id % column_tiles, blockIdx.x / 8 < share && id < total};
+    if (!t.live) return t;
+    int tile = int(id / column_tiles);
+    for (int base = 0; base < groups; base += kWave) {
+        const int e = base + lane;
+        const int lo = e < groups ? offsets[e] : 0, hi = e < groups ? offsets[e + 1] : 0;
+        const int n = (hi - lo + kTile - 1) / kTile;
+        int upto = n;
+        for (int d = 1; d < kWave; d <<= 1) {
+            const int v = __shfl_up(upto, d);
+            if (lane >= d) upto += v;
         }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t col = n0 + tx + 16 * j;
-            if (col >= n) continue;
-            if constexpr (P == Product::Weight) {
-                const int64_t row = m0 + ty + 16 * i;
-                if (row < p.width) p.c[(int64_t(group) * p.width + row) * n + col] = acc[i][j];
-            } else {
-                const int64_t row = begin + ty + 16 * i;
-                if (row < end) p.c[row * n + col] = acc[i][j];
-            }
+        const uint64_t past = __ballot(upto > tile);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            t.group = base + at;
+            t.begin = __shfl(lo, at) + (tile - __shfl(upto - n, at)) * kTile;
+            t.end = min(__shfl(hi, at), t.begin + kTile);
+            break;
         }
+        tile -= __shfl(upto, kWave - 1);
+    }
+    t.group = __builtin_amdgcn_readfirstlane(t.group);
+    t.begin = __builtin_amdgcn_readfirstlane(t.begin);
+    t.end = __builtin_amdgcn_readfirstlane(t.end);
+    return t;
 }
-
-unsigned tiles_of(size_t n) { return unsigned((n + kTile - 1) / kTile); }
-
-void row_product(Device& d, const Plan& plan, bool input, ProductArgs p) {
-    const unsigned row_tiles = unsigned(plan.rows / kTile + plan.experts + 1);
-    if (input)
-        launch(product_kernel<Product::Input>, dim3(tiles_of(p.width), row_tiles), dim3(256), 0, d.stream, p);
-    else
-        launch(product_kernel<Product::Forward>, dim3(tiles_of(p.columns), row_tiles), dim3(256), 0, d.stream, p);
-    after_launch("expert product");
-}
-
-// ---- the gated unit -------------------------------------------------------------------
 
 __device__ inline float sigmoid(float x) {
     const float e = expf(-fabsf(x));
     return (x >= 0.0f ? 1.0f : e) / (1.0f + e);
 }
 
-__global__ __launch_bounds__(256) void gate_kernel(const float* __restrict__ g, const float* __restrict__ u, int64_t count,
-                                                   float* __restrict__ out) {
-    const int64_t stride = int64_t(gridDim.x) * 256;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count; i += stride) out[i] = g[i] * sigmoid(g[i]) * u[i];
+// The loop over k: load(k0) reads a slice into registers, store() splits it
+// into LDS.
+template <class T, class Load, class Store>
+__device__ inline void run_tile(T& tile, split::Slice<S, kTile>& as, split::Slice<S, kTile>& bs, int64_t depth, Load&& load,
+                                Store&& store) {
+    load(int64_t(0));
+    for (int64_t k = 0; k < depth; k += split::kSliceK) {
+        store();
+        __syncthreads();
+        if (k + split::kSliceK < depth) load(k + split::kSliceK);
+        tile.multiply(as, bs);
+        __syncthreads();
+    }
 }
+
+// C[r] = x_r @ w[group], or silu(x_r @ gate) * (x_r @ up): there a tile holds 64
+// columns of both products, 32 of each side by side in every wave.
+template <bool Gated>
+__global__ __launch_bounds__(split::kThreads, 3) void forward_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, kTile> as, bs;
+    constexpr int kColumns = Gated ? kTile / 2 : kTile;
+    const RowTile t = find_tile(p.offsets, p.experts + 1, (p.columns + kColumns - 1) / kColumns);
+    if (!t.live) return;
+    const int64_t n0 = t.column * kColumns;
+    split::Tile<S, kTile, kTile> tile;
+    tile.clear();
+    const int64_t matrix = int64_t(t.group) * p.width * p.columns;
+    const auto source = [&](int r) { return p.a + int64_t(p.token ? p.token[r] : r) * p.width; };
+    if (t.group < p.experts) {
+        split::AlongK<kTile> a;
+        split::AcrossK<kTile> b;
+        const float *pa[a.kChunks], *pb[b.kChunks];
+        int valid[b.kChunks];
+#pragma unroll
+        for (int j = 0; j < a.kChunks; ++j) {
+            const int r = t.begin + a.row(j);
+            pa[j] = r < t.end ? source(r) : nullptr;
+        }
+#pragma unroll
+        for (int j = 0; j < b.kChunks; ++j) {
+            const int s = b.row(j);
+            const int64_t col = Gated ? n0 + s / 64 * 32 + s % 32 : n0 + s;
+            valid[j] = int(min(int64_t(2), max(int64_t(0), p.columns - col)));
+            pb[j] = (Gated && s / 32 % 2 ? p.b2 : p.b) + matrix + col;
+        }
+        run_tile(tile, as, bs, p.width,
+                 [&](int64_t k) {
+                     a.load(pa, k, p.width);
+                     b.load(pb, valid, k, p.width, [&](int64_t kk) { return kk * p.columns; });
+                 },
+                 [&] {
+                     a.store(as);
+                     b.store(bs);
+                 });
+    }
+    // A lost sum, value by value.
+    const auto again = [&](const float* w, int r, int64_t col) {
+        const float* const x = source(r);
+        float sum = 0.0f;
+        for (int64_t k = 0; k < p.width; ++k) sum = fmaf(x[k], w[matrix + k * p.columns + col], sum);
+        return sum;
+    };
+    if constexpr (Gated) {
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        const int64_t col = n0 + wave % 2 * 32 + lane % 32;
+        if (col >= p.columns) return;
+#pragma unroll
+        for (int m = 0; m < tile.kM; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int r = t.begin + wave / 2 * 64 + 32 * m + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
+                if (r >= t.end) continue;
+                float g = tile.acc[m][0][i], u = tile.acc[m][1][i];
+                if (!split::finite(g)) g = again(p.b, r, col);
+                if (!split::finite(u)) u = again(p.b2, r, col);
+                const int64_t at = int64_t(r) * p.columns + col;
+                p.c[at] = g * sigmoid(g) * u;
+                if (p.c2) {
+                    p.c2[at] = g;
+                    p.c3[at] = u;
+                }
+            }
+    } else {
+        tile.each([&](int m, int n, float v) {
+            const int r = t.begin + m;
+            const int64_t col = n0 + n;
+            if (r >= t.end || col >= p.columns) return;
+            if (!split::finite(v)) v = again(p.b, r, col);
+            p.c[int64_t(r) * p.columns + col] = v;
+        });
+    }
+}
+
+// C[r] = a[r] @ b[group]^T (+ a2[r] @ b2[group]^T).
+__global__ __launch_bounds__(split::kThreads, 2) void input_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, kTile> as, bs;
+    const RowTile t = find_tile(p.offsets, p.experts + 1, (p.width + kTile - 1) / kTile);
+    if (!t.live) return;
+    const int64_t n0 = t.column * kTile, matrix = int64_t(t.group) * p.width * p.columns;
+    split::Tile<S, kTile, kTile> tile;
+    tile.clear();
+    const int products = p.a2 ? 2 : 1;
+    if (t.group < p.experts) {
+        for (int product = 0; product < products; ++product) {
+            const float *const from = product ? p.a2 : p.a, *const w = (product ? p.b2 : p.b) + matrix;
+            split::AlongK<kTile> a, b;
+            const float *pa[a.kChunks], *pb[b.kChunks];
+#pragma unroll
+            for (int j = 0; j < a.kChunks; ++j) {
+                const int r = t.begin + a.row(j);
+                const int64_t n = n0 + b.row(j);
+                pa[j] = r < t.end ? from + int64_t(r) * p.columns : nullptr;
+                pb[j] = n < p.width ? w + n * p.columns : nullptr;
+            }
+            run_tile(tile, as, bs, p.columns,
+                     [&](int64_t k) {
+                         a.load(pa, k, p.columns);
+                         b.load(pb, k, p.columns);
+                     },
+                     [&] {
+                         a.store(as);
+                         b.store(bs);
+                     });
+        }
+    }
+    tile.each([&](int m, int n, float v) {
+        const int r = t.begin + m;
+        const int64_t col = n0 + n;
+        if (r >= t.end || col >= p.width) return;
+        if (!split::finite(v)) {
+            v = 0.0f;
+            for (int product = 0; product < products; ++product) {
+                const float *const x = (product ? p.a2 : p.a) + int64_t(r) * p.columns;
+                const float *const w = (product ? p.b2 : p.b) + matrix + col * p.columns;
+                for (int64_t k = 0; k < p.columns; ++k) v = fmaf(x[k], w[k], v);
+            }
+        }
+        p.c[int64_t(r) * p.width + col] = v;
+    });
+}
+
+// C[e] = sum over e's rows of x_r^T b[r]; workgroups in the order of experts, then tiles.
+__global__ __launch_bounds__(split::kThreads, 3) void weight_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, kTile> as, bs;
+    const int64_t row_tiles = (p.width + kTile - 1) / kTile, column_tiles = (p.columns + kTile - 1) / kTile;
+    const int64_t total = row_tiles * column_tiles * p.experts, share = (total + 7) / 8;
+    const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= share || id >= total) return;
+    const int group = int(id / (row_tiles * column_tiles));
+    const int64_t m0 = id / column_tiles % row_tiles * kTile, n0 = id % column_tiles * kTile;
+    const int begin = p.offsets[group], depth = p.offsets[group + 1] - begin;
+    const auto source = [&](int64_t r) { return int64_t(p.token ? p.token[r] : r) * p.width; };
+    split::Tile<S, kTile, kTile> tile;
+    tile.clear();
+    split::AcrossK<kTile> a, b;
+    const float *pa[a.kChunks], *pb[b.kChunks];
+    int va[a.kChunks], vb[b.kChunks];
+#pragma unroll
+    for (int j = 0; j < a.kChunks; ++j) {
+        const int64_t m = m0 + a.row(j), n = n0 + b.row(j);
+        va[j] = int(min(int64_t(2), max(int64_t(0), p.width - m)));
+        vb[j] = int(min(int64_t(2), max(int64_t(0), p.columns - n)));
+        pa[j] = p.a + m;
+        pb[j] = p.b + n;
+    }
+    run_tile(tile, as, bs, depth,
+             [&](int64_t k) {
+                 a.load(pa, va, k, depth, [&](int64_t kk) { return source(begin + kk); });
+                 b.load(pb, vb, k, depth, [&](int64_t kk) { return (begin + kk) * p.columns; });
+             },
+             [&] {
+                 a.store(as);
+                 b.store(bs);
+             });
+    tile.each([&](int m, int n, float v) {
+        const int64_t row = m0 + m, col = n0 + n;
+        if (row >= p.width || col >= p.columns) return;
+        if (!split::finite(v)) {
+            v = 0.0f;
+            for (int r = begin; r < begin + depth; ++r) v = fmaf(p.a[source(r) + row], p.b[int64_t(r) * p.columns + col], v);
+        }
+        p.c[(int64_t(group) * p.width + row) * p.columns + col] = v;
+    });
+}
+
+int64_t tiles_of(size_t n, int tile = kTile) { return int64_t((n + tile - 1) / tile); }
+
+// A grid for `tiles` tiles at most, in whole rounds of the eight dies.
+dim3 tile_grid(int64_t tiles) {
+    const int64_t blocks = (tiles + 7) / 8 * 8;
+    if (blocks >= int64_t(1) << 31) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
+    return dim3(unsigned(blocks));
+}
+int64_t row_tiles_at_most(const Plan& plan) { return int64_t(plan.rows / kTile + plan.experts + 1); }
+
+// ---- the gated unit -------------------------------------------------------------------
 
 // d silu(g) = s (1 + g (1 - s)) with s = sigmoid(g).
 __global__ __launch_bounds__(256) void gate_backward_kernel(const float* __restrict__ grad, const float* __restrict__ g,
@@ -355,8 +488,8 @@ int vc_hip_expert_plan_build(const float* chosen, size_t tokens, size_t top_k, s
         check_plan_sizes(tokens, top_k, experts);
         const size_t rows = tokens * top_k, chunks = plan_chunks(rows), chunk = plan_chunk(rows);
         if (!words || (rows && !chosen)) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert plan: null pointer");
-        int* const order = words + experts + 2;
-        int* const counts = order + 2 * rows;
+        int* const token = words + experts + 2;
+        int* const counts = token + 2 * rows;
         Profiled p("expert_plan", 0.0, 12.0 * rows);
         const uint32_t lds = uint32_t((2 + kPlanWaves) * (experts + 1) * sizeof(int));
         if (chunks > 1) {
@@ -365,8 +498,8 @@ int vc_hip_expert_plan_build(const float* chosen, size_t tokens, size_t top_k, s
             after_launch("expert plan counts");
         }
         launch(plan_place_kernel, dim3(unsigned(std::max<size_t>(chunks, 1))), dim3(kPlanBlock), lds, d.stream, chosen,
-               int(rows), int(chunk), int(experts), static_cast<const int*>(chunks > 1 ? counts : nullptr), words, order,
-               order + rows);
+               int(rows), int(chunk), int(experts), static_cast<const int*>(chunks > 1 ? counts : nullptr),
+               int(top_k), words, token, token + rows);
         after_launch("expert plan");
         p.done();
     });
@@ -380,9 +513,10 @@ int vc_hip_expert_linear_forward(const float* x, const float* w, const vc_hip_ex
         if (q.rows == 0 || columns == 0) return;
         if (!out || (width && (!x || !w))) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_linear: null pointer");
         Profiled p("expert_linear", 2.0 * q.rows * width * columns, 4.0 * (q.rows * (width + columns) + q.experts * width * columns));
-        row_product(d, q, false,
-                    ProductArgs{x, w, nullptr, nullptr, out, q.offsets, q.order, int(q.experts), ordered ? 0 : int(q.top_k),
-                                int64_t(width), int64_t(columns)});
+        launch(forward_kernel<false>, tile_grid(row_tiles_at_most(q) * tiles_of(columns)), dim3(split::kThreads), 0, d.stream,
+               ProductArgs{x, w, nullptr, nullptr, out, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token, int(q.experts),
+                           int64_t(width), int64_t(columns)});
+        after_launch("expert_linear");
         p.done();
     });
 }
@@ -397,18 +531,10 @@ int vc_hip_expert_gated_forward(const float* x, const float* gate, const float* 
         if (!out || (width && (!x || !gate || !up))) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_gated: null pointer");
         Profiled p("expert_gated", 4.0 * q.rows * width * columns,
                    4.0 * (q.rows * (width + (save_gate ? 3.0 : 1.0) * columns) + 2.0 * q.experts * width * columns));
-        const size_t count = q.rows * columns;
-        Scratch scratch(save_gate ? 4 : 2 * count * sizeof(float));
-        float* const g = save_gate ? save_gate : scratch.as<float>();
-        float* const u = save_up ? save_up : scratch.as<float>() + count;
-        ProductArgs args{x, gate, nullptr, nullptr, g, q.offsets, q.order, int(q.experts), ordered ? 0 : int(q.top_k),
-                         int64_t(width), int64_t(columns)};
-        row_product(d, q, false, args);
-        args.b = up;
-        args.c = u;
-        row_product(d, q, false, args);
-        launch(gate_kernel, dim3(grid_1d(count, 256, 8192)), dim3(256), 0, d.stream, static_cast<const float*>(g),
-               static_cast<const float*>(u), int64_t(count), out);
+        launch(forward_kernel<true>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, kTile / 2)), dim3(split::kThreads), 0,
+               d.stream,
+               ProductArgs{x, gate, nullptr, up, out, save_gate, save_up, q.offsets, ordered ? nullptr : q.token, int(q.experts),
+                           int64_t(width), int64_t(columns)});
         after_launch("expert_gated");
         p.done();
     });
@@ -440,9 +566,10 @@ int vc_hip_expert_linear_backward_input(const float* grad, const float* w, const
         const double products = grad2 ? 2.0 : 1.0;
         Profiled p("expert_backward_input", products * 2.0 * q.rows * width * columns,
                    4.0 * (q.rows * (width + products * columns) + products * q.experts * width * columns));
-        row_product(d, q, true,
-                    ProductArgs{grad, w, grad2, w2, grad_rows, q.offsets, q.order, int(q.experts), 0, int64_t(width),
-                                int64_t(columns)});
+        launch(input_kernel, tile_grid(row_tiles_at_most(q) * tiles_of(width)), dim3(split::kThreads), 0, d.stream,
+               ProductArgs{grad, w, grad2, w2, grad_rows, nullptr, nullptr, q.offsets, nullptr, int(q.experts), int64_t(width),
+                           int64_t(columns)});
+        after_launch("expert_backward_input");
         p.done();
     });
 }
@@ -454,13 +581,12 @@ int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, cons
         const Plan q = plan_of(plan);
         if (width == 0 || columns == 0) return;
         if (!grad_w || (q.rows && (!x || !grad))) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_linear_backward_weight: null pointer");
-        if (width > size_t(kTile) * 65535) fail(VC_HIP_ERR_OVERFLOW, "expert_linear_backward_weight: too many rows");
         Profiled p("expert_backward_weight", 2.0 * q.rows * width * columns,
                    4.0 * (q.rows * (width + columns) + q.experts * width * columns));
-        launch(product_kernel<Product::Weight>, dim3(tiles_of(columns), tiles_of(width), unsigned(q.experts)), dim3(256), 0,
+        launch(weight_kernel, tile_grid(int64_t(q.experts) * tiles_of(width) * tiles_of(columns)), dim3(split::kThreads), 0,
                d.stream,
-               ProductArgs{x, grad, nullptr, nullptr, grad_w, q.offsets, q.order, int(q.experts), ordered ? 0 : int(q.top_k),
-                           int64_t(width), int64_t(columns)});
+               ProductArgs{x, grad, nullptr, nullptr, grad_w, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
+                           int(q.experts), int64_t(width), int64_t(columns)});
         after_launch("expert_backward_weight");
         p.done();
     });

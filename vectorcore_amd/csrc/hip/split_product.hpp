@@ -1,0 +1,241 @@
+// Matrix products of float32 operands on the 16-bit matrix instructions, at
+// float32's precision.
+//
+// Every operand value is written as a sum of numbers of fewer bits, and the
+// product as the sum of their products that matter:
+//   Bf16x3: x = x1 + x2 + x3 with bfloat16 parts, each the rounding of what the
+//   earlier ones leave. |x2| <= 2^-9 |x|, |x3| <= 2^-18 |x|, and the parts' 24
+//   bits hold all of x. Of the nine products those below 2^-26 of the largest
+//   (x2 y3, x3 y2, x3 y3) are left out; six remain. bfloat16 has float32's
+//   exponents, so any magnitudes may meet.
+//   Fp16x2: x = x1 + x2 with half-precision parts, 22 bits of x; x2 y2 (2^-22)
+//   is left out, three products remain. For values known to lie near one.
+// All products are exact and summed in float32 by the matrix instructions, whose
+// 16-deep sums round less often than a float32 chain does. Six instructions of
+// 32 cycles take the place of eight of 64 (V_MFMA_F32_32X32X2_F32), three that
+// of eight.
+//
+// A workgroup of four waves computes a BM x BN tile of C, each wave a quarter
+// of it in 32 x 32 blocks, k in slices of 32. A thread loads its share of a
+// slice into registers while the slice before it is multiplied, splits it, and
+// stores the parts in LDS as the matrix instructions read them: [part][k / 8]
+// [row][8], so a fragment is one 16-byte read per lane and a transposed operand
+// costs nothing more than a k-contiguous one.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace vchip {
+namespace split {
+
+constexpr int kThreads = 256, kSliceK = 32, kGroups = kSliceK / 8;
+
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f2v __attribute__((ext_vector_type(2)));
+
+struct Bf16x3 {
+    static constexpr int kParts = 3, kProducts = 6;
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    // Parts of A and B of each product, the smallest products first.
+    static constexpr int kA[6] = {0, 2, 1, 0, 1, 0}, kB[6] = {2, 0, 1, 1, 0, 0};
+    static __device__ inline f16v multiply(v8 a, v8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+struct Fp16x2 {
+    static constexpr int kParts = 2, kProducts = 3;
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    static constexpr int kA[3] = {0, 1, 0}, kB[3] = {1, 0, 0};
+    static __device__ inline f16v multiply(v8 a, v8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+// The parts of eight values, packed.
+template <class S>
+__device__ inline void split8(const float (&v)[8], typename S::v8 (&out)[S::kParts]) {
+    f2v rest[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rest[i] = f2v{v[2 * i], v[2 * i + 1]};
+#pragma unroll
+    for (int p = 0; p < S::kParts; ++p) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const typename S::v2 part = __builtin_convertvector(rest[i], typename S::v2);
+            out[p][2 * i] = part[0];
+            out[p][2 * i + 1] = part[1];
+            if (p + 1 < S::kParts) {
+                rest[i][0] -= float(part[0]);
+                rest[i][1] -= float(part[1]);
+            }
+        }
+    }
+}
+
+// The LDS image of Rows rows of an operand's slice. A k-group's rows are four
+// 16-byte slots longer than they need to be: threads that store the four groups
+// of a row then meet different banks.
+template <class S, int Rows>
+struct Slice {
+    static constexpr int kStride = Rows + 4;
+    typename S::v8 at[S::kParts][kGroups][kStride];
+};
+
+// ---- operands: what one thread loads of a slice, and where it stores it -----------
+
+// k contiguous: element (row, k) at pointer(row)[k]. Thread t holds k-group
+// t % 4 of rows t / 4 + 64 j, so four threads read 128 contiguous bytes.
+template <int Rows>
+struct AlongK {
+    static constexpr int kChunks = Rows / 64;
+    float v[kChunks][8];
+
+    // p: the chunks' rows at k = 0, or null for rows that are zero.
+    __device__ inline void load(const float* const (&p)[kChunks], int64_t k0, int64_t depth) {
+        const int64_t k = k0 + 8 * (threadIdx.x % kGroups);
+        if (k0 + kSliceK <= depth) {
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                f4u lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+                if (p[j]) {
+                    lo = *reinterpret_cast<const f4u*>(p[j] + k);
+                    hi = *reinterpret_cast<const f4u*>(p[j] + k + 4);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[j][i] = lo[i];
+                    v[j][4 + i] = hi[i];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[j][i] = p[j] && k + i < depth ? p[j][k + i] : 0.0f;
+        }
+    }
+    template <class S>
+    __device__ inline void store(Slice<S, Rows>& lds) const {
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            typename S::v8 parts[S::kParts];
+            split8<S>(v[j], parts);
+#pragma unroll
+            for (int q = 0; q < S::kParts; ++q) lds.at[q][threadIdx.x % kGroups][threadIdx.x / kGroups + 64 * j] = parts[q];
+        }
+    }
+    static __device__ inline int row(int j) { return threadIdx.x / kGroups + 64 * j; }
+};
+
+// Rows contiguous: element (row, k) at line(k)[row]. Wave w holds k-group w,
+// lane l rows 2 l and 2 l + 1 (+ 128 j), so a wave reads 512 contiguous bytes
+// of each k.
+template <int Rows>
+struct AcrossK {
+    static constexpr int kChunks = Rows / 128;
+    float v[kChunks][2][8];
+
+    // p: the chunks' first rows at k = 0 of their matrix; valid: how many of the two rows there are.
+    // line(k): what to add to p for k; k < depth.
+    template <class Line>
+    __device__ inline void load(const float* const (&p)[kChunks], const int (&valid)[kChunks], int64_t k0, int64_t depth,
+                                Line&& line) {
+        const int64_t k = k0 + 8 * __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool inside = k + i < depth;  // uniform in the wave
+            const int64_t at = inside ? line(k + i) : 0;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                float x = 0.0f, y = 0.0f;
+                if (inside) {
+                    if (valid[j] == 2) {
+                        const f2u both = *reinterpret_cast<const f2u*>(p[j] + at);
+                        x = both[0];
+                        y = both[1];
+                    } else if (valid[j] == 1) {
+                        x = p[j][at];
+                    }
+                }
+                v[j][0][i] = x;
+                v[j][1][i] = y;
+            }
+        }
+    }
+    template <class S>
+    __device__ inline void store(Slice<S, Rows>& lds) const {
+        const int group = threadIdx.x / 64, lane = threadIdx.x % 64;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                typename S::v8 parts[S::kParts];
+                split8<S>(v[j][h], parts);
+#pragma unroll
+                for (int q = 0; q < S::kParts; ++q) lds.at[q][group][2 * lane + h + 128 * j] = parts[q];
+            }
+    }
+    static __device__ inline int row(int j) { return 2 * (threadIdx.x % 64) + 128 * j; }
+};
+
+// ---- the tile -----------------------------------------------------------------------
+
+template <class S, int BM, int BN>
+struct Tile {
+    static constexpr int kM = BM / 64, kN = BN / 64;  // 32 x 32 blocks of a wave
+    f16v acc[kM][kN];
+
+    __device__ inline void clear() {
+#pragma unroll
+        for (int a = 0; a < kM; ++a)
+#pragma unroll
+            for (int b = 0; b < kN; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.0f;
+    }
+
+    __device__ inline void multiply(const Slice<S, BM>& as, const Slice<S, BN>& bs) {
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        const int m0 = wave / 2 * (BM / 2) + lane % 32, n0 = wave % 2 * (BN / 2) + lane % 32;
+#pragma unroll
+        for (int k = 0; k < kGroups; k += 2) {
+            typename S::v8 a[kM][S::kParts], b[kN][S::kParts];
+#pragma unroll
+            for (int q = 0; q < S::kParts; ++q) {
+#pragma unroll
+                for (int i = 0; i < kM; ++i) a[i][q] = as.at[q][k + lane / 32][m0 + 32 * i];
+#pragma unroll
+                for (int i = 0; i < kN; ++i) b[i][q] = bs.at[q][k + lane / 32][n0 + 32 * i];
+            }
+#pragma unroll
+            for (int p = 0; p < S::kProducts; ++p)
+#pragma unroll
+                for (int i = 0; i < kM; ++i)
+#pragma unroll
+                    for (int j = 0; j < kN; ++j) acc[i][j] = S::multiply(a[i][S::kA[p]], b[j][S::kB[p]], acc[i][j]);
+        }
+    }
+
+    // f(row, column, value) for each value this thread holds; f may change it.
+    template <class F>
+    __device__ inline void each(F&& f) {
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+#pragma unroll
+        for (int a = 0; a < kM; ++a)
+#pragma unroll
+            for (int b = 0; b < kN; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    f(wave / 2 * (BM / 2) + 32 * a + 8 * (i / 4) + 4 * (lane / 32) + i % 4, wave % 2 * (BN / 2) + 32 * b + lane % 32,
+                      acc[a][b][i]);
+    }
+};
+
+// Is a sum of products lost to an infinity, a NaN or a value that rounds to an
+// infinity in 16 bits? Its parts give NaN or an infinity then.
+__device__ inline bool finite(float x) { return fabsf(x) < __builtin_huge_valf(); }
+
+}  // namespace split
+}  // namespace vchip
