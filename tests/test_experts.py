@@ -153,6 +153,35 @@ def test_linear(tokens, experts, top_k, width, columns, ordered, device):
     assert (np.abs(tw.grad.numpy() - dw) <= bound(len(group)) * mdw).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,top_k,width,columns", [(4099, 3, 2, 33, 2050), (4099, 3, 2, 2051, 33),
+                                                               (45, 5, 2, 2050, 2053), (9000, 6, 1, 96, 1024)])
+def test_many_tiles(tokens, experts, top_k, width, columns):
+    """Enough tiles for the whole chip: wide ones, each die its share, experts of unequal sizes, one without rows."""
+    rng = np.random.default_rng(tokens + width)
+    chosen = picks(rng, tokens, top_k, experts - 1, "skewed")
+    place, group, token = layout(chosen, experts)
+    x, w = rng.standard_normal((tokens, width)).astype(np.float32), rng.standard_normal((experts, width, columns)).astype(np.float32)
+    u, g = rng.standard_normal((experts, width, columns)).astype(np.float32), rng.standard_normal((len(group), columns)).astype(np.float32)
+    t = [vc.Tensor(a, requires_grad=True, device="hip") for a in (x, w)]
+    plan = vc.ExpertPlan(vc.Tensor(chosen, device="hip"), experts)
+    y = vc.expert_linear(*t, plan)
+    y.backward(vc.Tensor(g, device="hip"))
+    h = vc.expert_gated(t[0].detach(), t[1].detach(), vc.Tensor(u, device="hip"), plan).numpy()
+    y, dx, dw = y.numpy(), t[0].grad.numpy(), t[1].grad.numpy()
+    want_dx, mag_dx = np.zeros(x.shape), np.zeros(x.shape)
+    for e in range(experts):
+        r = np.nonzero(group == e)[0]
+        xe, ge, we, ue = (a.astype(np.float64) for a in (x[token[r]], g[r], w[e], u[e]))
+        a, b, mag, mag_u = xe @ we, xe @ ue, np.abs(xe) @ np.abs(we), np.abs(xe) @ np.abs(ue)
+        assert (np.abs(y[r] - a) <= bound(width) * mag).all()
+        assert (np.abs(h[r] - a / (1 + np.exp(-a)) * b) <= (bound(width, width, width) + 24 * UNIT) * mag * mag_u).all()
+        assert (np.abs(dw[e] - xe.T @ ge) <= bound(len(r)) * (np.abs(xe).T @ np.abs(ge))).all()
+        np.add.at(want_dx, token[r], ge @ we.T)
+        np.add.at(mag_dx, token[r], np.abs(ge) @ np.abs(we).T)
+    assert (np.abs(dx - want_dx) <= bound(columns, top_k) * mag_dx).all()
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_gradients_against_differences(device):
     rng = np.random.default_rng(5)

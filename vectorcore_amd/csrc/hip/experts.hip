@@ -143,7 +143,7 @@ Plan plan_of(const vc_hip_expert_plan* plan) {
 }
 
 // ---- products -----------------------------------------------------------------------
-// Tiles of 128 rows of one group by 128 columns (split_product.hpp).
+// Tiles of 128 rows of one group by 128 or 256 columns (split_product.hpp).
 
 constexpr int kTile = 128;
 using S = split::Bf16x3;
@@ -213,8 +213,8 @@ __device__ inline float sigmoid(float x) {
 
 // The loop over k: load(k0) reads a slice into registers, store() splits it
 // into LDS.
-template <class T, class Load, class Store>
-__device__ inline void run_tile(T& tile, split::Slice<S, kTile>& as, split::Slice<S, kTile>& bs, int64_t depth, Load&& load,
+template <class T, int BN, class Load, class Store>
+__device__ inline void run_tile(T& tile, split::Slice<S, kTile>& as, split::Slice<S, BN>& bs, int64_t depth, Load&& load,
                                 Store&& store) {
     load(int64_t(0));
     for (int64_t k = 0; k < depth; k += split::kSliceK) {
@@ -226,40 +226,42 @@ __device__ inline void run_tile(T& tile, split::Slice<S, kTile>& as, split::Slic
     }
 }
 
-// C[r] = x_r @ w[group], or silu(x_r @ gate) * (x_r @ up): there a tile holds 64
-// columns of both products, 32 of each side by side in every wave.
-template <bool Gated>
-__global__ __launch_bounds__(split::kThreads, 3) void forward_kernel(ProductArgs p) {
-    __shared__ split::Slice<S, kTile> as, bs;
-    constexpr int kColumns = Gated ? kTile / 2 : kTile;
+// Workgroups on a CU that registers and LDS have room for.
+constexpr int at_once(int columns) { return columns == 128 ? 3 : 2; }
+
+// C[r] = x_r @ w[group], or silu(x_r @ gate) * (x_r @ up): there a tile holds
+// half as many columns of both products, in turn 64 of each, so that a thread
+// holds both values of an element.
+template <bool Gated, int BN>
+__global__ __launch_bounds__(split::kThreads, at_once(BN)) void forward_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, kTile> as;
+    __shared__ split::Slice<S, BN> bs;
+    constexpr int kColumns = Gated ? BN / 2 : BN;
     const RowTile t = find_tile(p.offsets, p.experts + 1, (p.columns + kColumns - 1) / kColumns);
     if (!t.live) return;
     const int64_t n0 = t.column * kColumns;
-    split::Tile<S, kTile, kTile> tile;
+    split::Tile<S, kTile, BN> tile;
     tile.clear();
     const int64_t matrix = int64_t(t.group) * p.width * p.columns;
     const auto source = [&](int r) { return p.a + int64_t(p.token ? p.token[r] : r) * p.width; };
     if (t.group < p.experts) {
         split::AlongK<kTile> a;
-        split::AcrossK<kTile> b;
-        const float *pa[a.kChunks], *pb[b.kChunks];
-        int valid[b.kChunks];
+        split::AcrossK<BN> b;
+        const float* pa[a.kChunks];
+        unsigned at[b.kChunks];
 #pragma unroll
-        for (int j = 0; j < a.kChunks; ++j) {
-            const int r = t.begin + a.row(j);
-            pa[j] = r < t.end ? source(r) : nullptr;
-        }
+        for (int j = 0; j < a.kChunks; ++j) pa[j] = source(min(t.begin + a.row(j), t.end - 1));
 #pragma unroll
-        for (int j = 0; j < b.kChunks; ++j) {
-            const int s = b.row(j);
-            const int64_t col = Gated ? n0 + s / 64 * 32 + s % 32 : n0 + s;
-            valid[j] = int(min(int64_t(2), max(int64_t(0), p.columns - col)));
-            pb[j] = (Gated && s / 32 % 2 ? p.b2 : p.b) + matrix + col;
-        }
+        for (int j = 0; j < b.kChunks; ++j)
+            at[j] = unsigned(min(int64_t(Gated ? b.row(j / 2) : b.row(j)), p.columns - 1 - n0));
+        const float *const w = p.b + matrix + n0, *const w2 = Gated ? p.b2 + matrix + n0 : w;
         run_tile(tile, as, bs, p.width,
                  [&](int64_t k) {
                      a.load(pa, k, p.width);
-                     b.load(pb, valid, k, p.width, [&](int64_t kk) { return kk * p.columns; });
+                     b.load(at, k, p.width, [&](int64_t kk) {
+                         const int64_t line = kk * p.columns;
+                         return [=](int j) { return (Gated && j % 2 ? w2 : w) + line; };
+                     });
                  },
                  [&] {
                      a.store(as);
@@ -275,24 +277,27 @@ __global__ __launch_bounds__(split::kThreads, 3) void forward_kernel(ProductArgs
     };
     if constexpr (Gated) {
         const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-        const int64_t col = n0 + wave % 2 * 32 + lane % 32;
-        if (col >= p.columns) return;
 #pragma unroll
-        for (int m = 0; m < tile.kM; ++m)
+        for (int h = 0; h < tile.kN / 2; ++h) {
+            const int64_t col = n0 + 64 * h + wave % 2 * 32 + lane % 32;
+            if (col >= p.columns) continue;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int r = t.begin + wave / 2 * 64 + 32 * m + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
-                if (r >= t.end) continue;
-                float g = tile.acc[m][0][i], u = tile.acc[m][1][i];
-                if (!split::finite(g)) g = again(p.b, r, col);
-                if (!split::finite(u)) u = again(p.b2, r, col);
-                const int64_t at = int64_t(r) * p.columns + col;
-                p.c[at] = g * sigmoid(g) * u;
-                if (p.c2) {
-                    p.c2[at] = g;
-                    p.c3[at] = u;
+            for (int m = 0; m < tile.kM; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = t.begin + wave / 2 * 64 + 32 * m + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
+                    if (r >= t.end) continue;
+                    float g = tile.acc[m][2 * h][i], u = tile.acc[m][2 * h + 1][i];
+                    if (!split::finite(g)) g = again(p.b, r, col);
+                    if (!split::finite(u)) u = again(p.b2, r, col);
+                    const int64_t at = int64_t(r) * p.columns + col;
+                    p.c[at] = g * sigmoid(g) * u;
+                    if (p.c2) {
+                        p.c2[at] = g;
+                        p.c3[at] = u;
+                    }
                 }
-            }
+        }
     } else {
         tile.each([&](int m, int n, float v) {
             const int r = t.begin + m;
@@ -305,26 +310,26 @@ __global__ __launch_bounds__(split::kThreads, 3) void forward_kernel(ProductArgs
 }
 
 // C[r] = a[r] @ b[group]^T (+ a2[r] @ b2[group]^T).
-__global__ __launch_bounds__(split::kThreads, 2) void input_kernel(ProductArgs p) {
-    __shared__ split::Slice<S, kTile> as, bs;
-    const RowTile t = find_tile(p.offsets, p.experts + 1, (p.width + kTile - 1) / kTile);
+template <int BN>
+__global__ __launch_bounds__(split::kThreads, at_once(BN)) void input_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, kTile> as;
+    __shared__ split::Slice<S, BN> bs;
+    const RowTile t = find_tile(p.offsets, p.experts + 1, (p.width + BN - 1) / BN);
     if (!t.live) return;
-    const int64_t n0 = t.column * kTile, matrix = int64_t(t.group) * p.width * p.columns;
-    split::Tile<S, kTile, kTile> tile;
+    const int64_t n0 = t.column * BN, matrix = int64_t(t.group) * p.width * p.columns;
+    split::Tile<S, kTile, BN> tile;
     tile.clear();
     const int products = p.a2 ? 2 : 1;
     if (t.group < p.experts) {
         for (int product = 0; product < products; ++product) {
             const float *const from = product ? p.a2 : p.a, *const w = (product ? p.b2 : p.b) + matrix;
-            split::AlongK<kTile> a, b;
+            split::AlongK<kTile> a;
+            split::AlongK<BN> b;
             const float *pa[a.kChunks], *pb[b.kChunks];
 #pragma unroll
-            for (int j = 0; j < a.kChunks; ++j) {
-                const int r = t.begin + a.row(j);
-                const int64_t n = n0 + b.row(j);
-                pa[j] = r < t.end ? from + int64_t(r) * p.columns : nullptr;
-                pb[j] = n < p.width ? w + n * p.columns : nullptr;
-            }
+            for (int j = 0; j < a.kChunks; ++j) pa[j] = from + int64_t(min(t.begin + a.row(j), t.end - 1)) * p.columns;
+#pragma unroll
+            for (int j = 0; j < b.kChunks; ++j) pb[j] = w + min(n0 + b.row(j), p.width - 1) * p.columns;
             run_tile(tile, as, bs, p.columns,
                      [&](int64_t k) {
                          a.load(pa, k, p.columns);
@@ -352,34 +357,39 @@ __global__ __launch_bounds__(split::kThreads, 2) void input_kernel(ProductArgs p
     });
 }
 
-// C[e] = sum over e's rows of x_r^T b[r]; workgroups in the order of experts, then tiles.
-__global__ __launch_bounds__(split::kThreads, 3) void weight_kernel(ProductArgs p) {
-    __shared__ split::Slice<S, kTile> as, bs;
-    const int64_t row_tiles = (p.width + kTile - 1) / kTile, column_tiles = (p.columns + kTile - 1) / kTile;
-    const int64_t total = row_tiles * column_tiles * p.experts, share = (total + 7) / 8;
-    const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8;
-    if (blockIdx.x / 8 >= share || id >= total) return;
-    const int group = int(id / (row_tiles * column_tiles));
-    const int64_t m0 = id / column_tiles % row_tiles * kTile, n0 = id % column_tiles * kTile;
+// C[e] = sum over e's rows of x_r^T b[r]. Every die takes its part of each
+// expert's tiles, as experts differ in their rows.
+template <int BN>
+__global__ __launch_bounds__(split::kThreads, at_once(BN)) void weight_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, kTile> as;
+    __shared__ split::Slice<S, BN> bs;
+    const int64_t row_tiles = (p.width + kTile - 1) / kTile, column_tiles = (p.columns + BN - 1) / BN;
+    const int64_t total = row_tiles * column_tiles, share = (total + 7) / 8;
+    const int group = int(blockIdx.x / 8 / share);
+    const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8 % share;
+    if (id >= total) return;
+    const int64_t m0 = id / column_tiles * kTile, n0 = id % column_tiles * BN;
     const int begin = p.offsets[group], depth = p.offsets[group + 1] - begin;
     const auto source = [&](int64_t r) { return int64_t(p.token ? p.token[r] : r) * p.width; };
-    split::Tile<S, kTile, kTile> tile;
+    split::Tile<S, kTile, BN> tile;
     tile.clear();
-    split::AcrossK<kTile> a, b;
-    const float *pa[a.kChunks], *pb[b.kChunks];
-    int va[a.kChunks], vb[b.kChunks];
+    split::AcrossK<kTile> a;
+    split::AcrossK<BN> b;
+    unsigned at_a[a.kChunks], at_b[b.kChunks];
 #pragma unroll
-    for (int j = 0; j < a.kChunks; ++j) {
-        const int64_t m = m0 + a.row(j), n = n0 + b.row(j);
-        va[j] = int(min(int64_t(2), max(int64_t(0), p.width - m)));
-        vb[j] = int(min(int64_t(2), max(int64_t(0), p.columns - n)));
-        pa[j] = p.a + m;
-        pb[j] = p.b + n;
-    }
+    for (int j = 0; j < a.kChunks; ++j) at_a[j] = unsigned(min(int64_t(a.row(j)), p.width - 1 - m0));
+#pragma unroll
+    for (int j = 0; j < b.kChunks; ++j) at_b[j] = unsigned(min(int64_t(b.row(j)), p.columns - 1 - n0));
     run_tile(tile, as, bs, depth,
              [&](int64_t k) {
-                 a.load(pa, va, k, depth, [&](int64_t kk) { return source(begin + kk); });
-                 b.load(pb, vb, k, depth, [&](int64_t kk) { return (begin + kk) * p.columns; });
+                 a.load(at_a, k, depth, [&](int64_t kk) {
+                     const float* const line = p.a + m0 + source(begin + kk);
+                     return [=](int) { return line; };
+                 });
+                 b.load(at_b, k, depth, [&](int64_t kk) {
+                     const float* const line = p.b + n0 + (begin + kk) * p.columns;
+                     return [=](int) { return line; };
+                 });
              },
              [&] {
                  a.store(as);
@@ -396,7 +406,7 @@ __global__ __launch_bounds__(split::kThreads, 3) void weight_kernel(ProductArgs 
     });
 }
 
-int64_t tiles_of(size_t n, int tile = kTile) { return int64_t((n + tile - 1) / tile); }
+int64_t tiles_of(size_t n, int tile) { return int64_t((n + tile - 1) / tile); }
 
 // A grid for `tiles` tiles at most, in whole rounds of the eight dies.
 dim3 tile_grid(int64_t tiles) {
@@ -405,6 +415,14 @@ dim3 tile_grid(int64_t tiles) {
     return dim3(unsigned(blocks));
 }
 int64_t row_tiles_at_most(const Plan& plan) { return int64_t(plan.rows / kTile + plan.experts + 1); }
+
+// 256 columns a tile split the rows' operand half as often for the same
+// products; they need enough tiles for the chip.
+template <class F>
+void with_columns(Device& d, int64_t row_tiles, size_t columns, F&& f) {
+    if (row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) f(std::integral_constant<int, 256>());
+    else f(std::integral_constant<int, 128>());
+}
 
 // ---- the gated unit -------------------------------------------------------------------
 
@@ -513,9 +531,12 @@ int vc_hip_expert_linear_forward(const float* x, const float* w, const vc_hip_ex
         if (q.rows == 0 || columns == 0) return;
         if (!out || (width && (!x || !w))) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_linear: null pointer");
         Profiled p("expert_linear", 2.0 * q.rows * width * columns, 4.0 * (q.rows * (width + columns) + q.experts * width * columns));
-        launch(forward_kernel<false>, tile_grid(row_tiles_at_most(q) * tiles_of(columns)), dim3(split::kThreads), 0, d.stream,
-               ProductArgs{x, w, nullptr, nullptr, out, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token, int(q.experts),
-                           int64_t(width), int64_t(columns)});
+        const ProductArgs args{x, w, nullptr, nullptr, out, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
+                               int(q.experts), int64_t(width), int64_t(columns)};
+        with_columns(d, int64_t(q.rows / kTile), columns, [&](auto bn) {
+            launch(forward_kernel<false, bn()>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, bn())), dim3(split::kThreads),
+                   0, d.stream, args);
+        });
         after_launch("expert_linear");
         p.done();
     });
@@ -531,10 +552,12 @@ int vc_hip_expert_gated_forward(const float* x, const float* gate, const float* 
         if (!out || (width && (!x || !gate || !up))) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_gated: null pointer");
         Profiled p("expert_gated", 4.0 * q.rows * width * columns,
                    4.0 * (q.rows * (width + (save_gate ? 3.0 : 1.0) * columns) + 2.0 * q.experts * width * columns));
-        launch(forward_kernel<true>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, kTile / 2)), dim3(split::kThreads), 0,
-               d.stream,
-               ProductArgs{x, gate, nullptr, up, out, save_gate, save_up, q.offsets, ordered ? nullptr : q.token, int(q.experts),
-                           int64_t(width), int64_t(columns)});
+        const ProductArgs args{x, gate, nullptr, up, out, save_gate, save_up, q.offsets, ordered ? nullptr : q.token,
+                               int(q.experts), int64_t(width), int64_t(columns)};
+        with_columns(d, int64_t(q.rows / kTile), 2 * columns, [&](auto bn) {
+            launch(forward_kernel<true, bn()>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, bn() / 2)),
+                   dim3(split::kThreads), 0, d.stream, args);
+        });
         after_launch("expert_gated");
         p.done();
     });
@@ -566,9 +589,12 @@ int vc_hip_expert_linear_backward_input(const float* grad, const float* w, const
         const double products = grad2 ? 2.0 : 1.0;
         Profiled p("expert_backward_input", products * 2.0 * q.rows * width * columns,
                    4.0 * (q.rows * (width + products * columns) + products * q.experts * width * columns));
-        launch(input_kernel, tile_grid(row_tiles_at_most(q) * tiles_of(width)), dim3(split::kThreads), 0, d.stream,
-               ProductArgs{grad, w, grad2, w2, grad_rows, nullptr, nullptr, q.offsets, nullptr, int(q.experts), int64_t(width),
-                           int64_t(columns)});
+        const ProductArgs args{grad, w, grad2, w2, grad_rows, nullptr, nullptr, q.offsets, nullptr, int(q.experts),
+                               int64_t(width), int64_t(columns)};
+        with_columns(d, int64_t(q.rows / kTile), width, [&](auto bn) {
+            launch(input_kernel<bn()>, tile_grid(row_tiles_at_most(q) * tiles_of(width, bn())), dim3(split::kThreads), 0,
+                   d.stream, args);
+        });
         after_launch("expert_backward_input");
         p.done();
     });
@@ -583,10 +609,13 @@ int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, cons
         if (!grad_w || (q.rows && (!x || !grad))) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_linear_backward_weight: null pointer");
         Profiled p("expert_backward_weight", 2.0 * q.rows * width * columns,
                    4.0 * (q.rows * (width + columns) + q.experts * width * columns));
-        launch(weight_kernel, tile_grid(int64_t(q.experts) * tiles_of(width) * tiles_of(columns)), dim3(split::kThreads), 0,
-               d.stream,
-               ProductArgs{x, grad, nullptr, nullptr, grad_w, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
-                           int(q.experts), int64_t(width), int64_t(columns)});
+        const ProductArgs args{x, grad, nullptr, nullptr, grad_w, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
+                               int(q.experts), int64_t(width), int64_t(columns)};
+        const int64_t row_tiles = tiles_of(width, kTile);
+        with_columns(d, int64_t(q.experts) * row_tiles, columns, [&](auto bn) {
+            const int64_t share = tiles_of(row_tiles * tiles_of(columns, bn()), 8);
+            launch(weight_kernel<bn()>, tile_grid(int64_t(q.experts) * share * 8), dim3(split::kThreads), 0, d.stream, args);
+        });
         after_launch("expert_backward_weight");
         p.done();
     });

@@ -74,12 +74,12 @@ __device__ inline void split8(const float (&v)[8], typename S::v8 (&out)[S::kPar
     }
 }
 
-// The LDS image of Rows rows of an operand's slice. A k-group's rows are four
-// 16-byte slots longer than they need to be: threads that store the four groups
-// of a row then meet different banks.
+// The LDS image of Rows rows of an operand's slice. A k-group's rows are two
+// 16-byte slots longer than they need to be: eight threads that store the four
+// groups of two rows then meet different banks.
 template <class S, int Rows>
 struct Slice {
-    static constexpr int kStride = Rows + 4;
+    static constexpr int kStride = Rows + 2;
     typename S::v8 at[S::kParts][kGroups][kStride];
 };
 
@@ -92,17 +92,14 @@ struct AlongK {
     static constexpr int kChunks = Rows / 64;
     float v[kChunks][8];
 
-    // p: the chunks' rows at k = 0, or null for rows that are zero.
+    // p: the chunks' rows at k = 0. A row past the operand's end may be any
+    // row of it: what it gives is never stored.
     __device__ inline void load(const float* const (&p)[kChunks], int64_t k0, int64_t depth) {
         const int64_t k = k0 + 8 * (threadIdx.x % kGroups);
         if (k0 + kSliceK <= depth) {
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
-                f4u lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-                if (p[j]) {
-                    lo = *reinterpret_cast<const f4u*>(p[j] + k);
-                    hi = *reinterpret_cast<const f4u*>(p[j] + k + 4);
-                }
+                const f4u lo = *reinterpret_cast<const f4u*>(p[j] + k), hi = *reinterpret_cast<const f4u*>(p[j] + k + 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     v[j][i] = lo[i];
@@ -113,7 +110,7 @@ struct AlongK {
 #pragma unroll
             for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[j][i] = p[j] && k + i < depth ? p[j][k + i] : 0.0f;
+                for (int i = 0; i < 8; ++i) v[j][i] = k + i < depth ? p[j][k + i] : 0.0f;
         }
     }
     template <class S>
@@ -130,37 +127,32 @@ struct AlongK {
 };
 
 // Rows contiguous: element (row, k) at line(k)[row]. Wave w holds k-group w,
-// lane l rows 2 l and 2 l + 1 (+ 128 j), so a wave reads 512 contiguous bytes
-// of each k.
+// lane l rows l + 64 j: a wave reads 256 contiguous bytes of each k, whatever
+// the rows' alignment, and stores to neighbouring slots.
 template <int Rows>
 struct AcrossK {
-    static constexpr int kChunks = Rows / 128;
-    float v[kChunks][2][8];
+    static constexpr int kChunks = Rows / 64;
+    float v[kChunks][8];
 
-    // p: the chunks' first rows at k = 0 of their matrix; valid: how many of the two rows there are.
-    // line(k): what to add to p for k; k < depth.
+    // line(k): the line of k < depth, uniform in the wave. at: the chunks' places in a line; a row past the operand's
+    // end may be any place of it: what it gives is never stored.
     template <class Line>
-    __device__ inline void load(const float* const (&p)[kChunks], const int (&valid)[kChunks], int64_t k0, int64_t depth,
-                                Line&& line) {
+    __device__ inline void load(const unsigned (&at)[kChunks], int64_t k0, int64_t depth, Line&& line) {
         const int64_t k = k0 + 8 * __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        if (k0 + kSliceK <= depth) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool inside = k + i < depth;  // uniform in the wave
-            const int64_t at = inside ? line(k + i) : 0;
+            for (int i = 0; i < 8; ++i) {
+                const auto from = line(k + i);
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                float x = 0.0f, y = 0.0f;
-                if (inside) {
-                    if (valid[j] == 2) {
-                        const f2u both = *reinterpret_cast<const f2u*>(p[j] + at);
-                        x = both[0];
-                        y = both[1];
-                    } else if (valid[j] == 1) {
-                        x = p[j][at];
-                    }
-                }
-                v[j][0][i] = x;
-                v[j][1][i] = y;
+                for (int j = 0; j < kChunks; ++j) v[j][i] = from(j)[at[j]];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool inside = k + i < depth;
+                const auto from = line(inside ? k + i : 0);
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) v[j][i] = inside ? from(j)[at[j]] : 0.0f;
             }
         }
     }
@@ -168,20 +160,19 @@ struct AcrossK {
     __device__ inline void store(Slice<S, Rows>& lds) const {
         const int group = threadIdx.x / 64, lane = threadIdx.x % 64;
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j)
+        for (int j = 0; j < kChunks; ++j) {
+            typename S::v8 parts[S::kParts];
+            split8<S>(v[j], parts);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                typename S::v8 parts[S::kParts];
-                split8<S>(v[j][h], parts);
-#pragma unroll
-                for (int q = 0; q < S::kParts; ++q) lds.at[q][group][2 * lane + h + 128 * j] = parts[q];
-            }
+            for (int q = 0; q < S::kParts; ++q) lds.at[q][group][lane + 64 * j] = parts[q];
+        }
     }
-    static __device__ inline int row(int j) { return 2 * (threadIdx.x % 64) + 128 * j; }
+    static __device__ inline int row(int j) { return threadIdx.x % 64 + 64 * j; }
 };
 
 // ---- the tile -----------------------------------------------------------------------
 
+// Wave w computes rows BM / 2 (w / 2) .. and, of every 64 columns, the half w % 2.
 template <class S, int BM, int BN>
 struct Tile {
     static constexpr int kM = BM / 64, kN = BN / 64;  // 32 x 32 blocks of a wave
@@ -198,23 +189,24 @@ struct Tile {
 
     __device__ inline void multiply(const Slice<S, BM>& as, const Slice<S, BN>& bs) {
         const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-        const int m0 = wave / 2 * (BM / 2) + lane % 32, n0 = wave % 2 * (BN / 2) + lane % 32;
+        const int m0 = wave / 2 * (BM / 2) + lane % 32, n0 = wave % 2 * 32 + lane % 32;
 #pragma unroll
         for (int k = 0; k < kGroups; k += 2) {
-            typename S::v8 a[kM][S::kParts], b[kN][S::kParts];
+            typename S::v8 a[kM][S::kParts];
 #pragma unroll
-            for (int q = 0; q < S::kParts; ++q) {
+            for (int q = 0; q < S::kParts; ++q)
 #pragma unroll
                 for (int i = 0; i < kM; ++i) a[i][q] = as.at[q][k + lane / 32][m0 + 32 * i];
 #pragma unroll
-                for (int i = 0; i < kN; ++i) b[i][q] = bs.at[q][k + lane / 32][n0 + 32 * i];
+            for (int j = 0; j < kN; ++j) {
+                typename S::v8 b[S::kParts];
+#pragma unroll
+                for (int q = 0; q < S::kParts; ++q) b[q] = bs.at[q][k + lane / 32][n0 + 64 * j];
+#pragma unroll
+                for (int p = 0; p < S::kProducts; ++p)
+#pragma unroll
+                    for (int i = 0; i < kM; ++i) acc[i][j] = S::multiply(a[i][S::kA[p]], b[S::kB[p]], acc[i][j]);
             }
-#pragma unroll
-            for (int p = 0; p < S::kProducts; ++p)
-#pragma unroll
-                for (int i = 0; i < kM; ++i)
-#pragma unroll
-                    for (int j = 0; j < kN; ++j) acc[i][j] = S::multiply(a[i][S::kA[p]], b[j][S::kB[p]], acc[i][j]);
         }
     }
 
@@ -228,7 +220,7 @@ struct Tile {
             for (int b = 0; b < kN; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    f(wave / 2 * (BM / 2) + 32 * a + 8 * (i / 4) + 4 * (lane / 32) + i % 4, wave % 2 * (BN / 2) + 32 * b + lane % 32,
+                    f(wave / 2 * (BM / 2) + 32 * a + 8 * (i / 4) + 4 * (lane / 32) + i % 4, wave % 2 * 32 + 64 * b + lane % 32,
                       acc[a][b][i]);
     }
 };
