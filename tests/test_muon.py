@@ -51,6 +51,30 @@ def test_iterate(shape, steps, device):
         assert (np.linalg.svd(o, compute_uv=False).max(-1) <= max(values.max(), 1.3) + near(shape, steps)).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(700, 1500), (1501, 699), (24, 130, 258), (1100, 1100), (2, 300, 4097)])
+def test_iterate_of_many_tiles(shape):
+    g = (1e-3 * np.random.default_rng(sum(shape)).standard_normal(shape)).astype(np.float32)
+    for steps in (1, 5):
+        o = vc.orthogonalise(vc.Tensor(g, device="hip"), steps=steps).numpy().astype(np.float64)
+        error = np.sqrt(((o - exact(g, steps)) ** 2).sum((-2, -1)))
+        assert (error <= near(shape, steps)).all()
+
+
+@pytest.mark.gpu
+def test_more_parameters_than_a_launch_holds():
+    rng = np.random.default_rng(5)
+    shapes = [(int(a), int(b)) for a, b in rng.integers(1, 90, (31, 2))] + [(0, 7), (200, 300)]
+    g = [rng.standard_normal(s).astype(np.float32) for s in shapes]
+    p = [vc.Tensor.zeros(s, device="hip") for s in shapes]
+    m = [vc.Tensor.zeros(s, device="hip") for s in shapes]
+    vc.muon_step(p, m, 1.0, momentum=0.0, grads=[vc.Tensor(a, device="hip") for a in g])
+    for a, t, s in zip(g, p, shapes):
+        if a.size:
+            scale = np.sqrt(max(1.0, s[1] / s[0]))
+            assert np.sqrt(((t.numpy() + scale * exact(a, 5)) ** 2).sum()) <= scale * (near(s, 5) + 8 * UNIT * np.sqrt(min(s)))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_extreme_matrices(device):
     rng = np.random.default_rng(3)
@@ -153,6 +177,8 @@ def test_refusals(device):
                          (([p], [m]), dict(grads=[m])), (([p], [m]), dict(grads=[p]))):
         with pytest.raises(ValueError):
             vc.muon_step(*args, 0.1, **kwargs)
+    with pytest.raises(ValueError):
+        vc.muon_step([p], [m], 0.1, grads=[g], steps=0)
     assert (p.numpy() == 0).all() and (m.numpy() == 0).all()
     vc.muon_step([], [], 0.1, grads=[])
 

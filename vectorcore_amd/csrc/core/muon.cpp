@@ -53,6 +53,7 @@ void muon_step(const std::vector<Tensor*>& parameters, const std::vector<Tensor*
     if (!gradients.empty() && gradients.size() != parameters.size())
         throw std::invalid_argument("muon_step: " + std::to_string(gradients.size()) + " gradients for " +
                                     std::to_string(parameters.size()) + " parameters");
+    if (steps == 0) throw std::invalid_argument("muon_step needs at least one step");
     NoGradGuard guard;
     struct Item {
         Tensor *param, *momentum;

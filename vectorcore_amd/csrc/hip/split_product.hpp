@@ -219,9 +219,11 @@ struct Tile {
 #pragma unroll
             for (int b = 0; b < kN; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    f(wave / 2 * (BM / 2) + 32 * a + 8 * (i / 4) + 4 * (lane / 32) + i % 4, wave % 2 * 32 + 64 * b + lane % 32,
-                      acc[a][b][i]);
+                for (int i = 0; i < 16; ++i) {
+                    float v = acc[a][b][i];
+                    f(wave / 2 * (BM / 2) + 32 * a + 8 * (i / 4) + 4 * (lane / 32) + i % 4, wave % 2 * 32 + 64 * b + lane % 32, v);
+                    acc[a][b][i] = v;
+                }
     }
 };
 
