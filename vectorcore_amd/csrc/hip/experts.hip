@@ -211,21 +211,6 @@ __device__ inline float sigmoid(float x) {
     return (x >= 0.0f ? 1.0f : e) / (1.0f + e);
 }
 
-// The loop over k: load(k0) reads a slice into registers, store() splits it
-// into LDS.
-template <class T, int BN, class Load, class Store>
-__device__ inline void run_tile(T& tile, split::Slice<S, kTile>& as, split::Slice<S, BN>& bs, int64_t depth, Load&& load,
-                                Store&& store) {
-    load(int64_t(0));
-    for (int64_t k = 0; k < depth; k += split::kSliceK) {
-        store();
-        __syncthreads();
-        if (k + split::kSliceK < depth) load(k + split::kSliceK);
-        tile.multiply(as, bs);
-        __syncthreads();
-    }
-}
-
 // Workgroups on a CU that registers and LDS have room for.
 constexpr int at_once(int columns) { return columns == 128 ? 3 : 2; }
 
@@ -255,18 +240,20 @@ __global__ __launch_bounds__(split::kThreads, at_once(BN)) void forward_kernel(P
         for (int j = 0; j < b.kChunks; ++j)
             at[j] = unsigned(min(int64_t(Gated ? b.row(j / 2) : b.row(j)), p.columns - 1 - n0));
         const float *const w = p.b + matrix + n0, *const w2 = Gated ? p.b2 + matrix + n0 : w;
-        run_tile(tile, as, bs, p.width,
-                 [&](int64_t k) {
-                     a.load(pa, k, p.width);
-                     b.load(at, k, p.width, [&](int64_t kk) {
-                         const int64_t line = kk * p.columns;
-                         return [=](int j) { return (Gated && j % 2 ? w2 : w) + line; };
-                     });
-                 },
-                 [&] {
-                     a.store(as);
-                     b.store(bs);
-                 });
+        const auto line = [&](int64_t k) {
+            const int64_t at_k = k * p.columns;
+            return [=](int j) { return (Gated && j % 2 ? w2 : w) + at_k; };
+        };
+        split::accumulate(
+            tile, a, b, as, bs, p.width,
+            [&](int64_t k) {
+                a.load(pa, k);
+                b.load(at, k, line);
+            },
+            [&](int64_t k) {
+                a.load_rest(pa, k, p.width);
+                b.load_rest(at, k, p.width, line);
+            });
     }
     // A lost sum, value by value.
     const auto again = [&](const float* w, int r, int64_t col) {
@@ -330,15 +317,16 @@ __global__ __launch_bounds__(split::kThreads, at_once(BN)) void input_kernel(Pro
             for (int j = 0; j < a.kChunks; ++j) pa[j] = from + int64_t(min(t.begin + a.row(j), t.end - 1)) * p.columns;
 #pragma unroll
             for (int j = 0; j < b.kChunks; ++j) pb[j] = w + min(n0 + b.row(j), p.width - 1) * p.columns;
-            run_tile(tile, as, bs, p.columns,
-                     [&](int64_t k) {
-                         a.load(pa, k, p.columns);
-                         b.load(pb, k, p.columns);
-                     },
-                     [&] {
-                         a.store(as);
-                         b.store(bs);
-                     });
+            split::accumulate(
+                tile, a, b, as, bs, p.columns,
+                [&](int64_t k) {
+                    a.load(pa, k);
+                    b.load(pb, k);
+                },
+                [&](int64_t k) {
+                    a.load_rest(pa, k, p.columns);
+                    b.load_rest(pb, k, p.columns);
+                });
         }
     }
     tile.each([&](int m, int n, float v) {
@@ -380,21 +368,24 @@ __global__ __launch_bounds__(split::kThreads, at_once(BN)) void weight_kernel(Pr
     for (int j = 0; j < a.kChunks; ++j) at_a[j] = unsigned(min(int64_t(a.row(j)), p.width - 1 - m0));
 #pragma unroll
     for (int j = 0; j < b.kChunks; ++j) at_b[j] = unsigned(min(int64_t(b.row(j)), p.columns - 1 - n0));
-    run_tile(tile, as, bs, depth,
-             [&](int64_t k) {
-                 a.load(at_a, k, depth, [&](int64_t kk) {
-                     const float* const line = p.a + m0 + source(begin + kk);
-                     return [=](int) { return line; };
-                 });
-                 b.load(at_b, k, depth, [&](int64_t kk) {
-                     const float* const line = p.b + n0 + (begin + kk) * p.columns;
-                     return [=](int) { return line; };
-                 });
-             },
-             [&] {
-                 a.store(as);
-                 b.store(bs);
-             });
+    const auto line_a = [&](int64_t k) {
+        const float* const line = p.a + m0 + source(begin + k);
+        return [=](int) { return line; };
+    };
+    const auto line_b = [&](int64_t k) {
+        const float* const line = p.b + n0 + (begin + k) * p.columns;
+        return [=](int) { return line; };
+    };
+    split::accumulate(
+        tile, a, b, as, bs, depth,
+        [&](int64_t k) {
+            a.load(at_a, k, line_a);
+            b.load(at_b, k, line_b);
+        },
+        [&](int64_t k) {
+            a.load_rest(at_a, k, depth, line_a);
+            b.load_rest(at_b, k, depth, line_b);
+        });
     tile.each([&](int m, int n, float v) {
         const int64_t row = m0 + m, col = n0 + n;
         if (row >= p.width || col >= p.columns) return;

@@ -10,15 +10,18 @@
 //
 // All values stay near one by construction (|x| <= 1.21, |g| <= 1.5, |p| <= 3),
 // so the products run as three half-precision products of two parts each
-// (split_product.hpp), on values scaled by 2^14 in memory: below 2^15.6 they are
+// (packed_product.hpp), on values scaled by 2^14 in memory: below 2^15.6 they are
 // in half precision's range, and a part below its smallest step is 2^-38 of one.
 // The error is that of a float32 product relative to the norm, which is what the
 // iteration keeps of its input. The scale is a power of two and costs nothing.
 //
+// Every iterate is written twice, as X (of X and X^T the one with the shorter
+// side first) and transposed, as the products read it along the shared side.
+//
 // All matrices of a call run in the same launches, three an iteration: a train
 // step's matrices fill the chip together, and small ones share the latency.
+#include "packed_product.hpp"
 #include "reduce_common.hpp"
-#include "split_product.hpp"
 #include "vc_hip_internal.hpp"
 
 #include <algorithm>
@@ -31,26 +34,27 @@ namespace {
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScale = 16384.0f;
-constexpr int kNormBlocks = 64;   // partial sums of squares of a matrix
+constexpr int kNormBlocks = 1024;  // partial sums of squares of a matrix, at most
 constexpr int kAtOnce = 12;       // matrices (or batches of equal ones) of a launch
 constexpr int kMostSplit = 2048;  // tiles of a launch whose sums are split
-using S = split::Fp16x2;
+using packed::place;
+using half = _Float16;
 
 // `count` matrices [rows, cols].
 struct Matrix {
     const float* grad;
-    float *momentum, *param;     // null for a plain iterate
-    float *x, *y, *gram, *poly;  // scaled: the iterate, its successor; both squares
+    float *momentum, *param;  // null for a plain iterate
+    float *update, *out;      // what is orthogonalised; the plain iterate's result
+    half *x, *xt, *y, *yt;    // the scaled iterate [shorter, longer] and its transpose; the next one
+    half *gram, *poly;        // [shorter, shorter]
     double* partials;
-    int64_t rows, cols;
+    int64_t rows, cols, shorter, longer;  // the sides are padded to whole tiles
     int count, blocks;
     float rate;
     int first, splits, counters;  // of the launch: the first workgroup, parts of each tile's sum, its first count
 
     __host__ __device__ int64_t elements() const { return rows * cols; }
     __host__ __device__ bool wide() const { return rows <= cols; }
-    __host__ __device__ int64_t shorter() const { return rows <= cols ? rows : cols; }
-    __host__ __device__ int64_t longer() const { return rows <= cols ? cols : rows; }
 };
 struct Batch {
     Matrix of[kAtOnce];
@@ -71,7 +75,7 @@ __global__ __launch_bounds__(256) void update_kernel(Batch batch, float mu) {
     const int block = (blockIdx.x - m.first) % m.blocks, z = (blockIdx.x - m.first) / m.blocks;
     const int64_t count = m.elements(), base = z * count;
     const float* const grad = m.grad + base;
-    float *const momentum = m.momentum ? m.momentum + base : nullptr, *const x = m.x + base;
+    float *const momentum = m.momentum ? m.momentum + base : nullptr, *const x = m.update + base;
     double sum = 0.0;
     for (int64_t i = int64_t(block) * 256 + threadIdx.x; i < count; i += int64_t(m.blocks) * 256) {
         float v = grad[i];
@@ -89,17 +93,57 @@ __global__ __launch_bounds__(256) void update_kernel(Batch batch, float mu) {
     if (threadIdx.x == 0) m.partials[z * m.blocks + block] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
-// x becomes scale * x / ||x||.
-__global__ __launch_bounds__(256) void normalise_kernel(Batch batch, float scale) {
+// 1 / ||update|| (0 for zeros), by the whole workgroup.
+__device__ inline double inverse_norm(const Matrix& m, int z) {
+    __shared__ double sums[4];
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < m.blocks; i += 256) sum += m.partials[z * m.blocks + i];
+    sum = red::wave_sum(sum);
+    if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
+    __syncthreads();
+    const double norm = sqrt(sums[0] + sums[1] + sums[2] + sums[3]);
+    return norm == 0.0 ? 0.0 : 1.0 / norm;
+}
+
+// The first iterate without a step: out = update / ||update||.
+__global__ __launch_bounds__(256) void normalise_kernel(Batch batch) {
     const Matrix& m = batch.of[find(batch, blockIdx.x)];
     const int block = (blockIdx.x - m.first) % m.blocks, z = (blockIdx.x - m.first) / m.blocks;
-    double sum = 0.0;
-    for (int i = 0; i < m.blocks; ++i) sum += m.partials[z * m.blocks + i];
-    const double norm = sqrt(sum), factor = norm == 0.0 ? 0.0 : double(scale) / norm;
+    const double factor = inverse_norm(m, z);
     const int64_t count = m.elements();
-    float* const x = m.x + z * count;
     for (int64_t i = int64_t(block) * 256 + threadIdx.x; i < count; i += int64_t(m.blocks) * 256)
-        x[i] = float(double(x[i]) * factor);
+        m.out[z * count + i] = float(double(m.update[z * count + i]) * factor);
+}
+
+// x = kScale * update / ||update|| and its transpose, a 64 x 64 tile of both a workgroup.
+__global__ __launch_bounds__(256) void pack_kernel(Batch batch) {
+    __shared__ float tile[64][65];  // [shorter][longer]
+    const Matrix& m = batch.of[find(batch, blockIdx.x)];
+    const int64_t across = m.longer / 64, tiles = across * (m.shorter / 64);
+    const int64_t id = int(blockIdx.x) - m.first, z = id / tiles;
+    const int64_t s0 = id % tiles / across * 64, l0 = id % across * 64;
+    const double factor = double(kScale) * inverse_norm(m, int(z));
+    const float* const from = m.update + z * m.elements();
+    const bool wide = m.wide();
+    for (int i = threadIdx.x / 64; i < 64; i += 4) {  // lines of the update
+        const int64_t row = (wide ? s0 : l0) + i, col = (wide ? l0 : s0) + threadIdx.x % 64;
+        const float v = row < m.rows && col < m.cols ? float(double(from[row * m.cols + col]) * factor) : 0.0f;
+        if (wide) tile[i][threadIdx.x % 64] = v;
+        else tile[threadIdx.x % 64][i] = v;
+    }
+    __syncthreads();
+    half *const x = m.x + z * 2 * m.shorter * m.longer, *const xt = m.xt + z * 2 * m.shorter * m.longer;
+    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+        const int row = i / 16, k = i % 16 * 4;
+        float v[4], w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = tile[row][k + e];
+            w[e] = tile[k + e][row];
+        }
+        packed::store4(x + place(s0 + row, l0 + k, m.longer), v);
+        packed::store4(xt + place(l0 + row, s0 + k, m.shorter), w);
+    }
 }
 
 enum class Kind { Gram, Poly, Apply };
@@ -108,21 +152,21 @@ enum class Kind { Gram, Poly, Apply };
 // which the library's stream never overlaps.
 __device__ unsigned g_tile_done[kMostSplit];
 
-// A tile of G, P or the next X. last: the next X leaves the scale, to y or into
-// the parameter.
-template <Kind K, int BT>
-__global__ __launch_bounds__(split::kThreads, K == Kind::Apply && BT == 128 ? 2 : 3) void product_kernel(Batch batch, bool last, float keep, float* partial) {
-    __shared__ split::Slice<S, BT> as, bs;
+// A tile of G, P or the next X. last: the next X leaves the scale, to `out` or
+// into the parameter.
+template <Kind K, int BT, int Stages>
+__global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batch, bool last, float keep, float* partial) {
+    using Tile = packed::Tile<BT, Stages>;
+    __shared__ __align__(16) char lds[Tile::kLds];
     __shared__ bool finisher;
     const Matrix& m = batch.of[find(batch, blockIdx.x)];
-    const int64_t rows = K == Kind::Apply ? m.rows : m.shorter(), cols = K == Kind::Apply ? m.cols : m.shorter();
-    const int64_t depth = K == Kind::Gram ? m.longer() : m.shorter();
-    const int row_tiles = int((rows + BT - 1) / BT), column_tiles = int((cols + BT - 1) / BT);
+    const int row_tiles = int(m.shorter / BT), column_tiles = K == Kind::Apply ? int(m.longer / BT) : row_tiles;
     const int tiles = K == Kind::Apply ? row_tiles * column_tiles : row_tiles * (row_tiles + 1) / 2;
     int id = int(blockIdx.x) - m.first;
     const int part = id % m.splits;
     id /= m.splits;
-    const int z = id / tiles, tile_id = id % tiles;
+    const int64_t z = id / tiles;
+    const int tile_id = id % tiles;
     int i = tile_id / column_tiles, j = tile_id % column_tiles;
     if constexpr (K != Kind::Apply) {  // the tile_id-th with i <= j
         i = 0;
@@ -134,81 +178,25 @@ __global__ __launch_bounds__(split::kThreads, K == Kind::Apply && BT == 128 ? 2 
         j += i;
     }
     const int64_t m0 = int64_t(i) * BT, n0 = int64_t(j) * BT;
-    const float* const x = m.x + z * m.elements();
-    const int64_t square = z * m.shorter() * m.shorter();
-    // This part's slices of k.
-    const int64_t slices = (depth + split::kSliceK - 1) / split::kSliceK;
-    const int64_t begin = slices * part / m.splits * split::kSliceK;
-    const int64_t end = min(depth, slices * (part + 1) / m.splits * split::kSliceK);
-
-    split::Tile<S, BT, BT> tile;
+    const int64_t whole = z * 2 * m.shorter * m.longer, square = z * 2 * m.shorter * m.shorter;
+    const int64_t depth = K == Kind::Gram ? m.longer : m.shorter, slices = depth / packed::kSlice;
+    // The squares are their own transposes.
+    const half* const a = K == Kind::Gram ? m.x + whole : (K == Kind::Poly ? m.gram : m.poly) + square;
+    const half* const b = K == Kind::Gram ? a : K == Kind::Poly ? a : m.xt + whole;
+    Tile tile;
     tile.clear();
-    const auto run = [&](auto& a, auto& b, auto&& load_a, auto&& load_b) {
-        load_a(begin);
-        load_b(begin);
-        for (int64_t k = begin; k < end; k += split::kSliceK) {
-            a.store(as);
-            b.store(bs);
-            __syncthreads();
-            if (k + split::kSliceK < end) {
-                load_a(k + split::kSliceK);
-                load_b(k + split::kSliceK);
-            }
-            tile.multiply(as, bs);
-            __syncthreads();
-        }
-    };
-    using Along = split::AlongK<BT>;
-    using Across = split::AcrossK<BT>;
-    const auto along = [&](const float* from, int64_t first, int64_t many, int64_t ld, const float* (&p)[Along::kChunks]) {
-#pragma unroll
-        for (int c = 0; c < Along::kChunks; ++c) p[c] = from + min(first + Along::row(c), many - 1) * ld;
-    };
-    const auto across = [&](int64_t first, int64_t many, unsigned (&at)[Across::kChunks]) {
-#pragma unroll
-        for (int c = 0; c < Across::kChunks; ++c) at[c] = unsigned(min(int64_t(Across::row(c)), many - 1 - first));
-    };
-    const auto line_of = [](const float* from, int64_t ld) {
-        return [=](int64_t k) {
-            const float* const line = from + k * ld;
-            return [=](int) { return line; };
-        };
-    };
-    if (K == Kind::Poly || (K == Kind::Gram && m.wide()) || (K == Kind::Apply && !m.wide())) {
-        // The squares are their own transposes.
-        const float* const fa = K == Kind::Poly ? m.gram + square : x;
-        const float* const fb = K == Kind::Gram ? x : (K == Kind::Poly ? m.gram : m.poly) + square;
-        const int64_t lda = K == Kind::Poly ? m.shorter() : m.cols, ldb = K == Kind::Gram ? m.cols : m.shorter();
-        Along a, b;
-        const float *pa[Along::kChunks], *pb[Along::kChunks];
-        along(fa, m0, rows, lda, pa);
-        along(fb, n0, cols, ldb, pb);
-        run(a, b, [&](int64_t k) { a.load(pa, k, end); }, [&](int64_t k) { b.load(pb, k, end); });
-    } else if constexpr (K == Kind::Gram) {
-        Across a, b;
-        unsigned at_a[Across::kChunks], at_b[Across::kChunks];
-        across(m0, rows, at_a);
-        across(n0, cols, at_b);
-        run(a, b, [&](int64_t k) { a.load(at_a, k, end, line_of(x + m0, m.cols)); },
-            [&](int64_t k) { b.load(at_b, k, end, line_of(x + n0, m.cols)); });
-    } else if constexpr (K == Kind::Apply) {
-        Along a;
-        Across b;
-        const float* pa[Along::kChunks];
-        unsigned at_b[Across::kChunks];
-        along(m.poly + square, m0, rows, m.shorter(), pa);
-        across(n0, cols, at_b);
-        run(a, b, [&](int64_t k) { a.load(pa, k, end); }, [&](int64_t k) { b.load(at_b, k, end, line_of(x + n0, m.cols)); });
-    }
+    tile.accumulate(a + m0 * 2 * depth, b + n0 * 2 * depth, depth, slices * part / m.splits, slices * (part + 1) / m.splits, lds);
 
     if (m.splits > 1) {
         // The part that counts in last adds all of them in order.
-        constexpr int kValues = BT * BT / split::kThreads;
+        constexpr int kValues = BT * BT / packed::kThreads;
         float* const mine = partial + (int64_t(blockIdx.x) - part) * BT * BT + threadIdx.x;
         int at = 0;
-        tile.each([&](int, int, float& v) {
-            __hip_atomic_store(&mine[(int64_t(part) * kValues + at++) * split::kThreads], v, __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
+        tile.each4([&](int, int, float (&v)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                __hip_atomic_store(&mine[(int64_t(part) * kValues + at++) * packed::kThreads], v[e], __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
         });
         red::wait_stores_visible();
         __syncthreads();
@@ -222,36 +210,50 @@ __global__ __launch_bounds__(split::kThreads, K == Kind::Apply && BT == 128 ? 2 
         tile.clear();
         for (int q = 0; q < m.splits; ++q) {
             at = 0;
-            tile.each([&](int, int, float& v) {
-                v += __hip_atomic_load(&mine[(int64_t(q) * kValues + at++) * split::kThreads], __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT);
+            tile.each4([&](int, int, float (&v)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] += __hip_atomic_load(&mine[(int64_t(q) * kValues + at++) * packed::kThreads], __ATOMIC_RELAXED,
+                                              __HIP_MEMORY_SCOPE_AGENT);
             });
         }
     }
 
     const float unit = 1.0f / kScale;
     if constexpr (K == Kind::Apply) {
-        float* const out = m.y + z * m.elements();
-        float* const param = m.param ? m.param + z * m.elements() : nullptr;
-        tile.each([&](int r, int c, float& v) {
+        const half* const xt = m.xt + whole;
+        const bool wide = m.wide();
+        float *const out = m.out ? m.out + z * m.elements() : nullptr, *const param = m.param ? m.param + z * m.elements() : nullptr;
+        const int64_t rows = wide ? m.rows : m.cols, cols = wide ? m.cols : m.rows;  // without the padding
+        tile.each4([&](int r, int c, float (&v)[4]) {
             const int64_t row = m0 + r, col = n0 + c;
-            if (row >= rows || col >= cols) return;
-            const int64_t at = row * cols + col;
-            const float next = kA * x[at] + v * unit;
-            if (!last) out[at] = next;
-            else if (param) param[at] = keep * param[at] - m.rate * (next * unit);
-            else out[at] = next * unit;
+            float x[4];
+            packed::load4(xt + place(col, row, m.shorter), x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = kA * x[e] + v[e] * unit;
+            if (!last || col >= cols) return;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (row + e >= rows) return;
+                const int64_t at = wide ? (row + e) * cols + col : col * rows + row + e;
+                if (param) param[at] = keep * param[at] - m.rate * (v[e] * unit);
+                else out[at] = v[e] * unit;
+            }
         });
+        if (last) return;
+        tile.store(m.y + whole, m0, n0, m.longer);
+        tile.store_transposed(m.yt + whole, m0, n0, m.shorter);
     } else {
-        float* const out = (K == Kind::Gram ? m.gram : m.poly) + square;
-        tile.each([&](int r, int c, float& v) {
-            const int64_t row = m0 + r, col = n0 + c;
-            if (row >= rows || col >= cols) return;
-            v *= unit;
-            if constexpr (K == Kind::Poly) v = kB * m.gram[square + row * cols + col] + kC * v;
-            out[row * cols + col] = v;
-            if (i != j) out[col * cols + row] = v;
+        half* const out = (K == Kind::Gram ? m.gram : m.poly) + square;
+        const half* const gram = m.gram + square;
+        tile.each4([&](int r, int c, float (&v)[4]) {
+            float g[4];
+            if constexpr (K == Kind::Poly) packed::load4(gram + place(n0 + c, m0 + r, m.shorter), g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = K == Kind::Poly ? kB * g[e] + kC * (v[e] * unit) : v[e] * unit;
         });
+        tile.store_transposed(out, m0, n0, m.shorter);
+        if (i != j) tile.store(out, m0, n0, m.shorter);
     }
 }
 
@@ -268,95 +270,109 @@ int64_t assign(Batch& batch, F&& workgroups) {
 }
 
 int64_t tiles_of(Kind kind, const Matrix& m, int64_t bt) {
-    if (kind == Kind::Apply) return m.count * ((m.rows + bt - 1) / bt) * ((m.cols + bt - 1) / bt);
-    const int64_t t = (m.shorter() + bt - 1) / bt;
-    return m.count * (t * (t + 1) / 2);
-}
-int64_t all_tiles(Kind kind, const Batch& batch, int64_t bt) {
-    int64_t tiles = 0;
-    for (int i = 0; i < batch.n; ++i) tiles += tiles_of(kind, batch.of[i], bt);
-    return tiles;
+    const int64_t t = m.shorter / bt;
+    return m.count * (kind == Kind::Apply ? t * (m.longer / bt) : t * (t + 1) / 2);
 }
 
-// Where tiles are few, sums are split into parts of at least four slices.
+// Where tiles are few, sums are split into parts of at least four slices. More
+// stages in flight where a CU has one workgroup at most.
 template <Kind K, int BT>
-void product_tiles(Device& d, Batch& batch, bool last, float keep) {
-    const int64_t tiles = all_tiles(K, batch, BT);
-    const int64_t wanted = tiles > kMostSplit ? 1 : std::max<int64_t>(1, 2 * d.cu_count / std::max<int64_t>(1, tiles));
+void product(Device& d, Batch& batch, bool last = false, float keep = 0.0f) {
+    int64_t tiles = 0;
+    for (int i = 0; i < batch.n; ++i) tiles += tiles_of(K, batch.of[i], BT);
+    const int64_t wanted = tiles > kMostSplit ? 1 : std::max<int64_t>(1, d.cu_count / tiles);
     int64_t counters = 0;
     for (int i = 0; i < batch.n; ++i) {
         Matrix& m = batch.of[i];
-        const int64_t slices = ((K == Kind::Gram ? m.longer() : m.shorter()) + split::kSliceK - 1) / split::kSliceK;
+        const int64_t slices = (K == Kind::Gram ? m.longer : m.shorter) / packed::kSlice;
         m.splits = int(std::max<int64_t>(1, std::min(wanted, slices / 4)));
         m.counters = int(counters);
         counters += tiles_of(K, m, BT);
     }
     const int64_t blocks = assign(batch, [](const Matrix& m) { return tiles_of(K, m, BT) * m.splits; });
     Scratch partial(wanted > 1 ? size_t(blocks) * BT * BT * sizeof(float) : 4);
-    launch(product_kernel<K, BT>, dim3(unsigned(blocks)), dim3(split::kThreads), 0, d.stream, batch, last, keep,
-           partial.as<float>());
+    const dim3 grid{unsigned(blocks)}, threads{packed::kThreads};
+    if (blocks <= d.cu_count)
+        launch(product_kernel<K, BT, 4>, grid, threads, 0, d.stream, batch, last, keep, partial.as<float>());
+    else
+        launch(product_kernel<K, BT, 2>, grid, threads, 0, d.stream, batch, last, keep, partial.as<float>());
     after_launch("orthogonalise product");
 }
 
-// Tiles of 128 where they give every other CU work, else of 64.
-template <Kind K>
-void product(Device& d, Batch& batch, bool last = false, float keep = 0.0f) {
-    if (all_tiles(K, batch, 128) >= d.cu_count / 2) product_tiles<K, 128>(d, batch, last, keep);
-    else product_tiles<K, 64>(d, batch, last, keep);
+template <int BT>
+void iterate(Device& d, Batch& batch, float keep, size_t steps) {
+    for (size_t i = 0; i < steps; ++i) {
+        product<Kind::Gram, BT>(d, batch);
+        product<Kind::Poly, BT>(d, batch);
+        product<Kind::Apply, BT>(d, batch, i + 1 == steps, keep);
+        for (int k = 0; k < batch.n; ++k) {
+            std::swap(batch.of[k].x, batch.of[k].y);
+            std::swap(batch.of[k].xt, batch.of[k].yt);
+        }
+    }
 }
 
-// The iterates of a batch; x and its successor take turns.
+// The iterates of a batch; x and its successor take turns. Tiles of 128 where
+// they give every other CU work, else of 64.
 void run(Device& d, Batch& batch, float mu, float keep, size_t steps) {
-    int64_t partials = 0, squares = 0, elements = 0;
+    const auto padded = [](int64_t n, int64_t bt) { return (n + bt - 1) / bt * bt; };
+    int64_t tiles = 0;
     for (int i = 0; i < batch.n; ++i) {
-        Matrix& m = batch.of[i];
-        m.blocks = int(grid_1d(size_t(m.elements()), 2048, kNormBlocks));
-        partials += int64_t(m.count) * m.blocks;
-        squares += m.count * m.shorter() * m.shorter();
-        elements += m.count * m.elements();
+        const Matrix& m = batch.of[i];
+        tiles += m.count * (padded(m.rows, 128) / 128) * (padded(m.cols, 128) / 128);
     }
-    Scratch sums(partials * sizeof(double)), first(elements * sizeof(float)), second(elements * sizeof(float)),
-        gram(squares * sizeof(float)), poly(squares * sizeof(float));
-    std::vector<float*> out(batch.n);
-    partials = squares = elements = 0;
+    const int64_t bt = tiles >= d.cu_count / 2 ? 128 : 64;
+    int64_t partials = 0, squares = 0, wholes = 0;
     for (int i = 0; i < batch.n; ++i) {
         Matrix& m = batch.of[i];
-        out[i] = m.y;
-        m.x = steps == 0 ? out[i] : first.as<float>() + elements;
-        m.y = second.as<float>() + elements;
-        m.gram = gram.as<float>() + squares;
-        m.poly = poly.as<float>() + squares;
+        m.shorter = padded(std::min(m.rows, m.cols), bt);
+        m.longer = padded(std::max(m.rows, m.cols), bt);
+        m.blocks = int(grid_1d(size_t(m.elements()), 1024, kNormBlocks));
+        partials += int64_t(m.count) * m.blocks;
+        squares += m.count * m.shorter * m.shorter;
+        wholes += m.count * m.shorter * m.longer;
+    }
+    // Four bytes a value; the update lies where the second iterate will.
+    Scratch sums(partials * sizeof(double)), x(wholes * 4), xt(wholes * 4), y(wholes * 4), yt(wholes * 4), gram(squares * 4),
+        poly(squares * 4);
+    partials = squares = wholes = 0;
+    for (int i = 0; i < batch.n; ++i) {
+        Matrix& m = batch.of[i];
+        m.x = x.as<half>() + 2 * wholes;
+        m.xt = xt.as<half>() + 2 * wholes;
+        m.y = y.as<half>() + 2 * wholes;
+        m.yt = yt.as<half>() + 2 * wholes;
+        m.update = y.as<float>() + wholes;
+        m.gram = gram.as<half>() + 2 * squares;
+        m.poly = poly.as<half>() + 2 * squares;
         m.partials = sums.as<double>() + partials;
         partials += int64_t(m.count) * m.blocks;
-        squares += m.count * m.shorter() * m.shorter();
-        elements += m.count * m.elements();
+        squares += m.count * m.shorter * m.shorter;
+        wholes += m.count * m.shorter * m.longer;
     }
-    const auto pass = [&](auto kernel, float value) {
-        const int64_t blocks = assign(batch, [](const Matrix& m) { return int64_t(m.count) * m.blocks; });
-        launch(kernel, dim3(unsigned(blocks)), dim3(256), 0, d.stream, batch, value);
+    int64_t blocks = assign(batch, [](const Matrix& m) { return int64_t(m.count) * m.blocks; });
+    launch(update_kernel, dim3(unsigned(blocks)), dim3(256), 0, d.stream, batch, mu);
+    after_launch("muon update");
+    if (steps == 0) {
+        launch(normalise_kernel, dim3(unsigned(blocks)), dim3(256), 0, d.stream, batch);
         after_launch("orthogonalise");
-    };
-    pass(update_kernel, mu);
-    pass(normalise_kernel, steps == 0 ? 1.0f : kScale);
-    for (size_t i = 0; i < steps; ++i) {
-        const bool last = i + 1 == steps;
-        if (last)
-            for (int k = 0; k < batch.n; ++k) batch.of[k].y = out[k];
-        product<Kind::Gram>(d, batch);
-        product<Kind::Poly>(d, batch);
-        product<Kind::Apply>(d, batch, last, keep);
-        for (int k = 0; k < batch.n; ++k) std::swap(batch.of[k].x, batch.of[k].y);
+        return;
     }
+    blocks = assign(batch, [](const Matrix& m) { return m.count * (m.shorter / 64) * (m.longer / 64); });
+    launch(pack_kernel, dim3(unsigned(blocks)), dim3(256), 0, d.stream, batch);
+    after_launch("orthogonalise pack");
+    if (bt == 128) iterate<128>(d, batch, keep, steps);
+    else iterate<64>(d, batch, keep, steps);
 }
 
 void check_matrix(size_t count, size_t rows, size_t cols) {
-    const size_t most = size_t(1) << 30;
+    const size_t most = size_t(1) << 21;  // 128 rows of parts stay within a buffer load's 31-bit offsets
     if (count > 65535) fail(VC_HIP_ERR_INVALID_ARGUMENT, "orthogonalise: at most 65535 matrices");
     if (rows > most || cols > most) fail(VC_HIP_ERR_OVERFLOW, "orthogonalise: matrix too large");
 }
 
 double flops(const Matrix& m, size_t steps) {
-    const double s = double(m.shorter()), l = double(m.longer());
+    const double s = double(std::min(m.rows, m.cols)), l = double(std::max(m.rows, m.cols));
     return double(m.count) * double(steps) * (3.0 * s * s * l + s * s * s);
 }
 
@@ -377,7 +393,7 @@ int vc_hip_orthogonalise(const float* in, size_t count, size_t rows, size_t cols
         batch.n = 1;
         Matrix& m = batch.of[0];
         m.grad = in;
-        m.y = out;
+        m.out = out;
         m.rows = int64_t(rows);
         m.cols = int64_t(cols);
         m.count = int(count);

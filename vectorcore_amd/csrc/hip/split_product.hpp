@@ -1,19 +1,14 @@
 // Matrix products of float32 operands on the 16-bit matrix instructions, at
 // float32's precision.
 //
-// Every operand value is written as a sum of numbers of fewer bits, and the
-// product as the sum of their products that matter:
-//   Bf16x3: x = x1 + x2 + x3 with bfloat16 parts, each the rounding of what the
-//   earlier ones leave. |x2| <= 2^-9 |x|, |x3| <= 2^-18 |x|, and the parts' 24
-//   bits hold all of x. Of the nine products those below 2^-26 of the largest
-//   (x2 y3, x3 y2, x3 y3) are left out; six remain. bfloat16 has float32's
-//   exponents, so any magnitudes may meet.
-//   Fp16x2: x = x1 + x2 with half-precision parts, 22 bits of x; x2 y2 (2^-22)
-//   is left out, three products remain. For values known to lie near one.
-// All products are exact and summed in float32 by the matrix instructions, whose
-// 16-deep sums round less often than a float32 chain does. Six instructions of
-// 32 cycles take the place of eight of 64 (V_MFMA_F32_32X32X2_F32), three that
-// of eight.
+// Every value is written as a sum of three bfloat16 numbers, x = x1 + x2 + x3,
+// each the rounding of what the earlier ones leave: |x2| <= 2^-9 |x|, |x3| <=
+// 2^-18 |x|, and the parts' 24 bits hold all of x. Of the nine products of two
+// values' parts those below 2^-26 of the largest (x2 y3, x3 y2, x3 y3) are left
+// out. bfloat16 has float32's exponents, so any magnitudes may meet. The six
+// others are exact and summed in float32 by the matrix instructions, whose
+// 16-deep sums round less often than a float32 chain does: six instructions of
+// 32 cycles take the place of eight of 64 (V_MFMA_F32_32X32X2_F32).
 //
 // A workgroup of four waves computes a BM x BN tile of C, each wave a quarter
 // of it in 32 x 32 blocks, k in slices of 32. A thread loads its share of a
@@ -45,14 +40,6 @@ struct Bf16x3 {
     static constexpr int kA[6] = {0, 2, 1, 0, 1, 0}, kB[6] = {2, 0, 1, 1, 0, 0};
     static __device__ inline f16v multiply(v8 a, v8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
-struct Fp16x2 {
-    static constexpr int kParts = 2, kProducts = 3;
-    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
-    static constexpr int kA[3] = {0, 1, 0}, kB[3] = {1, 0, 0};
-    static __device__ inline f16v multiply(v8 a, v8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-};
-
 // The parts of eight values, packed.
 template <class S>
 __device__ inline void split8(const float (&v)[8], typename S::v8 (&out)[S::kParts]) {
@@ -94,24 +81,25 @@ struct AlongK {
 
     // p: the chunks' rows at k = 0. A row past the operand's end may be any
     // row of it: what it gives is never stored.
-    __device__ inline void load(const float* const (&p)[kChunks], int64_t k0, int64_t depth) {
+    __device__ inline void load(const float* const (&p)[kChunks], int64_t k0) {
         const int64_t k = k0 + 8 * (threadIdx.x % kGroups);
-        if (k0 + kSliceK <= depth) {
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                const f4u lo = *reinterpret_cast<const f4u*>(p[j] + k), hi = *reinterpret_cast<const f4u*>(p[j] + k + 4);
+        for (int j = 0; j < kChunks; ++j) {
+            const f4u lo = *reinterpret_cast<const f4u*>(p[j] + k), hi = *reinterpret_cast<const f4u*>(p[j] + k + 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[j][i] = lo[i];
-                    v[j][4 + i] = hi[i];
-                }
+            for (int i = 0; i < 4; ++i) {
+                v[j][i] = lo[i];
+                v[j][4 + i] = hi[i];
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[j][i] = k + i < depth ? p[j][k + i] : 0.0f;
         }
+    }
+    // The last slice, of which k < depth are there.
+    __device__ inline void load_rest(const float* const (&p)[kChunks], int64_t k0, int64_t depth) {
+        const int64_t k = k0 + 8 * (threadIdx.x % kGroups);
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] = k + i < depth ? p[j][k + i] : 0.0f;
     }
     template <class S>
     __device__ inline void store(Slice<S, Rows>& lds) const {
@@ -137,23 +125,24 @@ struct AcrossK {
     // line(k): the line of k < depth, uniform in the wave. at: the chunks' places in a line; a row past the operand's
     // end may be any place of it: what it gives is never stored.
     template <class Line>
-    __device__ inline void load(const unsigned (&at)[kChunks], int64_t k0, int64_t depth, Line&& line) {
+    __device__ inline void load(const unsigned (&at)[kChunks], int64_t k0, Line&& line) {
         const int64_t k = k0 + 8 * __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        if (k0 + kSliceK <= depth) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const auto from = line(k + i);
+        for (int i = 0; i < 8; ++i) {
+            const auto from = line(k + i);
 #pragma unroll
-                for (int j = 0; j < kChunks; ++j) v[j][i] = from(j)[at[j]];
-            }
-        } else {
+            for (int j = 0; j < kChunks; ++j) v[j][i] = from(j)[at[j]];
+        }
+    }
+    template <class Line>
+    __device__ inline void load_rest(const unsigned (&at)[kChunks], int64_t k0, int64_t depth, Line&& line) {
+        const int64_t k = k0 + 8 * __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool inside = k + i < depth;
-                const auto from = line(inside ? k + i : 0);
+        for (int i = 0; i < 8; ++i) {
+            const bool inside = k + i < depth;
+            const auto from = line(inside ? k + i : 0);
 #pragma unroll
-                for (int j = 0; j < kChunks; ++j) v[j][i] = inside ? from(j)[at[j]] : 0.0f;
-            }
+            for (int j = 0; j < kChunks; ++j) v[j][i] = inside ? from(j)[at[j]] : 0.0f;
         }
     }
     template <class S>
@@ -187,11 +176,11 @@ struct Tile {
                 for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.0f;
     }
 
-    __device__ inline void multiply(const Slice<S, BM>& as, const Slice<S, BN>& bs) {
+    // k-groups k and k + 1 of a slice.
+    __device__ inline void multiply(const Slice<S, BM>& as, const Slice<S, BN>& bs, int k) {
         const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
         const int m0 = wave / 2 * (BM / 2) + lane % 32, n0 = wave % 2 * 32 + lane % 32;
-#pragma unroll
-        for (int k = 0; k < kGroups; k += 2) {
+        {
             typename S::v8 a[kM][S::kParts];
 #pragma unroll
             for (int q = 0; q < S::kParts; ++q)
@@ -226,6 +215,28 @@ struct Tile {
                 }
     }
 };
+
+// The products of k < depth onto a tile: a slice is loaded into registers while
+// the one before it is multiplied. load(k) reads a whole slice, rest(k) the last
+// one, of which depth % 32 are there.
+template <class T, class A, class B, class SA, class SB, class Load, class Rest>
+__device__ inline void accumulate(T& tile, A& a, B& b, SA& as, SB& bs, int64_t depth, Load&& load, Rest&& rest) {
+    const auto next = [&](int64_t k) {
+        if (k + kSliceK <= depth) load(k);
+        else rest(k);
+    };
+    if (depth <= 0) return;
+    next(int64_t(0));
+    for (int64_t k = 0; k < depth; k += kSliceK) {
+        a.store(as);
+        b.store(bs);
+        __syncthreads();
+        if (k + kSliceK < depth) next(k + kSliceK);
+        tile.multiply(as, bs, 0);
+        tile.multiply(as, bs, 2);
+        __syncthreads();
+    }
+}
 
 // Is a sum of products lost to an infinity, a NaN or a value that rounds to an
 // infinity in 16 bits? Its parts give NaN or an infinity then.
