@@ -104,13 +104,13 @@ struct Tile {
     // acc += the products of k slices [begin, end) of BT rows of each operand;
     // a, b: their first rows; depth: k of a whole row. lds: kLds bytes.
     //
-    // Row r's chunk c (first parts 0 to 3, second 4 to 7) lies in slot c ^ (r % 8)
-    // of its 128 bytes: the rows of a fragment then meet different banks. Slice
+    // Row r's chunk c (first parts 0 to 3, second 4 to 7) lies in slot c ^ (r / 2 % 8)
+    // of its 128 bytes: 16 rows of a fragment then meet different banks. Slice
     // s + Stages - 1 is requested while slice s is multiplied.
     __device__ inline void accumulate(const _Float16* a, const _Float16* b, int64_t depth, int64_t begin, int64_t end, char* lds) {
         const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
         const uint32_t row_bytes = uint32_t(depth) * 4u;
-        const uint32_t off = uint32_t(8 * wave + lane / 8) * row_bytes + uint32_t((lane % 8) ^ (lane / 8)) * 16u;
+        const uint32_t off = uint32_t(8 * wave + lane / 8) * row_bytes + uint32_t((lane % 8) ^ (4 * (wave % 2) + lane / 16)) * 16u;
         const uint32_t to = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)lds)) + 1024u * uint32_t(wave));
         const auto request = [&](int64_t s, int stage) {
             const int64_t at = min(s, end - 1) * kLine;
@@ -120,7 +120,7 @@ struct Tile {
             load_rows<0, BT * 128>(__builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16*>(b + at), short(0), 0x7FFFFFFE, 0x00020000),
                                    off, 32u * row_bytes, dst);
         };
-        const int half = lane / 32, swizzle = lane % 8;
+        const int half = lane / 32, swizzle = lane / 2 % 8;
         const int row_a = wave / 2 * (BT / 2) + lane % 32, row_b = BT + wave % 2 * (BT / 2) + lane % 32;
         const auto multiply = [&](int stage) {
             const char* const from = lds + stage * kStage;
