@@ -162,6 +162,37 @@ struct RowTile {
     bool live;
 };
 
+// The tile-th of the groups' tiles of Rows rows.
+template <int Rows>
+__device__ inline RowTile find_rows(const int* __restrict__ offsets, int groups, int tile, int64_t column) {
+    const int lane = threadIdx.x % kWave;
+    RowTile t{0, 0, 0, column, false};
+    for (int base = 0; base < groups; base += kWave) {
+        const int e = base + lane;
+        const int lo = e < groups ? offsets[e] : 0, hi = e < groups ? offsets[e + 1] : 0;
+        const int n = (hi - lo + Rows - 1) / Rows;
+        int upto = n;
+        for (int d = 1; d < kWave; d <<= 1) {
+            const int v = __shfl_up(upto, d);
+            if (lane >= d) upto += v;
+        }
+        const uint64_t past = __ballot(upto > tile);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            t.live = true;
+            t.group = base + at;
+            t.begin = __shfl(lo, at) + (tile - __shfl(upto - n, at)) * Rows;
+            t.end = min(__shfl(hi, at), t.begin + Rows);
+            break;
+        }
+        tile -= __shfl(upto, kWave - 1);
+    }
+    t.group = __builtin_amdgcn_readfirstlane(t.group);
+    t.begin = __builtin_amdgcn_readfirstlane(t.begin);
+    t.end = __builtin_amdgcn_readfirstlane(t.end);
+    return t;
+}
+
 // The tile of this workgroup: tiles are numbered group by group, their columns
 // together, and dealt out so that each of the chip's eight dies (workgroups go
 // to them in turn) works on neighbouring ones, which read the same operands
@@ -178,32 +209,8 @@ __device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups,
     }
     const int64_t total = all * column_tiles, share = (total + 7) / 8;
     const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8;
-    RowTile t{0, 0, 0, id % column_tiles, blockIdx.x / 8 < share && id < total};
-    if (!t.live) return t;
-    int tile = int(id / column_tiles);
-    for (int base = 0; base < groups; base += kWave) {
-        const int e = base + lane;
-        const int lo = e < groups ? offsets[e] : 0, hi = e < groups ? offsets[e + 1] : 0;
-        const int n = (hi - lo + kTile - 1) / kTile;
-        int upto = n;
-        for (int d = 1; d < kWave; d <<= 1) {
-            const int v = __shfl_up(upto, d);
-            if (lane >= d) upto += v;
-        }
-        const uint64_t past = __ballot(upto > tile);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            t.group = base + at;
-            t.begin = __shfl(lo, at) + (tile - __shfl(upto - n, at)) * kTile;
-            t.end = min(__shfl(hi, at), t.begin + kTile);
-            break;
-        }
-        tile -= __shfl(upto, kWave - 1);
-    }
-    t.group = __builtin_amdgcn_readfirstlane(t.group);
-    t.begin = __builtin_amdgcn_readfirstlane(t.begin);
-    t.end = __builtin_amdgcn_readfirstlane(t.end);
-    return t;
+    if (blockIdx.x / 8 >= share || id >= total) return RowTile{0, 0, 0, 0, false};
+    return find_rows<kTile>(offsets, groups, int(id / column_tiles), id % column_tiles);
 }
 
 __device__ inline float sigmoid(float x) {
@@ -397,6 +404,173 @@ __global__ __launch_bounds__(split::kThreads, at_once(BN)) void weight_kernel(Pr
     });
 }
 
+// ---- few rows of each expert ----------------------------------------------------------
+// Bound by reading the weights, which every expert's rows need once: a workgroup
+// takes up to four rows of an expert, a tile of columns and a part of k. Each
+// lane reads four columns of eight k at a time, and each weight goes into as many
+// fused multiply-adds as there are rows; x is read from LDS. A wave reads whole
+// 1 KiB lines of 256 columns, or, where few rows reach few experts, 256-byte
+// lines of 64 columns at four places of k: the parts of k are then fewer and
+// longer. The sums of the waves' k are added in LDS, those of workgroups by the
+// one that counts in last, in order.
+
+constexpr int kThinRows = 4, kThinDepth = 512, kThinTiles = 4096;
+constexpr size_t kThinMost = 32;  // rows of an expert on average
+
+__device__ unsigned g_thin_done[kThinTiles];  // parts done of a tile; zero between launches
+
+// out: of column threadIdx.x of the tile.
+template <int Matrices, int Rows, int Columns>
+__device__ inline void thin_sums(const ProductArgs& p, const RowTile& t, int64_t begin, int64_t end, float (*xs)[kThinDepth],
+                                 float* sums, float (&out)[Rows][Matrices]) {
+    constexpr int kPlaces = 256 / Columns, kLanes = kWave / kPlaces;  // places of k in a wave, lanes of each
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int64_t n0 = t.column * Columns, col = n0 + 4 * (lane % kLanes);
+    const int64_t matrix = int64_t(t.group) * p.width * p.columns;
+    const int inside = int(min(int64_t(4), p.columns - col));  // of this lane's columns
+    split::f4u acc[Rows][Matrices];
+#pragma unroll
+    for (int r = 0; r < Rows; ++r)
+#pragma unroll
+        for (int m = 0; m < Matrices; ++m) acc[r][m] = split::f4u{0, 0, 0, 0};
+    for (int64_t k0 = begin; k0 < end; k0 += kThinDepth) {
+        const int depth = int(min(int64_t(kThinDepth), end - k0)), padded = (depth + 7) / 8 * 8;
+        for (int r = 0; r < Rows; ++r) {
+            const int row = min(t.begin + r, t.end - 1);
+            const float* const x = p.a + int64_t(p.token ? p.token[row] : row) * p.width + k0;
+            for (int k = threadIdx.x; k < padded; k += 256) xs[r][k] = k < depth ? x[k] : 0.0f;
+        }
+        __syncthreads();
+        for (int k = 8 * (kPlaces * wave + lane / kLanes); k < depth; k += 32 * kPlaces) {
+            split::f4u w[Matrices][8];
+            const unsigned at = unsigned(k) * unsigned(p.columns) + unsigned(col - n0);
+#pragma unroll
+            for (int m = 0; m < Matrices; ++m) {
+                const float* const from = (m ? p.b2 : p.b) + matrix + k0 * p.columns + n0;  // uniform
+                if (k + 8 <= depth && n0 + Columns <= p.columns) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[m][i] = *reinterpret_cast<const split::f4u*>(from + i * p.columns + at);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) w[m][i][c] = k + i < depth && c < inside ? (from + i * p.columns)[at + c] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < Rows; ++r)
+#pragma unroll
+                for (int m = 0; m < Matrices; ++m)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) acc[r][m][c] = fmaf(xs[r][k + i], w[m][i][c], acc[r][m][c]);
+        }
+        __syncthreads();
+    }
+    const int place = wave * kPlaces + lane / kLanes;
+#pragma unroll
+    for (int r = 0; r < Rows; ++r)
+#pragma unroll
+        for (int m = 0; m < Matrices; ++m) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sums[place * Columns + 4 * (lane % kLanes) + c] = acc[r][m][c];
+            __syncthreads();
+            float sum = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4 * kPlaces; ++q) sum += sums[q * Columns + threadIdx.x % Columns];
+            out[r][m] = sum;
+            __syncthreads();
+        }
+}
+
+template <bool Gated, int Rows, int Columns>
+__device__ inline void thin_tile(const ProductArgs& p, const RowTile& t, int part, int splits, int64_t tile, float* partial,
+                                 float (*xs)[kThinDepth], float* sums, bool& finisher) {
+    constexpr int kMatrices = Gated ? 2 : 1;
+    const int64_t groups = (p.width + 7) / 8;
+    const int64_t begin = min(p.width, groups * part / splits * 8), end = min(p.width, groups * (part + 1) / splits * 8);
+    float out[Rows][kMatrices];
+    thin_sums<kMatrices, Rows, Columns>(p, t, begin, end, xs, sums, out);
+    const bool mine = threadIdx.x < Columns;
+    if (splits > 1) {
+        constexpr int kValues = Rows * kMatrices;
+        float* const parts = partial + tile * splits * (kThinRows * kMatrices * Columns) + threadIdx.x % Columns;
+        if (mine) {
+#pragma unroll
+            for (int v = 0; v < kValues; ++v)
+                __hip_atomic_store(&parts[(part * kValues + v) * Columns], out[v / kMatrices][v % kMatrices], __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+        }
+        red::wait_stores_visible();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            unsigned* const done = &g_thin_done[tile];
+            finisher = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == unsigned(splits);
+            if (finisher) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!finisher) return;
+#pragma unroll
+        for (int v = 0; v < kValues; ++v) {
+            float sum = 0.0f;
+            for (int q = 0; q < splits; q += 8) {
+                float ahead[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    ahead[i] = __hip_atomic_load(&parts[(min(q + i, splits - 1) * kValues + v) * Columns], __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (q + i < splits) sum += ahead[i];
+            }
+            out[v / kMatrices][v % kMatrices] = sum;
+        }
+    }
+    const int64_t col = t.column * Columns + threadIdx.x;
+    if (!mine || col >= p.columns) return;
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        if (t.begin + r >= t.end) break;
+        const int64_t at = int64_t(t.begin + r) * p.columns + col;
+        if constexpr (Gated) {
+            const float g = out[r][0], u = out[r][1];
+            p.c[at] = g * sigmoid(g) * u;
+            if (p.c2) {
+                p.c2[at] = g;
+                p.c3[at] = u;
+            }
+        } else {
+            p.c[at] = out[r][0];
+        }
+    }
+}
+
+// Workgroups in the order of rows, columns, parts of k.
+template <bool Gated, int Columns>
+__global__ __launch_bounds__(256, Gated ? 2 : 3) void thin_kernel(ProductArgs p, int splits, float* partial) {
+    __shared__ float xs[kThinRows][kThinDepth], sums[1024];
+    __shared__ bool finisher;
+    const int64_t column_tiles = (p.columns + Columns - 1) / Columns;
+    const int part = int(blockIdx.x % splits);
+    const int64_t tile = blockIdx.x / splits;
+    const RowTile t = find_rows<kThinRows>(p.offsets, p.experts + 1, int(tile / column_tiles), tile % column_tiles);
+    if (!t.live) return;
+    if (t.group == p.experts) {  // dropped picks: zero rows
+        const int64_t col = t.column * Columns + threadIdx.x;
+        if (part || threadIdx.x >= Columns || col >= p.columns) return;
+        for (int64_t r = t.begin; r < t.end; ++r) {
+            p.c[r * p.columns + col] = 0.0f;
+            if (Gated && p.c2) p.c2[r * p.columns + col] = p.c3[r * p.columns + col] = 0.0f;
+        }
+        return;
+    }
+    const int rows = t.end - t.begin;
+    if (rows == 1) thin_tile<Gated, 1, Columns>(p, t, part, splits, tile, partial, xs, sums, finisher);
+    else if (rows == 2) thin_tile<Gated, 2, Columns>(p, t, part, splits, tile, partial, xs, sums, finisher);
+    else thin_tile<Gated, 4, Columns>(p, t, part, splits, tile, partial, xs, sums, finisher);
+}
+
 int64_t tiles_of(size_t n, int tile) { return int64_t((n + tile - 1) / tile); }
 
 // A grid for `tiles` tiles at most, in whole rounds of the eight dies.
@@ -413,6 +587,27 @@ template <class F>
 void with_columns(Device& d, int64_t row_tiles, size_t columns, F&& f) {
     if (row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) f(std::integral_constant<int, 256>());
     else f(std::integral_constant<int, 128>());
+}
+
+// (A lane's place in kThinDepth lines is a 32-bit offset.)
+bool thin(const Plan& plan, size_t columns) { return plan.rows <= kThinMost * plan.experts && columns <= size_t(1) << 20; }
+
+// Parts of k, of 64 to 128 at least, for three workgroups on every CU; narrow
+// tiles of columns where wide ones would leave that to more than six parts.
+template <bool Gated, int Columns>
+void launch_thin(Device& d, int64_t rows, const ProductArgs& args) {
+    const int64_t tiles = rows * tiles_of(size_t(args.columns), Columns), wanted = (3 * d.cu_count + tiles - 1) / tiles;
+    const int64_t splits = tiles > kThinTiles ? 1 : std::max<int64_t>(1, std::min(wanted, args.width / (Columns == 64 ? 128 : 64)));
+    if (tiles * splits >= int64_t(1) << 31) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
+    Scratch partial(splits > 1 ? size_t(tiles * splits) * kThinRows * Columns * (Gated ? 2 : 1) * sizeof(float) : 4);
+    launch(thin_kernel<Gated, Columns>, dim3(unsigned(tiles * splits)), dim3(256), 0, d.stream, args, int(splits),
+           partial.as<float>());
+}
+template <bool Gated>
+void launch_thin(Device& d, const Plan& plan, const ProductArgs& args) {
+    const int64_t rows = std::min<int64_t>(plan.rows, int64_t(plan.rows / kThinRows + plan.experts + 1));
+    if (2 * rows * tiles_of(size_t(args.columns), 256) < d.cu_count) launch_thin<Gated, 64>(d, rows, args);
+    else launch_thin<Gated, 256>(d, rows, args);
 }
 
 // ---- the gated unit -------------------------------------------------------------------
@@ -524,7 +719,8 @@ int vc_hip_expert_linear_forward(const float* x, const float* w, const vc_hip_ex
         Profiled p("expert_linear", 2.0 * q.rows * width * columns, 4.0 * (q.rows * (width + columns) + q.experts * width * columns));
         const ProductArgs args{x, w, nullptr, nullptr, out, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
                                int(q.experts), int64_t(width), int64_t(columns)};
-        with_columns(d, int64_t(q.rows / kTile), columns, [&](auto bn) {
+        if (thin(q, columns)) launch_thin<false>(d, q, args);
+        else with_columns(d, int64_t(q.rows / kTile), columns, [&](auto bn) {
             launch(forward_kernel<false, bn()>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, bn())), dim3(split::kThreads),
                    0, d.stream, args);
         });
@@ -545,7 +741,8 @@ int vc_hip_expert_gated_forward(const float* x, const float* gate, const float* 
                    4.0 * (q.rows * (width + (save_gate ? 3.0 : 1.0) * columns) + 2.0 * q.experts * width * columns));
         const ProductArgs args{x, gate, nullptr, up, out, save_gate, save_up, q.offsets, ordered ? nullptr : q.token,
                                int(q.experts), int64_t(width), int64_t(columns)};
-        with_columns(d, int64_t(q.rows / kTile), 2 * columns, [&](auto bn) {
+        if (thin(q, columns)) launch_thin<true>(d, q, args);
+        else with_columns(d, int64_t(q.rows / kTile), 2 * columns, [&](auto bn) {
             launch(forward_kernel<true, bn()>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, bn() / 2)),
                    dim3(split::kThreads), 0, d.stream, args);
         });

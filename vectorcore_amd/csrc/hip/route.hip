@@ -7,8 +7,13 @@
 // the lower index first among equals; weight_j = score_j / sum of the chosen
 // scores (renormalised) or score_j.
 //
-// One wavefront per row, all in double: choices next to a border between ranks
-// are those of the definition.
+// Choices next to a border between ranks are those of the definition: where a
+// row's 32-bit ranks cannot tell two candidates apart, its whole wavefront ranks
+// it again in double.
+//
+// Bound by HBM for many rows (the logits are read, the gradient is written), if
+// the vector instructions are few: sixteen lanes share a row, so four rows share
+// each step of a search or sum across lanes.
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"
 
@@ -90,37 +95,45 @@ __device__ inline void row_scores(const float* __restrict__ row, int experts, in
     for (int i = 0; i < NV; ++i) s[i] /= total;
 }
 
+struct RouteArgs {
+    const float *logits, *bias;
+    int64_t tokens;
+    int experts, top_k, groups, top_groups;
+    bool sigmoid, renormalise;
+    float *weights, *chosen;
+};
+
+// LDS that a wavefront has written is read by its other lanes.
+__device__ inline void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Row t by a whole wavefront, in double. ranks: 64 NV of LDS.
 template <int NV>
-__global__ __launch_bounds__(kWave* kWaves) void route_kernel(const float* __restrict__ logits, const float* __restrict__ bias,
-                                                             size_t tokens, int experts, int top_k, bool sigmoid, int groups,
-                                                             int top_groups, bool renormalise, float* __restrict__ weights,
-                                                             float* __restrict__ chosen) {
-    __shared__ double ranks[kWaves][kWave * NV];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const size_t t = size_t(blockIdx.x) * kWaves + wave;
-    const bool live = t < tokens;  // uniform in the wavefront
+__device__ void route_row(const RouteArgs& p, int64_t t, double* ranks) {
+    const int lane = threadIdx.x % kWave, experts = p.experts;
     double s[NV];
     uint64_t key[NV];
-    if (live) {
-        row_scores<NV>(logits + t * experts, experts, lane, sigmoid, s);
+    row_scores<NV>(p.logits + t * experts, experts, lane, p.sigmoid, s);
+    wave_fence();
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = lane + kWave * i;
-            const double rank = s[i] + (bias && e < experts ? double(bias[e]) : 0.0);
-            ranks[wave][e] = rank;
-            key[i] = e < experts ? rank_key(rank) : 0;
-        }
+    for (int i = 0; i < NV; ++i) {
+        const int e = lane + kWave * i;
+        const double rank = s[i] + (p.bias && e < experts ? double(p.bias[e]) : 0.0);
+        ranks[e] = rank;
+        key[i] = e < experts ? rank_key(rank) : 0;
     }
-    __syncthreads();
-    if (!live) return;
-    if (groups > 1) {
-        const int size = experts / groups;
+    wave_fence();
+    if (p.groups > 1) {
+        const int size = experts / p.groups;
         uint64_t strength = 0;
-        if (lane < groups) {
+        if (lane < p.groups) {
             double best = -__builtin_huge_val(), second = -__builtin_huge_val();
             bool nan = false;
             for (int i = 0; i < size; ++i) {
-                const double r = ranks[wave][lane * size + i];
+                const double r = ranks[lane * size + i];
                 nan |= r != r;
                 if (r > best) {
                     second = best;
@@ -132,9 +145,9 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(const float* __res
             strength = rank_key(nan ? __builtin_nan("") : size > 1 ? best + second : best);
         }
         uint64_t open = 0;
-        for (int j = 0; j < top_groups; ++j) {
+        for (int j = 0; j < p.top_groups; ++j) {
             const uint64_t best = wave_max_key(strength);
-            const int g = wave_min(strength == best && lane < groups ? lane : kWave);
+            const int g = wave_min(strength == best && lane < p.groups ? lane : kWave);
             open |= 1ull << g;
             if (lane == g) strength = 0;
         }
@@ -146,7 +159,7 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(const float* __res
     }
     int mine = 0;
     double score = 0.0, total = 0.0;
-    for (int j = 0; j < top_k; ++j) {
+    for (int j = 0; j < p.top_k; ++j) {
         uint64_t best = key[0];
 #pragma unroll
         for (int i = 1; i < NV; ++i) best = key[i] > best ? key[i] : best;
@@ -170,14 +183,289 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(const float* __res
             score = picked;
         }
     }
-    if (lane < top_k) {
-        weights[t * top_k + lane] = float(renormalise ? score / total : score);
-        chosen[t * top_k + lane] = float(mine);
+    if (lane < p.top_k) {
+        p.weights[t * p.top_k + lane] = float(p.renormalise ? score / total : score);
+        p.chosen[t * p.top_k + lane] = float(mine);
+    }
+}
+
+// A wavefront per row.
+template <int NV>
+__global__ __launch_bounds__(kWave* kWaves) void route_wide_kernel(RouteArgs p) {
+    __shared__ double ranks[kWaves][kWave * NV];
+    const int64_t t = int64_t(blockIdx.x) * kWaves + threadIdx.x / kWave;
+    if (t < p.tokens) route_row<NV>(p, t, ranks[threadIdx.x / kWave]);
+}
+
+// ---- sixteen lanes a row --------------------------------------------------------------
+// Up to 256 experts, 16 picks and 16 groups. Lane l of a row holds experts
+// 64 j + 4 l .. + 3.
+
+constexpr int kLanes = 16, kRows = kWave / kLanes;  // of a row; rows of a wavefront
+
+template <class F>
+__device__ inline float row_all(float v, F&& f) {
+    const int lane = red::lane_id();
+    v = f(v, red::partner<0>(v, lane));
+    v = f(v, red::partner<1>(v, lane));
+    v = f(v, red::partner<2>(v, lane));
+    return f(v, red::partner<3>(v, lane));
+}
+__device__ inline float row_sum(float v) {
+    return row_all(v, [](float a, float b) { return a + b; });
+}
+__device__ inline float row_max(float v) {
+    return row_all(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ inline uint32_t row_max_key(uint32_t v) {
+    const int lane = red::lane_id();
+    v = max(v, red::partner<0>(v, lane));
+    v = max(v, red::partner<1>(v, lane));
+    v = max(v, red::partner<2>(v, lane));
+    return max(v, red::partner<3>(v, lane));
+}
+__device__ inline int row_min(int v) {
+    const int lane = red::lane_id();
+    v = min(v, red::partner<0>(v, lane));
+    v = min(v, red::partner<1>(v, lane));
+    v = min(v, red::partner<2>(v, lane));
+    return min(v, red::partner<3>(v, lane));
+}
+
+// A number in its order (not NaN; -0 like 0), never 0.
+__device__ inline uint32_t order_key(float v) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v + 0.0f);
+    return bits >> 31 ? ~bits : bits | 0x80000000u;
+}
+__device__ inline float order_value(uint32_t key) {
+    return __builtin_bit_cast(float, key >> 31 ? key & 0x7FFFFFFFu : ~key);
+}
+
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// The row's logits; none past its end.
+template <int NV>
+__device__ inline void row_logits(const float* __restrict__ row, int experts, int l, float (&v)[NV]) {
+#pragma unroll
+    for (int j = 0; j < NV / 4; ++j) {
+        const int e = 64 * j + 4 * l;
+        if (e + 4 <= experts) {
+            const f4u x = *reinterpret_cast<const f4u*>(row + e);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[4 * j + c] = x[c];
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[4 * j + c] = e + c < experts ? row[e + c] : -__builtin_huge_valf();
+        }
+    }
+}
+
+__device__ inline float score_of(float logit, bool sigmoid, float top, float inverse) {
+    return sigmoid ? 1.0f / (1.0f + expf(-logit)) : expf(logit - top) * inverse;
+}
+
+// Exact: without a bias and groups the logits' own order is that of the ranks,
+// as long as doubles tell the scores apart. Otherwise the 32-bit ranks decide
+// where they are further apart than their errors: a score is within 2^-21 of
+// itself, a rank within 2^-20 of the largest score and bias.
+template <int NV, bool Exact>
+__global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
+    __shared__ double scratch[kWaves][kWave * NV / 2];  // floats of four rows, or doubles of one
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, l = lane % kLanes, r = lane / kLanes;
+    const int64_t first = (int64_t(blockIdx.x) * kWaves + wave) * kRows;
+    if (first >= p.tokens) return;  // uniform in the wavefront
+    const int64_t t = min(first + r, p.tokens - 1);
+    const int experts = p.experts;
+    const float* const row = p.logits + t * experts;
+    float v[NV];
+    row_logits<NV>(row, experts, l, v);
+    float top = -__builtin_huge_valf(), inverse = 1.0f;
+    bool again = false;  // this row in double
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        top = fmaxf(top, v[i]);
+        again |= v[i] != v[i];
+    }
+    top = row_max(top);
+    again |= !(fabsf(top) < __builtin_huge_valf());
+    if (!p.sigmoid) {
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) total += expf(v[i] - top);
+        inverse = 1.0f / row_sum(total);
+    }
+    uint32_t key[NV];
+    float margin = 0.0f;
+    if constexpr (Exact) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = 64 * (i / 4) + 4 * l + i % 4 < experts ? order_key(v[i]) : 0;
+    } else {
+        float most = 0.0f;
+        float* const ranks = reinterpret_cast<float*>(scratch[wave]) + r * (kWave * NV / 4);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = 64 * (i / 4) + 4 * l + i % 4;
+            const float score = score_of(v[i], p.sigmoid, top, inverse), bias = p.bias && e < experts ? p.bias[e] : 0.0f;
+            const float rank = score + bias;
+            again |= rank != rank;
+            most = fmaxf(most, fmaxf(score, fabsf(bias)));
+            key[i] = e < experts ? order_key(rank) : 0;
+            if (p.groups > 1) ranks[e] = rank;
+        }
+        margin = row_max(most) * 0x1p-18f;  // twice the errors of two ranks
+        again |= !(margin < __builtin_huge_valf());
+        if (p.groups > 1) {
+            wave_fence();
+            const int size = experts / p.groups;
+            float best = -__builtin_huge_valf(), second = best;
+            if (l < p.groups) {
+                int at = l % size;  // each lane begins elsewhere: other banks
+                for (int i = 0; i < size; ++i) {
+                    const float rank = ranks[l * size + at];
+                    second = fmaxf(second, fminf(best, rank));
+                    best = fmaxf(best, rank);
+                    at = at + 1 == size ? 0 : at + 1;
+                }
+            }
+            const float strength = size > 1 ? best + second : best;
+            wave_fence();
+            if (l < p.groups) ranks[l] = strength;
+            wave_fence();
+            int before = 0;
+            for (int g = 0; g < p.groups; ++g) {
+                const float other = ranks[g];
+                before += other > strength;
+                again |= g != l && l < p.groups && !(fabsf(other - strength) > 2.0f * margin);
+            }
+            const uint64_t open = __ballot(l < p.groups && before < p.top_groups) >> (kLanes * r);
+            const uint32_t inverse_size = (65536 + size - 1) / size;  // e / size for e < 256
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t e = 64 * (i / 4) + 4 * l + i % 4;
+                if (!(open >> (e * inverse_size >> 16) & 1)) key[i] = 0;
+            }
+        }
+    }
+    int mine = 0;
+    float previous = 0.0f;
+    for (int j = 0; j <= p.top_k; ++j) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) best = max(best, key[i]);
+        best = row_max_key(best);
+        // The candidate after the last pick is only compared with it.
+        const float value = order_value(best);
+        if (j > 0 && best != 0) {
+            const float gap = previous - value;
+            if (!Exact) again |= !(gap > margin);
+            else again |= gap > 0.0f && !(gap * (p.sigmoid ? expf(-fmaxf(value, 0.0f)) : 1.0f) > 1e-12f);
+            if (Exact) again |= (p.sigmoid ? value : value - top) < -600.0f && j < p.top_k;
+        }
+        previous = value;
+        if (j == p.top_k) break;
+        int at = 1 << 30;
+#pragma unroll
+        for (int i = NV - 1; i >= 0; --i)
+            if (key[i] == best) at = 64 * (i / 4) + 4 * l + i % 4;
+        at = row_min(at);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at == 64 * (i / 4) + 4 * l + i % 4) key[i] = 0;
+        if (l == j) mine = at;
+    }
+    const bool picked = l < p.top_k;
+    const float score = picked ? score_of(row[min(mine, experts - 1)], p.sigmoid, top, inverse) : 0.0f;
+    const float total = row_sum(score);
+    again |= !(total > 0.0f);
+    if (picked && first + r < p.tokens) {
+        p.weights[t * p.top_k + l] = p.renormalise ? score / total : score;
+        p.chosen[t * p.top_k + l] = float(mine);
+    }
+    uint64_t rows = __ballot(again);
+    for (int i = 0; i < kRows; ++i)
+        if (rows >> (kLanes * i) & 0xFFFF && first + i < p.tokens) route_row<(NV + 3) / 4>(p, first + i, scratch[wave]);
+}
+
+__device__ inline int expert_of(float chosen, int experts) { return min(max(int(chosen), 0), experts - 1); }
+
+// Up to 256 experts and 64 picks. Renormalised weights and sigmoid scores leave
+// the other logits no gradient, so only the chosen ones are read:
+//   softmax: w_j (g_j - sum g w), w over the chosen alone;
+//   sigmoid: p_j (1 - p_j) (g_j - sum g w) / sum p, or p_j (1 - p_j) g_j;
+// Dense (a softmax as it is): s_e (g_e - sum g p) for every expert.
+template <int NV, bool Dense>
+__global__ __launch_bounds__(kWave* kWaves) void route_gradient_kernel(const float* __restrict__ logits,
+                                                                      const float* __restrict__ chosen,
+                                                                      const float* __restrict__ grad, int64_t tokens,
+                                                                      int experts, int top_k, bool sigmoid, bool renormalise,
+                                                                      float* __restrict__ out) {
+    __shared__ __align__(16) float lds[kWaves][kRows][kLanes * NV];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, l = lane % kLanes, r = lane / kLanes;
+    const int64_t t = (int64_t(blockIdx.x) * kWaves + wave) * kRows + r;
+    const bool live = t < tokens;
+    const float* const row = logits + (live ? t : 0) * experts;
+    const float* const picks = chosen + (live ? t : 0) * top_k;
+    const float* const g = grad + (live ? t : 0) * top_k;
+    float* const place = lds[wave][r];
+    f4u zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NV / 4; ++j) *reinterpret_cast<f4u*>(place + 64 * j + 4 * l) = zero;
+    float v[NV], top = -__builtin_huge_valf(), inverse = 1.0f;
+    if constexpr (Dense) {
+        row_logits<NV>(row, experts, l, v);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) top = fmaxf(top, v[i]);
+        top = row_max(top);
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i] = expf(v[i] - top);
+            total += v[i];
+        }
+        inverse = 1.0f / row_sum(total);
+    } else if (!sigmoid) {
+        for (int j = l; j < top_k; j += kLanes) top = fmaxf(top, row[expert_of(picks[j], experts)]);
+        top = row_max(top);
+    }
+    float total = 0.0f, dot = 0.0f;
+    for (int j = l; j < top_k; j += kLanes) {
+        const float p = score_of(row[expert_of(picks[j], experts)], sigmoid, top, inverse);
+        total += p;
+        dot += p * g[j];
+    }
+    total = row_sum(total);
+    dot = row_sum(dot);
+    wave_fence();
+    for (int j = l; j < top_k; j += kLanes) {
+        const int e = expert_of(picks[j], experts);
+        const float p = score_of(row[e], sigmoid, top, inverse);
+        float d = Dense || !renormalise ? g[j] : top_k == 1 ? 0.0f : g[j] - dot / total;  // one weight alone is always 1
+        if (!Dense) d *= renormalise ? (sigmoid ? p / total * (1.0f - p) : p / total) : p * (1.0f - p);
+        place[e] = d;
+    }
+    wave_fence();
+    if (!live) return;
+    float* const to = out + t * experts;
+#pragma unroll
+    for (int j = 0; j < NV / 4; ++j) {
+        const int e = 64 * j + 4 * l;
+        f4u d = *reinterpret_cast<const f4u*>(place + e);
+        if constexpr (Dense) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) d[c] = v[4 * j + c] * inverse * (d[c] - dot);
+        }
+        if (e + 4 <= experts) {
+            *reinterpret_cast<f4u*>(to + e) = d;
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (e + c < experts) to[e + c] = d[c];
+        }
     }
 }
 
 template <int NV>
-__global__ __launch_bounds__(kWave* kWaves) void route_backward_kernel(const float* __restrict__ logits,
+__global__ __launch_bounds__(kWave* kWaves) void route_gradient_wide_kernel(const float* __restrict__ logits,
                                                                       const float* __restrict__ chosen,
                                                                       const float* __restrict__ grad, size_t tokens,
                                                                       int experts, int top_k, bool sigmoid,
@@ -189,7 +477,7 @@ __global__ __launch_bounds__(kWave* kWaves) void route_backward_kernel(const flo
     row_scores<NV>(logits + t * experts, experts, lane, sigmoid, s);
 #pragma unroll
     for (int i = 0; i < NV; ++i) d[i] = 0.0;
-    const int at = lane < top_k ? int(chosen[t * top_k + lane]) : 0;
+    const int at = lane < top_k ? expert_of(chosen[t * top_k + lane], experts) : 0;
     const double g = lane < top_k ? double(grad[t * top_k + lane]) : 0.0;
     double total = 0.0, dot = 0.0;  // of the chosen scores, of their products with the gradients
     double p = 0.0;
@@ -231,15 +519,23 @@ void check_route(const char* name, size_t tokens, size_t experts, size_t top_k, 
     if (tokens > (size_t(1) << 31)) fail(VC_HIP_ERR_INVALID_ARGUMENT, std::string(name) + ": too many tokens");
 }
 
-// f(std::integral_constant<int, NV>) with NV values per lane for a row of experts.
+// f(std::integral_constant<int, NV>) with NV values per lane for a row of experts, of 64 or of 16 lanes.
 template <typename F>
-void with_row_width(size_t experts, F&& f) {
+void with_wide_rows(size_t experts, F&& f) {
     if (experts <= 64) f(std::integral_constant<int, 1>());
     else if (experts <= 128) f(std::integral_constant<int, 2>());
     else if (experts <= 256) f(std::integral_constant<int, 4>());
     else if (experts <= 512) f(std::integral_constant<int, 8>());
     else f(std::integral_constant<int, 16>());
 }
+template <typename F>
+void with_rows(size_t experts, F&& f) {
+    if (experts <= 64) f(std::integral_constant<int, 4>());
+    else if (experts <= 128) f(std::integral_constant<int, 8>());
+    else f(std::integral_constant<int, 16>());
+}
+
+dim3 row_grid(size_t tokens, int rows) { return dim3(unsigned((tokens + rows - 1) / rows)); }
 
 }  // namespace
 }  // namespace vchip
@@ -260,11 +556,17 @@ int vc_hip_route_forward(const float* logits, const float* bias, size_t tokens, 
         if (!logits || !weights || !chosen) fail(VC_HIP_ERR_INVALID_ARGUMENT, "route: null pointer");
         const double n = double(tokens) * experts, picks = double(tokens) * top_k;
         Profiled p("route", 6.0 * n, 4.0 * (n + 2.0 * picks));
-        with_row_width(experts, [&](auto nv) {
-            launch(route_kernel<nv()>, dim3(unsigned((tokens + kWaves - 1) / kWaves)), dim3(kWave * kWaves), 0, d.stream, logits,
-                   bias, tokens, int(experts), int(top_k), score == VC_HIP_SCORE_SIGMOID, int(groups), int(top_groups),
-                   renormalise != 0, weights, chosen);
-        });
+        const RouteArgs args{logits, bias, int64_t(tokens), int(experts), int(top_k), int(groups), int(top_groups),
+                             score == VC_HIP_SCORE_SIGMOID, renormalise != 0, weights, chosen};
+        const dim3 block(kWave * kWaves);
+        if (experts > 256 || top_k > size_t(kLanes) || groups > size_t(kLanes))
+            with_wide_rows(experts, [&](auto nv) { launch(route_wide_kernel<nv()>, row_grid(tokens, kWaves), block, 0, d.stream, args); });
+        else
+            with_rows(experts, [&](auto nv) {
+                const dim3 grid = row_grid(tokens, kWaves * kRows);
+                if (!bias && groups == 1) launch(route_kernel<nv(), true>, grid, block, 0, d.stream, args);
+                else launch(route_kernel<nv(), false>, grid, block, 0, d.stream, args);
+            });
         after_launch("route");
         p.done();
     });
@@ -280,11 +582,23 @@ int vc_hip_route_backward(const float* logits, const float* chosen, const float*
             fail(VC_HIP_ERR_INVALID_ARGUMENT, "route_backward: null pointer");
         const double n = double(tokens) * experts, picks = double(tokens) * top_k;
         Profiled p("route_backward", 6.0 * n, 4.0 * (2.0 * n + 2.0 * picks));
-        with_row_width(experts, [&](auto nv) {
-            launch(route_backward_kernel<nv()>, dim3(unsigned((tokens + kWaves - 1) / kWaves)), dim3(kWave * kWaves), 0,
-                   d.stream, logits, chosen, grad_weights, tokens, int(experts), int(top_k), score == VC_HIP_SCORE_SIGMOID,
-                   renormalise != 0, grad_logits);
-        });
+        const bool sigmoid = score == VC_HIP_SCORE_SIGMOID, renorm = renormalise != 0;
+        const dim3 block(kWave * kWaves);
+        if (experts > 256)
+            with_wide_rows(experts, [&](auto nv) {
+                launch(route_gradient_wide_kernel<nv()>, row_grid(tokens, kWaves), block, 0, d.stream, logits, chosen,
+                       grad_weights, tokens, int(experts), int(top_k), sigmoid, renorm, grad_logits);
+            });
+        else
+            with_rows(experts, [&](auto nv) {
+                const dim3 grid = row_grid(tokens, kWaves * kRows);
+                if (!sigmoid && !renorm)
+                    launch(route_gradient_kernel<nv(), true>, grid, block, 0, d.stream, logits, chosen, grad_weights,
+                           int64_t(tokens), int(experts), int(top_k), sigmoid, renorm, grad_logits);
+                else
+                    launch(route_gradient_kernel<nv(), false>, grid, block, 0, d.stream, logits, chosen, grad_weights,
+                           int64_t(tokens), int(experts), int(top_k), sigmoid, renorm, grad_logits);
+            });
         after_launch("route_backward");
         p.done();
     });
