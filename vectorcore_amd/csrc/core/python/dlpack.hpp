@@ -131,27 +131,46 @@ inline std::uint64_t own_stream() {
     return stream;
 }
 
+// What is called of torch, looked up once it is loaded; never freed, as the
+// interpreter may be gone before static objects are.
+struct Torch {
+    py::object tensor, to_dlpack, stream_of, current_stream;
+    static const Torch* loaded() {
+        static const Torch* known = nullptr;  // under the interpreter's lock
+        if (!known) {
+            const py::object torch = py::reinterpret_borrow<py::object>(PyImport_GetModuleDict()).attr("get")("torch", py::none());
+            if (torch.is_none() || !py::hasattr(torch, "utils") || !py::hasattr(torch, "cuda")) return nullptr;  // or half loaded
+            const py::object c = torch.attr("_C");
+            // The stream's handle itself where torch offers it: it costs a tenth of the stream object.
+            known = new Torch{torch.attr("Tensor"), torch.attr("utils").attr("dlpack").attr("to_dlpack"),
+                              py::getattr(c, "_cuda_getCurrentRawStream", py::none()), torch.attr("cuda").attr("current_stream")};
+        }
+        return known;
+    }
+    [[nodiscard]] std::uint64_t stream() const {
+        return (stream_of.is_none() ? current_stream().attr("cuda_stream") : stream_of(0)).cast<std::uint64_t>();
+    }
+};
+
 // Tensors over the memory of `objects`, which have __dlpack__. torch's are
 // exported without a wait of their own: they are all ordered by torch's current
 // stream, which is waited for once.
 inline py::tuple import_(const py::args& objects) {
-    const py::object torch = py::reinterpret_borrow<py::object>(PyImport_GetModuleDict())
-                                 .attr("get")("torch", py::none());
-    const py::object tensor_type = torch.is_none() ? py::object(py::none()) : py::object(torch.attr("Tensor"));
+    const Torch* const torch = Torch::loaded();
     bool waited = false;
     py::tuple out(objects.size());
     for (std::size_t i = 0; i < objects.size(); ++i) {
         const py::object object = objects[i];
         py::object capsule;
-        if (!tensor_type.is_none() && py::isinstance(object, tensor_type)) {
+        if (torch && py::isinstance(object, torch->tensor)) {
             if (object.attr("requires_grad").cast<bool>())
                 throw std::invalid_argument("from_dlpack: detach() a torch tensor that requires gradients");
             if (!waited && object.attr("is_cuda").cast<bool>()) {
                 waited = true;
                 require_one_runtime();
-                check(vc_hip_wait_for_stream(torch.attr("cuda").attr("current_stream")().attr("cuda_stream").cast<std::uint64_t>()));
+                check(vc_hip_wait_for_stream(torch->stream()));
             }
-            capsule = torch.attr("utils").attr("dlpack").attr("to_dlpack")(object);
+            capsule = torch->to_dlpack(object);
         } else {
             const py::tuple device = object.attr("__dlpack_device__")();
             capsule = device[0].cast<int>() == kRocm ? object.attr("__dlpack__")(py::arg("stream") = own_stream())
