@@ -218,38 +218,33 @@ __device__ inline float sigmoid(float x) {
     return (x >= 0.0f ? 1.0f : e) / (1.0f + e);
 }
 
-// Workgroups on a CU that registers and LDS have room for.
-constexpr int at_once(int columns) { return columns == 128 ? 3 : 2; }
-
 // C[r] = x_r @ w[group], or silu(x_r @ gate) * (x_r @ up): there a tile holds
-// half as many columns of both products, in turn 64 of each, so that a thread
-// holds both values of an element.
-template <bool Gated, int BN>
-__global__ __launch_bounds__(split::kThreads, at_once(BN)) void forward_kernel(ProductArgs p) {
-    __shared__ split::Slice<S, kTile> as;
-    __shared__ split::Slice<S, BN> bs;
-    constexpr int kColumns = Gated ? BN / 2 : BN;
+// 64 columns of both products, so that a thread holds both values of an element.
+template <bool Gated>
+__global__ __launch_bounds__(split::kThreads, 3) void forward_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, kTile> as, bs;
+    constexpr int kColumns = Gated ? kTile / 2 : kTile;
     const RowTile t = find_tile(p.offsets, p.experts + 1, (p.columns + kColumns - 1) / kColumns);
     if (!t.live) return;
     const int64_t n0 = t.column * kColumns;
-    split::Tile<S, kTile, BN> tile;
+    split::Tile<S, kTile, kTile> tile;
     tile.clear();
     const int64_t matrix = int64_t(t.group) * p.width * p.columns;
     const auto source = [&](int r) { return p.a + int64_t(p.token ? p.token[r] : r) * p.width; };
     if (t.group < p.experts) {
         split::AlongK<kTile> a;
-        split::AcrossK<BN> b;
+        split::AcrossK<kTile> b;
         const float* pa[a.kChunks];
         unsigned at[b.kChunks];
 #pragma unroll
         for (int j = 0; j < a.kChunks; ++j) pa[j] = source(min(t.begin + a.row(j), t.end - 1));
 #pragma unroll
         for (int j = 0; j < b.kChunks; ++j)
-            at[j] = unsigned(min(int64_t(Gated ? b.row(j / 2) : b.row(j)), p.columns - 1 - n0));
+            at[j] = unsigned(min(int64_t(Gated ? b.row(0) : b.row(j)), p.columns - 1 - n0));
         const float *const w = p.b + matrix + n0, *const w2 = Gated ? p.b2 + matrix + n0 : w;
         const auto line = [&](int64_t k) {
             const int64_t at_k = k * p.columns;
-            return [=](int j) { return (Gated && j % 2 ? w2 : w) + at_k; };
+            return [=](int j) { return (j ? w2 : w) + at_k; };
         };
         split::accumulate(
             tile, a, b, as, bs, p.width,
@@ -271,27 +266,24 @@ __global__ __launch_bounds__(split::kThreads, at_once(BN)) void forward_kernel(P
     };
     if constexpr (Gated) {
         const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        const int64_t col = n0 + wave % 2 * 32 + lane % 32;
+        if (col >= p.columns) return;
 #pragma unroll
-        for (int h = 0; h < tile.kN / 2; ++h) {
-            const int64_t col = n0 + 64 * h + wave % 2 * 32 + lane % 32;
-            if (col >= p.columns) continue;
+        for (int m = 0; m < tile.kM; ++m)
 #pragma unroll
-            for (int m = 0; m < tile.kM; ++m)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = t.begin + wave / 2 * 64 + 32 * m + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
-                    if (r >= t.end) continue;
-                    float g = tile.acc[m][2 * h][i], u = tile.acc[m][2 * h + 1][i];
-                    if (!split::finite(g)) g = again(p.b, r, col);
-                    if (!split::finite(u)) u = again(p.b2, r, col);
-                    const int64_t at = int64_t(r) * p.columns + col;
-                    p.c[at] = g * sigmoid(g) * u;
-                    if (p.c2) {
-                        p.c2[at] = g;
-                        p.c3[at] = u;
-                    }
+            for (int i = 0; i < 16; ++i) {
+                const int r = t.begin + wave / 2 * 64 + 32 * m + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
+                if (r >= t.end) continue;
+                float g = tile.acc[m][0][i], u = tile.acc[m][1][i];
+                if (!split::finite(g)) g = again(p.b, r, col);
+                if (!split::finite(u)) u = again(p.b2, r, col);
+                const int64_t at = int64_t(r) * p.columns + col;
+                p.c[at] = g * sigmoid(g) * u;
+                if (p.c2) {
+                    p.c2[at] = g;
+                    p.c3[at] = u;
                 }
-        }
+            }
     } else {
         tile.each([&](int m, int n, float v) {
             const int r = t.begin + m;
@@ -304,21 +296,18 @@ __global__ __launch_bounds__(split::kThreads, at_once(BN)) void forward_kernel(P
 }
 
 // C[r] = a[r] @ b[group]^T (+ a2[r] @ b2[group]^T).
-template <int BN>
-__global__ __launch_bounds__(split::kThreads, at_once(BN)) void input_kernel(ProductArgs p) {
-    __shared__ split::Slice<S, kTile> as;
-    __shared__ split::Slice<S, BN> bs;
-    const RowTile t = find_tile(p.offsets, p.experts + 1, (p.width + BN - 1) / BN);
+__global__ __launch_bounds__(split::kThreads, 3) void input_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, kTile> as, bs;
+    const RowTile t = find_tile(p.offsets, p.experts + 1, (p.width + kTile - 1) / kTile);
     if (!t.live) return;
-    const int64_t n0 = t.column * BN, matrix = int64_t(t.group) * p.width * p.columns;
-    split::Tile<S, kTile, BN> tile;
+    const int64_t n0 = t.column * kTile, matrix = int64_t(t.group) * p.width * p.columns;
+    split::Tile<S, kTile, kTile> tile;
     tile.clear();
     const int products = p.a2 ? 2 : 1;
     if (t.group < p.experts) {
         for (int product = 0; product < products; ++product) {
             const float *const from = product ? p.a2 : p.a, *const w = (product ? p.b2 : p.b) + matrix;
-            split::AlongK<kTile> a;
-            split::AlongK<BN> b;
+            split::AlongK<kTile> a, b;
             const float *pa[a.kChunks], *pb[b.kChunks];
 #pragma unroll
             for (int j = 0; j < a.kChunks; ++j) pa[j] = from + int64_t(min(t.begin + a.row(j), t.end - 1)) * p.columns;
@@ -355,7 +344,7 @@ __global__ __launch_bounds__(split::kThreads, at_once(BN)) void input_kernel(Pro
 // C[e] = sum over e's rows of x_r^T b[r]. Every die takes its part of each
 // expert's tiles, as experts differ in their rows.
 template <int BN>
-__global__ __launch_bounds__(split::kThreads, at_once(BN)) void weight_kernel(ProductArgs p) {
+__global__ __launch_bounds__(split::kThreads, BN == 128 ? 3 : 2) void weight_kernel(ProductArgs p) {
     __shared__ split::Slice<S, kTile> as;
     __shared__ split::Slice<S, BN> bs;
     const int64_t row_tiles = (p.width + kTile - 1) / kTile, column_tiles = (p.columns + BN - 1) / BN;
@@ -581,14 +570,6 @@ dim3 tile_grid(int64_t tiles) {
 }
 int64_t row_tiles_at_most(const Plan& plan) { return int64_t(plan.rows / kTile + plan.experts + 1); }
 
-// 256 columns a tile split the rows' operand half as often for the same
-// products; they need enough tiles for the chip.
-template <class F>
-void with_columns(Device& d, int64_t row_tiles, size_t columns, F&& f) {
-    if (row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) f(std::integral_constant<int, 256>());
-    else f(std::integral_constant<int, 128>());
-}
-
 // (A lane's place in kThinDepth lines is a 32-bit offset.)
 bool thin(const Plan& plan, size_t columns) { return plan.rows <= kThinMost * plan.experts && columns <= size_t(1) << 20; }
 
@@ -720,10 +701,9 @@ int vc_hip_expert_linear_forward(const float* x, const float* w, const vc_hip_ex
         const ProductArgs args{x, w, nullptr, nullptr, out, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
                                int(q.experts), int64_t(width), int64_t(columns)};
         if (thin(q, columns)) launch_thin<false>(d, q, args);
-        else with_columns(d, int64_t(q.rows / kTile), columns, [&](auto bn) {
-            launch(forward_kernel<false, bn()>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, bn())), dim3(split::kThreads),
-                   0, d.stream, args);
-        });
+        else
+            launch(forward_kernel<false>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, kTile)), dim3(split::kThreads), 0,
+                   d.stream, args);
         after_launch("expert_linear");
         p.done();
     });
@@ -742,10 +722,9 @@ int vc_hip_expert_gated_forward(const float* x, const float* gate, const float* 
         const ProductArgs args{x, gate, nullptr, up, out, save_gate, save_up, q.offsets, ordered ? nullptr : q.token,
                                int(q.experts), int64_t(width), int64_t(columns)};
         if (thin(q, columns)) launch_thin<true>(d, q, args);
-        else with_columns(d, int64_t(q.rows / kTile), 2 * columns, [&](auto bn) {
-            launch(forward_kernel<true, bn()>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, bn() / 2)),
-                   dim3(split::kThreads), 0, d.stream, args);
-        });
+        else
+            launch(forward_kernel<true>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, kTile / 2)), dim3(split::kThreads), 0,
+                   d.stream, args);
         after_launch("expert_gated");
         p.done();
     });
@@ -779,10 +758,7 @@ int vc_hip_expert_linear_backward_input(const float* grad, const float* w, const
                    4.0 * (q.rows * (width + products * columns) + products * q.experts * width * columns));
         const ProductArgs args{grad, w, grad2, w2, grad_rows, nullptr, nullptr, q.offsets, nullptr, int(q.experts),
                                int64_t(width), int64_t(columns)};
-        with_columns(d, int64_t(q.rows / kTile), width, [&](auto bn) {
-            launch(input_kernel<bn()>, tile_grid(row_tiles_at_most(q) * tiles_of(width, bn())), dim3(split::kThreads), 0,
-                   d.stream, args);
-        });
+        launch(input_kernel, tile_grid(row_tiles_at_most(q) * tiles_of(width, kTile)), dim3(split::kThreads), 0, d.stream, args);
         after_launch("expert_backward_input");
         p.done();
     });
@@ -799,11 +775,15 @@ int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, cons
                    4.0 * (q.rows * (width + columns) + q.experts * width * columns));
         const ProductArgs args{x, grad, nullptr, nullptr, grad_w, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
                                int(q.experts), int64_t(width), int64_t(columns)};
+        // 256 columns a tile where they fill the chip: x is then split half as often. (8 experts, 1024 x 4096 over 16384
+        // rows: 809 us, with 128 columns 935. The products of rows gain nothing, as fewer tiles fit the CUs less evenly.)
         const int64_t row_tiles = tiles_of(width, kTile);
-        with_columns(d, int64_t(q.experts) * row_tiles, columns, [&](auto bn) {
+        const auto run = [&](auto bn) {
             const int64_t share = tiles_of(row_tiles * tiles_of(columns, bn()), 8);
             launch(weight_kernel<bn()>, tile_grid(int64_t(q.experts) * share * 8), dim3(split::kThreads), 0, d.stream, args);
-        });
+        };
+        if (int64_t(q.experts) * row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) run(std::integral_constant<int, 256>());
+        else run(std::integral_constant<int, 128>());
         after_launch("expert_backward_weight");
         p.done();
     });
