@@ -143,9 +143,8 @@ Plan plan_of(const vc_hip_expert_plan* plan) {
 }
 
 // ---- products -----------------------------------------------------------------------
-// Tiles of 128 rows of one group by 128 or 256 columns (split_product.hpp).
+// Tiles of 64 or 128 rows of one group (split_product.hpp).
 
-constexpr int kTile = 128;
 using S = split::Bf16x3;
 
 struct ProductArgs {
@@ -197,12 +196,13 @@ __device__ inline RowTile find_rows(const int* __restrict__ offsets, int groups,
 // together, and dealt out so that each of the chip's eight dies (workgroups go
 // to them in turn) works on neighbouring ones, which read the same operands
 // through its cache.
+template <int BM>
 __device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups, int64_t column_tiles) {
     const int lane = threadIdx.x % kWave;
     int all = 0;
     for (int base = 0; base < groups; base += kWave) {
         const int e = base + lane;
-        const int n = e < groups ? (offsets[e + 1] - offsets[e] + kTile - 1) / kTile : 0;
+        const int n = e < groups ? (offsets[e + 1] - offsets[e] + BM - 1) / BM : 0;
         int sum = n;
         for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
         all += sum;
@@ -210,7 +210,7 @@ __device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups,
     const int64_t total = all * column_tiles, share = (total + 7) / 8;
     const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8;
     if (blockIdx.x / 8 >= share || id >= total) return RowTile{0, 0, 0, 0, false};
-    return find_rows<kTile>(offsets, groups, int(id / column_tiles), id % column_tiles);
+    return find_rows<BM>(offsets, groups, int(id / column_tiles), id % column_tiles);
 }
 
 __device__ inline float sigmoid(float x) {
@@ -218,41 +218,46 @@ __device__ inline float sigmoid(float x) {
     return (x >= 0.0f ? 1.0f : e) / (1.0f + e);
 }
 
+// Workgroups on a CU, and slices on their way, of tiles of `rows` rows.
+constexpr int at_once(int rows) { return rows == 128 ? 3 : 2; }
+constexpr int ahead(int rows) { return rows == 128 ? 1 : 3; }
+
 // C[r] = x_r @ w[group], or silu(x_r @ gate) * (x_r @ up): there a tile holds
 // 64 columns of both products, so that a thread holds both values of an element.
-template <bool Gated>
-__global__ __launch_bounds__(split::kThreads, 3) void forward_kernel(ProductArgs p) {
-    __shared__ split::Slice<S, kTile> as, bs;
-    constexpr int kColumns = Gated ? kTile / 2 : kTile;
-    const RowTile t = find_tile(p.offsets, p.experts + 1, (p.columns + kColumns - 1) / kColumns);
+template <bool Gated, int BM>
+__global__ __launch_bounds__(split::kThreads, at_once(BM)) void forward_kernel(ProductArgs p) {
+    constexpr int BN = Gated ? 128 : BM, kColumns = Gated ? BN / 2 : BN;
+    __shared__ split::Slice<S, BM> as;
+    __shared__ split::Slice<S, BN> bs;
+    const RowTile t = find_tile<BM>(p.offsets, p.experts + 1, (p.columns + kColumns - 1) / kColumns);
     if (!t.live) return;
     const int64_t n0 = t.column * kColumns;
-    split::Tile<S, kTile, kTile> tile;
+    split::Tile<S, BM, BN> tile;
     tile.clear();
     const int64_t matrix = int64_t(t.group) * p.width * p.columns;
     const auto source = [&](int r) { return p.a + int64_t(p.token ? p.token[r] : r) * p.width; };
     if (t.group < p.experts) {
-        split::AlongK<kTile> a;
-        split::AcrossK<kTile> b;
-        const float* pa[a.kChunks];
-        unsigned at[b.kChunks];
+        using A = split::AlongK<BM>;
+        using B = split::AcrossK<BN>;
+        const float* pa[A::kChunks];
+        unsigned at[B::kChunks];
 #pragma unroll
-        for (int j = 0; j < a.kChunks; ++j) pa[j] = source(min(t.begin + a.row(j), t.end - 1));
+        for (int j = 0; j < A::kChunks; ++j) pa[j] = source(min(t.begin + A::row(j), t.end - 1));
 #pragma unroll
-        for (int j = 0; j < b.kChunks; ++j)
-            at[j] = unsigned(min(int64_t(Gated ? b.row(0) : b.row(j)), p.columns - 1 - n0));
+        for (int j = 0; j < B::kChunks; ++j)
+            at[j] = unsigned(min(int64_t(Gated ? B::row(0) : B::row(j)), p.columns - 1 - n0));
         const float *const w = p.b + matrix + n0, *const w2 = Gated ? p.b2 + matrix + n0 : w;
         const auto line = [&](int64_t k) {
             const int64_t at_k = k * p.columns;
             return [=](int j) { return (j ? w2 : w) + at_k; };
         };
-        split::accumulate(
-            tile, a, b, as, bs, p.width,
-            [&](int64_t k) {
+        split::accumulate<ahead(BM), A, B>(
+            tile, as, bs, p.width,
+            [&](A& a, B& b, int64_t k) {
                 a.load(pa, k);
                 b.load(at, k, line);
             },
-            [&](int64_t k) {
+            [&](A& a, B& b, int64_t k) {
                 a.load_rest(pa, k, p.width);
                 b.load_rest(at, k, p.width, line);
             });
@@ -272,7 +277,7 @@ __global__ __launch_bounds__(split::kThreads, 3) void forward_kernel(ProductArgs
         for (int m = 0; m < tile.kM; ++m)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int r = t.begin + wave / 2 * 64 + 32 * m + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
+                const int r = t.begin + wave / 2 * (BM / 2) + 32 * m + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
                 if (r >= t.end) continue;
                 float g = tile.acc[m][0][i], u = tile.acc[m][1][i];
                 if (!split::finite(g)) g = again(p.b, r, col);
@@ -296,30 +301,31 @@ __global__ __launch_bounds__(split::kThreads, 3) void forward_kernel(ProductArgs
 }
 
 // C[r] = a[r] @ b[group]^T (+ a2[r] @ b2[group]^T).
-__global__ __launch_bounds__(split::kThreads, 3) void input_kernel(ProductArgs p) {
-    __shared__ split::Slice<S, kTile> as, bs;
-    const RowTile t = find_tile(p.offsets, p.experts + 1, (p.width + kTile - 1) / kTile);
+template <int BM>
+__global__ __launch_bounds__(split::kThreads, at_once(BM)) void input_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, BM> as, bs;
+    const RowTile t = find_tile<BM>(p.offsets, p.experts + 1, (p.width + BM - 1) / BM);
     if (!t.live) return;
-    const int64_t n0 = t.column * kTile, matrix = int64_t(t.group) * p.width * p.columns;
-    split::Tile<S, kTile, kTile> tile;
+    const int64_t n0 = t.column * BM, matrix = int64_t(t.group) * p.width * p.columns;
+    split::Tile<S, BM, BM> tile;
     tile.clear();
     const int products = p.a2 ? 2 : 1;
     if (t.group < p.experts) {
         for (int product = 0; product < products; ++product) {
             const float *const from = product ? p.a2 : p.a, *const w = (product ? p.b2 : p.b) + matrix;
-            split::AlongK<kTile> a, b;
-            const float *pa[a.kChunks], *pb[b.kChunks];
+            using A = split::AlongK<BM>;
+            const float *pa[A::kChunks], *pb[A::kChunks];
 #pragma unroll
-            for (int j = 0; j < a.kChunks; ++j) pa[j] = from + int64_t(min(t.begin + a.row(j), t.end - 1)) * p.columns;
+            for (int j = 0; j < A::kChunks; ++j) pa[j] = from + int64_t(min(t.begin + A::row(j), t.end - 1)) * p.columns;
 #pragma unroll
-            for (int j = 0; j < b.kChunks; ++j) pb[j] = w + min(n0 + b.row(j), p.width - 1) * p.columns;
-            split::accumulate(
-                tile, a, b, as, bs, p.columns,
-                [&](int64_t k) {
+            for (int j = 0; j < A::kChunks; ++j) pb[j] = w + min(n0 + A::row(j), p.width - 1) * p.columns;
+            split::accumulate<ahead(BM), A, A>(
+                tile, as, bs, p.columns,
+                [&](A& a, A& b, int64_t k) {
                     a.load(pa, k);
                     b.load(pb, k);
                 },
-                [&](int64_t k) {
+                [&](A& a, A& b, int64_t k) {
                     a.load_rest(pa, k, p.columns);
                     b.load_rest(pb, k, p.columns);
                 });
@@ -343,27 +349,27 @@ __global__ __launch_bounds__(split::kThreads, 3) void input_kernel(ProductArgs p
 
 // C[e] = sum over e's rows of x_r^T b[r]. Every die takes its part of each
 // expert's tiles, as experts differ in their rows.
-template <int BN>
-__global__ __launch_bounds__(split::kThreads, BN == 128 ? 3 : 2) void weight_kernel(ProductArgs p) {
-    __shared__ split::Slice<S, kTile> as;
+template <int BM, int BN>
+__global__ __launch_bounds__(split::kThreads, BN == 256 ? 2 : at_once(BM)) void weight_kernel(ProductArgs p) {
+    __shared__ split::Slice<S, BM> as;
     __shared__ split::Slice<S, BN> bs;
-    const int64_t row_tiles = (p.width + kTile - 1) / kTile, column_tiles = (p.columns + BN - 1) / BN;
+    const int64_t row_tiles = (p.width + BM - 1) / BM, column_tiles = (p.columns + BN - 1) / BN;
     const int64_t total = row_tiles * column_tiles, share = (total + 7) / 8;
     const int group = int(blockIdx.x / 8 / share);
     const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8 % share;
     if (id >= total) return;
-    const int64_t m0 = id / column_tiles * kTile, n0 = id % column_tiles * BN;
+    const int64_t m0 = id / column_tiles * BM, n0 = id % column_tiles * BN;
     const int begin = p.offsets[group], depth = p.offsets[group + 1] - begin;
     const auto source = [&](int64_t r) { return int64_t(p.token ? p.token[r] : r) * p.width; };
-    split::Tile<S, kTile, BN> tile;
+    split::Tile<S, BM, BN> tile;
     tile.clear();
-    split::AcrossK<kTile> a;
-    split::AcrossK<BN> b;
-    unsigned at_a[a.kChunks], at_b[b.kChunks];
+    using A = split::AcrossK<BM>;
+    using B = split::AcrossK<BN>;
+    unsigned at_a[A::kChunks], at_b[B::kChunks];
 #pragma unroll
-    for (int j = 0; j < a.kChunks; ++j) at_a[j] = unsigned(min(int64_t(a.row(j)), p.width - 1 - m0));
+    for (int j = 0; j < A::kChunks; ++j) at_a[j] = unsigned(min(int64_t(A::row(j)), p.width - 1 - m0));
 #pragma unroll
-    for (int j = 0; j < b.kChunks; ++j) at_b[j] = unsigned(min(int64_t(b.row(j)), p.columns - 1 - n0));
+    for (int j = 0; j < B::kChunks; ++j) at_b[j] = unsigned(min(int64_t(B::row(j)), p.columns - 1 - n0));
     const auto line_a = [&](int64_t k) {
         const float* const line = p.a + m0 + source(begin + k);
         return [=](int) { return line; };
@@ -372,13 +378,13 @@ __global__ __launch_bounds__(split::kThreads, BN == 128 ? 3 : 2) void weight_ker
         const float* const line = p.b + n0 + (begin + k) * p.columns;
         return [=](int) { return line; };
     };
-    split::accumulate(
-        tile, a, b, as, bs, depth,
-        [&](int64_t k) {
+    split::accumulate<ahead(BM), A, B>(
+        tile, as, bs, depth,
+        [&](A& a, B& b, int64_t k) {
             a.load(at_a, k, line_a);
             b.load(at_b, k, line_b);
         },
-        [&](int64_t k) {
+        [&](A& a, B& b, int64_t k) {
             a.load_rest(at_a, k, depth, line_a);
             b.load_rest(at_b, k, depth, line_b);
         });
@@ -568,7 +574,15 @@ dim3 tile_grid(int64_t tiles) {
     if (blocks >= int64_t(1) << 31) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
     return dim3(unsigned(blocks));
 }
-int64_t row_tiles_at_most(const Plan& plan) { return int64_t(plan.rows / kTile + plan.experts + 1); }
+// Row tiles by column tiles at most.
+int64_t tiles_at_most(const Plan& plan, int rows, size_t width, int columns) {
+    return int64_t(plan.rows / rows + plan.experts + 1) * tiles_of(width, columns);
+}
+
+// Whether tiles of 128 rows give every CU one; otherwise tiles of 64 halve or
+// quarter what each of them computes (THIN64).
+bool enough(Device& d, int64_t tiles) { return tiles >= d.cu_count; }
+
 
 // (A lane's place in kThinDepth lines is a 32-bit offset.)
 bool thin(const Plan& plan, size_t columns) { return plan.rows <= kThinMost * plan.experts && columns <= size_t(1) << 20; }
@@ -700,10 +714,13 @@ int vc_hip_expert_linear_forward(const float* x, const float* w, const vc_hip_ex
         Profiled p("expert_linear", 2.0 * q.rows * width * columns, 4.0 * (q.rows * (width + columns) + q.experts * width * columns));
         const ProductArgs args{x, w, nullptr, nullptr, out, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
                                int(q.experts), int64_t(width), int64_t(columns)};
-        if (thin(q, columns)) launch_thin<false>(d, q, args);
+        const dim3 threads(split::kThreads);
+        if (thin(q, columns))
+            launch_thin<false>(d, q, args);
+        else if (enough(d, int64_t(q.rows / 128) * tiles_of(columns, 128)))
+            launch(forward_kernel<false, 128>, tile_grid(tiles_at_most(q, 128, columns, 128)), threads, 0, d.stream, args);
         else
-            launch(forward_kernel<false>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, kTile)), dim3(split::kThreads), 0,
-                   d.stream, args);
+            launch(forward_kernel<false, 64>, tile_grid(tiles_at_most(q, 64, columns, 64)), threads, 0, d.stream, args);
         after_launch("expert_linear");
         p.done();
     });
@@ -721,10 +738,13 @@ int vc_hip_expert_gated_forward(const float* x, const float* gate, const float* 
                    4.0 * (q.rows * (width + (save_gate ? 3.0 : 1.0) * columns) + 2.0 * q.experts * width * columns));
         const ProductArgs args{x, gate, nullptr, up, out, save_gate, save_up, q.offsets, ordered ? nullptr : q.token,
                                int(q.experts), int64_t(width), int64_t(columns)};
-        if (thin(q, columns)) launch_thin<true>(d, q, args);
+        const dim3 threads(split::kThreads);
+        if (thin(q, columns))
+            launch_thin<true>(d, q, args);
+        else if (enough(d, int64_t(q.rows / 128) * tiles_of(columns, 64)))
+            launch(forward_kernel<true, 128>, tile_grid(tiles_at_most(q, 128, columns, 64)), threads, 0, d.stream, args);
         else
-            launch(forward_kernel<true>, tile_grid(row_tiles_at_most(q) * tiles_of(columns, kTile / 2)), dim3(split::kThreads), 0,
-                   d.stream, args);
+            launch(forward_kernel<true, 64>, tile_grid(tiles_at_most(q, 64, columns, 64)), threads, 0, d.stream, args);
         after_launch("expert_gated");
         p.done();
     });
@@ -758,7 +778,11 @@ int vc_hip_expert_linear_backward_input(const float* grad, const float* w, const
                    4.0 * (q.rows * (width + products * columns) + products * q.experts * width * columns));
         const ProductArgs args{grad, w, grad2, w2, grad_rows, nullptr, nullptr, q.offsets, nullptr, int(q.experts),
                                int64_t(width), int64_t(columns)};
-        launch(input_kernel, tile_grid(row_tiles_at_most(q) * tiles_of(width, kTile)), dim3(split::kThreads), 0, d.stream, args);
+        const dim3 threads(split::kThreads);
+        if (enough(d, int64_t(q.rows / 128) * tiles_of(width, 128)))
+            launch(input_kernel<128>, tile_grid(tiles_at_most(q, 128, width, 128)), threads, 0, d.stream, args);
+        else
+            launch(input_kernel<64>, tile_grid(tiles_at_most(q, 64, width, 64)), threads, 0, d.stream, args);
         after_launch("expert_backward_input");
         p.done();
     });
@@ -777,13 +801,15 @@ int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, cons
                                int(q.experts), int64_t(width), int64_t(columns)};
         // 256 columns a tile where they fill the chip: x is then split half as often. (8 experts, 1024 x 4096 over 16384
         // rows: 809 us, with 128 columns 935. The products of rows gain nothing, as fewer tiles fit the CUs less evenly.)
-        const int64_t row_tiles = tiles_of(width, kTile);
-        const auto run = [&](auto bn) {
-            const int64_t share = tiles_of(row_tiles * tiles_of(columns, bn()), 8);
-            launch(weight_kernel<bn()>, tile_grid(int64_t(q.experts) * share * 8), dim3(split::kThreads), 0, d.stream, args);
+        const auto run = [&](auto bm, auto bn) {
+            const int64_t share = tiles_of(size_t(tiles_of(width, bm()) * tiles_of(columns, bn())), 8);
+            launch(weight_kernel<bm(), bn()>, tile_grid(int64_t(q.experts) * share * 8), dim3(split::kThreads), 0, d.stream, args);
         };
-        if (int64_t(q.experts) * row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) run(std::integral_constant<int, 256>());
-        else run(std::integral_constant<int, 128>());
+        using std::integral_constant;
+        const int64_t row_tiles = int64_t(q.experts) * tiles_of(width, 128);
+        if (row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) run(integral_constant<int, 128>(), integral_constant<int, 256>());
+        else if (enough(d, row_tiles * tiles_of(columns, 128))) run(integral_constant<int, 128>(), integral_constant<int, 128>());
+        else run(integral_constant<int, 64>(), integral_constant<int, 64>());
         after_launch("expert_backward_weight");
         p.done();
     });

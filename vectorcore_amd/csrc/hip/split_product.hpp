@@ -216,25 +216,54 @@ struct Tile {
     }
 };
 
-// The products of k < depth onto a tile: a slice is loaded into registers while
-// the one before it is multiplied. load(k) reads a whole slice, rest(k) the last
-// one, of which depth % 32 are there.
-template <class T, class A, class B, class SA, class SB, class Load, class Rest>
-__device__ inline void accumulate(T& tile, A& a, B& b, SA& as, SB& bs, int64_t depth, Load&& load, Rest&& rest) {
-    const auto next = [&](int64_t k) {
-        if (k + kSliceK <= depth) load(k);
-        else rest(k);
-    };
-    if (depth <= 0) return;
-    next(int64_t(0));
-    for (int64_t k = 0; k < depth; k += kSliceK) {
-        a.store(as);
-        b.store(bs);
+// The products of k < depth onto a tile. load(a, b, k) reads a whole slice,
+// rest(a, b, k) the last one, of which depth % 32 are there. Ahead register sets
+// hold slices that are on their way: one where other workgroups of the CU hide
+// the wait, more for grids that leave a CU one or two.
+template <int Ahead, class A, class B, class T, class SA, class SB, class Load, class Rest>
+__device__ inline void accumulate(T& tile, SA& as, SB& bs, int64_t depth, Load&& load, Rest&& rest) {
+    A a[Ahead];
+    B b[Ahead];
+    const auto multiply = [&](const A& x, const B& y, auto&& next) {
+        x.store(as);
+        y.store(bs);
         __syncthreads();
-        if (k + kSliceK < depth) next(k + kSliceK);
+        next();
         tile.multiply(as, bs, 0);
         tile.multiply(as, bs, 2);
         __syncthreads();
+    };
+    if constexpr (Ahead == 1) {
+        const auto next = [&](int64_t k) {
+            if (k + kSliceK <= depth) load(a[0], b[0], k);
+            else rest(a[0], b[0], k);
+        };
+        if (depth <= 0) return;
+        next(int64_t(0));
+        for (int64_t k = 0; k < depth; k += kSliceK)
+            multiply(a[0], b[0], [&] {
+                if (k + kSliceK < depth) next(k + kSliceK);
+            });
+    } else {
+        const int full = int(depth / kSliceK);
+        // Always the same number of loads on their way (past the end the last slice is read again), so that the compiler
+        // waits for just those it needs.
+        const auto at = [&](int s) { return int64_t(min(s, full - 1)) * kSliceK; };
+        if (full > 0) {
+#pragma unroll
+            for (int i = 0; i < Ahead; ++i) load(a[i], b[i], at(i));
+        }
+        for (int s = 0; s < full; s += Ahead) {
+#pragma unroll
+            for (int i = 0; i < Ahead; ++i) {
+                if (s + i >= full) break;
+                multiply(a[i], b[i], [&] { load(a[i], b[i], at(s + i + Ahead)); });
+            }
+        }
+        if (int64_t(full) * kSliceK < depth) {
+            rest(a[0], b[0], int64_t(full) * kSliceK);
+            multiply(a[0], b[0], [] {});
+        }
     }
 }
 
