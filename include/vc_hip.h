@@ -546,9 +546,11 @@ int vc_hip_expert_gated_backward(const float* grad, const float* saved_gate, con
 /* grad_rows[r] = grad[r] @ w[e]^T (+ grad2[r] @ w2[e]^T unless both are NULL), [rows, width]. */
 int vc_hip_expert_linear_backward_input(const float* grad, const float* w, const float* grad2, const float* w2,
                                         const vc_hip_expert_plan* plan, size_t width, size_t columns, float* grad_rows);
-/* grad_w[e] = sum over e's rows of x_r^T grad[r], zero for an expert without rows. */
-int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, const vc_hip_expert_plan* plan, size_t width,
-                                         size_t columns, int ordered, float* grad_w);
+/* grad_w[e] = sum over e's rows of x_r^T grad[r], zero for an expert without rows; likewise grad_w2 from grad2, unless
+ * both are NULL. */
+int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, const float* grad2,
+                                         const vc_hip_expert_plan* plan, size_t width, size_t columns, int ordered,
+                                         float* grad_w, float* grad_w2);
 /* out[t] = sum over t's picks of weights[pick] * rows[place], in pick order; weights NULL: all one. Dropped picks add
  * nothing. */
 int vc_hip_expert_combine_forward(const float* rows, const float* weights, const vc_hip_expert_plan* plan, size_t width,

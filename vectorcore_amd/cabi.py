@@ -168,7 +168,7 @@ _SIGNATURES = {
     "vc_hip_expert_gated_forward": ([_vp, _vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _sz, _i, _vp, _vp, _vp], _i),
     "vc_hip_expert_gated_backward": ([_vp, _vp, _vp, _sz, _vp, _vp], _i),
     "vc_hip_expert_linear_backward_input": ([_vp, _vp, _vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _sz, _vp], _i),
-    "vc_hip_expert_linear_backward_weight": ([_vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _sz, _i, _vp], _i),
+    "vc_hip_expert_linear_backward_weight": ([_vp, _vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _sz, _i, _vp, _vp], _i),
     "vc_hip_expert_combine_forward": ([_vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _vp], _i),
     "vc_hip_expert_combine_backward": ([_vp, _vp, _vp, ctypes.POINTER(ExpertPlan), _sz, _vp, _vp], _i),
     "vc_hip_orthogonalise": ([_vp, _sz, _sz, _sz, _sz, _vp], _i),

@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <utility>
 
 namespace vectorcore {
@@ -103,16 +104,25 @@ Tensor input_gradient(const Tensor& g, const Tensor& w, const Tensor* g2, const 
     return ordered ? rows : sum_rows(rows, nullptr, plan, width);
 }
 
-Tensor weight_gradient(const Tensor& x, const Tensor& g, const ExpertPlan& plan, std::size_t width, std::size_t columns,
-                       bool ordered) {
-    std::shared_ptr<Storage> out;
+// Of one or two matrices (g2 null: one) that multiply the same x.
+std::pair<Tensor, Tensor> weight_gradients(const Tensor& x, const Tensor& g, const Tensor* g2, const ExpertPlan& plan,
+                                           std::size_t width, std::size_t columns, bool ordered) {
+    std::shared_ptr<Storage> out, out2;
+    const std::size_t count = plan.experts() * width * columns;
     if (on_hip(g)) {
-        out = hip().expert_linear_backward_weight(st(x), off(x), st(g), off(g), device_rows(plan), width, columns, ordered);
+        std::tie(out, out2) = hip().expert_linear_backward_weight(st(x), off(x), st(g), off(g), g2 ? &st(*g2) : nullptr,
+                                                                  g2 ? off(*g2) : 0, device_rows(plan), width, columns, ordered);
     } else {
-        out = make_cpu_storage(plan.experts() * width * columns);
+        out = make_cpu_storage(count);
         cpu::expert_linear_backward_weight(x.data(), g.data(), host_rows(plan), width, columns, ordered, out->mutable_data());
+        if (g2) {
+            out2 = make_cpu_storage(count);
+            cpu::expert_linear_backward_weight(x.data(), g2->data(), host_rows(plan), width, columns, ordered, out2->mutable_data());
+        }
     }
-    return detail::make_tensor(std::move(out), {plan.experts(), width, columns}, false);
+    const Shape shape{plan.experts(), width, columns};
+    Tensor first = detail::make_tensor(std::move(out), shape, false);
+    return {first, out2 ? detail::make_tensor(std::move(out2), shape, false) : first};
 }
 
 }  // namespace
@@ -189,7 +199,7 @@ Tensor expert_linear(const Tensor& x, const Tensor& weight, const ExpertPlan& pl
         std::vector<Tensor> grads{Tensor(), Tensor()};
         const Tensor xv = sx.unpack(), wv = sw.unpack();
         if (nx) grads[0] = input_gradient(g, wv, nullptr, nullptr, plan, width, columns, ordered);
-        if (nw) grads[1] = weight_gradient(xv, g, plan, width, columns, ordered);
+        if (nw) grads[1] = weight_gradients(xv, g, nullptr, plan, width, columns, ordered).first;
         return grads;
     });
     return out;
@@ -231,8 +241,7 @@ Tensor expert_gated(const Tensor& x, const Tensor& gate, const Tensor& up, const
         const Tensor dgt = detail::make_tensor(std::move(dg), {rows, columns}, false);
         const Tensor dut = detail::make_tensor(std::move(du), {rows, columns}, false);
         if (nx) grads[0] = input_gradient(dgt, gv, &dut, &uv, plan, width, columns, ordered);
-        if (ng) grads[1] = weight_gradient(xv, dgt, plan, width, columns, ordered);
-        if (nu) grads[2] = weight_gradient(xv, dut, plan, width, columns, ordered);
+        if (ng || nu) std::tie(grads[1], grads[2]) = weight_gradients(xv, ng ? dgt : dut, ng && nu ? &dut : nullptr, plan, width, columns, ordered);
         return grads;
     });
     return result;

@@ -1657,16 +1657,19 @@ std::shared_ptr<Storage> HipBackend::expert_linear_backward_input(const Storage&
     return out;
 }
 
-std::shared_ptr<Storage> HipBackend::expert_linear_backward_weight(const Storage& x, std::size_t x_offset, const Storage& grad,
-                                                                   std::size_t grad_offset, const ExpertRows& plan,
-                                                                   std::size_t width, std::size_t columns, bool ordered) {
+std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> HipBackend::expert_linear_backward_weight(
+    const Storage& x, std::size_t x_offset, const Storage& grad, std::size_t grad_offset, const Storage* grad2,
+    std::size_t grad2_offset, const ExpertRows& plan, std::size_t width, std::size_t columns, bool ordered) {
     require(*this);
-    auto out = fresh(plan.experts * width * columns);
+    const std::size_t count = plan.experts * width * columns;
+    auto out = fresh(count);
+    std::shared_ptr<HipStorage> out2 = grad2 ? fresh(count) : nullptr;
     const auto rows = abi(plan);
-    check(vc_hip_expert_linear_backward_weight(dptr(x, x_offset), dptr(grad, grad_offset), &rows, width, columns, ordered,
-                                               out->ptr()),
+    check(vc_hip_expert_linear_backward_weight(dptr(x, x_offset), dptr(grad, grad_offset),
+                                               grad2 ? dptr(*grad2, grad2_offset) : nullptr, &rows, width, columns, ordered,
+                                               out->ptr(), out2 ? out2->ptr() : nullptr),
           "HIP expert product backward failed");
-    return out;
+    return {out, out2};
 }
 
 std::shared_ptr<Storage> HipBackend::expert_combine_forward(const Storage& rows, std::size_t rows_offset,

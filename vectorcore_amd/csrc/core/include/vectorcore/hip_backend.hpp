@@ -250,10 +250,10 @@ public:
                                                                         const Storage* w2, std::size_t w2_offset,
                                                                         const ExpertRows& plan, std::size_t width,
                                                                         std::size_t columns);
-    [[nodiscard]] std::shared_ptr<Storage> expert_linear_backward_weight(const Storage& x, std::size_t x_offset,
-                                                                         const Storage& grad, std::size_t grad_offset,
-                                                                         const ExpertRows& plan, std::size_t width,
-                                                                         std::size_t columns, bool ordered);
+    // Of one or two matrices (grad2 null: one) that multiply the same x.
+    [[nodiscard]] std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> expert_linear_backward_weight(
+        const Storage& x, std::size_t x_offset, const Storage& grad, std::size_t grad_offset, const Storage* grad2,
+        std::size_t grad2_offset, const ExpertRows& plan, std::size_t width, std::size_t columns, bool ordered);
     [[nodiscard]] std::shared_ptr<Storage> expert_combine_forward(const Storage& rows, std::size_t rows_offset,
                                                                   const Storage* weights, std::size_t weights_offset,
                                                                   const ExpertRows& plan, std::size_t width);

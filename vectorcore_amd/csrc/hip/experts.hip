@@ -54,6 +54,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(const float* __r
     for (int e = tid; e < groups; e += kPlanBlock) {
         int before = 0, all = 0;
         if (counts)
+#pragma unroll 8
             for (int c = 0; c < int(gridDim.x); ++c) {
                 const int n = counts[c * groups + e];
                 if (c < int(blockIdx.x)) before += n;
@@ -355,7 +356,9 @@ __global__ __launch_bounds__(split::kThreads, BN == 256 ? 2 : at_once(BM)) void 
     __shared__ split::Slice<S, BN> bs;
     const int64_t row_tiles = (p.width + BM - 1) / BM, column_tiles = (p.columns + BN - 1) / BN;
     const int64_t total = row_tiles * column_tiles, share = (total + 7) / 8;
-    const int group = int(blockIdx.x / 8 / share);
+    const int unit = int(blockIdx.x / 8 / share), group = unit % p.experts;
+    const float* const grad = unit < p.experts ? p.b : p.b2;
+    float* const out = unit < p.experts ? p.c : p.c2;
     const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8 % share;
     if (id >= total) return;
     const int64_t m0 = id / column_tiles * BM, n0 = id % column_tiles * BN;
@@ -375,7 +378,7 @@ __global__ __launch_bounds__(split::kThreads, BN == 256 ? 2 : at_once(BM)) void 
         return [=](int) { return line; };
     };
     const auto line_b = [&](int64_t k) {
-        const float* const line = p.b + n0 + (begin + k) * p.columns;
+        const float* const line = grad + n0 + (begin + k) * p.columns;
         return [=](int) { return line; };
     };
     split::accumulate<ahead(BM), A, B>(
@@ -393,9 +396,9 @@ __global__ __launch_bounds__(split::kThreads, BN == 256 ? 2 : at_once(BM)) void 
         if (row >= p.width || col >= p.columns) return;
         if (!split::finite(v)) {
             v = 0.0f;
-            for (int r = begin; r < begin + depth; ++r) v = fmaf(p.a[source(r) + row], p.b[int64_t(r) * p.columns + col], v);
+            for (int r = begin; r < begin + depth; ++r) v = fmaf(p.a[source(r) + row], grad[int64_t(r) * p.columns + col], v);
         }
-        p.c[(int64_t(group) * p.width + row) * p.columns + col] = v;
+        out[(int64_t(group) * p.width + row) * p.columns + col] = v;
     });
 }
 
@@ -788,25 +791,28 @@ int vc_hip_expert_linear_backward_input(const float* grad, const float* w, const
     });
 }
 
-int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, const vc_hip_expert_plan* plan, size_t width,
-                                         size_t columns, int ordered, float* grad_w) {
+int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, const float* grad2,
+                                         const vc_hip_expert_plan* plan, size_t width, size_t columns, int ordered,
+                                         float* grad_w, float* grad_w2) {
     return guard([&] {
         Device& d = require_device();
         const Plan q = plan_of(plan);
+        if (!grad_w2 != !grad2) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_linear_backward_weight: half of a second product");
         if (width == 0 || columns == 0) return;
         if (!grad_w || (q.rows && (!x || !grad))) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_linear_backward_weight: null pointer");
-        Profiled p("expert_backward_weight", 2.0 * q.rows * width * columns,
-                   4.0 * (q.rows * (width + columns) + q.experts * width * columns));
-        const ProductArgs args{x, grad, nullptr, nullptr, grad_w, nullptr, nullptr, q.offsets, ordered ? nullptr : q.token,
+        const int64_t products = grad2 ? 2 : 1;
+        Profiled p("expert_backward_weight", products * 2.0 * q.rows * width * columns,
+                   4.0 * (q.rows * (width + products * columns) + products * q.experts * width * columns));
+        const ProductArgs args{x, grad, nullptr, grad2, grad_w, grad_w2, nullptr, q.offsets, ordered ? nullptr : q.token,
                                int(q.experts), int64_t(width), int64_t(columns)};
         // 256 columns a tile where they fill the chip: x is then split half as often. (8 experts, 1024 x 4096 over 16384
         // rows: 809 us, with 128 columns 935. The products of rows gain nothing, as fewer tiles fit the CUs less evenly.)
         const auto run = [&](auto bm, auto bn) {
             const int64_t share = tiles_of(size_t(tiles_of(width, bm()) * tiles_of(columns, bn())), 8);
-            launch(weight_kernel<bm(), bn()>, tile_grid(int64_t(q.experts) * share * 8), dim3(split::kThreads), 0, d.stream, args);
+            launch(weight_kernel<bm(), bn()>, tile_grid(products * int64_t(q.experts) * share * 8), dim3(split::kThreads), 0, d.stream, args);
         };
         using std::integral_constant;
-        const int64_t row_tiles = int64_t(q.experts) * tiles_of(width, 128);
+        const int64_t row_tiles = products * int64_t(q.experts) * tiles_of(width, 128);
         if (row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) run(integral_constant<int, 128>(), integral_constant<int, 256>());
         else if (enough(d, row_tiles * tiles_of(columns, 128))) run(integral_constant<int, 128>(), integral_constant<int, 128>());
         else run(integral_constant<int, 64>(), integral_constant<int, 64>());

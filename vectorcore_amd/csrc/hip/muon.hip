@@ -38,7 +38,7 @@ constexpr int kNormBlocks = 1024;  // partial sums of squares of a matrix, at mo
 constexpr int kAtOnce = 12;       // matrices (or batches of equal ones) of a launch
 constexpr int kMostSplit = 2048;  // tiles of a launch whose sums are split
 using packed::place;
-using half = _Float16;
+using packed::half;
 
 // `count` matrices [rows, cols].
 struct Matrix {
@@ -221,17 +221,18 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
 
     const float unit = 1.0f / kScale;
     if constexpr (K == Kind::Apply) {
-        const half* const xt = m.xt + whole;
+        tile.mix(kA, m.x + whole, unit, m0, n0, m.longer);
+        if (!last) {
+            tile.store(m.y + whole, m0, n0, m.longer);
+            tile.store_transposed(m.yt + whole, m0, n0, m.shorter, lds);
+            return;
+        }
         const bool wide = m.wide();
         float *const out = m.out ? m.out + z * m.elements() : nullptr, *const param = m.param ? m.param + z * m.elements() : nullptr;
         const int64_t rows = wide ? m.rows : m.cols, cols = wide ? m.cols : m.rows;  // without the padding
         tile.each4([&](int r, int c, float (&v)[4]) {
             const int64_t row = m0 + r, col = n0 + c;
-            float x[4];
-            packed::load4(xt + place(col, row, m.shorter), x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = kA * x[e] + v[e] * unit;
-            if (!last || col >= cols) return;
+            if (col >= cols) return;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (row + e >= rows) return;
@@ -240,20 +241,18 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
                 else out[at] = v[e] * unit;
             }
         });
-        if (last) return;
-        tile.store(m.y + whole, m0, n0, m.longer);
-        tile.store_transposed(m.yt + whole, m0, n0, m.shorter);
     } else {
         half* const out = (K == Kind::Gram ? m.gram : m.poly) + square;
-        const half* const gram = m.gram + square;
-        tile.each4([&](int r, int c, float (&v)[4]) {
-            float g[4];
-            if constexpr (K == Kind::Poly) packed::load4(gram + place(n0 + c, m0 + r, m.shorter), g);
+        if constexpr (K == Kind::Poly) {
+            tile.mix(kB, m.gram + square, kC * unit, m0, n0, m.shorter);
+        } else {
+            tile.each4([&](int, int, float (&v)[4]) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = K == Kind::Poly ? kB * g[e] + kC * (v[e] * unit) : v[e] * unit;
-        });
-        tile.store_transposed(out, m0, n0, m.shorter);
-        if (i != j) tile.store(out, m0, n0, m.shorter);
+                for (int e = 0; e < 4; ++e) v[e] *= unit;
+            });
+        }
+        tile.store(out, m0, n0, m.shorter);
+        if (i != j) tile.store_transposed(out, m0, n0, m.shorter, lds);
     }
 }
 
@@ -274,7 +273,7 @@ int64_t tiles_of(Kind kind, const Matrix& m, int64_t bt) {
     return m.count * (kind == Kind::Apply ? t * (m.longer / bt) : t * (t + 1) / 2);
 }
 
-// Where tiles are few, sums are split into parts of at least four slices. More
+// Where tiles are few, sums are split into parts of at least eight slices. More
 // stages in flight where a CU has one workgroup at most.
 template <Kind K, int BT>
 void product(Device& d, Batch& batch, bool last = false, float keep = 0.0f) {
@@ -285,7 +284,7 @@ void product(Device& d, Batch& batch, bool last = false, float keep = 0.0f) {
     for (int i = 0; i < batch.n; ++i) {
         Matrix& m = batch.of[i];
         const int64_t slices = (K == Kind::Gram ? m.longer : m.shorter) / packed::kSlice;
-        m.splits = int(std::max<int64_t>(1, std::min(wanted, slices / 4)));
+        m.splits = int(std::max<int64_t>(1, std::min(wanted, slices / 8)));
         m.counters = int(counters);
         counters += tiles_of(K, m, BT);
     }

@@ -25,6 +25,7 @@ namespace packed {
 
 constexpr int kThreads = 256, kSlice = 32, kLine = 64;  // halves of a line
 
+typedef _Float16 half;
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -52,12 +53,6 @@ __device__ inline void store4(_Float16* to, const float (&v)[4]) {
     *reinterpret_cast<h4*>(to) = first;
     *reinterpret_cast<h4*>(to + kSlice) = second;
 }
-__device__ inline void load4(const _Float16* from, float (&v)[4]) {
-    const h4 first = *reinterpret_cast<const h4*>(from), second = *reinterpret_cast<const h4*>(from + kSlice);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = float(first[i]) + float(second[i]);
-}
-
 // s_waitcnt that leaves `loads` vector memory operations in flight.
 template <int Loads>
 __device__ inline void wait_loads() {
@@ -177,27 +172,71 @@ struct Tile {
                 }
     }
 
-    // The tile into a matrix from its element (m0, n0): 32 lanes write a line, the even ones first parts and the odd
-    // ones second parts of two neighbours.
-    __device__ inline void store(_Float16* to, int64_t m0, int64_t n0, int64_t depth) {
+    // This thread's place of the tile from element (m0, n0) of a matrix: 32 lanes hold a line, the even ones first parts and
+    // the odd ones second parts of two neighbours. f(place, value) for each value.
+    template <class P, class F>
+    __device__ inline void each_place(P* matrix, int64_t m0, int64_t n0, int64_t depth, F&& f) {
         const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-        const uint32_t select = lane % 2 ? 0x03020706u : 0x05040100u;
-        const int64_t column = n0 + wave % 2 * (BT / 2);
-        _Float16* const line = to + place(m0 + wave / 2 * (BT / 2) + 4 * (lane / 32), column, depth) + lane % 2 * kSlice + lane % 32 / 2 * 2;
+        P* const line = matrix + place(m0 + wave / 2 * (BT / 2) + 4 * (lane / 32), n0 + wave % 2 * (BT / 2), depth) +
+                        lane % 2 * kSlice + lane % 32 / 2 * 2;
 #pragma unroll
         for (int a = 0; a < kBlocks; ++a)
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const uint32_t mine = parts(acc[a][b][i]), other = red::partner<0>(mine, lane);
-                    *reinterpret_cast<uint32_t*>(line + (32 * a + 8 * (i / 4) + i % 4) * 2 * depth + b * kLine) =
-                        __builtin_amdgcn_perm(other, mine, select);
+                    float v = acc[a][b][i];
+                    f(line + (32 * a + 8 * (i / 4) + i % 4) * 2 * depth + b * kLine, v);
+                    acc[a][b][i] = v;
                 }
     }
-    // The same transposed: the tile's element (row, column) becomes (n0 + column, m0 + row).
-    __device__ inline void store_transposed(_Float16* to, int64_t m0, int64_t n0, int64_t depth) {
-        each4([&](int row, int column, float (&v)[4]) { store4(to + place(n0 + column, m0 + row, depth), v); });
+    // Two neighbours' parts, of one kind each, to one's parts of both kinds, and back.
+    static __device__ inline uint32_t exchange(uint32_t mine) {
+        const int lane = red::lane_id();
+        return __builtin_amdgcn_perm(red::partner<0>(mine, lane), mine, lane % 2 ? 0x03020706u : 0x05040100u);
+    }
+    __device__ inline void store(half* to, int64_t m0, int64_t n0, int64_t depth) {
+        each_place(to, m0, n0, depth, [](half* at, float& v) { *reinterpret_cast<uint32_t*>(at) = exchange(parts(v)); });
+    }
+    // tile = a * matrix + b * tile.
+    __device__ inline void mix(float a, const half* matrix, float b, int64_t m0, int64_t n0, int64_t depth) {
+        each_place(matrix, m0, n0, depth, [&](const half* at, float& v) {
+            const uint32_t both = exchange(*reinterpret_cast<const uint32_t*>(at));
+            const float x = float(__builtin_bit_cast(half, uint16_t(both))) + float(__builtin_bit_cast(half, uint16_t(both >> 16)));
+            v = a * x + b * v;
+        });
+    }
+    // The tile transposed: its element (row, column) becomes (n0 + column, m0 + row). A wave collects 32 rows of it in LDS,
+    // a line of each column, and writes whole lines. lds: of the finished accumulate().
+    __device__ inline void store_transposed(half* to, int64_t m0, int64_t n0, int64_t depth, char* lds) {
+        constexpr int kColumns = BT / 2, kStride = 128 + 16;  // of a wave; bytes, so that neighbours meet other banks
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        static_assert(4 * kColumns * kStride <= kLds, "the waves' lines exceed the stages");
+        char* const mine = lds + wave * kColumns * kStride;
+        __syncthreads();  // no wave reads the stages any more
+#pragma unroll
+        for (int a = 0; a < kBlocks; ++a) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = acc[a][b][4 * g + i];
+                    store4(reinterpret_cast<half*>(mine + (32 * b + lane % 32) * kStride) + 8 * g + 4 * (lane / 32), v);
+                }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            half* const line = to + place(n0 + wave % 2 * kColumns, m0 + wave / 2 * (BT / 2) + 32 * a, depth);
+#pragma unroll
+            for (int c = 0; c < kColumns; c += 8)
+                *reinterpret_cast<h8*>(line + (c + lane / 8) * 2 * depth + lane % 8 * 8) =
+                    *reinterpret_cast<const h8*>(mine + (c + lane / 8) * kStride + lane % 8 * 16);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
     }
 };
 
