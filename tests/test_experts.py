@@ -153,6 +153,14 @@ def test_linear(tokens, experts, top_k, width, columns, ordered, device):
     assert (np.abs(tw.grad.numpy() - dw) <= bound(len(group)) * mdw).all()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tokens,experts,top_k,width,hidden,kind", [(90, 2, 1, 1100, 60, "skewed"), (70, 1, 1, 70, 1290, "even"),
+                                                                    (44, 3, 3, 600, 700, "dropped"), (3000, 3, 1, 40, 70, "skewed")])
+def test_long_sums_of_few_tiles(tokens, experts, top_k, width, hidden, kind, device):
+    """Sums that are split over workgroups."""
+    test_gated_unit(tokens, experts, top_k, width, hidden, kind, device)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("tokens,experts,top_k,width,columns", [(4099, 3, 2, 33, 2050), (4099, 3, 2, 2051, 33),
                                                                (45, 5, 2, 2050, 2053), (9000, 6, 1, 96, 1024)])

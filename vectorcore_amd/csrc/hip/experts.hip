@@ -154,19 +154,36 @@ struct ProductArgs {
     const int *offsets, *token;  // token: of each row of a gathered A, null where A lies in row order
     int experts;
     int64_t width, columns;  // of each expert's matrix [width, columns]
+    // Tiles of 64: parts of each tile's sum, workgroup w the part w / (grid / parts).
+    int parts = 1;
+    float* partial = nullptr;
 };
 
 struct RowTile {
     int group, begin, end;  // rows of one group
     int64_t column;         // tile of columns
     bool live;
+    int64_t id;  // of a live tile among all
 };
+
+constexpr int64_t kSplitTiles = 4096;        // whose sums are split, at most
+__device__ unsigned g_tile_done[kSplitTiles];  // parts done; zero between launches, which never overlap
+
+// A part's k, in whole slices.
+struct Range {
+    int64_t begin, end;
+};
+__device__ inline Range part_of(int64_t depth, int part, int parts) {
+    if (parts == 1) return {0, depth};
+    const int64_t slices = (depth + split::kSliceK - 1) / split::kSliceK;
+    return {slices * part / parts * split::kSliceK, min(depth, slices * (part + 1) / parts * split::kSliceK)};
+}
 
 // The tile-th of the groups' tiles of Rows rows.
 template <int Rows>
 __device__ inline RowTile find_rows(const int* __restrict__ offsets, int groups, int tile, int64_t column) {
     const int lane = threadIdx.x % kWave;
-    RowTile t{0, 0, 0, column, false};
+    RowTile t{0, 0, 0, column, false, 0};
     for (int base = 0; base < groups; base += kWave) {
         const int e = base + lane;
         const int lo = e < groups ? offsets[e] : 0, hi = e < groups ? offsets[e + 1] : 0;
@@ -198,7 +215,7 @@ __device__ inline RowTile find_rows(const int* __restrict__ offsets, int groups,
 // to them in turn) works on neighbouring ones, which read the same operands
 // through its cache.
 template <int BM>
-__device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups, int64_t column_tiles) {
+__device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups, int64_t column_tiles, unsigned block) {
     const int lane = threadIdx.x % kWave;
     int all = 0;
     for (int base = 0; base < groups; base += kWave) {
@@ -209,9 +226,11 @@ __device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups,
         all += sum;
     }
     const int64_t total = all * column_tiles, share = (total + 7) / 8;
-    const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8;
-    if (blockIdx.x / 8 >= share || id >= total) return RowTile{0, 0, 0, 0, false};
-    return find_rows<BM>(offsets, groups, int(id / column_tiles), id % column_tiles);
+    const int64_t id = block % 8 * share + block / 8;
+    if (block / 8 >= share || id >= total) return RowTile{0, 0, 0, 0, false, 0};
+    RowTile t = find_rows<BM>(offsets, groups, int(id / column_tiles), id % column_tiles);
+    t.id = id;
+    return t;
 }
 
 __device__ inline float sigmoid(float x) {
@@ -219,18 +238,18 @@ __device__ inline float sigmoid(float x) {
     return (x >= 0.0f ? 1.0f : e) / (1.0f + e);
 }
 
-// Workgroups on a CU, and slices on their way, of tiles of `rows` rows.
-constexpr int at_once(int rows) { return rows == 128 ? 3 : 2; }
+// Slices on their way of tiles of `rows` rows.
 constexpr int ahead(int rows) { return rows == 128 ? 1 : 3; }
 
 // C[r] = x_r @ w[group], or silu(x_r @ gate) * (x_r @ up): there a tile holds
 // 64 columns of both products, so that a thread holds both values of an element.
 template <bool Gated, int BM>
-__global__ __launch_bounds__(split::kThreads, at_once(BM)) void forward_kernel(ProductArgs p) {
+__global__ __launch_bounds__(split::kThreads, Gated && BM == 128 ? 3 : 2) void forward_kernel(ProductArgs p) {
     constexpr int BN = Gated ? 128 : BM, kColumns = Gated ? BN / 2 : BN;
     __shared__ split::Slice<S, BM> as;
     __shared__ split::Slice<S, BN> bs;
-    const RowTile t = find_tile<BM>(p.offsets, p.experts + 1, (p.columns + kColumns - 1) / kColumns);
+    const int parts = BM == 64 ? p.parts : 1, tiles = int(gridDim.x) / parts, part = int(blockIdx.x) / tiles;
+    const RowTile t = find_tile<BM>(p.offsets, p.experts + 1, (p.columns + kColumns - 1) / kColumns, blockIdx.x % tiles);
     if (!t.live) return;
     const int64_t n0 = t.column * kColumns;
     split::Tile<S, BM, BN> tile;
@@ -240,6 +259,7 @@ __global__ __launch_bounds__(split::kThreads, at_once(BM)) void forward_kernel(P
     if (t.group < p.experts) {
         using A = split::AlongK<BM>;
         using B = split::AcrossK<BN>;
+        const Range range = part_of(p.width, part, parts);
         const float* pa[A::kChunks];
         unsigned at[B::kChunks];
 #pragma unroll
@@ -253,7 +273,7 @@ __global__ __launch_bounds__(split::kThreads, at_once(BM)) void forward_kernel(P
             return [=](int j) { return (j ? w2 : w) + at_k; };
         };
         split::accumulate<ahead(BM), A, B>(
-            tile, as, bs, p.width,
+            tile, as, bs, range.begin, range.end,
             [&](A& a, B& b, int64_t k) {
                 a.load(pa, k);
                 b.load(at, k, line);
@@ -262,6 +282,10 @@ __global__ __launch_bounds__(split::kThreads, at_once(BM)) void forward_kernel(P
                 a.load_rest(pa, k, p.width);
                 b.load_rest(at, k, p.width, line);
             });
+    }
+    if constexpr (BM == 64) {
+        __shared__ bool last;
+        if (parts > 1 && !split::join(tile, part, parts, p.partial + t.id * parts * (BM * BN), &g_tile_done[t.id], last)) return;
     }
     // A lost sum, value by value.
     const auto again = [&](const float* w, int r, int64_t col) {
@@ -291,26 +315,32 @@ __global__ __launch_bounds__(split::kThreads, at_once(BM)) void forward_kernel(P
                 }
             }
     } else {
+        if (tile.lost() && t.group < p.experts)
+            tile.each([&](int m, int n, float& v) {
+                const int r = t.begin + m;
+                const int64_t col = n0 + n;
+                if (!split::finite(v) && r < t.end && col < p.columns) v = again(p.b, r, col);
+            });
         tile.each([&](int m, int n, float v) {
             const int r = t.begin + m;
             const int64_t col = n0 + n;
-            if (r >= t.end || col >= p.columns) return;
-            if (!split::finite(v)) v = again(p.b, r, col);
-            p.c[int64_t(r) * p.columns + col] = v;
+            if (r < t.end && col < p.columns) p.c[int64_t(r) * p.columns + col] = v;
         });
     }
 }
 
 // C[r] = a[r] @ b[group]^T (+ a2[r] @ b2[group]^T).
 template <int BM>
-__global__ __launch_bounds__(split::kThreads, at_once(BM)) void input_kernel(ProductArgs p) {
+__global__ __launch_bounds__(split::kThreads, 2) void input_kernel(ProductArgs p) {
     __shared__ split::Slice<S, BM> as, bs;
-    const RowTile t = find_tile<BM>(p.offsets, p.experts + 1, (p.width + BM - 1) / BM);
+    const int parts = BM == 64 ? p.parts : 1, tiles = int(gridDim.x) / parts, part = int(blockIdx.x) / tiles;
+    const RowTile t = find_tile<BM>(p.offsets, p.experts + 1, (p.width + BM - 1) / BM, blockIdx.x % tiles);
     if (!t.live) return;
     const int64_t n0 = t.column * BM, matrix = int64_t(t.group) * p.width * p.columns;
     split::Tile<S, BM, BM> tile;
     tile.clear();
     const int products = p.a2 ? 2 : 1;
+    const Range range = part_of(p.columns, part, parts);
     if (t.group < p.experts) {
         for (int product = 0; product < products; ++product) {
             const float *const from = product ? p.a2 : p.a, *const w = (product ? p.b2 : p.b) + matrix;
@@ -321,7 +351,7 @@ __global__ __launch_bounds__(split::kThreads, at_once(BM)) void input_kernel(Pro
 #pragma unroll
             for (int j = 0; j < A::kChunks; ++j) pb[j] = w + min(n0 + A::row(j), p.width - 1) * p.columns;
             split::accumulate<ahead(BM), A, A>(
-                tile, as, bs, p.columns,
+                tile, as, bs, range.begin, range.end,
                 [&](A& a, A& b, int64_t k) {
                     a.load(pa, k);
                     b.load(pb, k);
@@ -332,34 +362,40 @@ __global__ __launch_bounds__(split::kThreads, at_once(BM)) void input_kernel(Pro
                 });
         }
     }
-    tile.each([&](int m, int n, float v) {
-        const int r = t.begin + m;
-        const int64_t col = n0 + n;
-        if (r >= t.end || col >= p.width) return;
-        if (!split::finite(v)) {
+    if constexpr (BM == 64) {
+        __shared__ bool last;
+        if (parts > 1 && !split::join(tile, part, parts, p.partial + t.id * parts * (BM * BM), &g_tile_done[t.id], last)) return;
+    }
+    if (tile.lost() && t.group < p.experts)  // sums again, value by value
+        tile.each([&](int m, int n, float& v) {
+            const int64_t r = t.begin + m, col = n0 + n;
+            if (split::finite(v) || r >= t.end || col >= p.width) return;
             v = 0.0f;
             for (int product = 0; product < products; ++product) {
-                const float *const x = (product ? p.a2 : p.a) + int64_t(r) * p.columns;
+                const float *const x = (product ? p.a2 : p.a) + r * p.columns;
                 const float *const w = (product ? p.b2 : p.b) + matrix + col * p.columns;
                 for (int64_t k = 0; k < p.columns; ++k) v = fmaf(x[k], w[k], v);
             }
-        }
-        p.c[int64_t(r) * p.width + col] = v;
+        });
+    tile.each([&](int m, int n, float v) {
+        const int64_t r = t.begin + m, col = n0 + n;
+        if (r < t.end && col < p.width) p.c[r * p.width + col] = v;
     });
 }
 
 // C[e] = sum over e's rows of x_r^T b[r]. Every die takes its part of each
 // expert's tiles, as experts differ in their rows.
 template <int BM, int BN>
-__global__ __launch_bounds__(split::kThreads, BN == 256 ? 2 : at_once(BM)) void weight_kernel(ProductArgs p) {
+__global__ __launch_bounds__(split::kThreads, 2) void weight_kernel(ProductArgs p) {
     __shared__ split::Slice<S, BM> as;
     __shared__ split::Slice<S, BN> bs;
     const int64_t row_tiles = (p.width + BM - 1) / BM, column_tiles = (p.columns + BN - 1) / BN;
     const int64_t total = row_tiles * column_tiles, share = (total + 7) / 8;
-    const int unit = int(blockIdx.x / 8 / share), group = unit % p.experts;
+    const int parts = BM == 64 ? p.parts : 1, blocks = int(gridDim.x) / parts, part = int(blockIdx.x) / blocks;
+    const int block = int(blockIdx.x) % blocks, unit = int(block / 8 / share), group = unit % p.experts;
     const float* const grad = unit < p.experts ? p.b : p.b2;
     float* const out = unit < p.experts ? p.c : p.c2;
-    const int64_t id = blockIdx.x % 8 * share + blockIdx.x / 8 % share;
+    const int64_t id = block % 8 * share + block / 8 % share;
     if (id >= total) return;
     const int64_t m0 = id / column_tiles * BM, n0 = id % column_tiles * BN;
     const int begin = p.offsets[group], depth = p.offsets[group + 1] - begin;
@@ -381,8 +417,9 @@ __global__ __launch_bounds__(split::kThreads, BN == 256 ? 2 : at_once(BM)) void 
         const float* const line = grad + n0 + (begin + k) * p.columns;
         return [=](int) { return line; };
     };
+    const Range range = part_of(depth, part, parts);
     split::accumulate<ahead(BM), A, B>(
-        tile, as, bs, depth,
+        tile, as, bs, range.begin, range.end,
         [&](A& a, B& b, int64_t k) {
             a.load(at_a, k, line_a);
             b.load(at_b, k, line_b);
@@ -391,14 +428,21 @@ __global__ __launch_bounds__(split::kThreads, BN == 256 ? 2 : at_once(BM)) void 
             a.load_rest(at_a, k, depth, line_a);
             b.load_rest(at_b, k, depth, line_b);
         });
-    tile.each([&](int m, int n, float v) {
-        const int64_t row = m0 + m, col = n0 + n;
-        if (row >= p.width || col >= p.columns) return;
-        if (!split::finite(v)) {
+    if constexpr (BM == 64) {
+        __shared__ bool last;
+        const int64_t at = unit * total + id;
+        if (parts > 1 && !split::join(tile, part, parts, p.partial + at * parts * (BM * BN), &g_tile_done[at], last)) return;
+    }
+    if (tile.lost())  // sums again, value by value
+        tile.each([&](int m, int n, float& v) {
+            const int64_t row = m0 + m, col = n0 + n;
+            if (split::finite(v) || row >= p.width || col >= p.columns) return;
             v = 0.0f;
             for (int r = begin; r < begin + depth; ++r) v = fmaf(p.a[source(r) + row], grad[int64_t(r) * p.columns + col], v);
-        }
-        out[(int64_t(group) * p.width + row) * p.columns + col] = v;
+        });
+    tile.each([&](int m, int n, float v) {
+        const int64_t row = m0 + m, col = n0 + n;
+        if (row < p.width && col < p.columns) out[(int64_t(group) * p.width + row) * p.columns + col] = v;
     });
 }
 
@@ -411,9 +455,12 @@ __global__ __launch_bounds__(split::kThreads, BN == 256 ? 2 : at_once(BM)) void 
 // lines of 64 columns at four places of k: the parts of k are then fewer and
 // longer. The sums of the waves' k are added in LDS, those of workgroups by the
 // one that counts in last, in order.
+//
+// Forward pass of 30 experts of 1024 x 1024, this and tiles of 64 rows: 4 rows an
+// expert on average 91 and 129 us, 8 rows 129 and 126, 16 rows 154 and 130.
 
 constexpr int kThinRows = 4, kThinDepth = 512, kThinTiles = 4096;
-constexpr size_t kThinMost = 32;  // rows of an expert on average
+constexpr size_t kThinMost = 6;  // rows of an expert on average
 
 __device__ unsigned g_thin_done[kThinTiles];  // parts done of a tile; zero between launches
 
@@ -582,6 +629,25 @@ int64_t tiles_at_most(const Plan& plan, int rows, size_t width, int columns) {
     return int64_t(plan.rows / rows + plan.experts + 1) * tiles_of(width, columns);
 }
 
+// Parts of a sum over `depth` for `tiles` tiles of 64, at least eight slices
+// each, and the memory for `values` of every tile and part.
+struct Parts {
+    int64_t parts;
+    Scratch partial;
+    Parts(Device& d, int64_t tiles, int64_t depth, int64_t values)
+        : parts(tiles > kSplitTiles ? 1 : std::max<int64_t>(1, std::min(2 * d.cu_count / std::max<int64_t>(1, tiles), depth / 256))),
+          partial(parts > 1 ? size_t(tiles * parts * values) * sizeof(float) : 4) {}
+    ProductArgs operator()(ProductArgs args) const {
+        args.parts = int(parts);
+        args.partial = partial.as<float>();
+        return args;
+    }
+};
+dim3 operator*(dim3 grid, int64_t parts) {
+    if (grid.x * parts >= int64_t(1) << 31) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
+    return dim3(unsigned(grid.x * parts));
+}
+
 // Whether tiles of 128 rows give every CU one; otherwise tiles of 64 halve or
 // quarter what each of them computes (THIN64).
 bool enough(Device& d, int64_t tiles) { return tiles >= d.cu_count; }
@@ -722,8 +788,11 @@ int vc_hip_expert_linear_forward(const float* x, const float* w, const vc_hip_ex
             launch_thin<false>(d, q, args);
         else if (enough(d, int64_t(q.rows / 128) * tiles_of(columns, 128)))
             launch(forward_kernel<false, 128>, tile_grid(tiles_at_most(q, 128, columns, 128)), threads, 0, d.stream, args);
-        else
-            launch(forward_kernel<false, 64>, tile_grid(tiles_at_most(q, 64, columns, 64)), threads, 0, d.stream, args);
+        else {
+            const int64_t tiles = tiles_at_most(q, 64, columns, 64);
+            const Parts parts(d, tiles, args.width, 64 * 64);
+            launch(forward_kernel<false, 64>, tile_grid(tiles) * parts.parts, threads, 0, d.stream, parts(args));
+        }
         after_launch("expert_linear");
         p.done();
     });
@@ -746,8 +815,11 @@ int vc_hip_expert_gated_forward(const float* x, const float* gate, const float* 
             launch_thin<true>(d, q, args);
         else if (enough(d, int64_t(q.rows / 128) * tiles_of(columns, 64)))
             launch(forward_kernel<true, 128>, tile_grid(tiles_at_most(q, 128, columns, 64)), threads, 0, d.stream, args);
-        else
-            launch(forward_kernel<true, 64>, tile_grid(tiles_at_most(q, 64, columns, 64)), threads, 0, d.stream, args);
+        else {
+            const int64_t tiles = tiles_at_most(q, 64, columns, 64);
+            const Parts parts(d, tiles, args.width, 64 * 128);
+            launch(forward_kernel<true, 64>, tile_grid(tiles) * parts.parts, threads, 0, d.stream, parts(args));
+        }
         after_launch("expert_gated");
         p.done();
     });
@@ -784,8 +856,11 @@ int vc_hip_expert_linear_backward_input(const float* grad, const float* w, const
         const dim3 threads(split::kThreads);
         if (enough(d, int64_t(q.rows / 128) * tiles_of(width, 128)))
             launch(input_kernel<128>, tile_grid(tiles_at_most(q, 128, width, 128)), threads, 0, d.stream, args);
-        else
-            launch(input_kernel<64>, tile_grid(tiles_at_most(q, 64, width, 64)), threads, 0, d.stream, args);
+        else {
+            const int64_t tiles = tiles_at_most(q, 64, width, 64);
+            const Parts parts(d, tiles, args.columns, 64 * 64);
+            launch(input_kernel<64>, tile_grid(tiles) * parts.parts, threads, 0, d.stream, parts(args));
+        }
         after_launch("expert_backward_input");
         p.done();
     });
@@ -815,7 +890,13 @@ int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, cons
         const int64_t row_tiles = products * int64_t(q.experts) * tiles_of(width, 128);
         if (row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) run(integral_constant<int, 128>(), integral_constant<int, 256>());
         else if (enough(d, row_tiles * tiles_of(columns, 128))) run(integral_constant<int, 128>(), integral_constant<int, 128>());
-        else run(integral_constant<int, 64>(), integral_constant<int, 64>());
+        else {
+            const int64_t tiles = products * int64_t(q.experts) * tiles_of(width, 64) * tiles_of(columns, 64);
+            const int64_t share = tiles_of(size_t(tiles_of(width, 64) * tiles_of(columns, 64)), 8);
+            const Parts parts(d, tiles, int64_t(q.rows / q.experts), 64 * 64);
+            launch(weight_kernel<64, 64>, tile_grid(products * int64_t(q.experts) * share * 8) * parts.parts, dim3(split::kThreads), 0,
+                   d.stream, parts(args));
+        }
         after_launch("expert_backward_weight");
         p.done();
     });

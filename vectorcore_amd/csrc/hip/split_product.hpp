@@ -18,6 +18,8 @@
 // costs nothing more than a k-contiguous one.
 #pragma once
 
+#include "reduce_common.hpp"
+
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -159,12 +161,17 @@ struct AcrossK {
     static __device__ inline int row(int j) { return threadIdx.x % 64 + 64 * j; }
 };
 
+// Is a sum of products lost to an infinity, a NaN or a value that rounds to an
+// infinity in 16 bits? Its parts give NaN or an infinity then.
+__device__ inline bool finite(float x) { return fabsf(x) < __builtin_huge_valf(); }
+
 // ---- the tile -----------------------------------------------------------------------
 
 // Wave w computes rows BM / 2 (w / 2) .. and, of every 64 columns, the half w % 2.
 template <class S, int BM, int BN>
 struct Tile {
     static constexpr int kM = BM / 64, kN = BN / 64;  // 32 x 32 blocks of a wave
+    static constexpr int kValues = 16 * kM * kN;      // of a thread
     f16v acc[kM][kN];
 
     __device__ inline void clear() {
@@ -199,6 +206,18 @@ struct Tile {
         }
     }
 
+    // Is one of this thread's values not finite? See finite().
+    __device__ inline bool lost() const {
+        bool any = false;
+#pragma unroll
+        for (int a = 0; a < kM; ++a)
+#pragma unroll
+            for (int b = 0; b < kN; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) any |= !finite(acc[a][b][i]);
+        return any;
+    }
+
     // f(row, column, value) for each value this thread holds; f may change it.
     template <class F>
     __device__ inline void each(F&& f) {
@@ -216,12 +235,12 @@ struct Tile {
     }
 };
 
-// The products of k < depth onto a tile. load(a, b, k) reads a whole slice,
-// rest(a, b, k) the last one, of which depth % 32 are there. Ahead register sets
+// The products of k in [begin, end) onto a tile. load(a, b, k) reads a whole
+// slice, rest(a, b, k) the last one, of which (end - begin) % 32 are there. Ahead register sets
 // hold slices that are on their way: one where other workgroups of the CU hide
 // the wait, more for grids that leave a CU one or two.
 template <int Ahead, class A, class B, class T, class SA, class SB, class Load, class Rest>
-__device__ inline void accumulate(T& tile, SA& as, SB& bs, int64_t depth, Load&& load, Rest&& rest) {
+__device__ inline void accumulate(T& tile, SA& as, SB& bs, int64_t begin, int64_t end, Load&& load, Rest&& rest) {
     A a[Ahead];
     B b[Ahead];
     const auto multiply = [&](const A& x, const B& y, auto&& next) {
@@ -235,20 +254,20 @@ __device__ inline void accumulate(T& tile, SA& as, SB& bs, int64_t depth, Load&&
     };
     if constexpr (Ahead == 1) {
         const auto next = [&](int64_t k) {
-            if (k + kSliceK <= depth) load(a[0], b[0], k);
+            if (k + kSliceK <= end) load(a[0], b[0], k);
             else rest(a[0], b[0], k);
         };
-        if (depth <= 0) return;
-        next(int64_t(0));
-        for (int64_t k = 0; k < depth; k += kSliceK)
+        if (end <= begin) return;
+        next(begin);
+        for (int64_t k = begin; k < end; k += kSliceK)
             multiply(a[0], b[0], [&] {
-                if (k + kSliceK < depth) next(k + kSliceK);
+                if (k + kSliceK < end) next(k + kSliceK);
             });
     } else {
-        const int full = int(depth / kSliceK);
+        const int full = int((end - begin) / kSliceK);
         // Always the same number of loads on their way (past the end the last slice is read again), so that the compiler
         // waits for just those it needs.
-        const auto at = [&](int s) { return int64_t(min(s, full - 1)) * kSliceK; };
+        const auto at = [&](int s) { return begin + int64_t(min(s, full - 1)) * kSliceK; };
         if (full > 0) {
 #pragma unroll
             for (int i = 0; i < Ahead; ++i) load(a[i], b[i], at(i));
@@ -260,16 +279,41 @@ __device__ inline void accumulate(T& tile, SA& as, SB& bs, int64_t depth, Load&&
                 multiply(a[i], b[i], [&] { load(a[i], b[i], at(s + i + Ahead)); });
             }
         }
-        if (int64_t(full) * kSliceK < depth) {
-            rest(a[0], b[0], int64_t(full) * kSliceK);
+        if (begin + int64_t(full) * kSliceK < end) {
+            rest(a[0], b[0], begin + int64_t(full) * kSliceK);
             multiply(a[0], b[0], [] {});
         }
     }
 }
 
-// Is a sum of products lost to an infinity, a NaN or a value that rounds to an
-// infinity in 16 bits? Its parts give NaN or an infinity then.
-__device__ inline bool finite(float x) { return fabsf(x) < __builtin_huge_valf(); }
+// One of `parts` workgroups that each hold a part of a tile's sums: false for
+// all but the one that counts in last on `done` (zero before and after), which
+// adds the parts in their order. partial: of this tile, parts * kValues values
+// of every thread.
+template <class T>
+__device__ inline bool join(T& tile, int part, int parts, float* partial, unsigned* done, bool& last) {
+    float* const mine = partial + threadIdx.x;
+    int at = 0;
+    tile.each([&](int, int, float& v) {
+        __hip_atomic_store(&mine[(part * T::kValues + at++) * kThreads], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    });
+    red::wait_stores_visible();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == unsigned(parts);
+        if (last) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return false;
+    tile.clear();
+    for (int q = 0; q < parts; ++q) {
+        at = 0;
+        tile.each([&](int, int, float& v) {
+            v += __hip_atomic_load(&mine[(q * T::kValues + at++) * kThreads], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        });
+    }
+    return true;
+}
 
 }  // namespace split
 }  // namespace vchip
