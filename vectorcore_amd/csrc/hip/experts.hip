@@ -157,6 +157,7 @@ struct ProductArgs {
     // Tiles of 64: parts of each tile's sum, workgroup w the part w / (grid / parts).
     int parts = 1;
     float* partial = nullptr;
+    int down = 1;  // of a weight's tiles: rectangles above each other, 8 / down side by side
 };
 
 struct RowTile {
@@ -210,10 +211,10 @@ __device__ inline RowTile find_rows(const int* __restrict__ offsets, int groups,
     return t;
 }
 
-// The tile of this workgroup: tiles are numbered group by group, their columns
-// together, and dealt out so that each of the chip's eight dies (workgroups go
-// to them in turn) works on neighbouring ones, which read the same operands
-// through its cache.
+// The tile of this workgroup. Row tiles are numbered group by group and taken
+// eight at a time, those of a column together; each of the chip's eight dies
+// (workgroups go to them in turn) gets neighbouring ones, which read the same
+// operands through its cache.
 template <int BM>
 __device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups, int64_t column_tiles, unsigned block) {
     const int lane = threadIdx.x % kWave;
@@ -228,7 +229,8 @@ __device__ inline RowTile find_tile(const int* __restrict__ offsets, int groups,
     const int64_t total = all * column_tiles, share = (total + 7) / 8;
     const int64_t id = block % 8 * share + block / 8;
     if (block / 8 >= share || id >= total) return RowTile{0, 0, 0, 0, false, 0};
-    RowTile t = find_rows<BM>(offsets, groups, int(id / column_tiles), id % column_tiles);
+    const int64_t strip = id / (8 * column_tiles), place = id % (8 * column_tiles), high = min(int64_t(8), all - 8 * strip);
+    RowTile t = find_rows<BM>(offsets, groups, int(8 * strip + place % high), place / high);
     t.id = id;
     return t;
 }
@@ -383,21 +385,23 @@ __global__ __launch_bounds__(split::kThreads, 2) void input_kernel(ProductArgs p
     });
 }
 
-// C[e] = sum over e's rows of x_r^T b[r]. Every die takes its part of each
-// expert's tiles, as experts differ in their rows.
+// C[e] = sum over e's rows of x_r^T b[r]. Every die takes a rectangle of each
+// expert's tiles (experts differ in their rows): that of `down` by `across`.
 template <int BM, int BN>
 __global__ __launch_bounds__(split::kThreads, 2) void weight_kernel(ProductArgs p) {
     __shared__ split::Slice<S, BM> as;
     __shared__ split::Slice<S, BN> bs;
     const int64_t row_tiles = (p.width + BM - 1) / BM, column_tiles = (p.columns + BN - 1) / BN;
-    const int64_t total = row_tiles * column_tiles, share = (total + 7) / 8;
+    const int64_t total = row_tiles * column_tiles, high = (row_tiles + p.down - 1) / p.down;
+    const int64_t wide = (column_tiles + 8 / p.down - 1) / (8 / p.down), share = high * wide;
     const int parts = BM == 64 ? p.parts : 1, blocks = int(gridDim.x) / parts, part = int(blockIdx.x) / blocks;
     const int block = int(blockIdx.x) % blocks, unit = int(block / 8 / share), group = unit % p.experts;
     const float* const grad = unit < p.experts ? p.b : p.b2;
     float* const out = unit < p.experts ? p.c : p.c2;
-    const int64_t id = block % 8 * share + block / 8 % share;
-    if (id >= total) return;
-    const int64_t m0 = id / column_tiles * BM, n0 = id % column_tiles * BN;
+    const int64_t row = block % 8 % p.down * high + block / 8 % share % high;
+    const int64_t column = block % 8 / p.down * wide + block / 8 % share / high, id = row * column_tiles + column;
+    if (row >= row_tiles || column >= column_tiles) return;
+    const int64_t m0 = row * BM, n0 = column * BN;
     const int begin = p.offsets[group], depth = p.offsets[group + 1] - begin;
     const auto source = [&](int64_t r) { return int64_t(p.token ? p.token[r] : r) * p.width; };
     split::Tile<S, BM, BN> tile;
@@ -882,20 +886,32 @@ int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, cons
                                int(q.experts), int64_t(width), int64_t(columns)};
         // 256 columns a tile where they fill the chip: x is then split half as often. (8 experts, 1024 x 4096 over 16384
         // rows: 809 us, with 128 columns 935. The products of rows gain nothing, as fewer tiles fit the CUs less evenly.)
-        const auto run = [&](auto bm, auto bn) {
-            const int64_t share = tiles_of(size_t(tiles_of(width, bm()) * tiles_of(columns, bn())), 8);
-            launch(weight_kernel<bm(), bn()>, tile_grid(products * int64_t(q.experts) * share * 8), dim3(split::kThreads), 0, d.stream, args);
+        const auto run = [&](auto bm, auto bn, ProductArgs a, int64_t parts) {
+            // The rectangles that read the least.
+            const int64_t rows = tiles_of(width, bm()), cols = tiles_of(columns, bn());
+            int64_t least = 0, share = 0;
+            for (int down = 1; down <= 8; down *= 2) {
+                const int64_t high = (rows + down - 1) / down, wide = (cols + 8 / down - 1) / (8 / down);
+                const int64_t reads = high * wide * 1024 + high * bm() + wide * bn();  // tiles first: rounding up adds empty ones
+                if (share == 0 || reads < least) {
+                    least = reads;
+                    share = high * wide;
+                    a.down = down;
+                }
+            }
+            launch(weight_kernel<bm(), bn()>, tile_grid(products * int64_t(q.experts) * share * 8) * parts, dim3(split::kThreads),
+                   0, d.stream, a);
         };
         using std::integral_constant;
         const int64_t row_tiles = products * int64_t(q.experts) * tiles_of(width, 128);
-        if (row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) run(integral_constant<int, 128>(), integral_constant<int, 256>());
-        else if (enough(d, row_tiles * tiles_of(columns, 128))) run(integral_constant<int, 128>(), integral_constant<int, 128>());
-        else {
+        if (row_tiles * tiles_of(columns, 256) >= 2 * d.cu_count) {
+            run(integral_constant<int, 128>(), integral_constant<int, 256>(), args, 1);
+        } else if (enough(d, row_tiles * tiles_of(columns, 128))) {
+            run(integral_constant<int, 128>(), integral_constant<int, 128>(), args, 1);
+        } else {
             const int64_t tiles = products * int64_t(q.experts) * tiles_of(width, 64) * tiles_of(columns, 64);
-            const int64_t share = tiles_of(size_t(tiles_of(width, 64) * tiles_of(columns, 64)), 8);
             const Parts parts(d, tiles, int64_t(q.rows / q.experts), 64 * 64);
-            launch(weight_kernel<64, 64>, tile_grid(products * int64_t(q.experts) * share * 8) * parts.parts, dim3(split::kThreads), 0,
-                   d.stream, parts(args));
+            run(integral_constant<int, 64>(), integral_constant<int, 64>(), parts(args), parts.parts);
         }
         after_launch("expert_backward_weight");
         p.done();
