@@ -51,7 +51,7 @@ struct Matrix {
     int64_t rows, cols, shorter, longer;  // the sides are padded to whole tiles
     int count, blocks;
     float rate;
-    int first, splits, counters;  // of the launch: the first workgroup, parts of each tile's sum, its first count
+    int first, splits, counters, parts;  // of the launch: the first workgroup (or die's), parts of a tile's sum, tiles and parts before
 
     __host__ __device__ int64_t elements() const { return rows * cols; }
     __host__ __device__ bool wide() const { return rows <= cols; }
@@ -159,23 +159,39 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
     using Tile = packed::Tile<BT, Stages>;
     __shared__ __align__(16) char lds[Tile::kLds];
     __shared__ bool finisher;
-    const Matrix& m = batch.of[find(batch, blockIdx.x)];
+    // Each of the chip's eight dies, which workgroups go to in turn, gets neighbouring tiles of every matrix,
+    // whose operands its cache then serves (16 of [1024, 4096] in order: see the figures above). Shares of the
+    // whole batch instead gave dies matrices of unlike depth, and the slowest took a quarter longer.
+    const Matrix& m = batch.of[find(batch, int(blockIdx.x) / 8)];
     const int row_tiles = int(m.shorter / BT), column_tiles = K == Kind::Apply ? int(m.longer / BT) : row_tiles;
     const int tiles = K == Kind::Apply ? row_tiles * column_tiles : row_tiles * (row_tiles + 1) / 2;
-    int id = int(blockIdx.x) - m.first;
+    const int blocks = m.count * tiles * m.splits, share = (blocks + 7) / 8;
+    int id = int(blockIdx.x) % 8 * share + int(blockIdx.x) / 8 - m.first;
+    if (id >= blocks) return;
     const int part = id % m.splits;
     id /= m.splits;
     const int64_t z = id / tiles;
-    const int tile_id = id % tiles;
-    int i = tile_id / column_tiles, j = tile_id % column_tiles;
-    if constexpr (K != Kind::Apply) {  // the tile_id-th with i <= j
-        i = 0;
-        j = tile_id;
-        while (j >= row_tiles - i) {
-            j -= row_tiles - i;
-            ++i;
+    // Strips of eight rows, column by column, of the tiles with i <= j where the product is symmetric.
+    int rest = id % tiles, i = 0, j = 0, high = 0;
+    for (;;) {
+        high = min(8, row_tiles - i);
+        const int triangle = K == Kind::Apply ? 0 : high * (high + 1) / 2, from = K == Kind::Apply ? 0 : i + high;
+        const int strip = triangle + high * (column_tiles - from);
+        if (rest >= strip) {
+            rest -= strip;
+            i += high;
+            continue;
         }
-        j += i;
+        if (rest < triangle) {
+            j = i;
+            for (int n = 1; rest >= n; ++n, ++j) rest -= n;
+            i += rest;
+        } else {
+            rest -= triangle;
+            j = from + rest / high;
+            i += rest % high;
+        }
+        break;
     }
     const int64_t m0 = int64_t(i) * BT, n0 = int64_t(j) * BT;
     const int64_t whole = z * 2 * m.shorter * m.longer, square = z * 2 * m.shorter * m.shorter;
@@ -190,7 +206,7 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
     if (m.splits > 1) {
         // The part that counts in last adds all of them in order.
         constexpr int kValues = BT * BT / packed::kThreads;
-        float* const mine = partial + (int64_t(blockIdx.x) - part) * BT * BT + threadIdx.x;
+        float* const mine = partial + (int64_t(m.parts) + int64_t(id) * m.splits) * BT * BT + threadIdx.x;
         int at = 0;
         tile.each4([&](int, int, float (&v)[4]) {
 #pragma unroll
@@ -201,7 +217,7 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
         red::wait_stores_visible();
         __syncthreads();
         if (threadIdx.x == 0) {
-            unsigned* const done = &g_tile_done[(int(blockIdx.x) - m.first) / m.splits + m.counters];
+            unsigned* const done = &g_tile_done[m.counters + id];
             finisher = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == unsigned(m.splits);
             if (finisher) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -280,17 +296,20 @@ void product(Device& d, Batch& batch, bool last = false, float keep = 0.0f) {
     int64_t tiles = 0;
     for (int i = 0; i < batch.n; ++i) tiles += tiles_of(K, batch.of[i], BT);
     const int64_t wanted = tiles > kMostSplit ? 1 : std::max<int64_t>(1, d.cu_count / tiles);
-    int64_t counters = 0;
+    int64_t counters = 0, blocks = 0;
     for (int i = 0; i < batch.n; ++i) {
         Matrix& m = batch.of[i];
         const int64_t slices = (K == Kind::Gram ? m.longer : m.shorter) / packed::kSlice;
         m.splits = int(std::max<int64_t>(1, std::min(wanted, slices / 8)));
         m.counters = int(counters);
+        m.parts = int(blocks);
         counters += tiles_of(K, m, BT);
+        blocks += tiles_of(K, m, BT) * m.splits;
+        if (blocks >= int64_t(1) << 30) fail(VC_HIP_ERR_OVERFLOW, "orthogonalise: too many tiles");
     }
-    const int64_t blocks = assign(batch, [](const Matrix& m) { return tiles_of(K, m, BT) * m.splits; });
+    const int64_t shares = assign(batch, [](const Matrix& m) { return (tiles_of(K, m, BT) * m.splits + 7) / 8; });
     Scratch partial(wanted > 1 ? size_t(blocks) * BT * BT * sizeof(float) : 4);
-    const dim3 grid{unsigned(blocks)}, threads{packed::kThreads};
+    const dim3 grid{unsigned(8 * shares)}, threads{packed::kThreads};
     if (blocks <= d.cu_count)
         launch(product_kernel<K, BT, 4>, grid, threads, 0, d.stream, batch, last, keep, partial.as<float>());
     else
