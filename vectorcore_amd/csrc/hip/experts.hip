@@ -653,9 +653,10 @@ dim3 operator*(dim3 grid, int64_t parts) {
 }
 
 // Whether tiles of 128 rows give every CU one; otherwise tiles of 64 halve or
-// quarter what each of them computes (THIN64).
+// quarter what each of them computes. A training pass of 8 experts, 1024 x 1024,
+// two a token, by tiles of 128 and of 64: 256 tokens 453 and 312 us, 1024 tokens
+// 555 and 505, 2048 tokens 800 and 799, 4096 tokens 1278 and 1327.
 bool enough(Device& d, int64_t tiles) { return tiles >= d.cu_count; }
-
 
 // (A lane's place in kThinDepth lines is a 32-bit offset.)
 bool thin(const Plan& plan, size_t columns) { return plan.rows <= kThinMost * plan.experts && columns <= size_t(1) << 20; }

@@ -20,6 +20,13 @@
 //
 // All matrices of a call run in the same launches, three an iteration: a train
 // step's matrices fill the chip together, and small ones share the latency.
+//
+// Bound by the matrix instructions where matrices are large: 1024 x 4096, 4096 x
+// 4096 and 4096 x 1000 take 434 us for the last product of an iteration (348
+// TFLOP/s), 258 for G (293) and 252 for P (279), of 408 TFLOP/s that a third of
+// the library's half-precision rate would be; the update and the first split are
+// 87 us each (4.3 TB/s). Small ones are bound by the latency of a launch and its
+// first loads: 784 x 256 and 256 x 10 take 24 us an iteration.
 #include "packed_product.hpp"
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"
@@ -289,8 +296,10 @@ int64_t tiles_of(Kind kind, const Matrix& m, int64_t bt) {
     return m.count * (kind == Kind::Apply ? t * (m.longer / bt) : t * (t + 1) / 2);
 }
 
-// Where tiles are few, sums are split into parts of at least eight slices. More
-// stages in flight where a CU has one workgroup at most.
+// Where tiles are few, sums are split into parts of at least eight slices (1024 x
+// 4096: 519 us, 817 with whole sums). More stages in flight where a CU has one
+// workgroup at most (1024 x 1024: 284 us, 348 with two stages; 2048 x 2048, with
+// more workgroups than that: 775 with two stages, 907 with four).
 template <Kind K, int BT>
 void product(Device& d, Batch& batch, bool last = false, float keep = 0.0f) {
     int64_t tiles = 0;
@@ -317,34 +326,39 @@ void product(Device& d, Batch& batch, bool last = false, float keep = 0.0f) {
     after_launch("orthogonalise product");
 }
 
-template <int BT>
-void iterate(Device& d, Batch& batch, float keep, size_t steps) {
-    for (size_t i = 0; i < steps; ++i) {
-        product<Kind::Gram, BT>(d, batch);
-        product<Kind::Poly, BT>(d, batch);
-        product<Kind::Apply, BT>(d, batch, i + 1 == steps, keep);
-        for (int k = 0; k < batch.n; ++k) {
-            std::swap(batch.of[k].x, batch.of[k].y);
-            std::swap(batch.of[k].xt, batch.of[k].yt);
-        }
-    }
-}
-
-// The iterates of a batch; x and its successor take turns. Tiles of 128 where
-// they give every other CU work, else of 64.
-void run(Device& d, Batch& batch, float mu, float keep, size_t steps) {
-    const auto padded = [](int64_t n, int64_t bt) { return (n + bt - 1) / bt * bt; };
-    int64_t tiles = 0;
+// Whether tiles of 128 give three of four CUs work, parts of a sum at least 1024
+// deep counted; four tiles of 64 read twice what one of 128 reads. Five
+// iterations, every product by tiles of 128 and of 64: 1024 x 1024 412 and 285
+// us, 2048 x 2048 869 and 814 (775 with 128 in the last product alone, as here),
+// 2816 x 2816 1535 and 1773, 4096 x 4096 4508 and 5087.
+bool wide_tiles(const Device& d, const Batch& batch, Kind kind) {
+    int64_t tiles = 0, blocks = 0;
+    for (int i = 0; i < batch.n; ++i) tiles += tiles_of(kind, batch.of[i], 128);
+    const int64_t wanted = std::max<int64_t>(1, d.cu_count / tiles);
     for (int i = 0; i < batch.n; ++i) {
         const Matrix& m = batch.of[i];
-        tiles += m.count * (padded(m.rows, 128) / 128) * (padded(m.cols, 128) / 128);
+        const int64_t depth = kind == Kind::Gram ? m.longer : m.shorter;
+        blocks += tiles_of(kind, m, 128) * std::max<int64_t>(1, std::min(wanted, depth / 1024));
     }
-    const int64_t bt = tiles >= d.cu_count / 2 ? 128 : 64;
+    return blocks >= d.cu_count * 3 / 4;
+}
+
+// The iterates of a batch; x and its successor take turns.
+void run(Device& d, Batch& batch, float mu, float keep, size_t steps) {
+    const auto pad = [&](int64_t to) {
+        for (int i = 0; i < batch.n; ++i) {
+            Matrix& m = batch.of[i];
+            m.shorter = (std::min(m.rows, m.cols) + to - 1) / to * to;
+            m.longer = (std::max(m.rows, m.cols) + to - 1) / to * to;
+        }
+    };
+    pad(128);
+    const bool wide_gram = wide_tiles(d, batch, Kind::Gram), wide_poly = wide_tiles(d, batch, Kind::Poly);
+    const bool wide_apply = wide_tiles(d, batch, Kind::Apply);
+    if (!wide_gram && !wide_poly && !wide_apply) pad(64);
     int64_t partials = 0, squares = 0, wholes = 0;
     for (int i = 0; i < batch.n; ++i) {
         Matrix& m = batch.of[i];
-        m.shorter = padded(std::min(m.rows, m.cols), bt);
-        m.longer = padded(std::max(m.rows, m.cols), bt);
         m.blocks = int(grid_1d(size_t(m.elements()), 1024, kNormBlocks));
         partials += int64_t(m.count) * m.blocks;
         squares += m.count * m.shorter * m.shorter;
@@ -379,8 +393,16 @@ void run(Device& d, Batch& batch, float mu, float keep, size_t steps) {
     blocks = assign(batch, [](const Matrix& m) { return m.count * (m.shorter / 64) * (m.longer / 64); });
     launch(pack_kernel, dim3(unsigned(blocks)), dim3(256), 0, d.stream, batch);
     after_launch("orthogonalise pack");
-    if (bt == 128) iterate<128>(d, batch, keep, steps);
-    else iterate<64>(d, batch, keep, steps);
+    for (size_t i = 0; i < steps; ++i) {
+        const bool last = i + 1 == steps;
+        wide_gram ? product<Kind::Gram, 128>(d, batch) : product<Kind::Gram, 64>(d, batch);
+        wide_poly ? product<Kind::Poly, 128>(d, batch) : product<Kind::Poly, 64>(d, batch);
+        wide_apply ? product<Kind::Apply, 128>(d, batch, last, keep) : product<Kind::Apply, 64>(d, batch, last, keep);
+        for (int k = 0; k < batch.n; ++k) {
+            std::swap(batch.of[k].x, batch.of[k].y);
+            std::swap(batch.of[k].xt, batch.of[k].yt);
+        }
+    }
 }
 
 void check_matrix(size_t count, size_t rows, size_t cols) {
