@@ -105,6 +105,36 @@ def test_ranks_a_rounding_apart(score, with_bias, device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_groups", [(256, 8, 3), (256, 1, 1), (128, 16, 5), (64, 16, 9), (192, 3, 2), (96, 8, 4)])
+@pytest.mark.parametrize("centre,spread", [(0.0, 1e-4), (-1.0, 1e-6), (3.0, 1e-7), (-30.0, 1.0), (-70.0, 4.0), (-90.0, 3.0)])
+@pytest.mark.parametrize("bias_scale", [1e-5, 1.0, 300.0])
+def test_ranks_at_all_distances(bias_scale, centre, spread, experts, groups, top_groups, score, device):
+    """Distances from far below 32 bits' to far above them, of scores and biases alone and together."""
+    rng = np.random.default_rng(experts + groups)
+    steps = np.exp(rng.uniform(-6, 0, (65, experts))) * rng.choice([-1, 1], (65, experts))
+    logits = (centre + spread * steps).astype(np.float32)
+    bias = (bias_scale * rng.choice([-1.0, 0.5, 0.5, 0.5, 1.0], experts)).astype(np.float32)
+    _, c = vc.route(vc.Tensor(logits, device=device), 7, score=score, groups=groups, top_groups=top_groups,
+                    bias=vc.Tensor(bias, device=device))
+    want = exact(logits, 7, bias, score, groups, top_groups)[1]
+    # Where 64 bits, too, cannot tell two ranks or groups' sums apart, the choice is either's: those rows are left out.
+    l = logits.astype(np.float64)
+    s = 1 / (1 + np.exp(-l)) if score == "sigmoid" else np.exp(l - l.max(1, keepdims=True))
+    ranks = (s if score == "sigmoid" else s / s.sum(1, keepdims=True)) + bias
+    least = 64 * np.finfo(np.float64).eps * np.abs(ranks).max()
+    strength = np.sort(np.sort(ranks.reshape(65, groups, -1), 2)[:, :, -2:].sum(2), 1)
+    cut = strength[:, -top_groups] - strength[:, -top_groups - 1] if top_groups < groups else np.full(65, np.inf)
+    kept = np.argsort(-np.sort(ranks.reshape(65, groups, -1), 2)[:, :, -2:].sum(2), axis=1, kind="stable")[:, :top_groups]
+    is_open = (kept[:, :, None] == np.arange(experts) // (experts // groups)).any(1)
+    best = np.sort(np.where(is_open, ranks, -np.inf), 1)[:, ::-1][:, :8]
+    clear = (np.minimum(cut, (best[:, :-1] - best[:, 1:]).min(1)) > least)
+    np.testing.assert_array_equal(c.numpy()[clear], want[clear])
+    if centre == 0.0 and bias_scale < 1e-3:
+        assert clear.sum() > 50
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalise", [True, False])
 def test_special_values(score, renormalise, device):
     """Masked experts (-inf), the lowest number, rows whose mask leaves nothing, NaN, +inf, saturated scores."""

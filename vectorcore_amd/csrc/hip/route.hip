@@ -11,9 +11,11 @@
 // row's 32-bit ranks cannot tell two candidates apart, its whole wavefront ranks
 // it again in double.
 //
-// Bound by HBM for many rows (the logits are read, the gradient is written), if
-// the vector instructions are few: sixteen lanes share a row, so four rows share
-// each step of a search or sum across lanes.
+// Many rows would be bound by HBM (the logits are read, the gradient is written)
+// and are, forward, by vector instructions still: sixteen lanes share a row, so
+// four rows share each step of a search or sum across lanes. 65536 rows of 256
+// experts: 50.6 us forward (1.4 TB/s), 17.1 us backward (67 MB written, 4.2 TB/s);
+// 4096 rows of 64: 4.1 and 3.9 us, a launch's latency.
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"
 
@@ -264,10 +266,56 @@ __device__ inline float score_of(float logit, bool sigmoid, float top, float inv
     return sigmoid ? 1.0f / (1.0f + expf(-logit)) : expf(logit - top) * inverse;
 }
 
+// The two largest of a set, joined with those of another set.
+__device__ inline void join_best(float& best, float& second, float other, float other_second) {
+    second = fmaxf(fminf(best, other), fmaxf(second, other_second));
+    best = fmaxf(best, other);
+}
+template <int Step, int N>
+__device__ inline void join_partners(float (&best)[N], float (&second)[N], int lane) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        join_best(best[j], second[j], red::partner<Step>(best[j], lane), red::partner<Step>(second[j], lane));
+}
+
+// Falling order, by odd-even merges.
+template <int N>
+__device__ inline void sort_keys(uint32_t (&key)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const uint32_t x = key[i + j], y = key[i + j + k];
+                        key[i + j] = max(x, y);
+                        key[i + j + k] = min(x, y);
+                    }
+}
+
+// 1 / (1 + exp(-x)) within 2^-21 of itself, or 2^-115 where x < -80: exp2(t)
+// with t = -x / ln 2, and what t's rounding leaves to first order.
+__device__ inline float quick_sigmoid(float x) {
+    const float log2e = 0x1.715476p+0f, rest = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;
+    x = fmaxf(x, -80.0f);
+    const float t = x * -log2e, low = fmaf(x, -rest, fmaf(x, -log2e, -t)), e = __builtin_amdgcn_exp2f(t);
+    return __builtin_amdgcn_rcpf(1.0f + fmaf(e, low * ln2, e));
+}
+
 // Exact: without a bias and groups the logits' own order is that of the ranks,
 // as long as doubles tell the scores apart. Otherwise the 32-bit ranks decide
-// where they are further apart than their errors: a score is within 2^-21 of
-// itself, a rank within 2^-20 of the largest score and bias.
+// where they are further apart than their errors: with M the largest score and
+// bias, a score is within 2^-21 of itself, a rank (at most 2 M) within 2^-20.6 M,
+// the difference of two within 2^-19.6 M and that of two groups' sums within 2^-18 M.
+//
+// A lane's ranks become fixed point numbers in units of 2^-26 of M's next power of
+// two, above four bits of the place in the lane: they differ, and are sorted once;
+// a pick is then the largest of sixteen first keys, and its lane moves up. (65536
+// rows of 256 experts, 8 of them in 4 of 8 groups: 50.6 us; 75.2 with every pick
+// looked for among all keys and each group's ranks read by one lane.)
 template <int NV, bool Exact>
 __global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
     __shared__ double scratch[kWaves][kWave * NV / 2];  // floats of four rows, or doubles of one
@@ -295,82 +343,155 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
         inverse = 1.0f / row_sum(total);
     }
     uint32_t key[NV];
-    float margin = 0.0f;
     if constexpr (Exact) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) key[i] = 64 * (i / 4) + 4 * l + i % 4 < experts ? order_key(v[i]) : 0;
     } else {
-        float most = 0.0f;
-        float* const ranks = reinterpret_cast<float*>(scratch[wave]) + r * (kWave * NV / 4);
+        float most = 0.0f, rank[NV];
+        if (p.bias) {
+            row_logits<NV>(p.bias, experts, l, rank);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) rank[i] = 0.0f;
+        }
+        // The scores take the logits' place.
+        if (p.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = quick_sigmoid(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = expf(v[i] - top) * inverse;
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = 64 * (i / 4) + 4 * l + i % 4;
-            const float score = score_of(v[i], p.sigmoid, top, inverse), bias = p.bias && e < experts ? p.bias[e] : 0.0f;
-            const float rank = score + bias;
-            again |= rank != rank;
-            most = fmaxf(most, fmaxf(score, fabsf(bias)));
-            key[i] = e < experts ? order_key(rank) : 0;
-            if (p.groups > 1) ranks[e] = rank;
+            const bool there = 64 * (i / 4) + 4 * l + i % 4 < experts;
+            const float score = v[i];
+            if (there) most = fmaxf(most, fmaxf(score, fabsf(rank[i])));
+            rank[i] = there ? score + rank[i] : -__builtin_huge_valf();
+            again |= rank[i] != rank[i];
         }
-        margin = row_max(most) * 0x1p-18f;  // twice the errors of two ranks
-        again |= !(margin < __builtin_huge_valf());
+        most = row_max(most);
+        again |= !(most > 0x1p-80f && most < __builtin_huge_valf());
+        const int unit = 26 - __builtin_amdgcn_frexp_expf(most);  // most < 2^(26 - unit)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int fixed = int(__builtin_amdgcn_ldexpf(rank[i], unit)) + (1 << 27);
+            key[i] = 64 * (i / 4) + 4 * l + i % 4 < experts ? uint32_t(fixed) << 4 | i : 0;
+        }
         if (p.groups > 1) {
-            wave_fence();
             const int size = experts / p.groups;
-            float best = -__builtin_huge_valf(), second = best;
-            if (l < p.groups) {
-                int at = l % size;  // each lane begins elsewhere: other banks
-                for (int i = 0; i < size; ++i) {
-                    const float rank = ranks[l * size + at];
-                    second = fmaxf(second, fminf(best, rank));
-                    best = fmaxf(best, rank);
-                    at = at + 1 == size ? 0 : at + 1;
+            const bool aligned = size >= 4 && size <= 64 && (size & (size - 1)) == 0;  // size / 4 lanes share a group
+            const int shift = 31 - __builtin_clz(size);
+            float* const ranks = reinterpret_cast<float*>(scratch[wave]) + r * (kWave * NV / 4);
+            float strength = 0.0f;
+            if (aligned) {
+                float best[NV / 4], second[NV / 4];
+#pragma unroll
+                for (int j = 0; j < NV / 4; ++j) {
+                    float other = fmaxf(rank[4 * j + 2], rank[4 * j + 3]);
+                    best[j] = fmaxf(rank[4 * j], rank[4 * j + 1]);
+                    second[j] = fminf(rank[4 * j], rank[4 * j + 1]);
+                    join_best(best[j], second[j], other, fminf(rank[4 * j + 2], rank[4 * j + 3]));
+                }
+                if (size > 4) join_partners<0>(best, second, lane);
+                if (size > 8) join_partners<1>(best, second, lane);
+                if (size > 16) join_partners<2>(best, second, lane);
+                if (size > 32) join_partners<3>(best, second, lane);
+                wave_fence();
+#pragma unroll
+                for (int j = 0; j < NV / 4; ++j) {
+                    const int e = 64 * j + 4 * l;
+                    if (e < experts && (e & (size - 1)) == 0) ranks[e >> shift] = best[j] + second[j];
+                }
+                wave_fence();
+                if (l < p.groups) strength = ranks[l];
+            } else {
+                wave_fence();
+#pragma unroll
+                for (int i = 0; i < NV; ++i) ranks[64 * (i / 4) + 4 * l + i % 4] = rank[i];
+                wave_fence();
+                float best = -__builtin_huge_valf(), second = best;
+                if (l < p.groups) {
+                    int at = l % size;  // each lane begins elsewhere: other banks
+                    for (int i = 0; i < size; ++i) {
+                        const float next = ranks[l * size + at];
+                        second = fmaxf(second, fminf(best, next));
+                        best = fmaxf(best, next);
+                        at = at + 1 == size ? 0 : at + 1;
+                    }
+                }
+                strength = size > 1 ? best + second : best;
+                wave_fence();
+                if (l < p.groups) ranks[l] = strength;
+                wave_fence();
+            }
+            const float margin = most * 0x1p-18f;
+            int before = 0, perhaps = -1;  // the groups that are stronger, and that may be (not itself)
+            for (int g = 0; g < p.groups; ++g) {
+                const float ahead = ranks[g] - strength;
+                before += ahead > margin;
+                perhaps += !(ahead < -margin);
+            }
+            again |= l < p.groups && before < p.top_groups && perhaps >= p.top_groups;
+            const uint32_t open = uint32_t(__ballot(l < p.groups && before < p.top_groups) >> (kLanes * r));
+            if (aligned) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (!(open >> ((64 * (i / 4) + 4 * l) >> shift) & 1)) key[i] = 0;
+            } else {
+                const uint32_t inverse_size = (65536 + size - 1) / size;  // e / size for e < 256
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const uint32_t e = 64 * (i / 4) + 4 * l + i % 4;
+                    if (!(open >> (e * inverse_size >> 16) & 1)) key[i] = 0;
                 }
             }
-            const float strength = size > 1 ? best + second : best;
-            wave_fence();
-            if (l < p.groups) ranks[l] = strength;
-            wave_fence();
-            int before = 0;
-            for (int g = 0; g < p.groups; ++g) {
-                const float other = ranks[g];
-                before += other > strength;
-                again |= g != l && l < p.groups && !(fabsf(other - strength) > 2.0f * margin);
-            }
-            const uint64_t open = __ballot(l < p.groups && before < p.top_groups) >> (kLanes * r);
-            const uint32_t inverse_size = (65536 + size - 1) / size;  // e / size for e < 256
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const uint32_t e = 64 * (i / 4) + 4 * l + i % 4;
-                if (!(open >> (e * inverse_size >> 16) & 1)) key[i] = 0;
-            }
         }
+        sort_keys(key);
     }
     int mine = 0;
-    float previous = 0.0f;
+    uint32_t previous = 0;
     for (int j = 0; j <= p.top_k; ++j) {
         uint32_t best = key[0];
+        if constexpr (Exact) {
 #pragma unroll
-        for (int i = 1; i < NV; ++i) best = max(best, key[i]);
+            for (int i = 1; i < NV; ++i) best = max(best, key[i]);
+        }
         best = row_max_key(best);
         // The candidate after the last pick is only compared with it.
-        const float value = order_value(best);
-        if (j > 0 && best != 0) {
-            const float gap = previous - value;
-            if (!Exact) again |= !(gap > margin);
-            else again |= gap > 0.0f && !(gap * (p.sigmoid ? expf(-fmaxf(value, 0.0f)) : 1.0f) > 1e-12f);
-            if (Exact) again |= (p.sigmoid ? value : value - top) < -600.0f && j < p.top_k;
+        if constexpr (Exact) {
+            const float value = order_value(best);
+            if (j > 0 && best != 0) {
+                const float gap = order_value(previous) - value;
+                again |= gap > 0.0f && !(gap * (p.sigmoid ? expf(-fmaxf(value, 0.0f)) : 1.0f) > 1e-12f);
+                again |= (p.sigmoid ? value : value - top) < -600.0f && j < p.top_k;
+            }
+        } else {
+            again |= j > 0 && best != 0 && (previous >> 4) - (best >> 4) <= 128;  // of 2^26: 2^-19
         }
-        previous = value;
+        previous = best;
         if (j == p.top_k) break;
         int at = 1 << 30;
+        if constexpr (Exact) {
 #pragma unroll
-        for (int i = NV - 1; i >= 0; --i)
-            if (key[i] == best) at = 64 * (i / 4) + 4 * l + i % 4;
-        at = row_min(at);
+            for (int i = NV - 1; i >= 0; --i)
+                if (key[i] == best) at = 64 * (i / 4) + 4 * l + i % 4;
+            at = row_min(at);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (at == 64 * (i / 4) + 4 * l + i % 4) key[i] = 0;
+            for (int i = 0; i < NV; ++i)
+                if (at == 64 * (i / 4) + 4 * l + i % 4) key[i] = 0;
+        } else {
+            const bool won = key[0] == best;
+            const uint32_t winners = uint32_t(__ballot(won) >> (kLanes * r)) & 0xFFFF;
+            const int i = best & 15;
+            again |= (winners & (winners - 1)) != 0;  // equal keys of two lanes
+            at = 64 * (i / 4) + 4 * (__ffs(winners) - 1) + i % 4;
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const uint32_t stays = key[n], next = n + 1 < NV ? key[n + 1] : 0u;
+                key[n] = won ? next : stays;
+            }
+        }
         if (l == j) mine = at;
     }
     const bool picked = l < p.top_k;
