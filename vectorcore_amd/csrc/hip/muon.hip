@@ -153,6 +153,131 @@ __global__ __launch_bounds__(256) void pack_kernel(Batch batch) {
     }
 }
 
+// ---- small matrices -----------------------------------------------------------------
+// Up to 64 by 256 or 32 by 512: a workgroup takes a matrix through the whole call in LDS, in
+// 32 x 32 tiles on the float32 matrix instructions, whose lane l holds row (of A)
+// or column (of B) l % 32 at k = l / 32. Which k meet is free as long as both
+// sides agree, so a lane reads four neighbouring ones at once.
+//
+// Five iterations, this and in tiles: 10 x 7 20 and 67 us, 64 x 64 39 and 72, 64 x
+// 256 80 and 83; 300 of 64 x 128 97 and 261. Bound by the chain of three products
+// and barriers on one CU; only for calls of such matrices alone, as next to larger
+// ones the tiles of small ones cost nothing.
+
+constexpr size_t kMostSteps = 64;  // of one launch
+constexpr int kShort = 64, kLong = 256, kSquareStride = kShort + 4;
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+__device__ inline f16v multiply4(f4 a, f4 b, f16v c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+// C += A B^T of 32 rows each, over k in [begin, end), multiples of 8.
+__device__ inline f16v multiply_rows(const float* a, const float* b, int stride, int begin, int end, f16v c) {
+    const int lane = red::lane_id(), at = lane % 32 * stride + lane / 32 * 4;
+#pragma unroll 2
+    for (int k = begin; k < end; k += 8)
+        c = multiply4(*reinterpret_cast<const f4*>(a + at + k), *reinterpret_cast<const f4*>(b + at + k), c);
+    return c;
+}
+// f(row, column, value) of a tile's values.
+template <class F>
+__device__ inline void each_value(const f16v& c, F&& f) {
+    const int lane = red::lane_id();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) f(e / 4 * 8 + lane / 32 * 4 + e % 4, lane % 32, c[e]);
+}
+
+__global__ __launch_bounds__(256) void small_kernel(Batch batch, float mu, float keep, int steps) {
+    __shared__ __align__(16) float x[kShort * (kLong + 4)], g[kShort * kSquareStride], q[kShort * kSquareStride];
+    __shared__ double sums[4];
+    const Matrix& m = batch.of[find(batch, blockIdx.x)];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int rows = int(m.rows), cols = int(m.cols), count = rows * cols;
+    const bool wide = m.wide();
+    const int tall_tiles = ((wide ? rows : cols) + 31) / 32, long_tiles = ((wide ? cols : rows) + 31) / 32;
+    const int stride = tall_tiles == 2 ? kLong + 4 : 2 * kLong + 4;  // rows of 16-byte groups that meet different banks
+    const int64_t base = int64_t(int(blockIdx.x) - m.first) * count;
+    for (int i = threadIdx.x; i < tall_tiles * 32 * stride; i += 256) x[i] = 0.0f;
+    __syncthreads();
+    const auto at = [&](int i) {
+        const int row = i / cols, col = i - row * cols;
+        return wide ? row * stride + col : col * stride + row;
+    };
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < count; i += 256) {
+        float v = m.grad[base + i];
+        if (m.momentum) {
+            const float next = m.momentum[base + i] * mu + v;
+            m.momentum[base + i] = next;
+            v = v + mu * next;
+        }
+        x[at(i)] = v;
+        sum += double(v) * double(v);
+    }
+    sum = red::wave_sum(sum);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    const double norm = sqrt(sums[0] + sums[1] + sums[2] + sums[3]), factor = norm == 0.0 ? 0.0 : 1.0 / norm;
+    for (int i = threadIdx.x; i < tall_tiles * 32 * stride; i += 256) x[i] = float(double(x[i]) * factor);
+    __syncthreads();
+    const f16v zero = {};
+    const int i0 = tall_tiles == 2 ? wave / 2 * 32 : 0, j0 = tall_tiles == 2 ? wave % 2 * 32 : 0;  // this wave's tile
+    for (int step = 0; step < steps; ++step) {
+        // G; a single tile's k is shared out to the waves.
+        if (tall_tiles == 2) {
+            each_value(multiply_rows(x + i0 * stride, x + j0 * stride, stride, 0, 32 * long_tiles, zero),
+                       [&](int r, int c, float v) { g[(i0 + r) * kSquareStride + j0 + c] = v; });
+        } else {
+            each_value(multiply_rows(x, x, stride, 8 * long_tiles * wave, 8 * long_tiles * (wave + 1), zero),
+                       [&](int r, int c, float v) { q[wave * 1024 + r * 32 + c] = v; });
+            __syncthreads();
+            for (int i = threadIdx.x; i < 1024; i += 256) {
+                const float* const part = q + i;
+                g[i / 32 * kSquareStride + i % 32] = (part[0] + part[1024]) + (part[2 * 1024] + part[3 * 1024]);
+            }
+        }
+        __syncthreads();
+        // Q = a I + b G + c G G
+        if (tall_tiles == 2 || wave == 0)
+            each_value(multiply_rows(g + i0 * kSquareStride, g + j0 * kSquareStride, kSquareStride, 0, 32 * tall_tiles, zero),
+                       [&](int r, int c, float v) {
+                           const int place = (i0 + r) * kSquareStride + j0 + c;
+                           q[place] = kB * g[place] + kC * v + (i0 + r == j0 + c ? kA : 0.0f);
+                       });
+        __syncthreads();
+        // X = Q X, whole columns a wave
+        for (int t = wave; t < long_tiles; t += 4) {
+            f16v upper = zero, lower = zero;
+            for (int k = 0; k < 32 * tall_tiles; k += 8) {
+                const int k0 = k + lane / 32 * 4, column = 32 * t + lane % 32;
+                f4 b;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) b[e] = x[(k0 + e) * stride + column];
+                upper = multiply4(*reinterpret_cast<const f4*>(q + lane % 32 * kSquareStride + k0), b, upper);
+                if (tall_tiles == 2)
+                    lower = multiply4(*reinterpret_cast<const f4*>(q + (32 + lane % 32) * kSquareStride + k0), b, lower);
+            }
+            each_value(upper, [&](int r, int c, float v) { x[r * stride + 32 * t + c] = v; });
+            if (tall_tiles == 2) each_value(lower, [&](int r, int c, float v) { x[(32 + r) * stride + 32 * t + c] = v; });
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < count; i += 256) {
+        if (m.param) m.param[base + i] = keep * m.param[base + i] - m.rate * x[at(i)];
+        else m.out[base + i] = x[at(i)];
+    }
+}
+
+bool small(const Matrix& m) {
+    const int64_t shorter = std::min(m.rows, m.cols);
+    return shorter <= kShort && std::max(m.rows, m.cols) <= (shorter <= 32 ? 2 * kLong : kLong);
+}
+
+// ---- matrices in tiles --------------------------------------------------------------
+
 enum class Kind { Gram, Poly, Apply };
 
 // Counts of the parts of a tile's sum that are done; zero between launches,
@@ -345,6 +470,12 @@ bool wide_tiles(const Device& d, const Batch& batch, Kind kind) {
 
 // The iterates of a batch; x and its successor take turns.
 void run(Device& d, Batch& batch, float mu, float keep, size_t steps) {
+    if (steps > 0 && steps <= kMostSteps && std::all_of(batch.of, batch.of + batch.n, small)) {
+        const int64_t matrices = assign(batch, [](const Matrix& m) { return int64_t(m.count); });
+        launch(small_kernel, dim3(unsigned(matrices)), dim3(256), 0, d.stream, batch, mu, keep, int(steps));
+        after_launch("orthogonalise small");
+        return;
+    }
     const auto pad = [&](int64_t to) {
         for (int i = 0; i < batch.n; ++i) {
             Matrix& m = batch.of[i];
