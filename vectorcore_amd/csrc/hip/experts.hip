@@ -633,13 +633,16 @@ int64_t tiles_at_most(const Plan& plan, int rows, size_t width, int columns) {
     return int64_t(plan.rows / rows + plan.experts + 1) * tiles_of(width, columns);
 }
 
-// Parts of a sum over `depth` for `tiles` tiles of 64, at least eight slices
-// each, and the memory for `values` of every tile and part.
+// Parts of a sum over `depth` for `tiles` tiles of 64, at least four slices each,
+// for four workgroups on every CU, and the memory for `values` of every tile and
+// part. (Training passes, this, two workgroups with eight slices, and six with
+// four: 256 tokens of 8 experts 1024 x 1024 207, 231 and 206 us; 999 of 5 experts
+// 131 x 515 144, 151 and 142; 2048 of 4 experts 512 x 512 184, 193 and 200.)
 struct Parts {
     int64_t parts;
     Scratch partial;
     Parts(Device& d, int64_t tiles, int64_t depth, int64_t values)
-        : parts(tiles > kSplitTiles ? 1 : std::max<int64_t>(1, std::min(2 * d.cu_count / std::max<int64_t>(1, tiles), depth / 256))),
+        : parts(tiles > kSplitTiles ? 1 : std::max<int64_t>(1, std::min(4 * d.cu_count / std::max<int64_t>(1, tiles), depth / 128))),
           partial(parts > 1 ? size_t(tiles * parts * values) * sizeof(float) : 4) {}
     ProductArgs operator()(ProductArgs args) const {
         args.parts = int(parts);
