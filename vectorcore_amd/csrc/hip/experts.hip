@@ -398,8 +398,9 @@ __global__ __launch_bounds__(split::kThreads, 2) void weight_kernel(ProductArgs 
     const int block = int(blockIdx.x) % blocks, unit = int(block / 8 / share), group = unit % p.experts;
     const float* const grad = unit < p.experts ? p.b : p.b2;
     float* const out = unit < p.experts ? p.c : p.c2;
-    const int64_t row = block % 8 % p.down * high + block / 8 % share % high;
-    const int64_t column = block % 8 / p.down * wide + block / 8 % share / high, id = row * column_tiles + column;
+    const int place = (block + unit) % 8;  // of the rectangle: those that are not whole go round the dies
+    const int64_t row = place % p.down * high + block / 8 % share % high;
+    const int64_t column = place / p.down * wide + block / 8 % share / high, id = row * column_tiles + column;
     if (row >= row_tiles || column >= column_tiles) return;
     const int64_t m0 = row * BM, n0 = column * BN;
     const int begin = p.offsets[group], depth = p.offsets[group + 1] - begin;
