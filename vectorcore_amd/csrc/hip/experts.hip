@@ -333,7 +333,7 @@ __global__ __launch_bounds__(split::kThreads, Gated && BM == 128 ? 3 : 2) void f
 
 // C[r] = a[r] @ b[group]^T (+ a2[r] @ b2[group]^T).
 template <int BM>
-__global__ __launch_bounds__(split::kThreads, 2) void input_kernel(ProductArgs p) {
+__global__ __launch_bounds__(split::kThreads, BM == 128 ? 3 : 2) void input_kernel(ProductArgs p) {
     __shared__ split::Slice<S, BM> as, bs;
     const int parts = BM == 64 ? p.parts : 1, tiles = int(gridDim.x) / parts, part = int(blockIdx.x) / tiles;
     const RowTile t = find_tile<BM>(p.offsets, p.experts + 1, (p.width + BM - 1) / BM, blockIdx.x % tiles);

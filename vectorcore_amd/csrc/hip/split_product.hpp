@@ -95,7 +95,16 @@ struct AlongK {
             }
         }
     }
-    // The last slice, of which k < depth are there.
+    // Zeros for the slice's first `n` k.
+    __device__ inline void drop(int n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool stays = 8 * int(threadIdx.x % kGroups) + i >= n;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) v[j][i] = stays ? v[j][i] : 0.0f;
+        }
+    }
+    // A slice of which k < depth are there.
     __device__ inline void load_rest(const float* const (&p)[kChunks], int64_t k0, int64_t depth) {
         const int64_t k = k0 + 8 * (threadIdx.x % kGroups);
 #pragma unroll
@@ -134,6 +143,14 @@ struct AcrossK {
             const auto from = line(k + i);
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) v[j][i] = from(j)[at[j]];
+        }
+    }
+    __device__ inline void drop(int n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool stays = 8 * int(threadIdx.x / 64) + i >= n;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) v[j][i] = stays ? v[j][i] : 0.0f;
         }
     }
     template <class Line>
@@ -235,14 +252,21 @@ struct Tile {
     }
 };
 
-// The products of k in [begin, end) onto a tile. load(a, b, k) reads a whole
-// slice, rest(a, b, k) the last one, of which (end - begin) % 32 are there. Ahead register sets
-// hold slices that are on their way: one where other workgroups of the CU hide
-// the wait, more for grids that leave a CU one or two.
+// The products of k in [begin, end) onto a tile. load(a, b, k) reads the slice
+// from k, rest(a, b, k) the last one, of which end - k are there. Ahead register
+// sets hold slices that are on their way: one where other workgroups of the CU
+// hide the wait, more for grids that leave a CU one or two.
+//
+// With one, the last slice ends at `end`, whatever the sum's length, so that it is
+// read like the others, and what it shares with the slice before it is dropped (a
+// training pass of 49152 rows of 64 experts, 1024 x 512, each with some other count:
+// 3388 us, 3444 with a last slice read value by value). With more this
+// gained nothing (2100 rows of 20 experts, 90 x 150: 105 and 100 us).
 template <int Ahead, class A, class B, class T, class SA, class SB, class Load, class Rest>
 __device__ inline void accumulate(T& tile, SA& as, SB& bs, int64_t begin, int64_t end, Load&& load, Rest&& rest) {
     A a[Ahead];
     B b[Ahead];
+    if (end <= begin) return;
     const auto multiply = [&](const A& x, const B& y, auto&& next) {
         x.store(as);
         y.store(bs);
@@ -253,16 +277,21 @@ __device__ inline void accumulate(T& tile, SA& as, SB& bs, int64_t begin, int64_
         __syncthreads();
     };
     if constexpr (Ahead == 1) {
-        const auto next = [&](int64_t k) {
-            if (k + kSliceK <= end) load(a[0], b[0], k);
-            else rest(a[0], b[0], k);
-        };
-        if (end <= begin) return;
-        next(begin);
-        for (int64_t k = begin; k < end; k += kSliceK)
+        const bool less = end < kSliceK;  // begin is a multiple of a slice
+        const int slices = int((end - begin + kSliceK - 1) / kSliceK);
+        const int shared = less ? 0 : int(begin + int64_t(slices) * kSliceK - end);
+        const auto at = [&](int s) { return min(begin + int64_t(s) * kSliceK, end - kSliceK); };
+        if (less) rest(a[0], b[0], begin);
+        else load(a[0], b[0], at(0));
+        for (int s = 0; s < slices; ++s) {
+            if (s + 1 == slices && shared) {
+                a[0].drop(shared);
+                b[0].drop(shared);
+            }
             multiply(a[0], b[0], [&] {
-                if (k + kSliceK < end) next(k + kSliceK);
+                if (s + 1 < slices) load(a[0], b[0], at(s + 1));
             });
+        }
     } else {
         const int full = int((end - begin) / kSliceK);
         // Always the same number of loads on their way (past the end the last slice is read again), so that the compiler
