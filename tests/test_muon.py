@@ -66,6 +66,16 @@ def test_iterate_around_the_largest_small_one(shape, steps):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("count,rows,cols", [(60, 500, 630), (60, 630, 500), (33, 513, 769)])
+def test_iterate_whose_last_round_of_tiles_is_split(count, rows, cols):
+    """More tiles than the chip holds at once; the ones left over belong to several matrices."""
+    g = (1e-3 * np.random.default_rng(count).standard_normal((count, rows, cols))).astype(np.float32)
+    for steps in (1, 2):
+        o = vc.orthogonalise(vc.Tensor(g, device="hip"), steps=steps).numpy().astype(np.float64)
+        assert (np.sqrt(((o - exact(g, steps)) ** 2).sum((-2, -1))) <= near((rows, cols), steps)).all()
+
+
+@pytest.mark.gpu
 def test_steps_of_small_matrices_with_and_without_a_large_one():
     rng = np.random.default_rng(3)
     shapes = [(64, 256), (10, 7), (4, 30, 64), (200, 40), (1, 1), (256, 10)]

@@ -22,10 +22,10 @@
 // step's matrices fill the chip together, and small ones share the latency.
 //
 // Bound by the matrix instructions where matrices are large: 1024 x 4096, 4096 x
-// 4096 and 4096 x 1000 take 434 us for the last product of an iteration (348
-// TFLOP/s), 258 for G (293) and 252 for P (279), of 408 TFLOP/s that a third of
+// 4096 and 4096 x 1000 take 449 us for the last product of an iteration (343
+// TFLOP/s), 271 for G (285) and 233 for P (304), of 408 TFLOP/s that a third of
 // the library's half-precision rate would be; the update and the first split are
-// 87 us each (4.3 TB/s). Small ones are bound by the latency of a launch and its
+// 88 us each (4.3 TB/s). Small ones are bound by the latency of a launch and its
 // first loads: 784 x 256 and 256 x 10 take 24 us an iteration.
 #include "packed_product.hpp"
 #include "reduce_common.hpp"
@@ -58,13 +58,14 @@ struct Matrix {
     int64_t rows, cols, shorter, longer;  // the sides are padded to whole tiles
     int count, blocks;
     float rate;
-    int first, splits, counters, parts;  // of the launch: the first workgroup (or die's), parts of a tile's sum, tiles and parts before
+    // Of the launch: the first workgroup (or die's); the tiles from `from`; parts of each one's sum; split tiles and parts before.
+    int first, from, tiles, splits, counters, parts;
 
     __host__ __device__ int64_t elements() const { return rows * cols; }
     __host__ __device__ bool wide() const { return rows <= cols; }
 };
 struct Batch {
-    Matrix of[kAtOnce];
+    Matrix of[kAtOnce + 1];  // of a product: also the tiles of the last round
     int n;
 };
 
@@ -297,14 +298,15 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
     const Matrix& m = batch.of[find(batch, int(blockIdx.x) / 8)];
     const int row_tiles = int(m.shorter / BT), column_tiles = K == Kind::Apply ? int(m.longer / BT) : row_tiles;
     const int tiles = K == Kind::Apply ? row_tiles * column_tiles : row_tiles * (row_tiles + 1) / 2;
-    const int blocks = m.count * tiles * m.splits, share = (blocks + 7) / 8;
+    const int blocks = m.tiles * m.splits, share = (blocks + 7) / 8;
     int id = int(blockIdx.x) % 8 * share + int(blockIdx.x) / 8 - m.first;
     if (id >= blocks) return;
     const int part = id % m.splits;
     id /= m.splits;
-    const int64_t z = id / tiles;
+    const int tile_id = id + m.from;
+    const int64_t z = tile_id / tiles;
     // Strips of eight rows, column by column, of the tiles with i <= j where the product is symmetric.
-    int rest = id % tiles, i = 0, j = 0, high = 0;
+    int rest = tile_id % tiles, i = 0, j = 0, high = 0;
     for (;;) {
         high = min(8, row_tiles - i);
         const int triangle = K == Kind::Apply ? 0 : high * (high + 1) / 2, from = K == Kind::Apply ? 0 : i + high;
@@ -425,24 +427,53 @@ int64_t tiles_of(Kind kind, const Matrix& m, int64_t bt) {
 // 4096: 519 us, 817 with whole sums). More stages in flight where a CU has one
 // workgroup at most (1024 x 1024: 284 us, 348 with two stages; 2048 x 2048, with
 // more workgroups than that: 775 with two stages, 907 with four).
+//
+// A CU has two workgroups with tiles of 128. Where the last round of them would
+// leave half of the places empty, its sums are split as well, and its tiles are
+// the last of the matrix with the most. (The matrices above, whose G and P have 600
+// tiles for 512 places: both products 532 to 504 us an iteration, P alone 264 to
+// 233; twice as many parts of the last round, or more, gained no more.)
 template <Kind K, int BT>
-void product(Device& d, Batch& batch, bool last = false, float keep = 0.0f) {
-    int64_t tiles = 0;
-    for (int i = 0; i < batch.n; ++i) tiles += tiles_of(K, batch.of[i], BT);
-    const int64_t wanted = tiles > kMostSplit ? 1 : std::max<int64_t>(1, d.cu_count / tiles);
-    int64_t counters = 0, blocks = 0;
+void product(Device& d, Batch batch, bool last = false, float keep = 0.0f) {
+    const auto slices = [](const Matrix& m) { return (K == Kind::Gram ? m.longer : m.shorter) / packed::kSlice; };
+    int64_t tiles = 0, most = 0;
     for (int i = 0; i < batch.n; ++i) {
         Matrix& m = batch.of[i];
-        const int64_t slices = (K == Kind::Gram ? m.longer : m.shorter) / packed::kSlice;
-        m.splits = int(std::max<int64_t>(1, std::min(wanted, slices / 8)));
+        const int64_t own = tiles_of(K, m, BT);
+        if (own >= int64_t(1) << 28) fail(VC_HIP_ERR_OVERFLOW, "orthogonalise: too many tiles");
+        m.from = 0;
+        m.tiles = int(own);
+        tiles += own;
+        if (own > batch.of[most].tiles) most = i;
+    }
+    const int64_t wanted = tiles > kMostSplit ? 1 : std::max<int64_t>(1, d.cu_count / tiles);
+    for (int i = 0; i < batch.n; ++i) {
+        Matrix& m = batch.of[i];
+        m.splits = int(std::max<int64_t>(1, std::min(wanted, slices(m) / 8)));
+    }
+    const int64_t places = 2 * d.cu_count, over = tiles % places;
+    if (BT == 128 && tiles > places && over && over <= places / 2 && batch.of[most].tiles > over && over <= kMostSplit) {
+        batch.of[most].tiles -= int(over);
+        Matrix& end = batch.of[batch.n++];
+        end = batch.of[most];
+        end.from = batch.of[most].tiles;
+        end.tiles = int(over);
+        end.splits = int(std::max<int64_t>(1, std::min(d.cu_count / over, slices(end) / 8)));
+    }
+    int64_t counters = 0, parts = 0, blocks = 0;
+    for (int i = 0; i < batch.n; ++i) {
+        Matrix& m = batch.of[i];
         m.counters = int(counters);
-        m.parts = int(blocks);
-        counters += tiles_of(K, m, BT);
-        blocks += tiles_of(K, m, BT) * m.splits;
+        m.parts = int(parts);
+        if (m.splits > 1) {
+            counters += m.tiles;
+            parts += int64_t(m.tiles) * m.splits;
+        }
+        blocks += int64_t(m.tiles) * m.splits;
         if (blocks >= int64_t(1) << 30) fail(VC_HIP_ERR_OVERFLOW, "orthogonalise: too many tiles");
     }
-    const int64_t shares = assign(batch, [](const Matrix& m) { return (tiles_of(K, m, BT) * m.splits + 7) / 8; });
-    Scratch partial(wanted > 1 ? size_t(blocks) * BT * BT * sizeof(float) : 4);
+    const int64_t shares = assign(batch, [](const Matrix& m) { return (int64_t(m.tiles) * m.splits + 7) / 8; });
+    Scratch partial(parts ? size_t(parts) * BT * BT * sizeof(float) : 4);
     const dim3 grid{unsigned(8 * shares)}, threads{packed::kThreads};
     if (blocks <= d.cu_count)
         launch(product_kernel<K, BT, 4>, grid, threads, 0, d.stream, batch, last, keep, partial.as<float>());
