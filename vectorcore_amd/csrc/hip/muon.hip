@@ -22,8 +22,8 @@
 // step's matrices fill the chip together, and small ones share the latency.
 //
 // Bound by the matrix instructions where matrices are large: 1024 x 4096, 4096 x
-// 4096 and 4096 x 1000 take 449 us for the last product of an iteration (343
-// TFLOP/s), 271 for G (285) and 233 for P (304), of 408 TFLOP/s that a third of
+// 4096 and 4096 x 1000 take 446 us for the last product of an iteration (346
+// TFLOP/s), 268 for G (288) and 231 for P (307), of 408 TFLOP/s that a third of
 // the library's half-precision rate would be; the update and the first split are
 // 88 us each (4.3 TB/s). Small ones are bound by the latency of a launch and its
 // first loads: 784 x 256 and 256 x 10 take 24 us an iteration.
