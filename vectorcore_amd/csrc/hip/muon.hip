@@ -24,8 +24,8 @@
 // Bound by the matrix instructions where matrices are large: 1024 x 4096, 4096 x
 // 4096 and 4096 x 1000 take 446 us for the last product of an iteration (346
 // TFLOP/s), 268 for G (288) and 231 for P (307), of 408 TFLOP/s that a third of
-// the library's half-precision rate would be; the update and the first split are
-// 88 us each (4.3 TB/s). Small ones are bound by the latency of a launch and its
+// the library's half-precision rate would be; the update and the first split
+// are 88 and 81 us (4.3 TB/s). Small ones are bound by the latency of a launch and its
 // first loads: 784 x 256 and 256 x 10 take 24 us an iteration.
 #include "packed_product.hpp"
 #include "reduce_common.hpp"
@@ -130,12 +130,19 @@ __global__ __launch_bounds__(256) void pack_kernel(Batch batch) {
     const int64_t across = m.longer / 64, tiles = across * (m.shorter / 64);
     const int64_t id = int(blockIdx.x) - m.first, z = id / tiles;
     const int64_t s0 = id % tiles / across * 64, l0 = id % across * 64;
-    const double factor = double(kScale) * inverse_norm(m, int(z));
     const float* const from = m.update + z * m.elements();
     const bool wide = m.wide();
-    for (int i = threadIdx.x / 64; i < 64; i += 4) {  // lines of the update
-        const int64_t row = (wide ? s0 : l0) + i, col = (wide ? l0 : s0) + threadIdx.x % 64;
-        const float v = row < m.rows && col < m.cols ? float(double(from[row * m.cols + col]) * factor) : 0.0f;
+    float line[16];  // of the update, read before the norm is known
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        const int64_t row = (wide ? s0 : l0) + threadIdx.x / 64 + 4 * n, col = (wide ? l0 : s0) + threadIdx.x % 64;
+        line[n] = row < m.rows && col < m.cols ? from[row * m.cols + col] : 0.0f;
+    }
+    const double factor = double(kScale) * inverse_norm(m, int(z));
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        const float v = float(double(line[n]) * factor);
+        const int i = threadIdx.x / 64 + 4 * n;
         if (wide) tile[i][threadIdx.x % 64] = v;
         else tile[threadIdx.x % 64][i] = v;
     }
@@ -293,8 +300,8 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
     __shared__ __align__(16) char lds[Tile::kLds];
     __shared__ bool finisher;
     // Each of the chip's eight dies, which workgroups go to in turn, gets neighbouring tiles of every matrix,
-    // whose operands its cache then serves (16 of [1024, 4096] in order: see the figures above). Shares of the
-    // whole batch instead gave dies matrices of unlike depth, and the slowest took a quarter longer.
+    // whose operands its cache then serves (an iteration of the large matrices above 1013 to 990 us). Shares of
+    // the whole batch instead gave dies matrices of unlike depth, and the last product took a quarter longer.
     const Matrix& m = batch.of[find(batch, int(blockIdx.x) / 8)];
     const int row_tiles = int(m.shorter / BT), column_tiles = K == Kind::Apply ? int(m.longer / BT) : row_tiles;
     const int tiles = K == Kind::Apply ? row_tiles * column_tiles : row_tiles * (row_tiles + 1) / 2;
