@@ -1,0 +1,165 @@
+"""Checks of recorded work and memory that another library writes: a result keeps the values that its operands had when
+it was asked for, once the work asked for is synchronised with the other library's write. test_shared_memory.py runs them;
+torch is imported first, so that the process has one HIP runtime."""
+
+import gc
+import sys
+from pathlib import Path
+
+import numpy as np
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
+
+import vectorcore_amd as vc  # noqa: E402
+
+N = 48
+
+
+def whole(seed, *shape):
+    """Small whole numbers: their products and sums are exact in any order."""
+    return np.random.default_rng(seed).integers(-4, 5, shape).astype(np.float32)
+
+
+def overwrite(*tensors):
+    """What a caller does before writing shared memory: the work asked for here is done, then the write is."""
+    vc.synchronize()
+    for t in tensors:
+        t.fill_(77.0)
+    if tensors[0].is_cuda:
+        torch.cuda.synchronize()
+
+
+def results(x, w, b):
+    """Name: result, of operations that may be recorded and computed later, which read x, w or b."""
+    other = vc.Tensor(whole(9, N, N), device=x.device)
+    return {"left": x @ other, "right": other @ w, "both": x @ w, "layer": other @ w + b, "bias": other @ other + b,
+            "relu": (x @ w + b).relu(), "late relu": (other @ other + b).relu()}
+
+
+def wanted(x, w, b):
+    o = whole(9, N, N)
+    return {"left": x @ o, "right": o @ w, "both": x @ w, "layer": o @ w + b, "bias": o @ o + b,
+            "relu": np.maximum(x @ w + b, 0), "late relu": np.maximum(o @ o + b, 0)}
+
+
+def elementwise(x, w):
+    """The same of elementwise operations whose operands want gradients."""
+    half = vc.Tensor(np.full((N, N), 0.5, np.float32), device=x.device)
+    return {"add": x + w, "chain": (x * 2.0 + w) * half - x, "one": x * 3.0, "rows": (x * w).sum(1), "columns": (x * w).sum(0),
+            "relu": (x - w).relu(), "mean": (x * 2.0).mean()}
+
+
+def elementwise_wanted(x, w):
+    return {"add": x + w, "chain": (x * 2 + w) * 0.5 - x, "one": x * 3, "rows": (x * w).sum(1), "columns": (x * w).sum(0),
+            "relu": np.maximum(x - w, 0), "mean": (x * 2).astype(np.float64).mean()}
+
+
+def compare(got, want):
+    for name in want:
+        np.testing.assert_allclose(got[name].numpy(), want[name], rtol=2.0 ** -23, atol=0, err_msg=name)
+
+
+def inputs(torch_device):
+    x, w, b = whole(1, N, N), whole(2, N, N), whole(3, N)
+    return (x, w, b), [torch.tensor(a, device=torch_device) for a in (x, w, b)]
+
+
+def check_results_of_imported_memory(device, torch_device):
+    host, shared = inputs(torch_device)
+    x, w, b = vc.from_dlpack(*shared)
+    got = results(x, w, b)
+    overwrite(*shared)
+    compare(got, wanted(*host))
+    compare(results(x, w, b), wanted(*(np.full_like(a, 77) for a in host)))  # what is asked for now reads what is there now
+
+
+def check_elementwise_results_of_imported_memory(device, torch_device):
+    host, shared = inputs(torch_device)
+    x, w, _ = vc.from_dlpack(*shared)
+    x.requires_grad = w.requires_grad = True
+    got = elementwise(x, w)
+    overwrite(*shared)
+    compare(got, elementwise_wanted(*host[:2]))
+
+
+def check_results_recorded_before_an_export(device, torch_device):
+    host, _ = inputs(torch_device)
+    x, w, b = (vc.Tensor(a, device=device) for a in host)
+    got = results(x, w, b)
+    leaves = [vc.Tensor(a, device=device, requires_grad=True) for a in host[:2]]
+    more = elementwise(*leaves)
+    shared = [torch.from_dlpack(t.detach()) for t in (x, w, b, *leaves)]
+    overwrite(*shared)
+    compare(got, wanted(*host))
+    compare(more, elementwise_wanted(*host[:2]))
+
+
+def check_results_of_exported_memory(device, torch_device):
+    host, _ = inputs(torch_device)
+    x, w, b = (vc.Tensor(a, device=device) for a in host)
+    shared = [torch.from_dlpack(t) for t in (x, w, b)]
+    got = results(x, w, b)
+    overwrite(*shared)
+    compare(got, wanted(*host))
+    # The other library lets go: nothing else writes the memory, and steps here keep what was recorded.
+    del shared
+    gc.collect()
+    got = results(x, w, b)
+    was = [t.numpy() for t in (x, w, b)]
+    vc.muon_step([x, w], [vc.Tensor.zeros((N, N), device=device) for _ in range(2)], 0.1,
+                 grads=[vc.Tensor(whole(5, N, N), device=device)] * 2)
+    compare(got, wanted(*was))
+    assert (x.numpy() != was[0]).any()
+
+
+def check_softmax_gradients(device, torch_device):
+    """The rule reads the operand as it was, also where another library writes it before the backward pass."""
+    values, up = np.random.default_rng(4).standard_normal((2, 70, 33)).astype(np.float32)
+    for log in (False, True):
+        def gradient(x, between):
+            x.requires_grad = True
+            y = x.log_softmax(1) if log else x.softmax(1)
+            between()
+            y.backward(vc.Tensor(up, device=device))
+            return x.grad.numpy()
+        want = gradient(vc.Tensor(values, device=device), lambda: None)
+        t = torch.tensor(values, device=torch_device)
+        np.testing.assert_array_equal(gradient(vc.from_dlpack(t)[0], lambda: overwrite(t)), want)
+        q = vc.Tensor(values, device=device)
+        np.testing.assert_array_equal(gradient(q, lambda: overwrite(torch.from_dlpack(q.detach()))), want)
+
+
+def check_gradients_of_a_pass_that_fails(device, torch_device):
+    """Gradients that a failing backward pass had stored already."""
+    seed = torch.tensor(whole(6, N, N), device=torch_device)
+    want = whole(6, N, N) * 2.0
+    a, b = (vc.Tensor(whole(s, N, N), device=device, requires_grad=True) for s in (7, 8))
+    spoilt = b * b
+    out = spoilt + a * 2.0
+    vc.muon_step([b], [vc.Tensor.zeros((N, N), device=device)], 0.1, grads=[vc.Tensor(whole(5, N, N), device=device)])
+    try:
+        out.backward(vc.from_dlpack(seed)[0])
+        raise AssertionError("the pass read an operand that had changed")
+    except RuntimeError as e:
+        assert "modified in place" in str(e)
+    overwrite(seed)
+    np.testing.assert_array_equal(a.grad.numpy(), want)
+
+
+RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_imported_memory,
+            check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
+            check_gradients_of_a_pass_that_fails]
+
+if __name__ == "__main__":
+    failed = []
+    for check in RECORDED:
+        try:
+            check("hip", "cuda")
+            print(check.__name__, "passed", flush=True)
+        except AssertionError as e:
+            failed.append(check.__name__)
+            print(check.__name__, "FAILED", str(e).strip().replace("\n", " ")[:300], flush=True)
+    torch.cuda.synchronize()
+    vc.synchronize()
+    print("all passed" if not failed else "failed", flush=True)

@@ -121,7 +121,7 @@ public:
 
     // Another library's memory (HipBackend::adopt).
     HipStorage(std::size_t elements, float* data, std::function<void()> release)
-        : elements_(elements), ptr_(data), shadow_valid_(false), pinned_(true),
+        : elements_(elements), ptr_(data), shadow_valid_(false),
           release_(std::make_unique<std::function<void()>>(std::move(release))) {}
 
     ~HipStorage() override {
@@ -348,15 +348,15 @@ public:
         }
         void* fresh_buffer = nullptr;
         check(vc_hip_alloc(bytes(), &fresh_buffer), "HIP allocation failed");
-        if (pinned_ || offset != 0 || count != elements_) {
+        if (shared() || offset != 0 || count != elements_) {
             const int status = vc_hip_copy(fresh_buffer, ptr_, bytes());
             if (status != VC_HIP_OK) {
                 (void)vc_hip_release(fresh_buffer);
                 throw_status(status, "HIP copy failed");
             }
         }
-        // Another library knows a pinned storage's buffer: the readers get the copy.
-        if (pinned_) std::swap(fresh_buffer, ptr_);
+        // Another library knows a shared storage's buffer: the readers get the copy.
+        if (shared()) std::swap(fresh_buffer, ptr_);
         auto previous = std::make_shared<HipStorage>(elements_, ptr_);  // takes over the current buffer
         ptr_ = fresh_buffer;
         for (const auto& r : waiting) {
@@ -369,12 +369,27 @@ public:
         return previous;
     }
 
-    // See HipBackend::expose: what is known of the contents here no longer holds
-    // once the other library writes them.
+    // Does another library hold this buffer's address? It may write the buffer
+    // without a word, so work that reads it is never left recorded, and nothing
+    // is kept of its contents.
+    bool shared() const {
+        std::lock_guard<std::recursive_mutex> lock(state_mutex());
+        return release_ != nullptr || exports_ > 0;
+    }
+
+    // See HipBackend::expose: work recorded on the contents is computed, and
+    // what is known of them here no longer holds once the other library writes.
     float* expose() {
         std::lock_guard<std::recursive_mutex> lock(state_mutex());
         (void)ptr();
-        pinned_ = true;
+        std::vector<std::shared_ptr<HipStorage>> waiting;
+        for (const auto& w : readers_) {
+            auto r = w.lock();
+            if (r && r.get() != this && r->reads_pending(this)) waiting.push_back(std::move(r));
+        }
+        for (const auto& r : waiting) r->settle();
+        readers_.clear();
+        ++exports_;
         shadow_valid_ = false;
         column_sum_.reset();
         row_argmax_.reset();
@@ -385,12 +400,36 @@ public:
         }
         return static_cast<float*>(ptr_);
     }
+    // The other library has let go.
+    void conceal() {
+        std::lock_guard<std::recursive_mutex> lock(state_mutex());
+        --exports_;
+    }
+
+    // Does a pending expression of this storage read memory shared with another library?
+    bool pending_on_shared() const;
 
 private:
     std::size_t bytes() const { return (elements_ ? elements_ : 1) * sizeof(float); }
     // Does work still deferred on this storage read s?
     bool reads_pending(const HipStorage* s) const {
         return (deferred_ && deferred_->reads(s)) || (map_ && expr_reads(*map_, s)) || (sum_of_ && expr_reads(*sum_of_, s));
+    }
+
+    // Computes what is recorded; a snapshot becomes a copy of what it stands for.
+    void settle() {
+        if (!map_ || map_->kind != MapNode::Kind::Input) {
+            (void)ptr();
+            return;
+        }
+        void* copy = nullptr;
+        check(vc_hip_alloc(bytes(), &copy), "HIP allocation failed");
+        const int status = vc_hip_copy(copy, map_->input->ptr() + map_->offset, elements_ * sizeof(float));
+        if (status != VC_HIP_OK) {
+            (void)vc_hip_release(copy);
+            throw_status(status, "HIP copy failed");
+        }
+        set_computed(copy);
     }
 
     std::size_t elements_;
@@ -411,7 +450,7 @@ private:
     mutable std::shared_ptr<HipStorage> relu_bits_;  // see relu_bits
     mutable std::size_t relu_bits_rows_ = 0, relu_bits_cols_ = 0;
     bool shadow_valid_;
-    bool pinned_ = false;  // another library holds this buffer's address
+    int exports_ = 0;  // that other libraries hold
     std::unique_ptr<std::function<void()>> release_;  // of another library's memory
 };
 
@@ -720,15 +759,28 @@ void expr_inputs(const MapNode& root, std::vector<std::shared_ptr<HipStorage>>& 
             out.push_back(n->input);
 }
 
+// A backward pass computes what it has recorded before it returns; anything
+// else that reads memory of another library is computed at once.
 std::shared_ptr<HipStorage> pending_storage(std::size_t elements, MapExpr expr, std::size_t summed = 0,
                                             bool row_sums = false) {
     auto out = summed ? std::make_shared<HipStorage>(elements, expr, summed, row_sums)
                       : std::make_shared<HipStorage>(elements, expr);
     std::vector<std::shared_ptr<HipStorage>> inputs;
     expr_inputs(*expr, inputs);
-    for (const auto& in : inputs) in->add_reader(out);
+    bool shared = false;
+    for (const auto& in : inputs) {
+        in->add_reader(out);
+        shared = shared || in->shared();
+    }
     if (t_elementwise_depth > 0) t_pending.push_back(out);
+    else if (shared) (void)out->ptr();
     return out;
+}
+
+bool reads_shared(const MapNode& root) {
+    for (const MapNode* n : nodes_of(root))
+        if (n->kind == MapNode::Kind::Input && n->input->shared()) return true;
+    return false;
 }
 
 // How an operand of `shape` (contiguous) broadcasts to out_shape viewed as a
@@ -829,6 +881,11 @@ bool views_agree(const Broadcast& a, const Broadcast& b) {
 }
 
 }  // namespace
+
+bool HipStorage::pending_on_shared() const {
+    std::lock_guard<std::recursive_mutex> lock(state_mutex());
+    return (map_ && reads_shared(*map_)) || (sum_of_ && reads_shared(*sum_of_));
+}
 
 HipBackend& HipBackend::instance() {
     static HipBackend backend;
@@ -1241,7 +1298,18 @@ HipBackend::ElementwiseScope::ElementwiseScope() {
     if (t_elementwise_depth++ == 0) t_pending.clear();
 }
 HipBackend::ElementwiseScope::~ElementwiseScope() {
-    if (--t_elementwise_depth == 0) t_pending.clear();  // what is still pending is computed on first use
+    if (--t_elementwise_depth > 0) return;
+    // What a pass that failed has recorded is computed on first use, or now where it reads another library's memory.
+    for (const auto& w : t_pending) {
+        const auto p = w.lock();
+        if (!p || !p->pending_on_shared()) continue;
+        try {
+            (void)p->ptr();
+        } catch (const std::exception&) {
+            continue;  // its first use will say so
+        }
+    }
+    t_pending.clear();
 }
 
 void HipBackend::flush_elementwise() {
@@ -1293,6 +1361,7 @@ std::shared_ptr<Storage> HipBackend::matmul_deferred(const std::shared_ptr<Stora
     if (!ha || !hb) throw std::invalid_argument("expected HIP storage");
     if (a_offset + m * k > ha->size() || b_offset + k * n > hb->size())
         throw std::out_of_range("HIP matmul operand exceeds storage");
+    if (ha->shared() || hb->shared()) return nullptr;
     // An operand that is itself a deferred product is computed now: nothing
     // more can join its epilogue once a product reads it, launching it here
     // lets the device start while the host records the rest, and no record
@@ -1326,7 +1395,7 @@ std::shared_ptr<Storage> HipBackend::add_bias_deferred(const Storage& product, s
         return nullptr;
     const bool row = (bias_shape == Shape{d->n} || bias_shape == Shape{1, d->n}) &&
                      bias_strides == contiguous_strides(bias_shape) && bias_offset + d->n <= hbias->size();
-    if (!row) return nullptr;
+    if (!row || hbias->shared()) return nullptr;
     (void)hbias->ptr();  // a deferred bias is computed now, as a product's operands are
     d->bias = hbias;
     d->bias_offset = bias_offset;
@@ -1422,6 +1491,11 @@ std::shared_ptr<Storage> HipBackend::snapshot(const std::shared_ptr<Storage>& so
     if (!h) throw std::invalid_argument("expected HIP storage");
     if (offset + count > h->size()) throw std::out_of_range("HIP snapshot exceeds storage");
     (void)h->ptr();
+    if (h->shared()) {
+        auto copy = fresh(count);
+        check(vc_hip_copy(copy->ptr(), h->ptr() + offset, count * sizeof(float)), "HIP copy failed");
+        return copy;
+    }
     auto n = std::make_shared<MapNode>();
     n->kind = MapNode::Kind::Input;
     n->input = h;
@@ -1733,6 +1807,7 @@ std::shared_ptr<Storage> HipBackend::adopt(float* data, std::size_t elements, st
 }
 
 float* HipBackend::expose(Storage& storage) { return as_hip(storage).expose(); }
+void HipBackend::conceal(Storage& storage) { as_hip(storage).conceal(); }
 
 std::optional<float> hip_host_scalar(const Storage& storage) {
     const auto* h = dynamic_cast<const HipStorage*>(&storage);

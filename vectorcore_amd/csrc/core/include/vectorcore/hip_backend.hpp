@@ -135,7 +135,9 @@ public:
     // gradient record expressions too (ForwardScope, one per op): the backward
     // pass computes again what its rules read of them, in the programs that
     // compute the gradients, and the pass's result with them (include); what
-    // else is read is computed then.
+    // else is read is computed then. Nothing stays recorded after the call that
+    // reads memory of another library (adopt, expose): who writes it has only
+    // the work enqueued here to wait for.
     class ForwardScope {
     public:
         explicit ForwardScope(bool defer);
@@ -281,9 +283,12 @@ public:
     // called, which is once the work enqueued before the storage died is done.
     // In-place ops write to that memory.
     [[nodiscard]] std::shared_ptr<Storage> adopt(float* data, std::size_t elements, std::function<void()> release);
-    // The buffer of a storage for another library, computed; it stays the
-    // storage's buffer from now on, also across in-place writes.
+    // The buffer of a storage for another library, computed, and with it what
+    // is recorded on its contents; it stays the storage's buffer, also across
+    // in-place writes, until the library that it was given to has let go
+    // (conceal, once for each expose).
     [[nodiscard]] float* expose(Storage& storage);
+    void conceal(Storage& storage);
 };
 
 // Host-side value of a one-element hip storage created from host data, if it

@@ -227,6 +227,7 @@ inline py::capsule export_(const Tensor& t, const py::object& stream, const py::
         const std::unique_ptr<Exported> mine(static_cast<Exported*>(m->context));
         // The buffer's next use here comes after the consumer's last one.
         if (mine->ordered) (void)vc_hip_wait_for_stream(mine->stream);
+        if (mine->managed.tensor.device.type == kRocm) HipBackend::instance().conceal(*mine->storage);
     };
     py::capsule out(&e->managed, "dltensor", [](PyObject* capsule) {
         if (!PyCapsule_IsValid(capsule, "dltensor")) return;  // taken
