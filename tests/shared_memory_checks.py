@@ -1,4 +1,4 @@
-"""Checks of recorded work and memory that another library writes: a result keeps the values that its operands had when
+"""Checks of recorded work, kept knowledge and memory that another library writes: a result keeps the values that its operands had when
 it was asked for, once the work asked for is synchronised with the other library's write. test_shared_memory.py runs them;
 torch is imported first, so that the process has one HIP runtime."""
 
@@ -147,13 +147,38 @@ def check_gradients_of_a_pass_that_fails(device, torch_device):
     np.testing.assert_array_equal(a.grad.numpy(), want)
 
 
+def check_largest_class_after_a_write(device, torch_device):
+    """The loss may keep each row's argmax; after a write from outside it is that of the new values."""
+    rows, classes = 40, 23
+    targets = list(range(10)) * 4
+    first, second = np.random.default_rng(5).standard_normal((2, rows, classes)).astype(np.float32)
+    t = torch.tensor(first, device=torch_device)
+    x = vc.from_dlpack(t)[0]
+    q = vc.Tensor(first, device=device)
+    shared = torch.from_dlpack(q)
+    for mine, theirs in ((x, t), (q, shared)):
+        vc.cross_entropy(mine, targets).item()
+        vc.synchronize()
+        theirs.copy_(torch.tensor(second))
+        if theirs.is_cuda:
+            torch.cuda.synchronize()
+        np.testing.assert_array_equal(mine.argmax(1).numpy(), second.argmax(1))
+    # One exported and let go of between the loss and the argmax.
+    q = vc.Tensor(first, device=device)
+    vc.cross_entropy(q, targets).item()
+    overwrite(torch.from_dlpack(q))
+    gc.collect()
+    np.testing.assert_array_equal(q.argmax(1).numpy(), np.zeros(rows))
+
+
 RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_imported_memory,
             check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
             check_gradients_of_a_pass_that_fails]
+KEPT = [check_largest_class_after_a_write]
 
 if __name__ == "__main__":
     failed = []
-    for check in RECORDED:
+    for check in RECORDED + KEPT:
         try:
             check("hip", "cuda")
             print(check.__name__, "passed", flush=True)

@@ -14,7 +14,7 @@ import shared_memory_checks as checks  # noqa: E402
 SCRIPT = Path(__file__).with_name("shared_memory_checks.py")
 
 
-@pytest.mark.parametrize("check", checks.RECORDED, ids=lambda c: c.__name__)
+@pytest.mark.parametrize("check", checks.RECORDED + checks.KEPT, ids=lambda c: c.__name__)
 def test_on_the_host(check):
     check("cpu", "cpu")
 

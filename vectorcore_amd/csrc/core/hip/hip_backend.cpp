@@ -253,6 +253,7 @@ public:
     void set_row_argmax(std::shared_ptr<HipStorage> indices, std::size_t offset, std::size_t rows,
                         std::size_t cols) const {
         std::lock_guard<std::recursive_mutex> lock(state_mutex());
+        if (shared()) return;  // the rows may change without a word
         row_argmax_ = std::move(indices);
         row_argmax_offset_ = offset;
         row_argmax_rows_ = rows;
