@@ -171,16 +171,46 @@ def check_largest_class_after_a_write(device, torch_device):
     np.testing.assert_array_equal(q.argmax(1).numpy(), np.zeros(rows))
 
 
+def check_order_of_later_writes():
+    """Neither side waits for the host: importing and exporting a tensor again orders what was enqueued since."""
+    n = 1 << 22
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.default_stream(), side):
+        with torch.cuda.stream(stream):
+            t = torch.zeros(n, device="cuda")
+            p = vc.from_dlpack(t)[0]
+            p.requires_grad = True
+            (p * 3.0).sum().backward()
+            m = torch.ones(2048, 2048, device="cuda")
+            for i in range(3):
+                for _ in range(6):  # keeps torch's stream busy
+                    m = (m @ m).clamp(max=1.0)
+                before = t + m[0, 0] - 1.0  # read late
+                vc.from_dlpack(t)           # the step waits for that
+                vc.sgd_step([p], 1.0)
+                torch.from_dlpack(p.detach())  # torch waits for the step
+                after = t.clone()
+                for _ in range(6):
+                    m = (m @ m).clamp(max=1.0)
+                t.add_(m[0, 0])
+                vc.from_dlpack(t)
+                late = p.detach() * 2.0
+                assert (before == -2.0 * i).all().item()
+                assert (after == -2.0 * i - 3.0).all().item()
+                assert (late.numpy() == 2 * (-2.0 * i - 2.0)).all()
+
+
 RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_imported_memory,
             check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
             check_gradients_of_a_pass_that_fails]
 KEPT = [check_largest_class_after_a_write]
+GPU = [check_order_of_later_writes]
 
 if __name__ == "__main__":
     failed = []
-    for check in RECORDED + KEPT:
+    for check in RECORDED + KEPT + GPU:
         try:
-            check("hip", "cuda")
+            check(*(() if check in GPU else ("hip", "cuda")))
             print(check.__name__, "passed", flush=True)
         except AssertionError as e:
             failed.append(check.__name__)

@@ -150,7 +150,7 @@ PYBIND11_MODULE(_vectorcore, m) {
              },
              py::kw_only(), py::arg("stream") = py::none(), py::arg("max_version") = py::none(),
              py::arg("dl_device") = py::none(), py::arg("copy") = py::none(),
-             "A DLPack capsule of the tensor's memory; the given stream waits for the work enqueued on it.")
+             "A DLPack capsule of the tensor's memory; the given stream waits for the work enqueued on it until now.")
         .def("__dlpack_device__", &dlpack::device_of)
         .def("__repr__", &Tensor::repr)
         .def("__matmul__", &Tensor::matmul, py::is_operator())
@@ -241,7 +241,8 @@ PYBIND11_MODULE(_vectorcore, m) {
         "lr * sqrt(max(1, cols / rows)) * orthogonalise(g + momentum * m). g: `grads`, or the parameters' own gradients.");
     m.def("from_dlpack", &dlpack::import_,
           "Tensors over the memory of the given objects (__dlpack__): float32, contiguous, on the host or the GPU. Always a "
-          "tuple.");
+          "tuple. Work asked for here from now on waits for what the other library's stream holds now; call it again, or "
+          "synchronise, after the other library has enqueued more that this one's writes or reads must wait for.");
     m.def("zero_grad", [](std::vector<Tensor> params) {
         for (auto& p : params) p.zero_grad();
     });

@@ -5,9 +5,16 @@
 // that the protocol fixes.
 //
 // Order of work: the hip device works on a stream of its own. An import makes
-// it wait for the producer's stream and an export makes the consumer's wait
-// for it, so neither side has to synchronise. A buffer that the other side
-// frees is kept until the work enqueued on it is done.
+// it wait for what the producer's stream holds then, and an export makes the
+// consumer's wait for what the hip device's holds then. Nothing orders what
+// either side enqueues later: before one side writes memory that the other may
+// still read, or reads what the other has written since, the program imports
+// (the other side's work first) or exports (this side's first) the tensor again,
+// or synchronises. Work asked for here counts as enqueued: none that reads
+// shared memory stays recorded. Versions count the writes made here alone, so an
+// operand that autograd has saved must not be written by the other side before
+// the backward pass. A buffer that the other side frees is kept until the work
+// enqueued on it is done.
 #include "vectorcore/detail/tensor_impl.hpp"
 #include "vectorcore/hip_backend.hpp"
 #include "vectorcore/vectorcore.hpp"
