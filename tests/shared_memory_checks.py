@@ -171,6 +171,18 @@ def check_largest_class_after_a_write(device, torch_device):
     np.testing.assert_array_equal(q.argmax(1).numpy(), np.zeros(rows))
 
 
+def check_negative_views(device, torch_device):
+    """torch negates these when it reads them: the memory holds other values."""
+    z = torch.tensor([1 + 2j], device=torch_device).conj()
+    for view in (z.imag, torch.arange(4.0, device=torch_device)._neg_view()):
+        try:
+            vc.from_dlpack(view)
+            raise AssertionError("taken with the wrong sign")
+        except ValueError as e:
+            assert "resolve_neg" in str(e)
+        np.testing.assert_array_equal(vc.from_dlpack(view.resolve_neg())[0].numpy(), view.resolve_neg().cpu().numpy())
+
+
 def check_order_of_later_writes():
     """Neither side waits for the host: importing and exporting a tensor again orders what was enqueued since."""
     n = 1 << 22
@@ -203,7 +215,7 @@ def check_order_of_later_writes():
 RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_imported_memory,
             check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
             check_gradients_of_a_pass_that_fails]
-KEPT = [check_largest_class_after_a_write]
+KEPT = [check_largest_class_after_a_write, check_negative_views]
 GPU = [check_order_of_later_writes]
 
 if __name__ == "__main__":

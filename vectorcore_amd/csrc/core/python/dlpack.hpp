@@ -172,6 +172,8 @@ inline py::tuple import_(const py::args& objects) {
         if (torch && py::isinstance(object, torch->tensor)) {
             if (object.attr("requires_grad").cast<bool>())
                 throw std::invalid_argument("from_dlpack: detach() a torch tensor that requires gradients");
+            if (object.attr("is_neg")().cast<bool>())  // its memory holds the negated values
+                throw std::invalid_argument("from_dlpack: resolve_neg() a torch tensor that is a negative view");
             if (!waited && object.attr("is_cuda").cast<bool>()) {
                 waited = true;
                 require_one_runtime();
