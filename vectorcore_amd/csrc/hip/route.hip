@@ -262,8 +262,14 @@ __device__ inline void row_logits(const float* __restrict__ row, int experts, in
     }
 }
 
+// exp(a - b), with what the difference's rounding leaves to first order: far
+// below the top that would be most of the error.
+__device__ inline float exp_difference(float a, float b) {
+    const float d = a - b, back = d - a, rest = (a - (d - back)) - (b + back), e = expf(d);
+    return fabsf(rest) < 1.0f ? fmaf(e, rest, e) : e;  // no rest of infinities
+}
 __device__ inline float score_of(float logit, bool sigmoid, float top, float inverse) {
-    return sigmoid ? 1.0f / (1.0f + expf(-logit)) : expf(logit - top) * inverse;
+    return sigmoid ? 1.0f / (1.0f + expf(-logit)) : exp_difference(logit, top) * inverse;
 }
 
 // The two largest of a set, joined with those of another set.
@@ -497,7 +503,7 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
     const bool picked = l < p.top_k;
     const float score = picked ? score_of(row[min(mine, experts - 1)], p.sigmoid, top, inverse) : 0.0f;
     const float total = row_sum(score);
-    again |= !(total > 0.0f);
+    again |= picked && !(score > 0x1p-100f);  // the least scores lose bits, and their quotients with them
     if (picked && first + r < p.tokens) {
         p.weights[t * p.top_k + l] = p.renormalise ? score / total : score;
         p.chosen[t * p.top_k + l] = float(mine);
