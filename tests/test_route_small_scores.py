@@ -41,13 +41,16 @@ def exact(logits, chosen, score, renormalise, grad):
 def check(logits, top_k, score, renormalise, device, **kwargs):
     rng = np.random.default_rng(top_k)
     grad = rng.standard_normal((len(logits), top_k)).astype(np.float32)
-    w, c = vc.route(vc.Tensor(logits, device=device), top_k, score=score, renormalise=renormalise, **kwargs)
+    l = vc.Tensor(logits, requires_grad=True, device=device)
+    w, c = vc.route(l, top_k, score=score, renormalise=renormalise, **kwargs)
+    w.backward(vc.Tensor(grad, device=device))
     chosen = c.numpy().astype(int)
     want_w, want_d, scale = exact(logits, chosen, score, renormalise, grad)
     # An exponential, its argument off by a rounding of a number below 16, a sum over the experts and a quotient. What
     # lies below the least normal number has fewer bits.
     rel = (48 + 2 * np.log2(logits.shape[1] + 1)) * UNIT
     np.testing.assert_allclose(w.numpy(), want_w, rtol=rel, atol=1e-38)
+    assert (np.abs(l.grad.numpy() - want_d) <= 4 * rel * scale + 1e-37).all()
     return chosen
 
 
@@ -90,3 +93,7 @@ def test_two_small_scores(device):
     w, c = vc.route(l, 2, score="sigmoid")
     np.testing.assert_array_equal(c.numpy(), [[2, 3]] * 3)
     np.testing.assert_allclose(w.numpy()[:2], [[0.7310585786, 0.2689414214]] * 2, rtol=64 * UNIT)
+    w.backward(vc.Tensor(np.array([[1, -1], [1, 0], [0.5, 0.5]], np.float32), device=device))
+    slope = 0.7310585786 * 0.2689414214
+    np.testing.assert_allclose(l.grad.numpy()[:2, 2:4], [[2 * slope, -2 * slope], [slope, -slope]], rtol=64 * UNIT)
+    np.testing.assert_allclose(l.grad.numpy()[2], np.zeros(8), atol=64 * UNIT)

@@ -118,9 +118,10 @@ void route_backward(const float* logits, const float* chosen, const float* grad_
                 d[static_cast<std::size_t>(chosen[t * top_k + j])] = renormalise ? (g - dot / total) / total : g;
             }
             const double mean = renormalise ? 0.0 : dot;  // the renormalised gradients cancel
-            for (std::size_t e = 0; e < experts; ++e)
-                grad_logits[t * experts + e] =
-                    static_cast<float>(sigmoid ? d[e] * s[e] * (1.0 - s[e]) : s[e] * (d[e] - mean));
+            for (std::size_t e = 0; e < experts; ++e) {  // (1 - s of a sigmoid is that of the negated logit)
+                const double rest = sigmoid && d[e] != 0.0 ? 1.0 / (1.0 + std::exp(static_cast<double>(logits[t * experts + e]))) : 0.0;
+                grad_logits[t * experts + e] = static_cast<float>(sigmoid ? d[e] * s[e] * rest : s[e] * (d[e] - mean));
+            }
         }
     });
 }

@@ -518,8 +518,11 @@ __device__ inline int expert_of(float chosen, int experts) { return min(max(int(
 // Up to 256 experts and 64 picks. Renormalised weights and sigmoid scores leave
 // the other logits no gradient, so only the chosen ones are read:
 //   softmax: w_j (g_j - sum g w), w over the chosen alone;
-//   sigmoid: p_j (1 - p_j) (g_j - sum g w) / sum p, or p_j (1 - p_j) g_j;
-// Dense (a softmax as it is): s_e (g_e - sum g p) for every expert.
+//   sigmoid: w_j (1 - p_j) (g_j - sum g w), or p_j (1 - p_j) g_j;
+// Dense (a softmax as it is): s_e (g_e - sum g p) for every expert. The weights
+// w are quotients of scores over a common factor that leaves the largest near
+// one, where the scores themselves may vanish, and 1 - p is the sigmoid of -l,
+// which has all its bits next to p = 1.
 template <int NV, bool Dense>
 __global__ __launch_bounds__(kWave* kWaves) void route_gradient_kernel(const float* __restrict__ logits,
                                                                       const float* __restrict__ chosen,
@@ -550,13 +553,20 @@ __global__ __launch_bounds__(kWave* kWaves) void route_gradient_kernel(const flo
             total += v[i];
         }
         inverse = 1.0f / row_sum(total);
-    } else if (!sigmoid) {
+    } else if (sigmoid && !renormalise) {
+        top = 0.0f;
+    } else {
         for (int j = l; j < top_k; j += kLanes) top = fmaxf(top, row[expert_of(picks[j], experts)]);
         top = row_max(top);
+        if (sigmoid) top = fminf(top, 0.0f);
     }
+    // sigmoid(x) = exp(min(x, 0)) / (1 + exp(-|x|)), over exp(top).
+    const auto score = [&](float x) {
+        return sigmoid ? exp_difference(fminf(x, 0.0f), top) / (1.0f + expf(-fabsf(x))) : score_of(x, false, top, inverse);
+    };
     float total = 0.0f, dot = 0.0f;
     for (int j = l; j < top_k; j += kLanes) {
-        const float p = score_of(row[expert_of(picks[j], experts)], sigmoid, top, inverse);
+        const float p = score(row[expert_of(picks[j], experts)]);
         total += p;
         dot += p * g[j];
     }
@@ -565,9 +575,10 @@ __global__ __launch_bounds__(kWave* kWaves) void route_gradient_kernel(const flo
     wave_fence();
     for (int j = l; j < top_k; j += kLanes) {
         const int e = expert_of(picks[j], experts);
-        const float p = score_of(row[e], sigmoid, top, inverse);
+        const float x = row[e], p = score(x);
         float d = Dense || !renormalise ? g[j] : top_k == 1 ? 0.0f : g[j] - dot / total;  // one weight alone is always 1
-        if (!Dense) d *= renormalise ? (sigmoid ? p / total * (1.0f - p) : p / total) : p * (1.0f - p);
+        if (!Dense) d *= renormalise ? p / total : p;
+        if (sigmoid) d *= score_of(-x, true, 0.0f, 1.0f);
         place[e] = d;
     }
     wave_fence();
@@ -631,7 +642,9 @@ __global__ __launch_bounds__(kWave* kWaves) void route_gradient_wide_kernel(cons
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int e = lane + kWave * i;
-        if (e < experts) out[t * experts + e] = float(sigmoid ? d[i] * s[i] * (1.0 - s[i]) : s[i] * (d[i] - mean));
+        if (e < experts)
+            out[t * experts + e] =
+                float(sigmoid ? d[i] * s[i] / (1.0 + exp(double(logits[t * experts + e]))) : s[i] * (d[i] - mean));
     }
 }
 
