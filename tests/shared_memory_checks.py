@@ -171,6 +171,21 @@ def check_largest_class_after_a_write(device, torch_device):
     np.testing.assert_array_equal(q.argmax(1).numpy(), np.zeros(rows))
 
 
+def check_picks_written_before_the_gradient(device, torch_device):
+    """No promise of a gradient's values, but of its bounds: numbers that are no expert's read and write nothing outside."""
+    for score in ("softmax", "sigmoid"):
+        for renormalise in (False, True):
+            logits = vc.Tensor(np.random.default_rng(6).standard_normal((6, 5)).astype(np.float32), requires_grad=True, device=device)
+            weights, chosen = vc.route(logits, 2, score=score, renormalise=renormalise)
+            vc.synchronize()
+            shared = torch.from_dlpack(chosen)
+            shared[:, 0] = torch.tensor([-1.0, 5.0, 1e9, float("nan"), float("inf"), 2.0 ** 33])
+            if shared.is_cuda:
+                torch.cuda.synchronize()
+            weights.backward(vc.Tensor(np.ones((6, 2), np.float32), device=device))
+            assert np.isfinite(logits.grad.numpy()).all()
+
+
 def check_negative_views(device, torch_device):
     """torch negates these when it reads them: the memory holds other values."""
     z = torch.tensor([1 + 2j], device=torch_device).conj()
@@ -215,7 +230,7 @@ def check_order_of_later_writes():
 RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_imported_memory,
             check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
             check_gradients_of_a_pass_that_fails]
-KEPT = [check_largest_class_after_a_write, check_negative_views]
+KEPT = [check_largest_class_after_a_write, check_negative_views, check_picks_written_before_the_gradient]
 GPU = [check_order_of_later_writes]
 
 if __name__ == "__main__":

@@ -35,6 +35,12 @@ std::size_t first_best(const std::vector<double>& ranks, const std::vector<char>
     return best;
 }
 
+// The expert of a saved pick, or one of them where another library has
+// written something else there since.
+std::size_t expert_of(float chosen, std::size_t experts) {
+    return chosen > 0.0F ? static_cast<std::size_t>(std::min(chosen, static_cast<float>(experts - 1))) : 0;
+}
+
 float sigmoid_of(float x) {
     const float e = std::exp(-std::fabs(x));
     return (x >= 0.0F ? 1.0F : e) / (1.0F + e);
@@ -108,14 +114,14 @@ void route_backward(const float* logits, const float* chosen, const float* grad_
             row_scores(logits + t * experts, experts, sigmoid, s);
             double total = 0.0, dot = 0.0;
             for (std::size_t j = 0; j < top_k; ++j) {
-                const double p = s[static_cast<std::size_t>(chosen[t * top_k + j])];
+                const double p = s[expert_of(chosen[t * top_k + j], experts)];
                 total += p;
                 dot += p * grad_weights[t * top_k + j];
             }
             std::fill(d.begin(), d.end(), 0.0);
             for (std::size_t j = 0; j < top_k; ++j) {
                 const double g = grad_weights[t * top_k + j];
-                d[static_cast<std::size_t>(chosen[t * top_k + j])] = renormalise ? (g - dot / total) / total : g;
+                d[expert_of(chosen[t * top_k + j], experts)] = renormalise ? (g - dot / total) / total : g;
             }
             const double mean = renormalise ? 0.0 : dot;  // the renormalised gradients cancel
             for (std::size_t e = 0; e < experts; ++e) {  // (1 - s of a sigmoid is that of the negated logit)

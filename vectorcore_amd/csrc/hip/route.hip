@@ -513,7 +513,9 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
         if (rows >> (kLanes * i) & 0xFFFF && first + i < p.tokens) route_row<(NV + 3) / 4>(p, first + i, scratch[wave]);
 }
 
-__device__ inline int expert_of(float chosen, int experts) { return min(max(int(chosen), 0), experts - 1); }
+// The expert of a saved pick, or one of them where another library has written
+// something else there since (before the conversion, which knows no NaN).
+__device__ inline int expert_of(float chosen, int experts) { return int(fminf(fmaxf(chosen, 0.0f), float(experts - 1))); }
 
 // Up to 256 experts and 64 picks. Renormalised weights and sigmoid scores leave
 // the other logits no gradient, so only the chosen ones are read:
