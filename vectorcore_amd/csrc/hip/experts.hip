@@ -937,6 +937,12 @@ int vc_hip_expert_linear_backward_weight(const float* x, const float* grad, cons
         if (!grad_w2 != !grad2) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_linear_backward_weight: half of a second product");
         if (width == 0 || columns == 0) return;
         if (!grad_w || (q.rows && (!x || !grad))) fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_linear_backward_weight: null pointer");
+        if (q.rows == 0) {  // zeros, without the plan's words, which no token needs
+            for (float* const out : {grad_w, grad_w2})
+                if (out)
+                    if (const int status = vc_hip_fill(out, q.experts * width * columns, 0.0f)) fail(status, vc_hip_last_error());
+            return;
+        }
         const int64_t products = grad2 ? 2 : 1;
         Profiled p("expert_backward_weight", products * 2.0 * q.rows * width * columns,
                    4.0 * (q.rows * (width + products * columns) + products * q.experts * width * columns));
