@@ -19,7 +19,8 @@ constexpr size_t kMaxExperts = 1024;
 // A counting sort that keeps equal experts in pick order. Chunks of picks are
 // counted by one launch; a second one adds up the counts before each chunk and
 // places the picks, a wavefront finding the lanes of equal experts by ballots.
-// Up to one round of picks a single workgroup does both.
+// Up to one round of picks a single workgroup does both. Picks are numbered
+// without a sign, as the last chunk and the last round may end behind 2^31.
 
 constexpr int kPlanBlock = 512, kPlanWaves = kPlanBlock / kWave;
 constexpr size_t kPlanChunks = 128;
@@ -34,8 +35,8 @@ __global__ __launch_bounds__(kPlanBlock) void plan_count_kernel(const float* __r
     extern __shared__ int lds[];
     for (int e = threadIdx.x; e <= experts; e += kPlanBlock) lds[e] = 0;
     __syncthreads();
-    const int begin = blockIdx.x * chunk, end = min(rows, begin + chunk);
-    for (int p = begin + int(threadIdx.x); p < end; p += kPlanBlock) atomicAdd(&lds[group_of(chosen[p], experts)], 1);
+    const unsigned begin = blockIdx.x * unsigned(chunk), end = min(unsigned(rows), begin + unsigned(chunk));
+    for (unsigned p = begin + threadIdx.x; p < end; p += kPlanBlock) atomicAdd(&lds[group_of(chosen[p], experts)], 1);
     __syncthreads();
     for (int e = threadIdx.x; e <= experts; e += kPlanBlock) counts[blockIdx.x * (experts + 1) + e] = lds[e];
 }
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(const float* __r
     int* const next = lds;                 // the chunk's next row of each group
     int* const total = lds + groups;       // all rows of each group, then their sum before it
     int* const found = lds + 2 * groups;   // [wave][group] of the round
-    const int begin = blockIdx.x * chunk, end = min(rows, begin + chunk);
+    const unsigned begin = blockIdx.x * unsigned(chunk), end = min(unsigned(rows), begin + unsigned(chunk));
     for (int e = tid; e < groups; e += kPlanBlock) {
         int before = 0, all = 0;
         if (counts)
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(const float* __r
     }
     __syncthreads();
     if (!counts) {
-        for (int p = begin + tid; p < end; p += kPlanBlock) atomicAdd(&total[group_of(chosen[p], experts)], 1);
+        for (unsigned p = begin + tid; p < end; p += kPlanBlock) atomicAdd(&total[group_of(chosen[p], experts)], 1);
         __syncthreads();
     }
     if (wave == 0) {
@@ -88,10 +89,10 @@ __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(const float* __r
     }
     if (blockIdx.x == 0 && tid == 0) offsets[groups] = rows;
     const int bits = 32 - __clz(groups);
-    for (int round = begin; round < end; round += kPlanBlock) {
+    for (unsigned round = begin; round < end; round += kPlanBlock) {
         for (int i = tid; i < kPlanWaves * groups; i += kPlanBlock) found[i] = 0;
         __syncthreads();
-        const int p = round + tid;
+        const unsigned p = round + tid;
         const int e = p < end ? group_of(chosen[p], experts) : groups;
         uint64_t same = ~0ull;
         for (int b = 0; b < bits; ++b) {
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(kPlanBlock) void plan_place_kernel(const float* __r
         if (p < end) {
             int row = next[e] + rank;
             for (int w = 0; w < wave; ++w) row += found[w * groups + e];
-            token[row] = p / top_k;
+            token[row] = int(p / unsigned(top_k));
             place[p] = row;
         }
         __syncthreads();
