@@ -1,4 +1,5 @@
-"""The expert and router entry points at the ends of their ranges: no tokens, and picks up to 2^31."""
+"""The expert and router entry points at the ends of their ranges: no tokens, picks up to 2^31, and more
+workgroups than one dimension of a grid holds."""
 
 import ctypes
 
@@ -67,6 +68,73 @@ def test_a_plan_of_nearly_2_31_picks(top_k):
     np.testing.assert_array_equal(window(plan, token + head, token + rows), (head + order) // top_k)
     for b in (chosen, plan):
         b.release()
+
+
+def windows(buffer, width, rows):
+    """Rows [begin, end) of a buffer at its start, inside and at its end."""
+    for at in (0, rows // 2, 2 ** 26 - 700, rows - 1500):
+        yield at, window(buffer, at * width, (at + 1500) * width).reshape(1500, width)
+
+
+def filled(*shape, value=7.0):
+    b = C.Buffer(shape)
+    C.check(C.lib().vc_hip_fill(b.ptr, int(np.prod(shape, dtype=np.int64)), value))
+    return b
+
+
+@pytest.mark.gpu
+def test_a_sum_over_more_than_2_26_picks():
+    lib, tokens, width = C.lib(), 2 ** 25 + 1000, 3
+    rows, words = 2 * tokens, ctypes.c_size_t()
+    C.check(lib.vc_hip_expert_plan_words(tokens, 2, 1, ctypes.byref(words)))
+    chosen, plan = filled(rows, value=0.0), C.Buffer((words.value,), np.int32)
+    C.check(lib.vc_hip_expert_plan_build(chosen.ptr, tokens, 2, 1, plan.ptr))
+    p = C.ExpertPlan(plan.ptr, tokens, 2, 1)
+    z, w, g = filled(rows, width, value=3.0), filled(rows, value=0.5), filled(tokens, width, value=2.0)
+    out, dz, dw = filled(tokens, width), filled(rows, width), filled(rows)
+    C.check(lib.vc_hip_expert_combine_forward(z.ptr, w.ptr, ctypes.byref(p), width, out.ptr))
+    C.check(lib.vc_hip_expert_combine_backward(g.ptr, z.ptr, w.ptr, ctypes.byref(p), width, dz.ptr, dw.ptr))
+    assert (window(out, 3 * (tokens - 1500), 3 * tokens) == 3.0).all()
+    assert all((v == 1.0).all() for _, v in windows(dz, width, rows))
+    assert all((v == 18.0).all() for _, v in windows(dw, 1, rows))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,top_k", [(2 ** 28 + 999, 2, 1), (2 ** 26 + 999, 17, 17)])
+def test_routes_of_more_rows_than_a_grids_dimension(tokens, experts, top_k):
+    """All rows are alike but windows of them, whose second expert is the best."""
+    lib = C.lib()
+    logits, w, c = filled(tokens, experts, value=0.0), filled(tokens, top_k), filled(tokens, top_k)
+    some = np.zeros((1500, experts), np.float32)
+    some[:, 1] = 1.0
+    for at, _ in windows(logits, experts, tokens):
+        C.check(lib.vc_hip_upload(logits.ptr + 4 * at * experts, some.ctypes.data, some.nbytes))
+    C.check(lib.vc_hip_route_forward(logits.ptr, None, tokens, experts, top_k, C.SOFTMAX, 1, 1, 0, w.ptr, c.ptr))
+    order = [1, 0, *range(2, experts)][:top_k]
+    p = np.exp(some[0].astype(np.float64)) / np.exp(some[0].astype(np.float64)).sum()
+    for _, v in windows(c, top_k, tokens):
+        np.testing.assert_array_equal(v, np.broadcast_to(order, v.shape))
+    for _, v in windows(w, top_k, tokens):
+        np.testing.assert_allclose(v, np.broadcast_to(p[order], v.shape), rtol=2.0 ** -19)
+    if experts > 2:
+        return
+    g, d = filled(tokens, 1, value=1.0), filled(tokens, 2)
+    C.check(lib.vc_hip_route_backward(logits.ptr, c.ptr, g.ptr, tokens, 2, 1, C.SOFTMAX, 0, d.ptr))
+    for _, v in windows(d, 2, tokens):
+        np.testing.assert_allclose(v, np.broadcast_to([-p[0] * p[1], p[0] * p[1]], v.shape), rtol=2.0 ** -18)
+
+
+@pytest.mark.gpu
+def test_too_many_tiles_are_refused():
+    """2^24 workgroups of 256 and more; nothing is launched."""
+    lib, p = C.lib(), C.Buffer((16,))
+    plan = C.ExpertPlan(p.ptr, 1 << 20, 1, 8)
+    most = 1 << 20
+    for call in (lambda: lib.vc_hip_expert_linear_forward(p.ptr, p.ptr, ctypes.byref(plan), 4, most, 0, p.ptr),
+                 lambda: lib.vc_hip_expert_gated_forward(p.ptr, p.ptr, p.ptr, ctypes.byref(plan), 4, most, 0, p.ptr, None, None),
+                 lambda: lib.vc_hip_expert_linear_backward_input(p.ptr, p.ptr, None, None, ctypes.byref(plan), most, 4, p.ptr),
+                 lambda: lib.vc_hip_expert_linear_backward_weight(p.ptr, p.ptr, None, ctypes.byref(plan), most, most, 0, p.ptr, None)):
+        assert call() == 3 and b"too many tiles" in lib.vc_hip_last_error()
 
 
 @pytest.mark.gpu

@@ -635,7 +635,7 @@ int64_t tiles_of(size_t n, int tile) { return int64_t((n + tile - 1) / tile); }
 // A grid for `tiles` tiles at most, in whole rounds of the eight dies.
 dim3 tile_grid(int64_t tiles) {
     const int64_t blocks = (tiles + 7) / 8 * 8;
-    if (blocks >= int64_t(1) << 31) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
+    if (blocks > int64_t(kMostBlocks)) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
     return dim3(unsigned(blocks));
 }
 // Row tiles by column tiles at most.
@@ -661,7 +661,7 @@ struct Parts {
     }
 };
 dim3 operator*(dim3 grid, int64_t parts) {
-    if (grid.x * parts >= int64_t(1) << 31) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
+    if (grid.x * parts > int64_t(kMostBlocks)) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
     return dim3(unsigned(grid.x * parts));
 }
 
@@ -680,7 +680,7 @@ template <bool Gated, int Columns>
 void launch_thin(Device& d, int64_t rows, const ProductArgs& args) {
     const int64_t tiles = rows * tiles_of(size_t(args.columns), Columns), wanted = (3 * d.cu_count + tiles - 1) / tiles;
     const int64_t splits = tiles > kThinTiles ? 1 : std::max<int64_t>(1, std::min(wanted, args.width / (Columns == 64 ? 128 : 64)));
-    if (tiles * splits >= int64_t(1) << 31) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
+    if (tiles * splits > int64_t(kMostBlocks)) fail(VC_HIP_ERR_OVERFLOW, "expert product: too many tiles");
     Scratch partial(splits > 1 ? size_t(tiles * splits) * kThinRows * Columns * (Gated ? 2 : 1) * sizeof(float) : 4);
     launch(thin_kernel<Gated, Columns>, dim3(unsigned(tiles * splits)), dim3(256), 0, d.stream, args, int(splits),
            partial.as<float>());
@@ -761,7 +761,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const float* __re
                                                                float* __restrict__ grad_rows,
                                                                float* __restrict__ grad_weights) {
     const int lane = threadIdx.x % kWave, kept = offsets[experts];
-    const int64_t p = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+    const int64_t p = block_id() * 4 + threadIdx.x / kWave;
     if (p >= picks) return;
     const int64_t r = place[p];
     const float* const g = grad + p / top_k * width;
@@ -995,7 +995,7 @@ int vc_hip_expert_combine_forward(const float* rows, const float* weights, const
         while (lanes < 256 && 4 * lanes < width) lanes *= 2;
         const unsigned tokens = 256 / lanes;
         const size_t across = (width + 4 * lanes - 1) / (4 * lanes);
-        if (across >= size_t(1) << 31) fail(VC_HIP_ERR_OVERFLOW, "expert_combine: rows too long");
+        if (across > kMostBlocks) fail(VC_HIP_ERR_OVERFLOW, "expert_combine: rows too long");
         launch(combine_kernel, dim3(unsigned(across), unsigned(std::min<size_t>((q.tokens + tokens - 1) / tokens, 65535))),
                dim3(lanes, tokens), 0, d.stream,
                rows, weights, q.place, q.offsets, int(q.experts), int64_t(q.tokens), int(q.top_k), int64_t(width), out);
@@ -1013,7 +1013,7 @@ int vc_hip_expert_combine_backward(const float* grad, const float* rows, const f
         if (width && (!grad || (grad_rows && !weights) || (grad_weights && !rows)))
             fail(VC_HIP_ERR_INVALID_ARGUMENT, "expert_combine_backward: null pointer");
         Profiled p("expert_combine_backward", 3.0 * q.rows * width, 4.0 * (q.tokens + 2.0 * q.rows) * width);
-        launch(combine_backward_kernel, dim3(unsigned((q.rows + 3) / 4)), dim3(256), 0, d.stream, grad, rows, weights, q.place,
+        launch(combine_backward_kernel, grid_2d((q.rows + 3) / 4), dim3(256), 0, d.stream, grad, rows, weights, q.place,
                q.offsets, int(q.experts), int64_t(q.rows), int(q.top_k), int64_t(width), grad_rows, grad_weights);
         after_launch("expert_combine_backward");
         p.done();

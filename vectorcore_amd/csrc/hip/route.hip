@@ -195,7 +195,7 @@ __device__ void route_row(const RouteArgs& p, int64_t t, double* ranks) {
 template <int NV>
 __global__ __launch_bounds__(kWave* kWaves) void route_wide_kernel(RouteArgs p) {
     __shared__ double ranks[kWaves][kWave * NV];
-    const int64_t t = int64_t(blockIdx.x) * kWaves + threadIdx.x / kWave;
+    const int64_t t = block_id() * kWaves + threadIdx.x / kWave;
     if (t < p.tokens) route_row<NV>(p, t, ranks[threadIdx.x / kWave]);
 }
 
@@ -326,7 +326,7 @@ template <int NV, bool Exact>
 __global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
     __shared__ double scratch[kWaves][kWave * NV / 2];  // floats of four rows, or doubles of one
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, l = lane % kLanes, r = lane / kLanes;
-    const int64_t first = (int64_t(blockIdx.x) * kWaves + wave) * kRows;
+    const int64_t first = (block_id() * kWaves + wave) * kRows;
     if (first >= p.tokens) return;  // uniform in the wavefront
     const int64_t t = min(first + r, p.tokens - 1);
     const int experts = p.experts;
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(kWave* kWaves) void route_gradient_kernel(const flo
                                                                       float* __restrict__ out) {
     __shared__ __align__(16) float lds[kWaves][kRows][kLanes * NV];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, l = lane % kLanes, r = lane / kLanes;
-    const int64_t t = (int64_t(blockIdx.x) * kWaves + wave) * kRows + r;
+    const int64_t t = (block_id() * kWaves + wave) * kRows + r;
     const bool live = t < tokens;
     const float* const row = logits + (live ? t : 0) * experts;
     const float* const picks = chosen + (live ? t : 0) * top_k;
@@ -611,7 +611,7 @@ __global__ __launch_bounds__(kWave* kWaves) void route_gradient_wide_kernel(cons
                                                                       int experts, int top_k, bool sigmoid,
                                                                       bool renormalise, float* __restrict__ out) {
     const int lane = threadIdx.x % kWave;
-    const size_t t = size_t(blockIdx.x) * kWaves + threadIdx.x / kWave;
+    const size_t t = size_t(block_id()) * kWaves + threadIdx.x / kWave;
     if (t >= tokens) return;
     double s[NV], d[NV];
     row_scores<NV>(logits + t * experts, experts, lane, sigmoid, s);
@@ -677,7 +677,7 @@ void with_rows(size_t experts, F&& f) {
     else f(std::integral_constant<int, 16>());
 }
 
-dim3 row_grid(size_t tokens, int rows) { return dim3(unsigned((tokens + rows - 1) / rows)); }
+dim3 row_grid(size_t tokens, int rows) { return grid_2d((tokens + rows - 1) / rows); }
 
 }  // namespace
 }  // namespace vchip

@@ -213,6 +213,16 @@ inline unsigned grid_1d(size_t items, unsigned block, unsigned max_blocks) {
     return static_cast<unsigned>(blocks);
 }
 
+// A dimension of a grid holds fewer than 2^32 threads: that many workgroups of
+// 256, or less where it is many. Beyond, a second dimension: workgroup
+// block_id() of at least `blocks`.
+constexpr size_t kMostBlocks = (size_t(1) << 24) - 1;
+inline dim3 grid_2d(size_t blocks) {
+    const size_t x = blocks < (size_t(1) << 20) ? blocks : size_t(1) << 20;
+    return dim3(static_cast<unsigned>(x), static_cast<unsigned>((blocks + x - 1) / x));
+}
+__device__ inline int64_t block_id() { return int64_t(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Shape metadata for broadcasting kernels (rank <= 8), passed by value.
