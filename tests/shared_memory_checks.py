@@ -171,6 +171,28 @@ def check_largest_class_after_a_write(device, torch_device):
     np.testing.assert_array_equal(q.argmax(1).numpy(), np.zeros(rows))
 
 
+def check_steps_of_overlapping_memory(device, torch_device):
+    """Tensors imported apart that lie over the same memory: refused before anything is written, but for gradients."""
+    memory = torch.tensor(whole(2, 4 * N), device=torch_device)
+    part = lambda begin, count=N: vc.from_dlpack(memory[begin:begin + count].reshape(4, -1))[0]
+    apart = lambda: vc.Tensor(whole(3, 4, N // 4), device=device)
+    for p, m, g in (([part(0)], [part(0)], [apart()]), ([part(0)], [apart()], [part(0)]), ([apart()], [part(5)], [part(0)]),
+                    ([part(0)], [part(N - 1)], [apart()]), ([part(0), part(2 * N), part(N)], [apart(), apart(), apart()], [apart(), apart(), part(3)]),
+                    ([apart(), part(0)], [part(8), apart()], [apart(), apart()])):
+        before = [t.numpy() for t in p + m]
+        try:
+            vc.muon_step(p, m, 0.1, grads=g)
+            raise AssertionError("taken")
+        except ValueError as e:
+            assert "overlap" in str(e)
+        for t, was in zip(p + m, before):
+            np.testing.assert_array_equal(t.numpy(), was)
+    p, m = [part(0), part(N)], [apart(), part(3 * N)]
+    vc.muon_step(p, m, 0.1, grads=[part(2 * N), part(2 * N)])  # neighbours, and one gradient twice
+    np.testing.assert_array_equal(vc.from_dlpack(memory)[0].numpy()[2 * N:3 * N], whole(2, 4 * N)[2 * N:3 * N])
+    assert (p[0].numpy() != whole(2, 4 * N)[:N].reshape(4, -1)).any() and (p[1].numpy() != whole(2, 4 * N)[N:2 * N].reshape(4, -1)).any()
+
+
 def check_picks_written_before_the_gradient(device, torch_device):
     """No promise of a gradient's values, but of its bounds: numbers that are no expert's read and write nothing outside."""
     for score in ("softmax", "sigmoid"):
@@ -230,7 +252,7 @@ def check_order_of_later_writes():
 RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_imported_memory,
             check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
             check_gradients_of_a_pass_that_fails]
-KEPT = [check_largest_class_after_a_write, check_negative_views, check_picks_written_before_the_gradient]
+KEPT = [check_largest_class_after_a_write, check_negative_views, check_picks_written_before_the_gradient, check_steps_of_overlapping_memory]
 GPU = [check_order_of_later_writes]
 
 if __name__ == "__main__":

@@ -1807,6 +1807,7 @@ std::shared_ptr<Storage> HipBackend::adopt(float* data, std::size_t elements, st
     return std::make_shared<HipStorage>(elements, data, std::move(release));
 }
 
+const float* HipBackend::address(const Storage& storage) const { return as_hip(storage).ptr(); }
 float* HipBackend::expose(Storage& storage) { return as_hip(storage).expose(); }
 void HipBackend::conceal(Storage& storage) { as_hip(storage).conceal(); }
 

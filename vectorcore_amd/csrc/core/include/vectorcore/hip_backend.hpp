@@ -275,10 +275,13 @@ public:
         const Storage* grad;
         std::size_t grad_offset, count, rows, cols;
     };
-    // Distinct storages but for the gradients. The caller bumps the versions.
+    // No memory in common but that of gradients. The caller bumps the versions.
     void muon_step(const std::vector<MuonItem>& items, float rate, float mu, float decay, std::size_t steps);
 
     // --- memory shared with other libraries ---
+    // Where a storage's values lie, computed: two storages over memory of
+    // another library may overlap.
+    [[nodiscard]] const float* address(const Storage& storage) const;
     // A storage over device memory that its owner keeps until `release` is
     // called, which is once the work enqueued before the storage died is done.
     // In-place ops write to that memory.

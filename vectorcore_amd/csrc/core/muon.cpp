@@ -5,9 +5,11 @@
 #include "vectorcore/hip_backend.hpp"
 
 #include <algorithm>
+#include <cstdint>
 #include <stdexcept>
 #include <string>
 #include <unordered_set>
+#include <utility>
 
 namespace vectorcore {
 
@@ -21,6 +23,18 @@ Matrices matrices_of(const char* op, const Shape& shape) {
     if (shape.size() < 2)
         throw std::invalid_argument(std::string(op) + " takes matrices [..., rows, cols], got " + shape_string(shape));
     return {numel(Shape(shape.begin(), shape.end() - 2)), shape[shape.size() - 2], shape.back()};
+}
+
+// The memory of a tensor of n > 0 elements.
+struct Range {
+    std::uintptr_t begin, end;
+    bool writes;
+};
+Range range_of(const Tensor& t, std::size_t n, bool writes) {
+    const float* const data = t.device() == Device::hip() ? HipBackend::instance().address(*t.impl()->storage) + t.impl()->offset
+                                                           : t.data();
+    const auto begin = reinterpret_cast<std::uintptr_t>(data);
+    return {begin, begin + n * sizeof(float), writes};
 }
 
 void require_known(Device device) {
@@ -81,6 +95,19 @@ void muon_step(const std::vector<Tensor*>& parameters, const std::vector<Tensor*
     for (const Item& it : items)
         if (written.count(it.grad.impl()->storage.get()))
             throw std::invalid_argument("muon_step: a gradient shares storage with a parameter or momentum");
+    // Storages taken from another library may lie over the same memory.
+    std::vector<Range> ranges;
+    for (const Item& it : items)
+        for (const auto& [tensor, writes] : {std::pair<const Tensor*, bool>{it.param, true}, {it.momentum, true}, {&it.grad, false}})
+            if (const std::size_t n = tensor->numel()) ranges.push_back(range_of(*tensor, n, writes));
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    std::uintptr_t end = 0, written_end = 0;  // of what lies before
+    for (const Range& r : ranges) {
+        if (r.begin < (r.writes ? end : written_end))
+            throw std::invalid_argument("muon_step: parameters, momenta and gradients must not overlap in memory");
+        end = std::max(end, r.end);
+        if (r.writes) written_end = std::max(written_end, r.end);
+    }
     std::vector<HipBackend::MuonItem> batch;
     for (const Item& it : items) {
         const auto &p = it.param->impl(), &m = it.momentum->impl(), &g = it.grad.impl();
