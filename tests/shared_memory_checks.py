@@ -193,6 +193,25 @@ def check_steps_of_overlapping_memory(device, torch_device):
     assert (p[0].numpy() != whole(2, 4 * N)[:N].reshape(4, -1)).any() and (p[1].numpy() != whole(2, 4 * N)[N:2 * N].reshape(4, -1)).any()
 
 
+def check_steps_of_one_buffer_imported_twice(device, torch_device):
+    """Tied weights: every import's update counts, in the order of the list."""
+    memory = torch.zeros(40, 50, device=torch_device)
+    tied = [vc.from_dlpack(memory)[0] for _ in range(3)]
+    part = vc.from_dlpack(memory[3:9])[0]
+    own = vc.Tensor(np.zeros((40, 50), np.float32), device=device)
+    lent = torch.from_dlpack(own)
+    again = vc.from_dlpack(lent)[0]
+    params = [tied[0], part, tied[1], own, again, tied[2]]
+    for i, p in enumerate(params):
+        p.requires_grad = True
+        (p * float(2 ** i)).sum().backward()
+    vc.sgd_step(params, 1.0)
+    want = np.full((40, 50), -(1.0 + 4 + 32))
+    want[3:9] -= 2
+    np.testing.assert_array_equal(tied[1].numpy(), want)
+    np.testing.assert_array_equal(own.numpy(), np.full((40, 50), -(8.0 + 16)))
+
+
 def check_picks_written_before_the_gradient(device, torch_device):
     """No promise of a gradient's values, but of its bounds: numbers that are no expert's read and write nothing outside."""
     for score in ("softmax", "sigmoid"):
@@ -252,7 +271,8 @@ def check_order_of_later_writes():
 RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_imported_memory,
             check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
             check_gradients_of_a_pass_that_fails]
-KEPT = [check_largest_class_after_a_write, check_negative_views, check_picks_written_before_the_gradient, check_steps_of_overlapping_memory]
+KEPT = [check_largest_class_after_a_write, check_negative_views, check_picks_written_before_the_gradient, check_steps_of_overlapping_memory,
+        check_steps_of_one_buffer_imported_twice]
 GPU = [check_order_of_later_writes]
 
 if __name__ == "__main__":

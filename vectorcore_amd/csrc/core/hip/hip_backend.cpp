@@ -1808,6 +1808,13 @@ std::shared_ptr<Storage> HipBackend::adopt(float* data, std::size_t elements, st
 }
 
 const float* HipBackend::address(const Storage& storage) const { return as_hip(storage).ptr(); }
+bool HipBackend::shared(const Storage& storage) const { return as_hip(storage).shared(); }
+bool HipBackend::overlap(const Storage& a, const Storage& b) const {
+    if (&a == &b) return true;
+    if (!shared(a) || !shared(b)) return false;
+    const auto p = reinterpret_cast<std::uintptr_t>(address(a)), q = reinterpret_cast<std::uintptr_t>(address(b));
+    return p < q + b.size() * sizeof(float) && q < p + a.size() * sizeof(float);
+}
 float* HipBackend::expose(Storage& storage) { return as_hip(storage).expose(); }
 void HipBackend::conceal(Storage& storage) { as_hip(storage).conceal(); }
 

@@ -91,11 +91,16 @@ void sgd_step(const std::vector<Tensor*>& parameters, float learning_rate) {
     // hip parameters are updated in batches (one launch for up to 16), in
     // parameter order: a batch is flushed before anything that the reference's
     // one-at-a-time loop would order after it (an error, a cpu parameter, a
-    // parameter sharing a batched storage).
+    // parameter sharing a batched storage, or its memory where that is another
+    // library's).
     std::vector<HipBackend::AxpyItem> batch;
     std::vector<Storage*> touched;        // targets in the batch
     std::vector<const Storage*> read;     // sources in the batch
-    const auto contains = [](const auto& v, const Storage* s) { return std::find(v.begin(), v.end(), s) != v.end(); };
+    const auto contains = [](const auto& v, const Storage* s) {
+        if (std::find(v.begin(), v.end(), s) != v.end()) return true;
+        const HipBackend& hip = HipBackend::instance();
+        return !v.empty() && hip.shared(*s) && std::any_of(v.begin(), v.end(), [&](const Storage* o) { return hip.overlap(*o, *s); });
+    };
     const auto flush = [&] {
         if (batch.empty()) return;
         HipBackend::instance().axpy_batch(batch, -learning_rate);
