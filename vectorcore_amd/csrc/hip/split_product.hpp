@@ -5,7 +5,10 @@
 // each the rounding of what the earlier ones leave: |x2| <= 2^-9 |x|, |x3| <=
 // 2^-18 |x|, and the parts' 24 bits hold all of x. Of the nine products of two
 // values' parts those below 2^-26 of the largest (x2 y3, x3 y2, x3 y3) are left
-// out. bfloat16 has float32's exponents, so any magnitudes may meet. The six
+// out. bfloat16 has float32's exponents, so values of 2^-110 (8e-34) or more may
+// meet any others; its least step is 2^-133, by half of which a smaller value may
+// be off (2^-120 by 2^-14 of itself), which shows where it meets one above 2^80.
+// The six
 // others are exact and summed in float32 by the matrix instructions, whose
 // 16-deep sums round less often than a float32 chain does: six instructions of
 // 32 cycles take the place of eight of 64 (V_MFMA_F32_32X32X2_F32).
