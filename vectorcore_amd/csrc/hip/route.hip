@@ -303,7 +303,9 @@ __device__ inline void sort_keys(uint32_t (&key)[N]) {
 }
 
 // 1 / (1 + exp(-x)) within 2^-21 of itself, or 2^-115 where x < -80: exp2(t)
-// with t = -x / ln 2, and what t's rounding leaves to first order.
+// with t = -x / ln 2, and what t's rounding leaves to first order; 1 / ln 2 in
+// two terms, as in Cody and Waite's reduction (Software Manual for the Elementary
+// Functions, 1980).
 __device__ inline float quick_sigmoid(float x) {
     const float log2e = 0x1.715476p+0f, rest = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;
     x = fmaxf(x, -80.0f);
