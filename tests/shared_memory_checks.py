@@ -171,6 +171,26 @@ def check_largest_class_after_a_write(device, torch_device):
     np.testing.assert_array_equal(q.argmax(1).numpy(), np.zeros(rows))
 
 
+def check_gradients_that_are_the_seed(device, torch_device):
+    """Sums and views pass the gradient on as it is: a stored one is no part of the seed's memory."""
+    up = whole(6, N, N)
+    for lend in (False, True):
+        if lend:
+            seed = vc.Tensor(up, device=device)
+            memory = torch.from_dlpack(seed)
+        else:
+            memory = torch.tensor(up, device=torch_device)
+            seed = vc.from_dlpack(memory)[0]
+        a, b, c = (vc.Tensor(whole(s, N, N), device=device, requires_grad=True) for s in (7, 8, 9))
+        kept = a + c.reshape([N * N]).reshape([N, N])
+        kept.retain_grad()
+        (kept + b).backward(seed)
+        b.backward(seed)
+        overwrite(memory)
+        for t, times in ((a, 1), (c, 1), (kept, 1), (b, 2)):
+            np.testing.assert_array_equal(t.grad.numpy(), times * up)
+
+
 def check_steps_of_overlapping_memory(device, torch_device):
     """Tensors imported apart that lie over the same memory: refused before anything is written, but for gradients."""
     memory = torch.tensor(whole(2, 4 * N), device=torch_device)
@@ -272,7 +292,7 @@ RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_impor
             check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
             check_gradients_of_a_pass_that_fails]
 KEPT = [check_largest_class_after_a_write, check_negative_views, check_picks_written_before_the_gradient, check_steps_of_overlapping_memory,
-        check_steps_of_one_buffer_imported_twice]
+        check_steps_of_one_buffer_imported_twice, check_gradients_that_are_the_seed]
 GPU = [check_order_of_later_writes]
 
 if __name__ == "__main__":

@@ -373,7 +373,7 @@ public:
     // Does another library hold this buffer's address? It may write the buffer
     // without a word, so work that reads it is never left recorded, and nothing
     // is kept of its contents.
-    bool shared() const {
+    [[nodiscard]] bool shared() const override {
         std::lock_guard<std::recursive_mutex> lock(state_mutex());
         return release_ != nullptr || exports_ > 0;
     }
@@ -1808,10 +1808,9 @@ std::shared_ptr<Storage> HipBackend::adopt(float* data, std::size_t elements, st
 }
 
 const float* HipBackend::address(const Storage& storage) const { return as_hip(storage).ptr(); }
-bool HipBackend::shared(const Storage& storage) const { return as_hip(storage).shared(); }
 bool HipBackend::overlap(const Storage& a, const Storage& b) const {
     if (&a == &b) return true;
-    if (!shared(a) || !shared(b)) return false;
+    if (!a.shared() || !b.shared()) return false;
     const auto p = reinterpret_cast<std::uintptr_t>(address(a)), q = reinterpret_cast<std::uintptr_t>(address(b));
     return p < q + b.size() * sizeof(float) && q < p + a.size() * sizeof(float);
 }

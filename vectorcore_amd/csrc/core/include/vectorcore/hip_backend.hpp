@@ -282,8 +282,6 @@ public:
     // Where a storage's values lie, computed: two storages over memory of
     // another library may overlap.
     [[nodiscard]] const float* address(const Storage& storage) const;
-    // Does another library hold the storage's address (adopt, expose)?
-    [[nodiscard]] bool shared(const Storage& storage) const;
     // Have two storages memory in common? Only shared ones that differ can.
     [[nodiscard]] bool overlap(const Storage& a, const Storage& b) const;
     // A storage over device memory that its owner keeps until `release` is

@@ -23,8 +23,14 @@ public:
     [[nodiscard]] std::uint64_t version() const noexcept { return version_; }
     void bump_version() noexcept { ++version_; }
 
+    // May another library hold the memory's address? What is to stay must then
+    // not be this storage. (Of the hip device: until the library has let go.)
+    [[nodiscard]] virtual bool shared() const { return shared_; }
+    void set_shared() noexcept { shared_ = true; }
+
 private:
     std::uint64_t version_{0};
+    bool shared_ = false;
 };
 
 std::shared_ptr<Storage> make_cpu_storage(std::size_t elements);

@@ -99,7 +99,7 @@ void sgd_step(const std::vector<Tensor*>& parameters, float learning_rate) {
     const auto contains = [](const auto& v, const Storage* s) {
         if (std::find(v.begin(), v.end(), s) != v.end()) return true;
         const HipBackend& hip = HipBackend::instance();
-        return !v.empty() && hip.shared(*s) && std::any_of(v.begin(), v.end(), [&](const Storage* o) { return hip.overlap(*o, *s); });
+        return !v.empty() && s->shared() && std::any_of(v.begin(), v.end(), [&](const Storage* o) { return hip.overlap(*o, *s); });
     };
     const auto flush = [&] {
         if (batch.empty()) return;

@@ -226,6 +226,7 @@ inline py::capsule export_(const Tensor& t, const py::object& stream, const py::
     } else {
         if (!stream.is_none()) throw std::runtime_error("__dlpack__: a tensor in host memory has no stream");
         data = e->storage->mutable_data();
+        e->storage->set_shared();
     }
     e->shape.assign(t.shape().begin(), t.shape().end());
     e->strides.assign(t.strides().begin(), t.strides().end());

@@ -27,7 +27,9 @@ private:
 class AdoptedStorage final : public Storage {
 public:
     AdoptedStorage(float* values, std::size_t n, std::function<void()> release)
-        : values_(values), n_(n), release_(std::move(release)) {}
+        : values_(values), n_(n), release_(std::move(release)) {
+        set_shared();
+    }
     ~AdoptedStorage() override { release_(); }
     AdoptedStorage(const AdoptedStorage&) = delete;
     AdoptedStorage& operator=(const AdoptedStorage&) = delete;

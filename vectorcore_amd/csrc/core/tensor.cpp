@@ -303,6 +303,16 @@ void Tensor::backward(const Tensor& gradient) const {
 
 namespace {
 
+// A gradient to store. The seed, which rules may pass on as it is, can lie in
+// another library's memory: a copy of it then.
+std::shared_ptr<detail::TensorImpl> stored(const Tensor& g) {
+    const auto& storage = g.impl()->storage;
+    if (!storage->shared()) return g.detach().impl();
+    auto copy = g.device() == Device::hip() ? HipBackend::instance().snapshot(storage, g.impl()->offset, g.numel())
+                                            : make_cpu_storage(g.data(), g.numel());
+    return detail::make_tensor(std::move(copy), g.shape(), false).impl();
+}
+
 // The node loop of Tensor::backward over `order` (depth-first post-order from
 // root), seeded with `gradient` at root.
 void run_backward(const std::shared_ptr<detail::TensorImpl>& root,
@@ -323,7 +333,7 @@ void run_backward(const std::shared_ptr<detail::TensorImpl>& root,
         const Tensor upstream = found->second;
         pending.erase(found);
         if (node->requires_grad && (node->leaf || node->retains_grad)) {
-            node->grad = node->grad ? (detail::from_impl(node->grad) + upstream).detach().impl() : upstream.detach().impl();
+            node->grad = node->grad ? (detail::from_impl(node->grad) + upstream).detach().impl() : stored(upstream);
         }
         if (!node->grad_fn) continue;
         std::vector<Tensor> grads;
