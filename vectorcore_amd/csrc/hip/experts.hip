@@ -147,10 +147,16 @@ Plan plan_of(const vc_hip_expert_plan* plan) {
 // ---- products -----------------------------------------------------------------------
 // Tiles of 64 or 128 rows of one group (split_product.hpp). Bound by the matrix
 // instructions and, beside them, by the vector instructions that split operands:
-// 16384 rows of 8 experts, 1024 x 4096, reach 174 TFLOP/s forward, 175 to the rows
-// and 177 to the weights, of 215 that a sixth of the library's bfloat16 rate would
-// be. 49152 rows of 64 experts, 1024 x 512: 156, 167 and 120, as sums of 768 rows
-// leave prologues and stores a larger share.
+// 16384 rows of 8 experts, 1024 x 4096, reach 180 TFLOP/s in the gated unit, 158 in
+// the plain product, 172 to the rows and 171 to the weights, of 215 that a sixth of
+// the library's bfloat16 rate would be. 49152 rows of 64 experts, 1024 x 512: 156,
+// 153, 165 and 121, as sums of 768 rows leave prologues and stores a larger share.
+//
+// A sum that is not finite (an infinity or NaN among its operands, or a value that
+// rounds to an infinity) is computed again by its lane, term after term: right, but
+// slow where there are many. A training pass of the first batch: 8.0 ms, 174 with
+// one token of NaN (all of its experts' gradients are), 388 with one such weight
+// and 628 with one such expert.
 
 using S = split::Bf16x3;
 
@@ -471,7 +477,10 @@ __global__ __launch_bounds__(split::kThreads, 2) void weight_kernel(ProductArgs 
 // expert on average 91 and 129 us, 8 rows 129 and 126, 16 rows 154 and 130. One
 // token of 2 of 16 experts, 1024 x 4096: 19.9 us for the two products of the gated
 // unit (67 MB, 3.4 TB/s) and 14.1 for the third; 16 tokens that reach some 42 of 64
-// experts, 1024 x 512: 36.8 and 21.0 us (174 and 87 MB, 4.7 and 4.1 TB/s).
+// experts, 1024 x 512: 36.8 and 21.0 us (174 and 87 MB, 4.7 and 4.1 TB/s). The
+// average decides, as the host does not know the load. An uneven one costs no more:
+// 384 rows of 64 experts, 1024 x 512, take 90 and 35 us evenly, 45 and 19 on six
+// experts, 41 and 19 on one, whose weights the caches serve after the first rows.
 
 constexpr int kThinRows = 4, kThinDepth = 512, kThinTiles = 4096;
 constexpr size_t kThinMost = 6;  // rows of an expert on average

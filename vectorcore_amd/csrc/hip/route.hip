@@ -9,12 +9,15 @@
 //
 // Choices next to a border between ranks are those of the definition: where a
 // row's 32-bit ranks cannot tell two candidates apart, its whole wavefront ranks
-// it again in double.
+// it again in double, weights included. So it does where a chosen score is below
+// 2^-100, which float32 would soon not hold. A bias far above the scores, as one
+// that masks an expert, makes that every row, as 32-bit ranks next to it have no
+// digits of the scores (65536 rows of 256 experts: 200 us with one bias of -1e4).
 //
 // Many rows would be bound by HBM (the logits are read, the gradient is written)
 // and are, forward, by vector instructions still: sixteen lanes share a row, so
 // four rows share each step of a search or sum across lanes. 65536 rows of 256
-// experts: 50.6 us forward (1.4 TB/s), 17.1 us backward (67 MB written, 4.2 TB/s);
+// experts: 50.2 us forward (1.4 TB/s), 18.1 us backward (67 MB written, 3.7 TB/s);
 // 4096 rows of 64: 4.1 and 3.9 us, a launch's latency.
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"
