@@ -462,6 +462,12 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
     }
     int mine = 0;
     uint32_t previous = 0;
+    bool tied = false;  // the candidate after the last pick with that pick
+    // Of two logits in falling order: may doubles not tell their scores apart?
+    const auto near = [&](float ahead, float value) {
+        const float gap = ahead - value;
+        return gap > 0.0f && !(gap * (p.sigmoid ? expf(-fmaxf(value, 0.0f)) : 1.0f) > 1e-12f);
+    };
     for (int j = 0; j <= p.top_k; ++j) {
         uint32_t best = key[0];
         if constexpr (Exact) {
@@ -473,8 +479,8 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
         if constexpr (Exact) {
             const float value = order_value(best);
             if (j > 0 && best != 0) {
-                const float gap = order_value(previous) - value;
-                again |= gap > 0.0f && !(gap * (p.sigmoid ? expf(-fmaxf(value, 0.0f)) : 1.0f) > 1e-12f);
+                again |= near(order_value(previous), value);
+                tied = best == previous;
                 again |= (p.sigmoid ? value : value - top) < -600.0f && j < p.top_k;
             }
         } else {
@@ -504,6 +510,15 @@ __global__ __launch_bounds__(kWave* kWaves) void route_kernel(RouteArgs p) {
             }
         }
         if (l == j) mine = at;
+    }
+    if constexpr (Exact) {
+        if (__ballot(tied)) {  // the next logit below the tied ones may have their score, and a lower index
+            uint32_t below = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) below = max(below, key[i] < previous ? key[i] : 0);
+            below = row_max_key(below);
+            again |= tied && below != 0 && near(order_value(previous), order_value(below));
+        }
     }
     const bool picked = l < p.top_k;
     const float score = picked ? score_of(row[min(mine, experts - 1)], p.sigmoid, top, inverse) : 0.0f;
