@@ -191,6 +191,15 @@ def check_gradients_that_are_the_seed(device, torch_device):
             np.testing.assert_array_equal(t.grad.numpy(), times * up)
 
 
+def check_numbers_that_are_no_stream(device, torch_device):
+    for stream in (-2, "default"):
+        try:
+            vc.Tensor(np.zeros(3, np.float32), device=device).__dlpack__(stream=stream)
+            raise AssertionError("taken")
+        except RuntimeError:
+            pass
+
+
 def check_steps_of_overlapping_memory(device, torch_device):
     """Tensors imported apart that lie over the same memory: refused before anything is written, but for gradients."""
     memory = torch.tensor(whole(2, 4 * N), device=torch_device)
@@ -292,7 +301,8 @@ RECORDED = [check_results_of_imported_memory, check_elementwise_results_of_impor
             check_results_recorded_before_an_export, check_results_of_exported_memory, check_softmax_gradients,
             check_gradients_of_a_pass_that_fails]
 KEPT = [check_largest_class_after_a_write, check_negative_views, check_picks_written_before_the_gradient, check_steps_of_overlapping_memory,
-        check_steps_of_one_buffer_imported_twice, check_gradients_that_are_the_seed]
+        check_steps_of_one_buffer_imported_twice, check_gradients_that_are_the_seed,
+        check_numbers_that_are_no_stream]
 GPU = [check_order_of_later_writes]
 
 if __name__ == "__main__":

@@ -69,7 +69,8 @@ namespace nn {
 // In place, for every parameter [..., rows, cols]: momentum = mu * momentum + g;
 // p = (1 - rate * decay) * p - rate * sqrt(max(1, cols / rows)) *
 // orthogonalise(g + mu * momentum). g: its entry of `gradients`, or its own
-// gradient where that is empty; a parameter without one is left out.
+// gradient where that is empty; a parameter without one is left out. What is
+// written must not overlap with anything else of the call in memory.
 void muon_step(const std::vector<Tensor*>& parameters, const std::vector<Tensor*>& momenta, float rate, float mu = 0.95F,
                float decay = 0.0F, std::size_t steps = 5, const std::vector<Tensor>& gradients = {});
 

@@ -238,7 +238,8 @@ PYBIND11_MODULE(_vectorcore, m) {
         py::arg("params"), py::arg("momenta"), py::arg("lr"), py::arg("momentum") = 0.95F, py::arg("weight_decay") = 0.0F,
         py::arg("steps") = 5, py::arg("grads") = py::none(),
         "Orthogonalised momentum update in place: m = momentum * m + g; p = (1 - lr * weight_decay) * p - "
-        "lr * sqrt(max(1, cols / rows)) * orthogonalise(g + momentum * m). g: `grads`, or the parameters' own gradients.");
+        "lr * sqrt(max(1, cols / rows)) * orthogonalise(g + momentum * m). g: `grads`, or the parameters' own gradients. "
+        "Parameters and momenta must not overlap with each other or a gradient in memory.");
     m.def("from_dlpack", &dlpack::import_,
           "Tensors over the memory of the given objects (__dlpack__): float32, contiguous, on the host or the GPU. Always a "
           "tuple. Work asked for here from now on waits for what the other library's stream holds now; call it again, or "

@@ -216,8 +216,9 @@ inline py::capsule export_(const Tensor& t, const py::object& stream, const py::
     float* data = nullptr;
     if (type == kRocm) {
         require_one_runtime();
-        data = HipBackend::instance().expose(*e->storage);
         const std::int64_t consumer = stream.is_none() ? 0 : stream.cast<std::int64_t>();
+        if (consumer < -1) throw std::runtime_error("__dlpack__: a stream is a handle, 0 or -1");
+        data = HipBackend::instance().expose(*e->storage);
         if (consumer != -1) {
             e->ordered = true;
             e->stream = static_cast<std::uint64_t>(consumer);
