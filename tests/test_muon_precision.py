@@ -81,6 +81,19 @@ def test_error_of_many_matrices(count, rows, cols, kind):
             assert all(norm(o - want) <= most for o in got[i::3])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,rows,cols", [(16, 26, 3266), (31, 3266, 26), (8, 60, 1000), (8, 200, 300), (40, 12, 700), (4, 130, 900)])
+def test_error_is_no_larger_than_float32s(count, rows, cols):
+    """Random matrices with a short side have nearly equal singular values, which pass a rounding on together. Half as much
+    again as the same iterations in float32 leaves room for the luck of single roundings."""
+    g = [matrix("random", rows, cols, 50 + i) for i in range(count)]
+    got = vc.orthogonalise(vc.Tensor(np.stack(g), device="hip")).numpy()
+    want = [iterate(a, 5, np.float64) for a in g]
+    mine = norm(np.array([norm(o - w) for o, w in zip(got, want)]))
+    float32 = norm(np.array([norm(iterate(a, 5, np.float32) - w) for a, w in zip(g, want)]))
+    assert mine <= 1.5 * float32
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_a_step_at_float32s_precision(device):
     """The parameter itself: keep * p - rate * O, its own rounding beside the iterate's error."""

@@ -8,12 +8,14 @@
 // P = b G + c G G, symmetric, of which the tiles on and above the diagonal are
 // computed and stored twice, and a X + P X: m m n + m m m + 2 m m n operations.
 //
-// All values stay near one by construction (|x| <= 1.21, |g| <= 1.5, |p| <= 3),
+// All values stay near one by construction (|x| <= 1.21, |g| <= 1.5, |p| <= 3; G and
+// P are held around an identity from some iteration on, see Quintic),
 // so the products run as three half-precision products of two parts each
 // (packed_product.hpp), on values scaled by 2^14 in memory: below 2^15.6 they are
 // in half precision's range, and a part below its smallest step is 2^-38 of one.
-// The error is that of a float32 product relative to the norm, which is what the
-// iteration keeps of its input. The scale is a power of two and costs nothing.
+// The error relative to the norm, which is what the iteration keeps of its input, is
+// no larger than that of float32 products (test_muon_precision.py), at half of it for
+// most shapes. The scale is a power of two and costs nothing.
 //
 // Every iterate is written twice, as X (of X and X^T the one with the shorter
 // side first) and transposed, as the products read it along the shared side.
@@ -22,7 +24,7 @@
 // step's matrices fill the chip together, and small ones share the latency.
 //
 // Bound by the matrix instructions where matrices are large: 1024 x 4096, 4096 x
-// 4096 and 4096 x 1000 take 446 us for the last product of an iteration (346
+// 4096 and 4096 x 1000 take 448 us for the last product of an iteration (346
 // TFLOP/s), 268 for G (288) and 231 for P (307), of 408 TFLOP/s that a third of
 // the library's half-precision rate would be; the update and the first split
 // are 88 and 81 us (4.3 TB/s). Small ones are bound by the latency of a launch and its
@@ -39,8 +41,32 @@
 namespace vchip {
 namespace {
 
-constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScale = 16384.0f;
+
+// a, b and c of an iteration around G = H + shift: a X + (b G + c G G) X is
+// (a + b shift + c shift^2) X + ((b + 2 c shift) H + c H H) X. The first iterations
+// bring singular values up from far below one, and G holds them best. In later ones
+// most are near one, where a X and P X cancel to a fifth, and a rounding of P
+// counts five times; with shift 1 nothing cancels and P is small. So is H's
+// diagonal, beside whose squares the matrix instructions cut the other products of
+// a sum short, always to one side (G G: 2 ulp of each diagonal element). 26 x 3266,
+// error relative to the norm: 2.4e-6 with shift 0 throughout, 8.3e-7 so.
+constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
+struct Quintic {
+    float a, b, c, shift;
+};
+__device__ inline Quintic quintic_of(bool shifted) {
+    return shifted ? Quintic{float(kA + kB + kC), float(kB + 2.0 * kC), float(kC), 1.0f} : Quintic{float(kA), float(kB), float(kC), 0.0f};
+}
+// The first iteration with shift 1: where equal singular values, 1 / sqrt(shorter)
+// at first, have passed sqrt(1/2), the third at the latest, which the largest of
+// unlike ones reach by then.
+int turn_of(int64_t shorter) {
+    double s = 1.0 / std::sqrt(double(shorter));
+    int step = 0;
+    for (; step < 2 && s * s < 0.5; ++step) s *= kA + s * s * (kB + s * s * kC);
+    return step;
+}
 constexpr int kNormBlocks = 1024;  // partial sums of squares of a matrix, at most
 constexpr int kAtOnce = 12;       // matrices (or batches of equal ones) of a launch
 constexpr int kMostSplit = 2048;  // tiles of a launch whose sums are split
@@ -56,7 +82,7 @@ struct Matrix {
     half *gram, *poly;        // [shorter, shorter]
     double* partials;
     int64_t rows, cols, shorter, longer;  // the sides are padded to whole tiles
-    int count, blocks;
+    int count, blocks, turn;  // turn: of the iterations, see turn_of
     float rate;
     // Of the launch: the first workgroup (or die's); the tiles from `from`; parts of each one's sum; split tiles and parts before.
     int first, from, tiles, splits, counters, parts;
@@ -234,26 +260,28 @@ __global__ __launch_bounds__(256) void small_kernel(Batch batch, float mu, float
     const f16v zero = {};
     const int i0 = tall_tiles == 2 ? wave / 2 * 32 : 0, j0 = tall_tiles == 2 ? wave % 2 * 32 : 0;  // this wave's tile
     for (int step = 0; step < steps; ++step) {
-        // G; a single tile's k is shared out to the waves.
+        const Quintic f = quintic_of(step >= m.turn);
+        // H; a single tile's k is shared out to the waves.
         if (tall_tiles == 2) {
             each_value(multiply_rows(x + i0 * stride, x + j0 * stride, stride, 0, 32 * long_tiles, zero),
-                       [&](int r, int c, float v) { g[(i0 + r) * kSquareStride + j0 + c] = v; });
+                       [&](int r, int c, float v) { g[(i0 + r) * kSquareStride + j0 + c] = v - (i0 + r == j0 + c ? f.shift : 0.0f); });
         } else {
             each_value(multiply_rows(x, x, stride, 8 * long_tiles * wave, 8 * long_tiles * (wave + 1), zero),
                        [&](int r, int c, float v) { q[wave * 1024 + r * 32 + c] = v; });
             __syncthreads();
             for (int i = threadIdx.x; i < 1024; i += 256) {
                 const float* const part = q + i;
-                g[i / 32 * kSquareStride + i % 32] = (part[0] + part[1024]) + (part[2 * 1024] + part[3 * 1024]);
+                g[i / 32 * kSquareStride + i % 32] =
+                    (part[0] + part[1024]) + (part[2 * 1024] + part[3 * 1024]) - (i / 32 == i % 32 ? f.shift : 0.0f);
             }
         }
         __syncthreads();
-        // Q = a I + b G + c G G
+        // Q = a I + b H + c H H
         if (tall_tiles == 2 || wave == 0)
             each_value(multiply_rows(g + i0 * kSquareStride, g + j0 * kSquareStride, kSquareStride, 0, 32 * tall_tiles, zero),
                        [&](int r, int c, float v) {
                            const int place = (i0 + r) * kSquareStride + j0 + c;
-                           q[place] = kB * g[place] + kC * v + (i0 + r == j0 + c ? kA : 0.0f);
+                           q[place] = f.b * g[place] + f.c * v + (i0 + r == j0 + c ? f.a : 0.0f);
                        });
         __syncthreads();
         // X = Q X, whole columns a wave
@@ -295,7 +323,7 @@ __device__ unsigned g_tile_done[kMostSplit];
 // A tile of G, P or the next X. last: the next X leaves the scale, to `out` or
 // into the parameter.
 template <Kind K, int BT, int Stages>
-__global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batch, bool last, float keep, float* partial) {
+__global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batch, int step, bool last, float keep, float* partial) {
     using Tile = packed::Tile<BT, Stages>;
     __shared__ __align__(16) char lds[Tile::kLds];
     __shared__ bool finisher;
@@ -303,6 +331,7 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
     // whose operands its cache then serves (an iteration of the large matrices above 1013 to 990 us). Shares of
     // the whole batch instead gave dies matrices of unlike depth, and the last product took a quarter longer.
     const Matrix& m = batch.of[find(batch, int(blockIdx.x) / 8)];
+    const bool shifted = step >= m.turn;  // (read with the rest of m)
     const int row_tiles = int(m.shorter / BT), column_tiles = K == Kind::Apply ? int(m.longer / BT) : row_tiles;
     const int tiles = K == Kind::Apply ? row_tiles * column_tiles : row_tiles * (row_tiles + 1) / 2;
     const int blocks = m.tiles * m.splits, share = (blocks + 7) / 8;
@@ -342,7 +371,7 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
     const half* const b = K == Kind::Gram ? a : K == Kind::Poly ? a : m.xt + whole;
     Tile tile;
     tile.clear();
-    tile.accumulate(a + m0 * 2 * depth, b + n0 * 2 * depth, depth, slices * part / m.splits, slices * (part + 1) / m.splits, lds);
+    tile.template accumulate<K == Kind::Gram>(a + m0 * 2 * depth, b + n0 * 2 * depth, depth, slices * part / m.splits, slices * (part + 1) / m.splits, lds);
 
     if (m.splits > 1) {
         // The part that counts in last adds all of them in order.
@@ -377,8 +406,9 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
     }
 
     const float unit = 1.0f / kScale;
+    const Quintic f = quintic_of(shifted);
     if constexpr (K == Kind::Apply) {
-        tile.mix(kA, m.x + whole, unit, m0, n0, m.longer);
+        tile.mix(f.a, m.x + whole, unit, m0, n0, m.longer);
         if (!last) {
             tile.store(m.y + whole, m0, n0, m.longer);
             tile.store_transposed(m.yt + whole, m0, n0, m.shorter, lds);
@@ -401,11 +431,11 @@ __global__ __launch_bounds__(packed::kThreads, 2) void product_kernel(Batch batc
     } else {
         half* const out = (K == Kind::Gram ? m.gram : m.poly) + square;
         if constexpr (K == Kind::Poly) {
-            tile.mix(kB, m.gram + square, kC * unit, m0, n0, m.shorter);
+            tile.mix(f.b, m.gram + square, f.c * unit, m0, n0, m.shorter);
         } else {
-            tile.each4([&](int, int, float (&v)[4]) {
+            tile.each4([&](int r, int c, float (&v)[4]) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= unit;
+                for (int e = 0; e < 4; ++e) v[e] = v[e] * unit - (i == j && r + e == c ? f.shift * kScale : 0.0f);
             });
         }
         tile.store(out, m0, n0, m.shorter);
@@ -441,7 +471,7 @@ int64_t tiles_of(Kind kind, const Matrix& m, int64_t bt) {
 // tiles for 512 places: both products 532 to 504 us an iteration, P alone 264 to
 // 233; twice as many parts of the last round, or more, gained no more.)
 template <Kind K, int BT>
-void product(Device& d, Batch batch, bool last = false, float keep = 0.0f) {
+void product(Device& d, Batch batch, int step, bool last = false, float keep = 0.0f) {
     const auto slices = [](const Matrix& m) { return (K == Kind::Gram ? m.longer : m.shorter) / packed::kSlice; };
     int64_t tiles = 0, most = 0;
     for (int i = 0; i < batch.n; ++i) {
@@ -483,9 +513,9 @@ void product(Device& d, Batch batch, bool last = false, float keep = 0.0f) {
     Scratch partial(parts ? size_t(parts) * BT * BT * sizeof(float) : 4);
     const dim3 grid{unsigned(8 * shares)}, threads{packed::kThreads};
     if (blocks <= d.cu_count)
-        launch(product_kernel<K, BT, 4>, grid, threads, 0, d.stream, batch, last, keep, partial.as<float>());
+        launch(product_kernel<K, BT, 4>, grid, threads, 0, d.stream, batch, step, last, keep, partial.as<float>());
     else
-        launch(product_kernel<K, BT, 2>, grid, threads, 0, d.stream, batch, last, keep, partial.as<float>());
+        launch(product_kernel<K, BT, 2>, grid, threads, 0, d.stream, batch, step, last, keep, partial.as<float>());
     after_launch("orthogonalise product");
 }
 
@@ -508,6 +538,7 @@ bool wide_tiles(const Device& d, const Batch& batch, Kind kind) {
 
 // The iterates of a batch; x and its successor take turns.
 void run(Device& d, Batch& batch, float mu, float keep, size_t steps) {
+    for (int i = 0; i < batch.n; ++i) batch.of[i].turn = turn_of(std::min(batch.of[i].rows, batch.of[i].cols));
     if (steps > 0 && steps <= kMostSteps && std::all_of(batch.of, batch.of + batch.n, small)) {
         const int64_t matrices = assign(batch, [](const Matrix& m) { return int64_t(m.count); });
         launch(small_kernel, dim3(unsigned(matrices)), dim3(256), 0, d.stream, batch, mu, keep, int(steps));
@@ -564,9 +595,10 @@ void run(Device& d, Batch& batch, float mu, float keep, size_t steps) {
     after_launch("orthogonalise pack");
     for (size_t i = 0; i < steps; ++i) {
         const bool last = i + 1 == steps;
-        wide_gram ? product<Kind::Gram, 128>(d, batch) : product<Kind::Gram, 64>(d, batch);
-        wide_poly ? product<Kind::Poly, 128>(d, batch) : product<Kind::Poly, 64>(d, batch);
-        wide_apply ? product<Kind::Apply, 128>(d, batch, last, keep) : product<Kind::Apply, 64>(d, batch, last, keep);
+        const int step = int(std::min<size_t>(i, 2));  // all later ones are like the third
+        wide_gram ? product<Kind::Gram, 128>(d, batch, step) : product<Kind::Gram, 64>(d, batch, step);
+        wide_poly ? product<Kind::Poly, 128>(d, batch, step) : product<Kind::Poly, 64>(d, batch, step);
+        wide_apply ? product<Kind::Apply, 128>(d, batch, step, last, keep) : product<Kind::Apply, 64>(d, batch, step, last, keep);
         for (int k = 0; k < batch.n; ++k) {
             std::swap(batch.of[k].x, batch.of[k].y);
             std::swap(batch.of[k].xt, batch.of[k].yt);
