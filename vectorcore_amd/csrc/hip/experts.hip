@@ -147,10 +147,10 @@ Plan plan_of(const vc_hip_expert_plan* plan) {
 // ---- products -----------------------------------------------------------------------
 // Tiles of 64 or 128 rows of one group (split_product.hpp). Bound by the matrix
 // instructions and, beside them, by the vector instructions that split operands:
-// 16384 rows of 8 experts, 1024 x 4096, reach 180 TFLOP/s in the gated unit, 158 in
-// the plain product, 172 to the rows and 171 to the weights, of 215 that a sixth of
-// the library's bfloat16 rate would be. 49152 rows of 64 experts, 1024 x 512: 156,
-// 153, 165 and 121, as sums of 768 rows leave prologues and stores a larger share.
+// 16384 rows of 8 experts, 1024 x 4096, reach 177 TFLOP/s in the gated unit, 154 in
+// the plain product, 170 to the rows and 170 to the weights, of 215 that a sixth of
+// the library's bfloat16 rate would be. 49152 rows of 64 experts, 1024 x 512: 154,
+// 151, 162 and 119, as sums of 768 rows leave prologues and stores a larger share.
 //
 // A sum that is not finite (an infinity or NaN among its operands, or a value that
 // rounds to an infinity) is computed again by its lane, term after term: right, but

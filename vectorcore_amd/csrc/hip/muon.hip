@@ -24,11 +24,11 @@
 // step's matrices fill the chip together, and small ones share the latency.
 //
 // Bound by the matrix instructions where matrices are large: 1024 x 4096, 4096 x
-// 4096 and 4096 x 1000 take 448 us for the last product of an iteration (346
-// TFLOP/s), 268 for G (288) and 231 for P (307), of 408 TFLOP/s that a third of
+// 4096 and 4096 x 1000 take 453 us for the last product of an iteration (340
+// TFLOP/s), 277 for G (279) and 232 for P (305), of 408 TFLOP/s that a third of
 // the library's half-precision rate would be; the update and the first split
-// are 88 and 81 us (4.3 TB/s). Small ones are bound by the latency of a launch and its
-// first loads: 784 x 256 and 256 x 10 take 24 us an iteration.
+// are 88 and 80 us (4.3 TB/s). Small ones are bound by the latency of a launch and its
+// first loads: 784 x 256 and 256 x 10 take 25 us an iteration.
 #include "packed_product.hpp"
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"

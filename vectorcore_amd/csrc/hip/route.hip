@@ -17,7 +17,7 @@
 // Many rows would be bound by HBM (the logits are read, the gradient is written)
 // and are, forward, by vector instructions still: sixteen lanes share a row, so
 // four rows share each step of a search or sum across lanes. 65536 rows of 256
-// experts: 50.2 us forward (1.4 TB/s), 18.1 us backward (67 MB written, 3.7 TB/s);
+// experts: 50.9 us forward (1.4 TB/s), 18.1 us backward (67 MB written, 3.7 TB/s);
 // 4096 rows of 64: 4.1 and 3.9 us, a launch's latency.
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"
