@@ -500,6 +500,38 @@ int vc_hip_release_to_stream(uint64_t stream);
  * libraries that must not be freed before. */
 int vc_hip_when_done(void (*done)(void*), void* context);
 
+/* ---- layer normalisation ----------------------------------------------------------------
+ * No counterpart in the reference. */
+/* y = (x - mean) / sqrt(variance + eps) * weight + bias for each row of x [rows, width]; weight and bias [width], each
+ * may be NULL. stats [rows, 4], on a 16-byte boundary, or NULL: what the backward needs of each row. eps >= 0. */
+int vc_hip_layer_norm_forward(const float* x, const float* weight, const float* bias, size_t rows, size_t width, float eps,
+                              float* y, float* stats);
+/* The gradients of x, weight and bias from that of y; each may be NULL, and weight as in the forward. */
+int vc_hip_layer_norm_backward(const float* grad, const float* x, const float* weight, const float* stats, size_t rows,
+                               size_t width, float* grad_x, float* grad_weight, float* grad_bias);
+
+/* ---- dropout ---------------------------------------------------------------------------
+ * No counterpart in the reference. */
+/* out[i] = (kept(i) ? x[i] / (1 - p) : 0) + residual[i]; residual may be NULL. Element i is kept where word i % 4 of
+ * Philox 4x32-10 of the 128-bit counter (i / 4, stream) under the 64-bit key seed is at least round(p 2^32). Also the
+ * gradient of x from that of out, without the residual. 0 <= p <= 1. */
+int vc_hip_dropout(const float* x, const float* residual, size_t count, double p, uint64_t seed, uint64_t stream,
+                   float* out);
+
+/* ---- the loss of a linear layer -------------------------------------------------------
+ * No counterpart in the reference. */
+/* The softmax cross entropy of z = x W + bias for each row of x [rows, width], W [width, classes], bias [classes] or
+ * NULL, without keeping z. targets [rows]: class numbers as floats; a row whose target is no class number is left out:
+ * its loss is zero, whatever its values. losses [rows], mean [1] (over the rows that count, zero if none does): either
+ * may be NULL. */
+int vc_hip_linear_xent_forward(const float* x, const float* weight, const float* bias, const float* targets, size_t rows,
+                               size_t width, size_t classes, float* losses, float* mean);
+/* The gradients of sum_t shares[t] loss_t; each may be NULL. shares NULL: those of the mean loss, which then goes to
+ * mean (or NULL). A row that is left out has a gradient of zero and no part in the others. */
+int vc_hip_linear_xent_gradient(const float* x, const float* weight, const float* bias, const float* targets,
+                                const float* shares, size_t rows, size_t width, size_t classes, float* mean,
+                                float* grad_x, float* grad_weight, float* grad_bias);
+
 /* ---- mixture of experts -------------------------------------------------------------
  * No counterpart in the reference. */
 /* Scores of a router: softmax over the experts, or a sigmoid of each logit. */

@@ -12,6 +12,7 @@ from ._vectorcore import (  # noqa: F401
     Linear,
     Tensor,
     cross_entropy,
+    dropout,
     expert_combine,
     expert_gated,
     expert_linear,
@@ -27,6 +28,8 @@ from ._vectorcore import (  # noqa: F401
     hip_profile,
     hip_profile_read,
     hip_profile_reset,
+    layer_norm,
+    linear_cross_entropy,
     log_softmax,
     metal_available,
     metal_device_name,

@@ -30,14 +30,16 @@ OBJ = PKG / "_build"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
-HIP_SOURCES = ["runtime.hip", "elementwise.hip", "reduce.hip", "xent.hip", "softmax.hip", "gemm.hip", "route.hip",
+HIP_SOURCES = ["runtime.hip", "elementwise.hip", "reduce.hip", "xent.hip", "softmax.hip", "gemm.hip", "layer_norm.hip", "dropout.hip",
+               "linear_xent.hip", "route.hip",
                "experts.hip", "muon.hip", "fused_map.hip"]
 # Sources compiled once per define set: the fused-map interpreters, one object
 # per input count, so that they compile in parallel.
 HIP_VARIANT_SOURCES = {"fused_map_inputs.hip": [[f"-DVC_MAP_NIN={k}"] for k in range(1, 9)]}
-LIB_SOURCES = ["shape.cpp", "storage.cpp", "tensor.cpp", "autograd.cpp", "ops.cpp", "nn.cpp", "experts.cpp",
+LIB_SOURCES = ["shape.cpp", "storage.cpp", "tensor.cpp", "autograd.cpp", "ops.cpp", "nn.cpp", "layers.cpp", "experts.cpp",
                "muon.cpp",
-               "cpu/parallel.cpp", "cpu/cpu_backend.cpp", "cpu/expert_backend.cpp", "hip/hip_backend.cpp"]
+               "cpu/parallel.cpp", "cpu/cpu_backend.cpp", "cpu/layer_backend.cpp",
+               "cpu/expert_backend.cpp", "hip/hip_backend.cpp"]
 BINDINGS = "python/bindings.cpp"
 CPP_TEST = ROOT / "tests" / "cpp" / "test_vectorcore.cpp"
 ORACLE_C = ROOT / "oracle" / "vc_oracle.c"

@@ -160,6 +160,11 @@ _SIGNATURES = {
     "vc_hip_wait_for_stream": ([ctypes.c_uint64], _i),
     "vc_hip_release_to_stream": ([ctypes.c_uint64], _i),
     "vc_hip_when_done": ([WHEN_DONE, _vp], _i),
+    "vc_hip_layer_norm_forward": ([_vp, _vp, _vp, _sz, _sz, _f, _vp, _vp], _i),
+    "vc_hip_layer_norm_backward": ([_vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp], _i),
+    "vc_hip_dropout": ([_vp, _vp, _sz, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _vp], _i),
+    "vc_hip_linear_xent_forward": ([_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp], _i),
+    "vc_hip_linear_xent_gradient": ([_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp], _i),
     "vc_hip_route_forward": ([_vp, _vp, _sz, _sz, _sz, _i, _sz, _sz, _i, _vp, _vp], _i),
     "vc_hip_route_backward": ([_vp, _vp, _vp, _sz, _sz, _sz, _i, _i, _vp], _i),
     "vc_hip_expert_plan_words": ([_sz, _sz, _sz, _szp], _i),

@@ -1628,6 +1628,79 @@ std::shared_ptr<Storage> HipBackend::cross_entropy_backward(const Storage& logit
     return out;
 }
 
+// ---- layer normalisation, dropout, the loss of a linear layer ----------------------
+
+namespace {
+float* optional_ptr(const Storage* s, std::size_t offset) { return s ? dptr(*s, offset) : nullptr; }
+// A new storage of `count` elements in *out, if that is wanted; its address.
+float* output(std::shared_ptr<Storage>* out, std::size_t count) {
+    if (!out) return nullptr;
+    auto made = fresh(count);
+    *out = made;
+    return made->ptr();
+}
+}  // namespace
+
+std::shared_ptr<Storage> HipBackend::layer_norm_forward(const Storage& x, std::size_t x_offset, const Storage* weight,
+                                                        std::size_t weight_offset, const Storage* bias, std::size_t bias_offset,
+                                                        std::size_t rows, std::size_t width, float eps,
+                                                        std::shared_ptr<Storage>* stats) {
+    require(*this);
+    auto out = fresh(rows * width);
+    check(vc_hip_layer_norm_forward(dptr(x, x_offset), optional_ptr(weight, weight_offset), optional_ptr(bias, bias_offset), rows,
+                                    width, eps, out->ptr(), output(stats, 4 * rows)),
+          "HIP layer_norm failed");
+    return out;
+}
+
+void HipBackend::layer_norm_backward(const Storage& grad, std::size_t grad_offset, const Storage& x, std::size_t x_offset,
+                                     const Storage* weight, std::size_t weight_offset, const Storage& stats, std::size_t rows,
+                                     std::size_t width, std::shared_ptr<Storage>* grad_x, std::shared_ptr<Storage>* grad_weight,
+                                     std::shared_ptr<Storage>* grad_bias) {
+    require(*this);
+    check(vc_hip_layer_norm_backward(dptr(grad, grad_offset), dptr(x, x_offset), optional_ptr(weight, weight_offset),
+                                     dptr(stats, 0), rows, width, output(grad_x, rows * width), output(grad_weight, width),
+                                     output(grad_bias, width)),
+          "HIP layer_norm backward failed");
+}
+
+std::shared_ptr<Storage> HipBackend::dropout(const Storage& x, std::size_t x_offset, const Storage* residual,
+                                             std::size_t residual_offset, std::size_t count, double p, std::uint64_t seed,
+                                             std::uint64_t stream) {
+    require(*this);
+    auto out = fresh(count);
+    check(vc_hip_dropout(dptr(x, x_offset), optional_ptr(residual, residual_offset), count, p, seed, stream, out->ptr()),
+          "HIP dropout failed");
+    return out;
+}
+
+std::shared_ptr<Storage> HipBackend::linear_xent_forward(const Storage& x, std::size_t x_offset, const Storage& weight,
+                                                         std::size_t weight_offset, const Storage* bias, std::size_t bias_offset,
+                                                         const Storage& targets, std::size_t targets_offset, std::size_t rows,
+                                                         std::size_t width, std::size_t classes, bool mean) {
+    require(*this);
+    auto out = fresh(mean ? 1 : rows);
+    check(vc_hip_linear_xent_forward(dptr(x, x_offset), dptr(weight, weight_offset), optional_ptr(bias, bias_offset),
+                                     dptr(targets, targets_offset), rows, width, classes, mean ? nullptr : out->ptr(),
+                                     mean ? out->ptr() : nullptr),
+          "HIP linear_cross_entropy failed");
+    return out;
+}
+
+void HipBackend::linear_xent_gradient(const Storage& x, std::size_t x_offset, const Storage& weight, std::size_t weight_offset,
+                                      const Storage* bias, std::size_t bias_offset, const Storage& targets,
+                                      std::size_t targets_offset, const Storage* shares, std::size_t shares_offset,
+                                      std::size_t rows, std::size_t width, std::size_t classes, std::shared_ptr<Storage>* mean,
+                                      std::shared_ptr<Storage>* grad_x, std::shared_ptr<Storage>* grad_weight,
+                                      std::shared_ptr<Storage>* grad_bias) {
+    require(*this);
+    check(vc_hip_linear_xent_gradient(dptr(x, x_offset), dptr(weight, weight_offset), optional_ptr(bias, bias_offset),
+                                      dptr(targets, targets_offset), optional_ptr(shares, shares_offset), rows, width, classes,
+                                      output(mean, 1), output(grad_x, rows * width), output(grad_weight, width * classes),
+                                      output(grad_bias, classes)),
+          "HIP linear_cross_entropy gradient failed");
+}
+
 // ---- a mixture of experts ----------------------------------------------------------
 
 std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> HipBackend::route_forward(

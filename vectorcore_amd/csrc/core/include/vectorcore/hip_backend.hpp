@@ -216,6 +216,35 @@ public:
                                                                   std::size_t rows, std::size_t classes,
                                                                   bool column_sum = false);
 
+    // --- layer normalisation, dropout, the loss of a linear layer (the entry points of the same names) ---
+    // weight, bias: or null. stats: receives the rows' statistics, or null.
+    [[nodiscard]] std::shared_ptr<Storage> layer_norm_forward(const Storage& x, std::size_t x_offset, const Storage* weight,
+                                                              std::size_t weight_offset, const Storage* bias,
+                                                              std::size_t bias_offset, std::size_t rows, std::size_t width,
+                                                              float eps, std::shared_ptr<Storage>* stats);
+    // The gradients that are not null are computed.
+    void layer_norm_backward(const Storage& grad, std::size_t grad_offset, const Storage& x, std::size_t x_offset,
+                             const Storage* weight, std::size_t weight_offset, const Storage& stats, std::size_t rows,
+                             std::size_t width, std::shared_ptr<Storage>* grad_x, std::shared_ptr<Storage>* grad_weight,
+                             std::shared_ptr<Storage>* grad_bias);
+    // residual: or null.
+    [[nodiscard]] std::shared_ptr<Storage> dropout(const Storage& x, std::size_t x_offset, const Storage* residual,
+                                                   std::size_t residual_offset, std::size_t count, double p,
+                                                   std::uint64_t seed, std::uint64_t stream);
+    // The mean loss (one element) or the rows' losses.
+    [[nodiscard]] std::shared_ptr<Storage> linear_xent_forward(const Storage& x, std::size_t x_offset, const Storage& weight,
+                                                               std::size_t weight_offset, const Storage* bias,
+                                                               std::size_t bias_offset, const Storage& targets,
+                                                               std::size_t targets_offset, std::size_t rows,
+                                                               std::size_t width, std::size_t classes, bool mean);
+    // The gradients that are not null are computed; shares null: those of the mean loss, which goes to *mean.
+    void linear_xent_gradient(const Storage& x, std::size_t x_offset, const Storage& weight, std::size_t weight_offset,
+                              const Storage* bias, std::size_t bias_offset, const Storage& targets,
+                              std::size_t targets_offset, const Storage* shares, std::size_t shares_offset, std::size_t rows,
+                              std::size_t width, std::size_t classes, std::shared_ptr<Storage>* mean,
+                              std::shared_ptr<Storage>* grad_x, std::shared_ptr<Storage>* grad_weight,
+                              std::shared_ptr<Storage>* grad_bias);
+
     // --- a mixture of experts (the entry points of the same names) ---
     // {weights, chosen}.
     [[nodiscard]] std::pair<std::shared_ptr<Storage>, std::shared_ptr<Storage>> route_forward(

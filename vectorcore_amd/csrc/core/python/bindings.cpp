@@ -68,6 +68,14 @@ std::vector<std::size_t> targets_from(const py::object& obj) {
     return py::cast<std::vector<std::size_t>>(obj);
 }
 
+// Integer targets with -1 for rows that are left out, of one dimension.
+std::vector<std::int64_t> signed_targets_from(const py::object& obj) {
+    if (!py::isinstance<py::array>(obj)) return py::cast<std::vector<std::int64_t>>(obj);
+    auto arr = py::array_t<std::int64_t, py::array::c_style | py::array::forcecast>::ensure(obj);
+    if (!arr || arr.ndim() != 1) throw std::invalid_argument("linear_cross_entropy expects targets of shape [rows]");
+    return {arr.data(), arr.data() + arr.size()};
+}
+
 void check(int status) {
     if (status != VC_HIP_OK) throw std::runtime_error(vc_hip_last_error());
 }
@@ -181,6 +189,29 @@ PYBIND11_MODULE(_vectorcore, m) {
           },
           py::arg("logits"), py::arg("targets"),
           "Mean softmax cross-entropy of [batch, classes] logits and integer class targets.");
+    m.def("layer_norm", &nn::layer_norm, py::arg("x"), py::arg("weight") = py::none(), py::arg("bias") = py::none(),
+          py::arg("eps") = 1e-5F,
+          "(x - mean) / sqrt(variance + eps) over the last axis of x, times weight, plus bias, both [width] or None.");
+    m.def("dropout", &nn::dropout, py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("stream") = 0,
+          py::arg("residual") = py::none(),
+          "Each element of x with probability p zero, else divided by 1 - p; plus residual, of x's shape, if given. Which "
+          "elements is a function of their flat index, seed and stream alone (Philox 4x32-10): the mask is not kept, and each "
+          "call that is to draw its own takes a seed or stream of its own. p = 0 gives x (plus residual).");
+    m.def(
+        "linear_cross_entropy",
+        [](const Tensor& x, const Tensor& weight, const py::object& targets, std::optional<Tensor> bias,
+           const std::string& reduction) {
+            if (reduction != "mean" && reduction != "none") throw std::invalid_argument("reduction must be 'mean' or 'none'");
+            const auto r = reduction == "mean" ? nn::Reduction::Mean : nn::Reduction::None;
+            if (py::isinstance<Tensor>(targets))
+                return nn::linear_cross_entropy(x, weight, py::cast<Tensor>(targets), bias, r);
+            return nn::linear_cross_entropy(x, weight, signed_targets_from(targets), bias, r);
+        },
+        py::arg("x"), py::arg("weight"), py::arg("targets"), py::arg("bias") = py::none(), py::arg("reduction") = "mean",
+        "Softmax cross entropy of x @ weight + bias, whose [rows, classes] logits are never kept. targets: class numbers, as "
+        "integers or as a Tensor of floats on x's device; -1 (in a Tensor anything that is no class number) leaves a row out. "
+        "reduction 'mean': over the rows that count, zero if none does, its gradients computed with it; 'none': the loss of "
+        "each row, zero for one left out.");
     m.def("softmax", [](const Tensor& t, std::int64_t axis) { return t.softmax(axis); }, py::arg("value"),
           py::arg("axis") = -1);
     m.def("log_softmax", [](const Tensor& t, std::int64_t axis) { return t.log_softmax(axis); }, py::arg("value"),

@@ -1,0 +1,490 @@
+// Layer normalisation over the last axis of [rows, width], and its gradients.
+//
+// With m and v a row's mean and variance, r = 1 / sqrt(v + eps) and
+// h = (x - m) r:
+//   y  = h w + b
+//   dx = r (d - mean(d) - h mean(d h)),  d = dy w
+//   dw = the sum over rows of dy h,      db = the sum over rows of dy.
+//
+// Bound by HBM: the forward reads x and writes y, the backward reads x and dy
+// and writes dx. So a row stays in registers between its statistics and what is
+// made of it, and the backward collects dw and db on the way: a thread holds the
+// same columns of every row of its workgroup, each workgroup leaves one partial
+// row of either sum, and a second launch adds those in a fixed order, in double.
+//
+// A row's mean is kept as a float and what the float is off by: x - m would
+// otherwise lose the bits of a row that lies far from zero. The statistics are
+// sums of at most 64 values a lane, then a tree.
+#include "reduce_common.hpp"
+#include "vc_hip_internal.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+namespace vchip {
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+// 16 bytes on any 4-byte boundary, as rows of any length start.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// What the forward leaves of a row: x - mean - rest is exact to a rounding, times scale it is h.
+struct alignas(16) RowStats {
+    float mean, rest, scale, unused;
+};
+
+// G threads hold a row of up to 4 G NV values: values 4 t + 4 G u .. of thread t. Groups of up to a wavefront share a
+// workgroup of 256 threads; a larger group is a workgroup.
+template <int G>
+constexpr int kThreadsOf = G > 256 ? G : 256;
+template <int G, int NV>
+struct Shape {
+    static constexpr int kThreads = kThreadsOf<G>, kGroups = kThreads / G, kMost = 4 * G * NV;
+    static constexpr int kWaves = G > 64 ? G / 64 : 1;  // of a group
+    // Of 16 wavefronts 128 registers a thread do not hold four groups of x, dy, w, dw and db.
+    static constexpr bool kHoldsSums = G < 1024 || NV < 4;
+};
+
+template <int G>
+__device__ inline float lanes_sum(float v) {
+    const int lane = red::lane_id();
+    v += red::partner<0>(v, lane);
+    v += red::partner<1>(v, lane);
+    if constexpr (G >= 8) v += red::partner<2>(v, lane);
+    if constexpr (G >= 16) v += red::partner<3>(v, lane);
+    if constexpr (G >= 32) v += red::partner<4>(v, lane);
+    if constexpr (G >= 64) v += red::partner<5>(v, lane);
+    return v;
+}
+
+// Sums of N values over a group; every thread of it gets them. A group of several wavefronts exchanges through one of two
+// places in turn: who is a whole reduction ahead has passed a barrier that all others reached after reading.
+template <int G, int N>
+struct GroupSum {
+    float (*place)[Shape<G, 1>::kWaves][N];  // [2]
+    int turn = 0;
+    __device__ inline void operator()(float (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = lanes_sum<(G < 64 ? G : 64)>(v[i]);
+        if constexpr (G > 64) {
+            if (threadIdx.x % 64 == 0) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) place[turn][threadIdx.x / 64][i] = v[i];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                v[i] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < Shape<G, 1>::kWaves; ++w) v[i] += place[turn][w][i];
+            }
+            turn ^= 1;
+        }
+    }
+};
+
+template <int G, int NV>
+__device__ inline void load(const float* __restrict__ row, int width, int t, float fill, f4 (&v)[NV]) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        const int a = 4 * t + 4 * G * u;
+        if (a + 3 < width) {
+            v[u] = *reinterpret_cast<const f4u*>(row + a);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[u][e] = a + e < width ? row[a + e] : fill;
+        }
+    }
+}
+template <int G, int NV>
+__device__ inline void store(float* __restrict__ row, int width, int t, const f4 (&v)[NV]) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        const int a = 4 * t + 4 * G * u;
+        if (a + 3 < width) {
+            *reinterpret_cast<f4u*>(row + a) = v[u];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (a + e < width) row[a + e] = v[u][e];
+        }
+    }
+}
+
+// The row's values become x - mean - rest, zeros past its end; the same for every thread of the group.
+template <int G, int NV>
+__device__ inline RowStats statistics(f4 (&v)[NV], int width, int t, float eps, GroupSum<G, 2>& sum) {
+    const float n = float(width);
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0] += v[u][e];
+    sum(s);
+    RowStats st;
+    st.mean = s[0] / n;
+    s[0] = s[1] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[u][e] = 4 * t + 4 * G * u + e < width ? v[u][e] - st.mean : 0.0f;
+            s[0] += v[u][e];
+            s[1] = __builtin_fmaf(v[u][e], v[u][e], s[1]);
+        }
+    sum(s);
+    st.rest = s[0] / n;
+    // The mean of (x - mean)^2 exceeds the variance by rest^2, which is 2^-48 of mean^2 at most.
+    st.scale = 1.0f / sqrtf(fmaxf(s[1] / n - st.rest * st.rest, 0.0f * s[1]) + eps);
+    st.unused = 0.0f;
+    return st;
+}
+
+template <int G, int NV>
+__global__ __launch_bounds__(kThreadsOf<G>) void rows_forward_kernel(
+    const float* __restrict__ x, const float* __restrict__ weight, const float* __restrict__ bias, float* __restrict__ y,
+    RowStats* __restrict__ stats, int64_t rows, int width, float eps) {
+    constexpr int kGroups = Shape<G, NV>::kGroups;
+    __shared__ float place[2][Shape<G, 1>::kWaves][2];
+    GroupSum<G, 2> sum{place};
+    const int t = threadIdx.x % G;
+    f4 w[NV], b[NV];
+    if (weight) load<G>(weight, width, t, 0.0f, w);
+    if (bias) load<G>(bias, width, t, 0.0f, b);
+    for (int64_t first = int64_t(blockIdx.x) * kGroups; first < rows; first += int64_t(gridDim.x) * kGroups) {
+        const int64_t r = first + threadIdx.x / G;
+        const bool there = r < rows;  // the wavefront stays whole
+        f4 v[NV];
+        load<G>(x + (there ? r : rows - 1) * width, width, t, 0.0f, v);
+        const RowStats st = statistics<G>(v, width, t, eps, sum);
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float h = (v[u][e] - st.rest) * st.scale;
+                v[u][e] = weight ? h * w[u][e] : h;
+                if (bias) v[u][e] += b[u][e];
+            }
+        if (there) {
+            store<G>(y + r * width, width, t, v);
+            if (stats && t == 0) stats[r] = st;
+        }
+    }
+}
+
+// Columns: dw and db wanted; sums [gridDim.x][2][width], this workgroup's rows.
+template <int G, int NV, bool Columns>
+__global__ __launch_bounds__(kThreadsOf<G>) void rows_backward_kernel(
+    const float* __restrict__ grad, const float* __restrict__ x, const float* __restrict__ weight,
+    const RowStats* __restrict__ stats, float* __restrict__ dx, float* __restrict__ sums, int64_t rows, int width) {
+    constexpr int kGroups = Shape<G, NV>::kGroups, kMost = Shape<G, NV>::kMost;
+    __shared__ float place[2][Shape<G, 1>::kWaves][2];
+    __shared__ float columns[Columns && kGroups > 1 ? kGroups * kMost : 1];
+    GroupSum<G, 2> sum{place};
+    const int t = threadIdx.x % G;
+    const float n = float(width);
+    f4 w[NV], dw[Columns ? NV : 1] = {}, db[Columns ? NV : 1] = {};
+    if (weight) load<G>(weight, width, t, 0.0f, w);
+    for (int64_t first = int64_t(blockIdx.x) * kGroups; first < rows; first += int64_t(gridDim.x) * kGroups) {
+        const int64_t r = first + threadIdx.x / G;
+        const bool there = r < rows;
+        const int64_t at = there ? r : rows - 1;
+        f4 h[NV], d[NV];
+        load<G>(x + at * width, width, t, 0.0f, h);
+        load<G>(grad + at * width, width, t, 0.0f, d);
+        const RowStats st = stats[at];
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                h[u][e] = 4 * t + 4 * G * u + e < width ? (h[u][e] - st.mean - st.rest) * st.scale : 0.0f;
+                if constexpr (Columns) {
+                    if (there) {
+                        dw[u][e] = __builtin_fmaf(d[u][e], h[u][e], dw[u][e]);
+                        db[u][e] += d[u][e];
+                    }
+                }
+                if (weight) d[u][e] *= w[u][e];
+                s[0] += d[u][e];
+                s[1] = __builtin_fmaf(d[u][e], h[u][e], s[1]);
+            }
+        if (!dx) continue;  // the same in every thread
+        sum(s);
+        s[0] /= n;
+        s[1] /= n;
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[u][e] = (d[u][e] - s[0] - h[u][e] * s[1]) * st.scale;
+        if (there) store<G>(dx + r * width, width, t, d);
+    }
+    if constexpr (Columns) {
+        float* const out = sums + int64_t(blockIdx.x) * 2 * width;
+        if constexpr (kGroups == 1) {
+            store<G>(out, width, t, dw);
+            store<G>(out + width, width, t, db);
+        } else {
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                __syncthreads();
+#pragma unroll
+                for (int u = 0; u < NV; ++u)
+                    *reinterpret_cast<f4*>(columns + threadIdx.x / G * kMost + 4 * t + 4 * G * u) = which ? db[u] : dw[u];
+                __syncthreads();
+                for (int c = threadIdx.x; c < width; c += Shape<G, NV>::kThreads) {
+                    float total = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) total += columns[g * kMost + c];
+                    out[which * width + c] = total;
+                }
+            }
+        }
+    }
+}
+
+// ---- rows that no workgroup holds: read once for each sum ------------------------------
+
+constexpr int kWideThreads = 1024;
+
+// Sums of N doubles over the workgroup, on every thread.
+template <int N>
+__device__ inline void workgroup_sum(double (&v)[N], double (*place)[kWideThreads / 64]) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = red::wave_sum(v[i]);
+        if (threadIdx.x % 64 == 0) place[i][threadIdx.x / 64] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = 0.0;
+        for (int w = 0; w < kWideThreads / 64; ++w) v[i] += place[i][w];
+    }
+}
+
+__global__ __launch_bounds__(kWideThreads) void wide_forward_kernel(const float* __restrict__ x, const float* __restrict__ weight,
+                                                                    const float* __restrict__ bias, float* __restrict__ y,
+                                                                    RowStats* __restrict__ stats, int64_t rows, int64_t width,
+                                                                    float eps) {
+    __shared__ double place[2][kWideThreads / 64];
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const float* const row = x + r * width;
+        double s[1] = {0.0}, q[1] = {0.0};
+        for (int64_t c = threadIdx.x; c < width; c += kWideThreads) s[0] += double(row[c]);
+        workgroup_sum(s, place);
+        const double mean = s[0] / double(width);
+        for (int64_t c = threadIdx.x; c < width; c += kWideThreads) {
+            const double d = double(row[c]) - mean;
+            q[0] += d * d;
+        }
+        workgroup_sum(q, place);
+        RowStats st;
+        st.mean = float(mean);
+        st.rest = float(mean - double(st.mean));
+        st.scale = float(1.0 / sqrt(q[0] / double(width) + double(eps)));
+        st.unused = 0.0f;
+        for (int64_t c = threadIdx.x; c < width; c += kWideThreads) {
+            float h = (row[c] - st.mean - st.rest) * st.scale;
+            if (weight) h *= weight[c];
+            if (bias) h += bias[c];
+            y[r * width + c] = h;
+        }
+        if (stats && threadIdx.x == 0) stats[r] = st;
+    }
+}
+
+__global__ __launch_bounds__(kWideThreads) void wide_backward_kernel(const float* __restrict__ grad, const float* __restrict__ x,
+                                                                     const float* __restrict__ weight,
+                                                                     const RowStats* __restrict__ stats, float* __restrict__ dx,
+                                                                     int64_t rows, int64_t width) {
+    __shared__ double place[2][kWideThreads / 64];
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const float *const g = grad + r * width, *const row = x + r * width;
+        const RowStats st = stats[r];
+        double s[2] = {0.0, 0.0};
+        for (int64_t c = threadIdx.x; c < width; c += kWideThreads) {
+            const float h = (row[c] - st.mean - st.rest) * st.scale, d = weight ? g[c] * weight[c] : g[c];
+            s[0] += double(d);
+            s[1] += double(d) * double(h);
+        }
+        workgroup_sum(s, place);
+        const float first = float(s[0] / double(width)), second = float(s[1] / double(width));
+        for (int64_t c = threadIdx.x; c < width; c += kWideThreads) {
+            const float h = (row[c] - st.mean - st.rest) * st.scale, d = weight ? g[c] * weight[c] : g[c];
+            dx[r * width + c] = (d - first - h * second) * st.scale;
+        }
+    }
+}
+
+// Workgroup (i, j): columns 256 i .., rows j, j + gridDim.y, ...
+__global__ __launch_bounds__(256) void wide_columns_kernel(const float* __restrict__ grad, const float* __restrict__ x,
+                                                           const RowStats* __restrict__ stats, float* __restrict__ sums,
+                                                           int64_t rows, int64_t width) {
+    const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= width) return;
+    double dw = 0.0, db = 0.0;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        const RowStats st = stats[r];
+        const float g = grad[r * width + c];
+        dw += double(g) * double((x[r * width + c] - st.mean - st.rest) * st.scale);
+        db += double(g);
+    }
+    float* const out = sums + int64_t(blockIdx.y) * 2 * width;
+    out[c] = float(dw);
+    out[width + c] = float(db);
+}
+
+// ---- the partial rows -----------------------------------------------------------------
+
+constexpr int kFinishWaves = 16;
+
+// Column c of 2 width: dw, then db. Wave w adds the parts w, w + 16, ... of 64 columns, then the waves are added in order.
+__global__ __launch_bounds__(64 * kFinishWaves) void finish_kernel(const float* __restrict__ sums, int parts, int64_t width,
+                                                                   float* __restrict__ dw, float* __restrict__ db) {
+    __shared__ double waves[kFinishWaves][64];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int64_t c = int64_t(blockIdx.x) * 64 + lane;
+    double total = 0.0;
+    if (c < 2 * width) {
+        for (int p = wave; p < parts; p += 8 * kFinishWaves) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = p + u * kFinishWaves < parts ? sums[int64_t(p + u * kFinishWaves) * 2 * width + c] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) total += double(v[u]);
+        }
+    }
+    waves[wave][lane] = total;
+    __syncthreads();
+    if (wave != 0 || c >= 2 * width) return;
+    for (int w = 1; w < kFinishWaves; ++w) total += waves[w][lane];
+    float* const out = c < width ? dw : db;
+    if (out) out[c < width ? c : c - width] = float(total);
+}
+
+// f(G, NV) for the least shape that holds a row; false where none does.
+template <class F>
+bool with_shape(size_t width, F&& f) {
+#define VC_SHAPE(G, NV) \
+    if (width <= size_t(Shape<G, NV>::kMost)) return f(std::integral_constant<int, G>{}, std::integral_constant<int, NV>{}), true
+    VC_SHAPE(4, 1);
+    VC_SHAPE(16, 1);
+    VC_SHAPE(32, 1);
+    VC_SHAPE(64, 1);
+    VC_SHAPE(64, 2);
+    VC_SHAPE(64, 3);
+    VC_SHAPE(64, 4);
+    VC_SHAPE(256, 2);
+    VC_SHAPE(256, 3);
+    VC_SHAPE(256, 4);
+    VC_SHAPE(1024, 2);
+    VC_SHAPE(1024, 3);
+    VC_SHAPE(1024, 4);
+#undef VC_SHAPE
+    return false;
+}
+
+void check_sizes(const char* op, size_t rows, size_t width) {
+    if (width == 0) fail(VC_HIP_ERR_INVALID_ARGUMENT, std::string(op) + ": no values in a row");
+    if (rows > (size_t(1) << 40) || width > (size_t(1) << 26) || rows > (size_t(1) << 46) / width)
+        fail(VC_HIP_ERR_OVERFLOW, std::string(op) + ": too many values");
+}
+
+}  // namespace
+}  // namespace vchip
+
+using namespace vchip;
+
+extern "C" {
+
+int vc_hip_layer_norm_forward(const float* x, const float* weight, const float* bias, size_t rows, size_t width, float eps,
+                              float* y, float* stats) {
+    return guard([&] {
+        Device& d = require_device();
+        check_sizes("layer_norm", rows, width);
+        if (!(eps >= 0.0f) || std::isinf(eps)) fail(VC_HIP_ERR_INVALID_ARGUMENT, "layer_norm: eps must be a number from zero up");
+        if (rows == 0) return;
+        if (!x || !y) fail(VC_HIP_ERR_INVALID_ARGUMENT, "layer_norm: null pointer");
+        if (stats && !aligned16(stats)) fail(VC_HIP_ERR_INVALID_ARGUMENT, "layer_norm: stats must lie on a 16-byte boundary");
+        auto* const st = reinterpret_cast<RowStats*>(stats);
+        const double count = double(rows) * double(width);
+        Profiled p("layer_norm", 8.0 * count, 8.0 * count);
+        const bool held = with_shape(width, [&](auto g, auto nv) {
+            using S = Shape<g(), nv()>;
+            const unsigned grid = grid_1d(rows, S::kGroups, 8u * unsigned(d.cu_count));
+            launch(rows_forward_kernel<g(), nv()>, dim3(grid), dim3(S::kThreads), 0, d.stream, x, weight, bias, y, st,
+                   int64_t(rows), int(width), eps);
+        });
+        if (!held)
+            launch(wide_forward_kernel, dim3(grid_1d(rows, 1, 2u * unsigned(d.cu_count))), dim3(kWideThreads), 0, d.stream, x, weight,
+                   bias, y, st, int64_t(rows), int64_t(width), eps);
+        after_launch("layer_norm");
+        p.done();
+    });
+}
+
+int vc_hip_layer_norm_backward(const float* grad, const float* x, const float* weight, const float* stats, size_t rows,
+                               size_t width, float* grad_x, float* grad_weight, float* grad_bias) {
+    return guard([&] {
+        Device& d = require_device();
+        check_sizes("layer_norm_backward", rows, width);
+        const bool columns = grad_weight || grad_bias;
+        if (!grad_x && !columns) return;
+        if (rows == 0) {
+            for (float* out : {grad_weight, grad_bias})
+                if (out && vc_hip_fill(out, width, 0.0f) != VC_HIP_OK) fail(VC_HIP_ERR_RUNTIME, vc_hip_last_error());
+            return;
+        }
+        if (!grad || !x || !stats) fail(VC_HIP_ERR_INVALID_ARGUMENT, "layer_norm_backward: null pointer");
+        if (!aligned16(stats)) fail(VC_HIP_ERR_INVALID_ARGUMENT, "layer_norm_backward: stats must lie on a 16-byte boundary");
+        const auto* const st = reinterpret_cast<const RowStats*>(stats);
+        const double count = double(rows) * double(width);
+        Profiled p("layer_norm_backward", 10.0 * count, 12.0 * count);
+        unsigned parts = 0;
+        std::unique_ptr<Scratch> sums;
+        const auto scratch = [&](unsigned n) {
+            parts = n;
+            if (columns) sums = std::make_unique<Scratch>(size_t(n) * 2 * width * sizeof(float));
+            return sums ? sums->as<float>() : nullptr;
+        };
+        bool collected = !columns;  // are the sums made with dx?
+        const bool held = with_shape(width, [&](auto g, auto nv) {
+            using S = Shape<g(), nv()>;
+            if constexpr (S::kHoldsSums) {
+                if (columns) {
+                    const unsigned grid = grid_1d(rows, S::kGroups, 2u * unsigned(d.cu_count));
+                    launch(rows_backward_kernel<g(), nv(), true>, dim3(grid), dim3(S::kThreads), 0, d.stream, grad, x, weight, st,
+                           grad_x, scratch(grid), int64_t(rows), int(width));
+                    collected = true;
+                    return;
+                }
+            }
+            if (grad_x)
+                launch(rows_backward_kernel<g(), nv(), false>, dim3(grid_1d(rows, S::kGroups, 8u * unsigned(d.cu_count))),
+                       dim3(S::kThreads), 0, d.stream, grad, x, weight, st, grad_x, nullptr, int64_t(rows), int(width));
+        });
+        if (!collected || !held) {
+            if (grad_x && !held)
+                launch(wide_backward_kernel, dim3(grid_1d(rows, 1, 2u * unsigned(d.cu_count))), dim3(kWideThreads), 0, d.stream, grad,
+                       x, weight, st, grad_x, int64_t(rows), int64_t(width));
+            if (columns) {
+                const unsigned across = unsigned((width + 255) / 256);
+                const unsigned down = unsigned(std::min<size_t>(rows, std::max<size_t>(1, 4 * size_t(d.cu_count) / across)));
+                launch(wide_columns_kernel, dim3(across, down), dim3(256), 0, d.stream, grad, x, st, scratch(down), int64_t(rows),
+                       int64_t(width));
+            }
+        }
+        after_launch("layer_norm_backward");
+        if (columns) {
+            launch(finish_kernel, dim3(unsigned((2 * width + 63) / 64)), dim3(64 * kFinishWaves), 0, d.stream, sums->as<float>(),
+                   int(parts), int64_t(width), grad_weight, grad_bias);
+            after_launch("layer_norm_backward columns");
+        }
+        p.done();
+    });
+}
+
+}  // extern "C"
