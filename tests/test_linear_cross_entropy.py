@@ -79,6 +79,9 @@ def run(x, w, t, b, device, reduction="mean", dy=None, host=False):
 
 SIZES = [(1, 1, 1), (1, 1, 2), (3, 5, 2), (1, 64, 10), (7, 64, 10), (64, 16, 256), (65, 33, 129), (33, 130, 257), (130, 96, 1000),
          (257, 128, 2049), (64, 511, 4099), (5, 300, 20001)]
+# Products of 2^28 multiplications and more, on either side of whole tiles and lines.
+LARGE = [(1000, 96, 3001), (129, 515, 5003), (2049, 64, 2500), (40, 700, 12000), (700, 1030, 400), (256, 1024, 1024)]
+SIZES += LARGE
 
 
 @pytest.mark.parametrize("device", DEVICES)

@@ -1,0 +1,240 @@
+// Products C = A B^T of float32 values on the half-precision matrix instructions,
+// for operands that are used whole and once: each is packed into memory first.
+//
+// A value is scaled by a power of two of its row and split, x 2^e = x1 + x2, with
+// half-precision parts. e brings the row's largest magnitude to 2^13 .. 2^14, so a
+// value keeps 22 bits or an error of 2^-39 of the largest, whichever is more. Of
+// the four products of two values' parts x2 y2 (2^-22 of the largest) is left out.
+// Three instructions of 32 cycles take the place of eight of 64 of the float32
+// matrix instruction.
+//
+// 32 neighbouring values of a row are one 128-byte line of eight 16-byte chunks:
+// chunk 2 g + p holds part p of the values 8 g .. 8 g + 7. Rows are padded to 256 and
+// lines to whole ones with zeros, so the loads of a tile need no check and go
+// straight to LDS.
+#pragma once
+
+#include "reduce_common.hpp"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+namespace vchip {
+namespace halves {
+
+constexpr int kThreads = 512, kTile = 256, kSlice = 32, kLineBytes = 128;
+
+typedef _Float16 half;
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// The exponent that brings a largest magnitude, as a float's bits, to 2^13 .. 2^14.
+__device__ inline int exponent_of(uint32_t bits) {
+    return bits == 0 ? 0 : 14 - __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, bits));
+}
+
+// The chunks of eight values along k, scaled by 2^e.
+__device__ inline void split8(const float (&v)[8], int e, h8& first, h8& second) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = __builtin_amdgcn_ldexpf(v[i], e);
+        first[i] = half(x);
+        second[i] = half(x - float(first[i]));
+    }
+}
+
+// s_waitcnt that leaves `loads` vector memory operations in flight.
+template <int Loads>
+__device__ inline void wait_loads() {
+    __builtin_amdgcn_s_waitcnt((Loads & 15) | (Loads >> 4) << 14 | 0x0F70);
+}
+
+// A tile of 256 x 256 by eight waves, wave w rows 128 (w / 4) .. and columns 64 (w % 4) .. in 32 x 32 blocks. Two waves a SIMD
+// and one workgroup a CU: a 16-deep step of a wave reads 12 KiB of LDS for 24 instructions, and a slice of 32 k (64 KiB of
+// loads) takes 3072 cycles, which covers the loads of the next.
+struct Tile {
+    static constexpr int kStage = 2 * kTile * kLineBytes, kLds = 2 * kStage, kValues = 128;
+    f16v acc[4][2];
+
+    __device__ inline void clear() {
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.0f;
+    }
+
+    // One load: 64 chunks of 16 bytes, lane l's to byte 16 l of the wave's part of the stage. Inline assembly, as the compiler
+    // would wait for every load in flight before LDS reads that it cannot tell apart; what a stage's loads have written is
+    // waited for before the barrier that hands it on.
+    template <int At>
+    static __device__ inline void load_one(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t uniform, uint32_t lds) {
+        asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                     :
+                     : "s"(lds), "v"(off), "s"(rs), "s"(uniform), "i"(At)
+                     : "memory", "m0", "scc");
+    }
+    template <int At>
+    static __device__ inline void load_rows(const half* from, uint32_t off, uint32_t step, uint32_t lds) {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<half*>(from), short(0), 0x7FFFFFFE, 0x00020000);
+        load_one<At>(rs, off, 0, lds);
+        load_one<At + 8192>(rs, off, step, lds);
+        load_one<At + 16384>(rs, off, 2 * step, lds);
+        load_one<At + 24576>(rs, off, 3 * step, lds);
+    }
+
+    // acc += the products of lines [begin, end) of 256 rows of each operand; a, b: their first rows; lines: of a row, fewer
+    // than 2^16 (a load's offset has 31 bits). lds: kLds bytes. Row r's chunk c lies in slot c ^ (r / 2 % 8) of its 128 bytes:
+    // the rows of a fragment then meet different banks.
+    __device__ inline void accumulate(const half* a, const half* b, int lines, int begin, int end, char* lds) {
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        const uint32_t row_bytes = uint32_t(lines) * kLineBytes;
+        const uint32_t off = uint32_t(8 * wave + lane / 8) * row_bytes + uint32_t((lane % 8) ^ (4 * (wave % 2) + lane / 16)) * 16u;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((lds_ptr_t)lds)) + 1024u * uint32_t(wave));
+        const auto request = [&](int s, int stage) {
+            const int64_t at = int64_t(s) * (kLineBytes / 2);
+            const uint32_t dst = to + uint32_t(stage) * kStage;
+            load_rows<0>(a + at, off, 64u * row_bytes, dst);
+            load_rows<kTile * kLineBytes>(b + at, off, 64u * row_bytes, dst);
+        };
+        const int row_a = 128 * (wave / 4) + lane % 32, row_b = kTile + 64 * (wave % 4) + lane % 32;
+        const int half_wave = lane / 32, swizzle = lane / 2 % 8;
+        const auto multiply = [&](int stage) {
+            const char* const from = lds + stage * kStage;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                h8 x[4][2], y[2][2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int slot = ((4 * t + 2 * half_wave + q) ^ swizzle) * 16;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i][q] = *reinterpret_cast<const h8*>(from + (row_a + 32 * i) * kLineBytes + slot);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) y[j][q] = *reinterpret_cast<const h8*>(from + (row_b + 32 * j) * kLineBytes + slot);
+                }
+#pragma unroll
+                for (int p = 0; p < 3; ++p)  // the small products first
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i][p == 1], y[j][p == 0], acc[i][j], 0, 0, 0);
+            }
+        };
+        if (end <= begin) return;
+        request(begin, 0);
+        int stage = 0;
+        for (int s = begin; s < end; ++s) {
+            wait_loads<0>();
+            __syncthreads();  // slice s is there, and slice s - 1 has been read
+            request(min(s + 1, end - 1), stage ^ 1);
+            multiply(stage);
+            stage ^= 1;
+        }
+        wait_loads<0>();  // no load may land in LDS that others use by then
+    }
+
+    // f(row, column, v) for the four values of neighbouring rows of a column; f may change them.
+    template <class F>
+    __device__ inline void each4(F&& f) {
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = acc[a][b][4 * g + i];
+                    f(128 * (wave / 4) + 32 * a + 8 * g + 4 * (lane / 32), 64 * (wave % 4) + 32 * b + lane % 32, v);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[a][b][4 * g + i] = v[i];
+                }
+    }
+
+    // One of `parts` workgroups that each hold a part of the tile's sums: false for all but the one that counts in last on
+    // `done` (zero before and after), which adds the parts in their order. partial: of this tile, parts * kValues values of
+    // every thread.
+    __device__ inline bool join(int part, int parts, float* partial, unsigned* done, bool& last) {
+        float* const mine = partial + threadIdx.x;
+        int at = 0;
+        each4([&](int, int, float(&v)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                __hip_atomic_store(&mine[(part * kValues + at++) * kThreads], v[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        });
+        red::wait_stores_visible();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == unsigned(parts);
+            if (last) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last) return false;
+        clear();
+        for (int q = 0; q < parts; ++q) {
+            at = 0;
+            each4([&](int, int, float(&v)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[i] += __hip_atomic_load(&mine[(q * kValues + at++) * kThreads], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            });
+        }
+        return true;
+    }
+};
+
+// The tiles of a product: `whole` workgroups compute one each, the others' sums are split over `parts` each, so that the last
+// round of workgroups fills the CUs.
+struct Tiles {
+    int down, across;  // tiles of A's and of B's rows
+    int lines;
+    int whole, rest, parts;
+    int blocks() const { return whole + rest * parts; }
+};
+inline Tiles tiles_of(int64_t rows_a, int64_t rows_b, int64_t lines, int cu_count) {
+    Tiles t{};
+    t.down = int((rows_a + kTile - 1) / kTile);
+    t.across = int((rows_b + kTile - 1) / kTile);
+    t.lines = int(lines);
+    const int all = t.down * t.across;
+    t.whole = all;
+    const int rest = all % cu_count;
+    if (rest) {
+        const int parts = std::min(cu_count / rest, std::max(1, t.lines / 8));
+        if (parts > 1) {
+            t.whole = all - rest;
+            t.rest = rest;
+            t.parts = parts;
+        }
+    }
+    return t;
+}
+
+// Which tile a workgroup computes. Neighbouring workgroups go to the eight XCDs in turn: each XCD takes a run of the order, in
+// which eight tiles of A's rows by all of B's follow each other, so what its 32 CUs read at a time is shared in its L2.
+struct Place {
+    int m, n, part;
+    bool split;
+};
+__device__ inline Place place_of(const Tiles& t, int block) {
+    int id = block, part = 0;
+    const bool split = block >= t.whole;
+    if (split) {
+        id = t.whole + (block - t.whole) % t.rest;
+        part = (block - t.whole) / t.rest;
+    } else {
+        const int each = t.whole / 8, over = t.whole % 8, xcd = block % 8;
+        id = xcd * each + min(xcd, over) + block / 8;
+    }
+    const int run = 8 * t.across, first = id / run * 8, high = min(8, t.down - first), in = id % run;
+    return Place{first + in % high, in / high, part, split};
+}
+
+}  // namespace halves
+}  // namespace vchip
