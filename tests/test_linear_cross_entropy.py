@@ -231,6 +231,25 @@ def test_upstream_gradients_scale_and_add_up(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_gradients_given_away_may_be_written(device):
+    """What a first pass stores may be written to in place: a later pass through the same graph gives the same again."""
+    x, w, t, b = problem(20, 10, 15)
+    tx, tw = (vc.Tensor(v, requires_grad=True, device=device) for v in (x, w))
+    loss = vc.linear_cross_entropy(tx, tw, t)
+    loss.backward()
+    once = tx.grad.numpy().copy(), tw.grad.numpy().copy()
+    held = tw.grad
+    held.requires_grad = True
+    held.sum().backward()
+    vc.sgd_step([held], 1.0)  # subtracts one everywhere
+    np.testing.assert_array_equal(held.numpy(), once[1] - 1)
+    tx.zero_grad(), tw.zero_grad()
+    loss.backward()
+    np.testing.assert_array_equal(tx.grad.numpy(), once[0])
+    np.testing.assert_array_equal(tw.grad.numpy(), once[1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_gradient_against_differences(device):
     x, w, t, b = problem(4, 6, 9)
     _, dx, dw, db = run(x, w, t, b, device)

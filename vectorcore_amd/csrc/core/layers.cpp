@@ -133,7 +133,19 @@ constexpr const char* kLoss = "linear_cross_entropy";
 
 struct LossGradients {
     std::shared_ptr<Storage> x, weight, bias;
+    bool given = false;
+    // The storages have been given away: a later pass reads their values as they are now, also if they are written to.
+    void keep() {
+        for (auto* s : {&x, &weight, &bias})
+            if (*s) *s = hip().snapshot(*s, 0, (*s)->size());
+        given = true;
+    }
 };
+
+// backward()'s own upstream gradient, known on the host.
+bool is_one(const Tensor& g) {
+    return on_hip(g) && off(g) == 0 && hip_host_scalar(st(g)) == std::optional<float>(1.0F);
+}
 
 // The gradients that are wanted, with shares of their own (null: the mean loss's, which it then leaves in *mean).
 LossGradients loss_gradients(const Tensor& x, const Tensor& weight, const Tensor& targets, const std::optional<Tensor>& bias,
@@ -212,10 +224,15 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
     if (!gradient) return made(loss_of(x, weight, targets, bias, mean), mean ? Shape{} : Shape{rows});
     if (mean) {
         std::shared_ptr<Storage> value;
-        const LossGradients unit = loss_gradients(x, weight, targets, bias, nullptr, nx, nw, nb, &value);
+        const auto unit = std::make_shared<LossGradients>(loss_gradients(x, weight, targets, bias, nullptr, nx, nw, nb, &value));
         Tensor out = made(std::move(value), {});
         detail::attach_grad_fn(out, parents, [=](const Tensor& g) {
-            return listed(unit, [&](const std::shared_ptr<Storage>& s, const Shape& shape) { return made(s, shape) * g; });
+            if (!unit->given && is_one(g)) {
+                const LossGradients whole = *unit;
+                unit->keep();
+                return listed(whole, [](const std::shared_ptr<Storage>& s, const Shape& shape) { return made(s, shape); });
+            }
+            return listed(*unit, [&](const std::shared_ptr<Storage>& s, const Shape& shape) { return made(s, shape) * g; });
         });
         return out;
     }

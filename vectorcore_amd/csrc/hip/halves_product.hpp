@@ -8,17 +8,14 @@
 // Three instructions of 32 cycles take the place of eight of 64 of the float32
 // matrix instruction.
 //
-// 32 neighbouring values of a row are one 128-byte line of eight 16-byte chunks:
-// chunk 2 g + p holds part p of the values 8 g .. 8 g + 7. Rows are padded to 256 and
-// lines to whole ones with zeros, so the loads of a tile need no check and go
-// straight to LDS.
+// 32 neighbouring values of a row are one 128-byte line, their first parts, then
+// their second ones: four threads that hold eight values each then write 64
+// neighbouring bytes at a time. Rows are padded to 256 and lines to whole ones with
+// zeros, so the loads of a tile need no check and go straight to LDS.
 #pragma once
-
-#include "reduce_common.hpp"
 
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
 #include <cstdint>
 
 namespace vchip {
@@ -90,7 +87,9 @@ struct Tile {
     // acc += the products of lines [begin, end) of 256 rows of each operand; a, b: their first rows; lines: of a row, fewer
     // than 2^16 (a load's offset has 31 bits). lds: kLds bytes. Row r's chunk c lies in slot c ^ (r / 2 % 8) of its 128 bytes:
     // the rows of a fragment then meet different banks.
-    __device__ inline void accumulate(const half* a, const half* b, int lines, int begin, int end, char* lds) {
+    // Run lines at a time (0: all), from a multiple of that many, before(s) and after(s) around those from s.
+    template <int Run, class Before, class After>
+    __device__ inline void accumulate(const half* a, const half* b, int lines, int begin, int end, char* lds, Before&& before, After&& after) {
         const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
         const uint32_t row_bytes = uint32_t(lines) * kLineBytes;
         const uint32_t off = uint32_t(8 * wave + lane / 8) * row_bytes + uint32_t((lane % 8) ^ (4 * (wave % 2) + lane / 16)) * 16u;
@@ -110,7 +109,7 @@ struct Tile {
                 h8 x[4][2], y[2][2];
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    const int slot = ((4 * t + 2 * half_wave + q) ^ swizzle) * 16;
+                    const int slot = ((4 * q + 2 * t + half_wave) ^ swizzle) * 16;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i][q] = *reinterpret_cast<const h8*>(from + (row_a + 32 * i) * kLineBytes + slot);
 #pragma unroll
@@ -128,12 +127,22 @@ struct Tile {
         if (end <= begin) return;
         request(begin, 0);
         int stage = 0;
-        for (int s = begin; s < end; ++s) {
+        const auto slice = [&](int s) {
             wait_loads<0>();
             __syncthreads();  // slice s is there, and slice s - 1 has been read
             request(min(s + 1, end - 1), stage ^ 1);
             multiply(stage);
             stage ^= 1;
+        };
+        if constexpr (Run == 0) {
+            for (int s = begin; s < end; ++s) slice(s);
+        } else {
+            for (int first = begin; first < end; first += Run) {
+                const int last = min(end, first + Run);
+                before(first);
+                for (int s = first; s < last; ++s) slice(s);
+                after(first);
+            }
         }
         wait_loads<0>();  // no load may land in LDS that others use by then
     }
@@ -148,6 +157,7 @@ struct Tile {
             for (int g = 0; g < 4; ++g)
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
+                    asm volatile("" ::: "memory");  // addresses and loads of one group at a time: all do not fit the registers
                     float v[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = acc[a][b][4 * g + i];
@@ -157,35 +167,59 @@ struct Tile {
                 }
     }
 
-    // One of `parts` workgroups that each hold a part of the tile's sums: false for all but the one that counts in last on
-    // `done` (zero before and after), which adds the parts in their order. partial: of this tile, parts * kValues values of
-    // every thread.
-    __device__ inline bool join(int part, int parts, float* partial, unsigned* done, bool& last) {
-        float* const mine = partial + threadIdx.x;
-        int at = 0;
-        each4([&](int, int, float(&v)[4]) {
+    // Of a tile whose sums are split: this part's, kValues values of every thread.
+    __device__ inline void store_part(float* partial) const {
+        float* to = partial + threadIdx.x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                __hip_atomic_store(&mine[(part * kValues + at++) * kThreads], v[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        });
-        red::wait_stores_visible();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == unsigned(parts);
-            if (last) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (!last) return false;
-        clear();
-        for (int q = 0; q < parts; ++q) {
-            at = 0;
-            each4([&](int, int, float(&v)[4]) {
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                asm volatile("" : "+v"(to)::"memory");
+#pragma unroll
+                for (int i = 0; i < 16; ++i) to[i * kThreads] = acc[a][b][i];
+                to += 16 * kThreads;
+            }
+    }
+    // The sum of all parts, in their order, of a cleared tile; four parts' loads of 16 values in flight.
+    __device__ inline void load_parts(const float* partial, int parts) {
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float* from = partial + (2 * a + b) * 16 * kThreads + threadIdx.x;
+                for (int p = 0; p < parts; p += 4) {
+                    float v[4][16];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            v[q][i] = p + q < parts ? from[(int64_t(p + q) * kValues + i) * kThreads] : 0.0f;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[a][b][i] += v[q][i];
+                }
+            }
+    }
+    // The same for four values alone: group q of 32 of a thread, f(row, column, v).
+    template <class F>
+    static __device__ inline void each_part(const float* partial, int parts, int q, F&& f) {
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int p = 0; p < parts; p += 4) {
+            float w[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    v[i] += __hip_atomic_load(&mine[(q * kValues + at++) * kThreads], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            });
+                    w[u][i] = p + u < parts ? partial[(int64_t(p + u) * kValues + 4 * q + i) * kThreads + threadIdx.x] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += w[u][i];
         }
-        return true;
+        const int block = q / 4, g = q % 4;
+        f(128 * (wave / 4) + 32 * (block / 2) + 8 * g + 4 * (lane / 32), 64 * (wave % 4) + 32 * (block % 2) + lane % 32, v);
     }
 };
 
@@ -193,47 +227,43 @@ struct Tile {
 // round of workgroups fills the CUs.
 struct Tiles {
     int down, across;  // tiles of A's and of B's rows
-    int lines;
     int whole, rest, parts;
-    int blocks() const { return whole + rest * parts; }
 };
-inline Tiles tiles_of(int64_t rows_a, int64_t rows_b, int64_t lines, int cu_count) {
-    Tiles t{};
-    t.down = int((rows_a + kTile - 1) / kTile);
-    t.across = int((rows_b + kTile - 1) / kTile);
-    t.lines = int(lines);
-    const int all = t.down * t.across;
-    t.whole = all;
-    const int rest = all % cu_count;
-    if (rest) {
-        const int parts = std::min(cu_count / rest, std::max(1, t.lines / 8));
-        if (parts > 1) {
-            t.whole = all - rest;
-            t.rest = rest;
-            t.parts = parts;
-        }
-    }
+__device__ inline Tiles tiles_of(int64_t rows_a, int64_t rows_b, int lines, int places) {
+    Tiles t{int((rows_a + kTile - 1) / kTile), int((rows_b + kTile - 1) / kTile), 0, 0, 1};
+    const int all = t.down * t.across, rest = all % places, parts = rest ? min(places / rest, lines / 8) : 1;
+    t.rest = parts > 1 ? rest : 0;
+    t.parts = parts > 1 ? parts : 1;
+    t.whole = all - t.rest;
     return t;
+}
+// At least as many workgroups as tiles_of asks for, of these rows or fewer.
+inline int64_t most_blocks(int64_t rows_a, int64_t rows_b, int64_t places) {
+    const int64_t all = ((rows_a + kTile - 1) / kTile) * ((rows_b + kTile - 1) / kTile);
+    return (all + places - 1) / places * places;
 }
 
 // Which tile a workgroup computes. Neighbouring workgroups go to the eight XCDs in turn: each XCD takes a run of the order, in
 // which eight tiles of A's rows by all of B's follow each other, so what its 32 CUs read at a time is shared in its L2.
 struct Place {
-    int m, n, part;
-    bool split;
+    int m, n;
+    int rest, part;  // of a split tile: which, and which of its parts; else -1
 };
-__device__ inline Place place_of(const Tiles& t, int block) {
-    int id = block, part = 0;
-    const bool split = block >= t.whole;
-    if (split) {
-        id = t.whole + (block - t.whole) % t.rest;
-        part = (block - t.whole) / t.rest;
-    } else {
-        const int each = t.whole / 8, over = t.whole % 8, xcd = block % 8;
-        id = xcd * each + min(xcd, over) + block / 8;
-    }
+__device__ inline Place tile_at(const Tiles& t, int id) {
     const int run = 8 * t.across, first = id / run * 8, high = min(8, t.down - first), in = id % run;
-    return Place{first + in % high, in / high, part, split};
+    return Place{first + in % high, in / high, -1, -1};
+}
+// block < t.whole + t.rest * t.parts
+__device__ inline Place place_of(const Tiles& t, int block) {
+    if (block < t.whole) {
+        const int each = t.whole / 8, over = t.whole % 8, xcd = block % 8;
+        return tile_at(t, xcd * each + min(xcd, over) + block / 8);
+    }
+    const int rest = (block - t.whole) % t.rest;
+    Place p = tile_at(t, t.whole + rest);
+    p.rest = rest;
+    p.part = (block - t.whole) / t.rest;
+    return p;
 }
 
 }  // namespace halves

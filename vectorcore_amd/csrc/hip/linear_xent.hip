@@ -18,6 +18,7 @@
 #include <cmath>
 #include <memory>
 #include <string>
+#include <type_traits>
 
 namespace vchip {
 namespace {
@@ -33,16 +34,75 @@ __device__ inline int64_t class_of(float target, int64_t classes) {
     return float(c) == target ? c : -1;
 }
 
-constexpr int kCountThreads = 1024;
+constexpr int kCountThreads = 1024, kCountRows = 4;  // rows of a thread and turn
 
-// share[0] = one over the number of rows that count, or zero.
-__global__ __launch_bounds__(kCountThreads) void count_kernel(const float* __restrict__ targets, int64_t rows, int64_t classes,
-                                                              float* __restrict__ share) {
-    __shared__ double lds[kCountThreads / 64];
-    double n = 0.0;
-    for (int64_t r = threadIdx.x; r < rows; r += kCountThreads) n += class_of(targets[r], classes) >= 0 ? 1.0 : 0.0;
-    n = red::block_sum(n, lds);
-    if (threadIdx.x == 0) share[0] = n > 0.0 ? float(1.0 / n) : 0.0f;
+// The rows that count: how many (counted), one over it or zero (share), and which, in order (place, or null), for the packed
+// route with the largest finite magnitude of their shares (most, or null). losses: zeros for the others, or null.
+__global__ __launch_bounds__(kCountThreads) void count_kernel(const float* __restrict__ targets, const float* __restrict__ shares,
+                                                              int64_t rows, int64_t classes, int* __restrict__ counted,
+                                                              float* __restrict__ share, int* __restrict__ place,
+                                                              uint32_t* __restrict__ most, float* __restrict__ losses) {
+    __shared__ int of_wave[kCountThreads / 64];
+    __shared__ uint32_t most_of_wave[kCountThreads / 64];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int before = 0;
+    uint32_t high = 0;
+    for (int64_t r0 = 0; r0 < rows; r0 += kCountThreads * kCountRows) {
+        const int64_t first = r0 + int64_t(threadIdx.x) * kCountRows;
+        int flags = 0;
+#pragma unroll
+        for (int i = 0; i < kCountRows; ++i) {
+            const int64_t r = first + i;
+            if (r >= rows) continue;
+            if (class_of(targets[r], classes) >= 0) {
+                flags |= 1 << i;
+                if (most && shares) {
+                    const uint32_t bits = __builtin_bit_cast(uint32_t, shares[r]) & 0x7FFFFFFFu;
+                    high = max(high, bits < 0x7F800000u ? bits : 0u);
+                }
+            } else if (losses) {
+                losses[r] = 0.0f;
+            }
+        }
+        const int own = __popc(flags);
+        int upto = own;  // of this wavefront's lanes up to this one
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int other = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += other;
+        }
+        if (lane == 63) of_wave[wave] = upto;
+        __syncthreads();
+        int all = 0, at = before + upto - own;
+        for (int w = 0; w < kCountThreads / 64; ++w) {
+            if (w < wave) at += of_wave[w];
+            all += of_wave[w];
+        }
+        if (place) {
+#pragma unroll
+            for (int i = 0; i < kCountRows; ++i)
+                if (flags >> i & 1) place[at++] = int(first + i);
+        }
+        before += all;
+        __syncthreads();
+    }
+    if (most) {
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) high = max(high, uint32_t(__shfl_xor(int(high), d, 64)));
+        if (lane == 0) most_of_wave[wave] = high;
+        __syncthreads();
+    }
+    if (threadIdx.x != 0) return;
+    const float one = before > 0 ? float(1.0 / double(before)) : 0.0f;
+    if (counted) counted[0] = before;
+    share[0] = one;
+    if (!most) return;
+    if (!shares) {
+        most[0] = __builtin_bit_cast(uint32_t, one);
+        return;
+    }
+    for (int w = 1; w < kCountThreads / 64; ++w) high = max(high, most_of_wave[w]);
+    most[0] = max(high, most_of_wave[0]);
 }
 
 // mean[0] = share[0] times the sum of the losses.
@@ -130,32 +190,61 @@ __global__ __launch_bounds__(kRowThreads) void logits_kernel(float* __restrict__
 
 // ---- large products: packed halves -----------------------------------------------------
 //
-// The three products of a piece read packed operands (halves_product.hpp), each made once:
+// The rows that count are taken together, so that the others cost nothing. The three products of a piece of them read packed
+// operands (halves_product.hpp), each made once:
 //   z^T = W^T x^T  from the columns of W and the rows of x, along the features,
 //   dx  = dz W^T   from the rows of dz and of W, along the classes,
-//   dW  = x^T dz   from the columns of x and of dz, along the rows of the piece.
+//   dW  = x^T dz   from the columns of x and of dz, along the tokens of the piece.
 // The logits are made transposed: a thread of the product then holds 64 classes of a token, whose maximum and sum need no
-// exchange but one, and the largest gradient of a class is that of a row in memory.
+// exchange but one, and a class's gradients, packed along the tokens, take the place of its logits.
+//
+// A class's gradients may be small at every token (a rare class) and are scaled by a power of two of their own, for each block
+// of 256 tokens that of the largest in it: the product's sums change their unit with the block.
 
 using halves::half;
 using halves::h8;
 
 constexpr int kPackThreads = 256, kPackRows = 32, kPackColumns = 128;
+constexpr int kBlockTokens = 256, kBlockLines = kBlockTokens / halves::kSlice;
 constexpr float kLog2e = 1.44269504f;
 
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// A matrix of floats whose left out rows are zeros.
-struct Plain {
-    const float* values;
-    const float* targets;  // null: every row counts
-    int64_t rows, columns, classes;
-    const uint32_t *row_most, *column_most;  // the largest magnitudes, as bits
-    __device__ inline bool row_counts(int64_t r) const { return r < rows && (!targets || class_of(targets[r], classes) >= 0); }
-    // Eight values of a row from column c, a multiple of eight.
-    __device__ inline void load(int64_t r, bool counts, int64_t c, float (&v)[8]) const {
-        const float* const at = values + r * columns + c;
-        if (counts && c + 8 <= columns) {
+// A piece of the rows that count: rows place[first] .. of the call, as many as there are, at most `most`.
+struct Piece {
+    const int *counted, *place;
+    int64_t first, most;
+    __device__ inline int64_t tokens() const { return max(int64_t(0), min(most, int64_t(counted[0]) - first)); }
+    __device__ inline int64_t row(int64_t t) const { return place[first + t]; }
+};
+
+// Packs a matrix of floats [rows, columns] by its rows (along columns, row_lines a row) and by its columns (along rows,
+// column_lines a column); either may be null. of.place: the matrix's rows are the piece's; else `rows` of them in order. The
+// largest magnitudes are those of the whole matrix's rows and columns. A workgroup takes 32 rows and 128 columns, past the
+// ends zeros.
+__global__ __launch_bounds__(kPackThreads) void pack_kernel(const float* __restrict__ values, Piece of, int64_t rows, int64_t columns,
+                                                            const uint32_t* __restrict__ row_most,
+                                                            const uint32_t* __restrict__ column_most, half* __restrict__ by_row,
+                                                            int row_lines, half* __restrict__ by_column, int column_lines, int down, int across) {
+    __shared__ float tile[kPackRows][kPackColumns + 4];
+    const int64_t block = block_id();
+    const int64_t row0 = block / across * kPackRows, column0 = block % across * kPackColumns;
+    if (block / across >= down) return;
+    if (of.place) {
+        rows = of.tokens();
+        if (row0 >= (rows + halves::kTile - 1) / halves::kTile * halves::kTile) return;
+    }
+    // Sixteen threads read 512 neighbouring bytes of a row.
+    const int c = 8 * (threadIdx.x % 16);
+    const int64_t column = column0 + c;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int r = threadIdx.x / 16 + 16 * j;
+        const bool there = row0 + r < rows;
+        const int64_t row = there && of.place ? of.row(row0 + r) : row0 + r;
+        const float* const at = values + row * columns + column;
+        float v[8];
+        if (there && column + 8 <= columns) {
             const f4u lo = *reinterpret_cast<const f4u*>(at), hi = *reinterpret_cast<const f4u*>(at + 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -164,95 +253,16 @@ struct Plain {
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = counts && c + i < columns ? at[i] : 0.0f;
+            for (int i = 0; i < 8; ++i) v[i] = there && column + i < columns ? at[i] : 0.0f;
         }
-    }
-    struct Columns {
-        __device__ inline float along_row(float v, int) const { return v; }
-    };
-    __device__ inline Columns hold(int64_t) const { return {}; }
-    __device__ inline void load(int64_t r, bool counts, int64_t c, const Columns&, float (&v)[8]) const { load(r, counts, c, v); }
-    __device__ inline uint32_t row_bits(int64_t r) const { return r < rows ? row_most[r] : 0u; }
-    __device__ inline uint32_t column_bits(int64_t c) const { return c < columns ? column_most[c] : 0u; }
-};
-
-// What a token's gradients are made of, from its logits' statistics.
-struct Token {
-    float most, scale;  // exp(z - most) * scale is the share of a class
-    float others;       // the share of all classes but the target's, which is minus the target's gradient
-    int target;         // -1: left out
-};
-
-// dz^T [classes, tokens], for shares of one, of the logits z^T. Along a class (a row) times the tokens' shares.
-struct Gradients {
-    const float* logits;
-    int64_t stride;
-    const Token* tokens;
-    const float* shares;
-    bool one_share;
-    int64_t rows, columns;  // classes, tokens
-    const uint32_t* row_most;
-    __device__ inline bool row_counts(int64_t r) const { return r < rows; }
-    static __device__ inline float of(float z, int64_t r, const Token& t) {
-        if (t.target < 0) return 0.0f;
-        return t.target == int(r) ? -t.others : exp_of(z - t.most) * t.scale;
-    }
-    struct Columns {
-        Token token[8];
-        float share[8];
-        __device__ inline float along_row(float v, int i) const { return v * share[i]; }
-    };
-    __device__ inline Columns hold(int64_t c) const {
-        Columns held;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            held.token[i] = c + i < columns ? tokens[c + i] : Token{0.0f, 0.0f, 0.0f, -1};
-            held.share[i] = held.token[i].target < 0 ? 0.0f : shares[one_share ? 0 : c + i];
-        }
-        return held;
-    }
-    // The stride is a multiple of 256, and whole rows are there to read.
-    __device__ inline void load(int64_t r, bool counts, int64_t c, const Columns& held, float (&v)[8]) const {
-        const float* const at = logits + r * stride + c;
-        const red::f4 none{0.0f, 0.0f, 0.0f, 0.0f}, lo = counts ? red::ld4(at) : none, hi = counts ? red::ld4(at + 4) : none;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = counts ? of(i < 4 ? lo[i % 4] : hi[i % 4], r, held.token[i]) : 0.0f;
-    }
-    __device__ inline uint32_t row_bits(int64_t r) const { return r < rows ? row_most[r] : 0u; }
-    __device__ inline uint32_t column_bits(int64_t c) const {
-        return c < columns ? __builtin_bit_cast(uint32_t, tokens[c].others) : 0u;
-    }
-};
-
-// Packs a matrix by its rows (along columns, row_lines a row) and by its columns (along rows, column_lines a column); either may
-// be null. A workgroup takes 32 rows and 128 columns, past the ends zeros.
-template <class Source>
-__global__ __launch_bounds__(kPackThreads) void pack_kernel(Source from, half* __restrict__ by_row, int row_lines,
-                                                            half* __restrict__ by_column, int column_lines, int across) {
-    __shared__ float tile[kPackRows][kPackColumns + 4];
-    const int64_t block = block_id();
-    const int64_t row0 = block / across * kPackRows, column0 = block % across * kPackColumns;
-    // Sixteen threads read 512 neighbouring bytes of a row.
-    const int c = 8 * (threadIdx.x % 16);
-    const int64_t column = column0 + c;
-    const auto held = from.hold(column);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int r = threadIdx.x / 16 + 16 * j;
-        const int64_t row = row0 + r;
-        float v[8], scaled[8];
-        from.load(row, from.row_counts(row), column, held, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            tile[r][c + i] = v[i];
-            scaled[i] = held.along_row(v[i], i);
-        }
+        for (int i = 0; i < 8; ++i) tile[r][c + i] = v[i];
         if (by_row && column / 32 < row_lines) {
             h8 first, second;
-            halves::split8(scaled, halves::exponent_of(from.row_bits(row)), first, second);
-            half* const to = by_row + (row * row_lines + column / 32) * 64 + column % 32 * 2;
+            halves::split8(v, there ? halves::exponent_of(row_most[row]) : 0, first, second);
+            half* const to = by_row + ((row0 + r) * row_lines + column / 32) * 64 + column % 32;
             *reinterpret_cast<h8*>(to) = first;
-            *reinterpret_cast<h8*>(to + 8) = second;
+            *reinterpret_cast<h8*>(to + 32) = second;
         }
     }
     if (!by_column) return;
@@ -266,41 +276,56 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(Source from, half* _
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = tile[8 * g + i][at];
         h8 first, second;
-        halves::split8(v, halves::exponent_of(from.column_bits(column0 + at)), first, second);
-        half* const to = by_column + ((column0 + at) * column_lines + line) * 64 + 16 * g;
+        halves::split8(v, column0 + at < columns ? halves::exponent_of(column_most[column0 + at]) : 0, first, second);
+        half* const to = by_column + ((column0 + at) * column_lines + line) * 64 + 8 * g;
         *reinterpret_cast<h8*>(to) = first;
-        *reinterpret_cast<h8*>(to + 8) = second;
+        *reinterpret_cast<h8*>(to + 32) = second;
     }
 }
 
 constexpr int kMostRows = 64, kMostColumns = 256;
 
 // The largest finite magnitudes of a matrix's rows and columns, as bits, into arrays of zeros: bits of positive floats are
-// ordered as the floats are, so the order of the atomics does not matter. A workgroup takes 64 rows and 256 columns.
+// ordered as the floats are, so the order of the atomics does not matter. Rows that targets (or null) leave out have no part;
+// cleared (or null) gets zeros for them. A workgroup takes 64 rows and 256 columns.
 __global__ __launch_bounds__(256) void most_kernel(const float* __restrict__ values, const float* __restrict__ targets,
                                                    int64_t rows, int64_t columns, int64_t classes, int across,
-                                                   uint32_t* __restrict__ row_most, uint32_t* __restrict__ column_most) {
+                                                   uint32_t* __restrict__ row_most, uint32_t* __restrict__ column_most,
+                                                   float* __restrict__ cleared) {
     __shared__ uint32_t of_column[4][kMostColumns];
     const int64_t block = block_id();
     const int64_t row0 = block / across * kMostRows, column0 = block % across * kMostColumns;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int64_t c = column0 + 4 * lane;
-    uint32_t most[4] = {0, 0, 0, 0};
-    for (int j = 0; j < kMostRows / 4; ++j) {
-        const int64_t r = row0 + wave + 4 * j;
-        if (r >= rows) break;  // the same in the whole wavefront
-        if (targets && class_of(targets[r], classes) < 0) continue;
-        uint32_t row = 0;
-        f4u v{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kRows = kMostRows / 4;  // of a wavefront
+    f4u v[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+        const int64_t r = row0 + kRows * wave + j;
+        v[j] = f4u{0.0f, 0.0f, 0.0f, 0.0f};
+        if (r >= rows) continue;
+        if (targets && class_of(targets[r], classes) < 0) {
+            if (cleared) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < columns) cleared[r * columns + c + e] = 0.0f;
+            }
+            continue;
+        }
         if (c + 4 <= columns) {
-            v = *reinterpret_cast<const f4u*>(values + r * columns + c);
+            v[j] = *reinterpret_cast<const f4u*>(values + r * columns + c);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = c + e < columns ? values[r * columns + c + e] : 0.0f;
+            for (int e = 0; e < 4; ++e) v[j][e] = c + e < columns ? values[r * columns + c + e] : 0.0f;
         }
+    }
+    uint32_t most[4] = {0, 0, 0, 0}, of_row = 0;  // lane j: of the wavefront's row j
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+        uint32_t row = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            uint32_t bits = __builtin_bit_cast(uint32_t, v[e]) & 0x7FFFFFFFu;
+            uint32_t bits = __builtin_bit_cast(uint32_t, v[j][e]) & 0x7FFFFFFFu;
             bits = bits < 0x7F800000u ? bits : 0u;
             most[e] = max(most[e], bits);
             row = max(row, bits);
@@ -312,9 +337,10 @@ __global__ __launch_bounds__(256) void most_kernel(const float* __restrict__ val
             row = max(row, red::partner<3>(row, lane));
             row = max(row, red::partner<4>(row, lane));
             row = max(row, red::partner<5>(row, lane));
-            if (lane == 0) atomicMax(&row_most[r], row);
+            of_row = lane == j ? row : of_row;
         }
     }
+    if (of_row) atomicMax(&row_most[row0 + kRows * wave + lane], of_row);  // a row past the end has none
     if (!column_most) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) of_column[wave][4 * lane + e] = most[e];
@@ -326,67 +352,148 @@ __global__ __launch_bounds__(256) void most_kernel(const float* __restrict__ val
     if (column < columns && all) atomicMax(&column_most[column], all);
 }
 
-// The largest |dz share| of each class, as bits, into zeros; and, where Sums, of every 512 tokens the class's sum of them, into
-// sums [token groups][classes]. A wavefront holds 512 tokens and takes 16 classes. The largest without its exponential: of
-// the exponents' maximum one is taken at the end.
-constexpr int kGroupTokens = 512, kGroupClasses = 16;
+// What a token's gradients are made of, from its logits' statistics.
+struct Token {
+    float most, scale;  // exp(z - most) * scale is the share of a class
+    float others;       // the share of all classes but the target's, which is minus the target's gradient
+    int target;
+};
+
+// The exponent of a class's gradients in a block of tokens: that of the largest, but no unit is smaller than 2^-82 of the one
+// that the largest of all could have, so that sums of larger units, 2^44 at most, stay finite in it.
+__device__ inline int class_exponent(uint32_t most, uint32_t most_share) {
+    return min(halves::exponent_of(most), halves::exponent_of(most_share) + 82);
+}
+
+constexpr int kGradientStride = kBlockTokens + 2;  // four threads that read eight classes of a token each meet different banks
+
+// The gradients dz^T of a piece from its logits z^T [classes, stride]: times the tokens' shares, packed along the tokens, in
+// their place; and for shares of one packed along the classes (by_token, or null). most [blocks][whole classes]: the largest of
+// each class, as bits. Sums: of each class, into sums [blocks][classes]. A workgroup takes 32 classes and a block of tokens;
+// four lanes of a wavefront read a line of the logits, and then write it.
 template <bool Sums>
-__global__ __launch_bounds__(64) void class_most_kernel(Gradients from, uint32_t* __restrict__ most, double* __restrict__ sums,
-                                                        int groups) {
-    const int lane = threadIdx.x;
-    const int64_t block = block_id(), group = block % groups;
-    const int64_t c0 = group * kGroupTokens + 8 * lane, v0 = block / groups * kGroupClasses;
-    const bool inside = c0 < from.stride;
-    const Gradients::Columns held = from.hold(c0);
-    float offset[8], own[8];
+__global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t stride, Piece piece, const Token* __restrict__ tokens,
+                                                        const float* __restrict__ shares, const uint32_t* __restrict__ most_share,
+                                                        int64_t classes, int64_t whole_classes, uint32_t* __restrict__ most,
+                                                        half* __restrict__ by_token, int lines, double* __restrict__ sums,
+                                                        int blocks) {
+    __shared__ float tile[32][kGradientStride];
+    const int64_t id = block_id(), block = id % blocks, v0 = id / blocks * 32;
+    if (v0 >= classes) return;
+    const int64_t t0 = block * kBlockTokens, n = piece.tokens();
+    if (t0 >= n) {
+        if constexpr (Sums)
+            if (threadIdx.x < 32 && v0 + threadIdx.x < classes) sums[block * classes + v0 + threadIdx.x] = 0.0;
+        return;
+    }
+    const int lane = threadIdx.x % 64, c = 8 * (threadIdx.x % 32);
+    float* const at = logits + (v0 + threadIdx.x / 32) * stride + t0 + c;
+    red::f4 z[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (v0 + threadIdx.x / 32 + 8 * j < classes) {
+            z[j][0] = red::ld4(at + 8 * j * stride);
+            z[j][1] = red::ld4(at + 8 * j * stride + 4);
+        }
+    Token token[8];
+    float share[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float share = __builtin_amdgcn_logf(fabsf(held.share[i]));
-        offset[i] = __builtin_amdgcn_logf(held.token[i].scale) + share;
-        own[i] = __builtin_amdgcn_logf(held.token[i].others) + share;
+        token[i] = t0 + c + i < n ? tokens[t0 + c + i] : Token{0.0f, 0.0f, 0.0f, -1};
+        share[i] = t0 + c + i < n ? shares[t0 + c + i] : 0.0f;
     }
-    for (int k = 0; k < kGroupClasses; ++k) {
-        const int64_t v = v0 + k;
-        if (v >= from.rows) break;
-        const float* const at = from.logits + v * from.stride + c0;
-        const red::f4 none{0.0f, 0.0f, 0.0f, 0.0f}, lo = inside ? red::ld4(at) : none, hi = inside ? red::ld4(at + 4) : none;
-        float top = kLowest;
+    const uint32_t top = most_share[0];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int r = threadIdx.x / 32 + 8 * j;
+        const int v = int(v0) + r;
+        const bool there = v < classes;
+        float d[8];
+        uint32_t high = 0;
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float z = i < 4 ? lo[i % 4] : hi[i % 4];
-            const Token& t = held.token[i];
-            if (t.target >= 0) top = fmaxf(top, t.target == int(v) ? own[i] : __builtin_fmaf(z - t.most, kLog2e, offset[i]));
-            if constexpr (Sums) sum += double(Gradients::of(z, v, t) * held.share[i]);
+            const float e = exp_of(z[j][i / 4][i % 4] - token[i].most) * token[i].scale;
+            const float g = token[i].target == v ? -token[i].others : e;
+            const bool counts = there && token[i].target >= 0;
+            tile[r][c + i] = counts ? g : 0.0f;
+            d[i] = counts ? g * share[i] : 0.0f;
+            const uint32_t bits = __builtin_bit_cast(uint32_t, d[i]) & 0x7FFFFFFFu;
+            high = max(high, bits < 0x7F800000u ? bits : 0u);
+            if constexpr (Sums) sum += double(d[i]);
         }
-        top = fmaxf(top, red::partner<0>(top, lane));
-        top = fmaxf(top, red::partner<1>(top, lane));
-        top = fmaxf(top, red::partner<2>(top, lane));
-        top = fmaxf(top, red::partner<3>(top, lane));
-        top = fmaxf(top, red::partner<4>(top, lane));
-        top = fmaxf(top, red::partner<5>(top, lane));
-        if constexpr (Sums) sum = red::wave_sum(sum);
-        if (lane == 0) {
-            const uint32_t bits = __builtin_bit_cast(uint32_t, __builtin_amdgcn_exp2f(top));
-            if (bits && bits < 0x7F800000u) atomicMax(&most[v], bits);
-            if constexpr (Sums) sums[group * from.rows + v] = sum;
+        high = max(high, red::partner<0>(high, lane));
+        high = max(high, red::partner<1>(high, lane));
+        high = max(high, red::partner<2>(high, lane));
+        high = max(high, red::partner<3>(high, lane));
+        high = max(high, red::partner<4>(high, lane));
+        if constexpr (Sums) {
+            sum += red::partner<0>(sum, lane);
+            sum += red::partner<1>(sum, lane);
+            sum += red::partner<2>(sum, lane);
+            sum += red::partner<3>(sum, lane);
+            sum += red::partner<4>(sum, lane);
         }
+        if (!there) continue;
+        h8 first, second;
+        halves::split8(d, class_exponent(high, top), first, second);
+        half* const to = reinterpret_cast<half*>(at - c % 32 + 8 * j * stride) + c % 32;
+        *reinterpret_cast<h8*>(to) = first;
+        *reinterpret_cast<h8*>(to + 32) = second;
+        if (threadIdx.x % 32 == 0) {
+            most[block * whole_classes + v] = high;
+            if constexpr (Sums) sums[block * classes + v] = sum;
+        }
+    }
+    if (!by_token) return;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int t = threadIdx.x / 4 + 64 * j, g = threadIdx.x % 4;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = tile[8 * g + i][t];
+        const uint32_t others = t0 + t < n ? __builtin_bit_cast(uint32_t, tokens[t0 + t].others) : 0u;
+        h8 first, second;
+        halves::split8(v, halves::exponent_of(others), first, second);
+        half* const to = by_token + ((t0 + t) * lines + v0 / 32) * 64 + 8 * g;
+        *reinterpret_cast<h8*>(to) = first;
+        *reinterpret_cast<h8*>(to + 32) = second;
     }
 }
 
 // ---- the products -----------------------------------------------------------------------
 
-// z^T: scaled back, with the bias, stored if wanted; and of each 128 classes of a token the maximum, the sum of the exponentials
-// over it, and the target's logit.
+// Of each class the exponent of W's column, and the bias or zero, or minus infinity for the classes that fill the last tile.
+__global__ __launch_bounds__(256) void classes_kernel(const float* __restrict__ bias, const uint32_t* __restrict__ most,
+                                                      int* __restrict__ exponents, float* __restrict__ out, int64_t classes,
+                                                      int64_t whole_classes) {
+    const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (v >= whole_classes) return;
+    exponents[v] = v < classes ? halves::exponent_of(most[v]) : 0;
+    out[v] = v >= classes ? kLowest : bias ? bias[v] : 0.0f;
+}
+
+// z^T: scaled back, with the bias, stored for a gradient (Store); and of each 128 classes of a token the maximum, the sum of the
+// exponentials over it but the target's, and the target's logit. exponents, bias and out reach to the end of the last tile.
+template <bool Store>
 struct Logits {
-    const uint32_t *class_most, *token_most;
+    static constexpr bool kElementwise = false, kUnits = false;
+    Piece piece;
+    const int* exponents;
+    const uint32_t* row_most;
     const float *bias, *targets;
     float *out, *most, *sum, *at_target;
-    int64_t classes, tokens, stride;
+    int64_t classes, stride;
+    int lines;
+    __device__ inline int64_t rows_a() const { return classes; }
+    __device__ inline int64_t rows_b() const { return piece.tokens(); }
+    __device__ inline int depth() const { return lines; }
+    __device__ inline bool idle() const { return false; }
     __device__ inline void operator()(halves::Tile& tile, int m, int n) const {
         const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
         const int64_t v0 = int64_t(m) * halves::kTile, t0 = int64_t(n) * halves::kTile + 64 * (wave % 4) + lane % 32;
-        const int left = int(min(classes - v0, int64_t(halves::kTile)));  // classes of this tile
+        const int64_t tokens = piece.tokens();
         const int row0 = 128 * (wave / 4) + 4 * (lane / 32);
         float top[2], others[2];
         int e_token[2], target[2];  // the target's row in this tile
@@ -395,56 +502,59 @@ struct Logits {
             top[b] = kLowest;
             others[b] = 0.0f;
             const int64_t t = t0 + 32 * b;
-            e_token[b] = t < tokens ? halves::exponent_of(token_most[t]) : 0;
-            const int64_t own = t < tokens ? class_of(targets[t], classes) - v0 : -1;
+            const int64_t row = t < tokens ? piece.row(t) : 0;
+            e_token[b] = t < tokens ? halves::exponent_of(row_most[row]) : 0;
+            const int64_t own = t < tokens ? class_of(targets[row], classes) - v0 : -1;
             target[b] = own >= 0 && own < halves::kTile ? int(own) : -1;
         }
-        const uint32_t* bits = class_most + v0 + row0;  // padded to whole tiles
-        const float* of_bias = bias + v0 + row0;
-        float* to = out + (v0 + row0) * stride + t0;
+        const int* const of_class = exponents + v0;
+        const float* const of_bias = bias + v0;
+        // A row of the tile is a scalar offset: 256 rows of at most 2^16 floats stay within a buffer's 31 bits.
+        const __amdgpu_buffer_rsrc_t rows =
+            __builtin_amdgcn_make_buffer_rsrc(out + v0 * stride + int64_t(n) * halves::kTile, short(0), 0x7FFFFFFE, 0x00020000);
+        const uint32_t row_bytes = uint32_t(stride) * 4u, at = uint32_t(row0) * row_bytes + uint32_t(64 * (wave % 4) + lane % 32) * 4u;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
+        for (int a = 0; a < 4; ++a) {       // 32 rows of the tile, 16 of this thread's, at a time:
+            asm volatile("" ::: "memory");  // the exponents of all do not fit the registers
+            const int r0 = 32 * a;
             int e[16];
-            // Of 32 rows at a time: the addresses and exponents of all do not fit the registers.
-            asm volatile("" : "+v"(bits), "+v"(to), "+v"(of_bias));
+            float add[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const uint4 of = *reinterpret_cast<const uint4*>(bits + 8 * g);
-                e[4 * g] = halves::exponent_of(of.x);
-                e[4 * g + 1] = halves::exponent_of(of.y);
-                e[4 * g + 2] = halves::exponent_of(of.z);
-                e[4 * g + 3] = halves::exponent_of(of.w);
+                const int4 of = *reinterpret_cast<const int4*>(of_class + row0 + r0 + 8 * g);
+                const red::f4 more = red::ld4(of_bias + row0 + r0 + 8 * g);
+                e[4 * g] = of.x;
+                e[4 * g + 1] = of.y;
+                e[4 * g + 2] = of.z;
+                e[4 * g + 3] = of.w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) add[4 * g + i] = more[i];
             }
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                float z[16], high = top[b];
+                int own = target[b] - row0 - r0;  // the target's among these rows, if it is
+                float z[16], high = top[b], found = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int r = row0 + 32 * a + 8 * (i / 4) + i % 4;
-                    z[i] = __builtin_amdgcn_ldexpf(tile.acc[a][b][i], -(e[i] + e_token[b]));
-                    if (r < left) {
-                        if (bias) z[i] += of_bias[8 * (i / 4) + i % 4];
-                        if (out) to[(8 * (i / 4) + i % 4) * stride + 32 * b] = z[i];
-                        if (r == target[b]) at_target[t0 + 32 * b] = z[i];
-                    } else {
-                        z[i] = kLowest;
-                    }
+                    const int r = 8 * (i / 4) + i % 4;
+                    z[i] = __builtin_amdgcn_ldexpf(tile.acc[a][b][i], -(e[i] + e_token[b])) + add[i];
+                    if constexpr (Store)
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, z[i]), rows, at + 128u * b,
+                                                              uint32_t(r0 + r) * row_bytes, 0);
+                    found = own == r ? z[i] : found;
                     high = z[i] > high ? z[i] : high;
                 }
+                if (own >= 0 && own < 32 && (own & 4) == 0) at_target[t0 + 32 * b] = found;
+                asm volatile("" : "+v"(own));  // the comparisons are cheaper made twice than kept
                 // Sums without the target's exponential: beside a share near one the others' would lose their bits. The
                 // maximum is no NaN; where all are minus infinity the exponentials over zero are zeros (or NaN).
                 const float over = high == kLowest ? 0.0f : high;
                 others[b] *= top[b] == high ? 1.0f : exp_of(top[b] - high);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = row0 + 32 * a + 8 * (i / 4) + i % 4;
-                    others[b] += r == target[b] ? 0.0f : exp_of(z[i] - over);
-                }
+                for (int i = 0; i < 16; ++i) others[b] += own == 8 * (i / 4) + i % 4 ? 0.0f : exp_of(z[i] - over);
                 top[b] = high;
+                asm volatile("" : "+v"(others[b]));  // here, not behind all the rows, whose logits would have to be kept
             }
-            bits += 32;
-            of_bias += 32;
-            to += 32 * stride;
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -460,113 +570,173 @@ struct Logits {
     }
 };
 
-// The statistics of a piece's tokens from those of every 128 classes, and the losses. A token's parts are shared by four
-// threads, wavefront w taking every fourth.
-__global__ __launch_bounds__(256) void token_kernel(const float* __restrict__ most, const float* __restrict__ sum,
-                                                    const float* __restrict__ at_target, const float* __restrict__ targets,
-                                                    int parts, int64_t stride, int64_t tokens, int64_t classes,
-                                                    Token* __restrict__ out, float* __restrict__ losses) {
-    __shared__ float tops[4][64];
-    __shared__ double totals[4][64];
+// The statistics of a piece's tokens from those of every 128 classes, their shares in a row, and their losses. A workgroup takes
+// 64 tokens, wavefront w every sixteenth part.
+constexpr int kTokenWaves = 16;
+__global__ __launch_bounds__(64 * kTokenWaves) void token_kernel(Piece piece, const float* __restrict__ most,
+                                                                 const float* __restrict__ sum, const float* __restrict__ at_target,
+                                                                 const float* __restrict__ targets, int parts, int64_t stride,
+                                                                 int64_t classes, const float* __restrict__ shares, bool one_share,
+                                                                 Token* __restrict__ out, float* __restrict__ own_shares,
+                                                                 float* __restrict__ losses) {
+    __shared__ float tops[kTokenWaves][64];
+    __shared__ double totals[kTokenWaves][64];
+    const int64_t n = piece.tokens();
+    if (int64_t(blockIdx.x) * 64 >= n) return;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int64_t t = int64_t(blockIdx.x) * 64 + lane;  // below the stride
     float top = kLowest;
-    for (int p = wave; p < parts; p += 4) top = fmaxf(top, most[p * stride + t]);
+#pragma unroll 8
+    for (int p = wave; p < parts; p += kTokenWaves) top = fmaxf(top, most[p * stride + t]);
     tops[wave][lane] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(tops[0][lane], tops[1][lane]), fmaxf(tops[2][lane], tops[3][lane]));
+    for (int w = 0; w < kTokenWaves; ++w) top = fmaxf(top, tops[w][lane]);
     double others = 0.0;
-    for (int p = wave; p < parts; p += 4) {
+#pragma unroll 8
+    for (int p = wave; p < parts; p += kTokenWaves) {
         const float m = most[p * stride + t];
         others += double(sum[p * stride + t]) * (m == top ? 1.0 : double(exp_of(m - top)));
     }
     totals[wave][lane] = others;
     __syncthreads();
-    if (wave != 0 || t >= tokens) return;
-    const int64_t target = class_of(targets[t], classes);
-    if (target < 0) {
-        if (out) out[t] = Token{0.0f, 0.0f, 0.0f, -1};
-        if (losses) losses[t] = 0.0f;
-        return;
-    }
-    others = ((totals[0][lane] + totals[1][lane]) + totals[2][lane]) + totals[3][lane];
+    if (wave != 0 || t >= n) return;
+    for (int w = 1; w < kTokenWaves; ++w) others += totals[w][lane];
+    const int64_t row = piece.row(t);
     const float at = at_target[t] - top;
     const double total = others + double(expf(at));
-    if (losses) losses[t] = float(log(total) - double(at));
-    if (out) out[t] = Token{top, float(1.0 / total), float(others / total), int(target)};
+    if (losses) losses[row] = float(log(total) - double(at));
+    if (!out) return;
+    out[t] = Token{top, float(1.0 / total), float(others / total), int(class_of(targets[row], classes))};
+    own_shares[t] = shares[one_share ? 0 : row];
 }
 
-// dx [tokens, width], times the tokens' shares.
+// dx [rows, width], times the tokens' shares.
 struct InputGradient {
+    static constexpr bool kElementwise = true, kUnits = false;
+    Piece piece;
     const Token* of_token;
     const uint32_t* feature_most;
     const float* shares;
-    bool one_share;
     float* out;
-    int64_t tokens, width;
-    __device__ inline void operator()(halves::Tile& tile, int m, int n) const {
-        tile.each4([&](int r, int c, float(&v)[4]) {
-            const int64_t t = int64_t(m) * halves::kTile + r, d = int64_t(n) * halves::kTile + c;
-            if (d >= width) return;
-            const int e = halves::exponent_of(feature_most[d]);
+    int64_t width;
+    int lines;
+    __device__ inline int64_t rows_a() const { return piece.tokens(); }
+    __device__ inline int64_t rows_b() const { return width; }
+    __device__ inline int depth() const { return lines; }
+    __device__ inline bool idle() const { return false; }
+    __device__ inline void store(int m, int n, int r, int c, const float (&v)[4]) const {
+        const int64_t t = int64_t(m) * halves::kTile + r, d = int64_t(n) * halves::kTile + c, tokens = piece.tokens();
+        if (d >= width) return;
+        const int e = halves::exponent_of(feature_most[d]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (t + i >= tokens) continue;
-                const Token token = of_token[t + i];
-                const float share = token.target < 0 ? 0.0f : shares[one_share ? 0 : t + i];
-                const int others = halves::exponent_of(__builtin_bit_cast(uint32_t, token.others));
-                out[(t + i) * width + d] = token.target < 0 ? 0.0f : __builtin_amdgcn_ldexpf(v[i], -(e + others)) * share;
-            }
-        });
+        for (int i = 0; i < 4; ++i) {
+            if (t + i >= tokens) continue;
+            const int others = halves::exponent_of(__builtin_bit_cast(uint32_t, of_token[t + i].others));
+            out[piece.row(t + i) * width + d] = __builtin_amdgcn_ldexpf(v[i], -(e + others)) * shares[t + i];
+        }
     }
 };
 
 // dW [width, classes], added to what is there for all pieces but the first.
 struct WeightGradient {
-    const uint32_t *feature_most, *class_most;
+    static constexpr bool kElementwise = true, kUnits = true;
+    Piece piece;
+    const uint32_t *feature_most, *class_most, *most_share;
     float* out;
-    int64_t width, classes;
+    int64_t width, classes, whole_classes;
     bool add;
-    __device__ inline void operator()(halves::Tile& tile, int m, int n) const {
-        tile.each4([&](int r, int c, float(&v)[4]) {
-            const int64_t d = int64_t(m) * halves::kTile + r, k = int64_t(n) * halves::kTile + c;
-            if (k >= classes) return;
-            const int e = halves::exponent_of(class_most[k]);
+    __device__ inline int64_t rows_a() const { return width; }
+    __device__ inline int64_t rows_b() const { return classes; }
+    __device__ inline int depth() const { return int((piece.tokens() + halves::kSlice - 1) / halves::kSlice); }
+    __device__ inline bool idle() const { return add && piece.tokens() == 0; }
+    __device__ inline void store(int m, int n, int r, int c, const float (&v)[4]) const {
+        const int64_t d = int64_t(m) * halves::kTile + r, k = int64_t(n) * halves::kTile + c;
+        if (k >= classes) return;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (d + i >= width) continue;
-                float* const to = out + (d + i) * classes + k;
-                const float g = __builtin_amdgcn_ldexpf(v[i], -(e + halves::exponent_of(feature_most[d + i])));
-                *to = add ? *to + g : g;
-            }
-        });
+        for (int i = 0; i < 4; ++i) {
+            if (d + i >= width) continue;
+            float* const to = out + (d + i) * classes + k;
+            const float g = __builtin_amdgcn_ldexpf(v[i], -halves::exponent_of(feature_most[d + i]));
+            *to = add ? *to + g : g;
+        }
     }
 };
 
-// How many of a split tile's parts are there, zero between launches (which follow each other on one stream).
-constexpr int kMostSplit = 1024;
-__device__ unsigned g_parts_done[kMostSplit];
-
-template <class Epilogue>
-__global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* __restrict__ a, const half* __restrict__ b,
-                                                                   halves::Tiles tiles, float* __restrict__ partial,
-                                                                   Epilogue epilogue) {
+// lines: a row's of either operand, of which depth() are multiplied. The parts of split tiles go to partial, for join_kernel.
+template <class Of>
+__global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* __restrict__ a, const half* __restrict__ b, int lines,
+                                                                   int places, float* __restrict__ partial, Of of) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
-    __shared__ bool last;
+    if (of.idle()) return;
+    const int depth = of.depth();
+    const halves::Tiles tiles = halves::tiles_of(of.rows_a(), of.rows_b(), depth, places);
+    if (int(blockIdx.x) >= tiles.whole + tiles.rest * tiles.parts) return;
     const halves::Place at = halves::place_of(tiles, blockIdx.x);
-    const int parts = at.split ? tiles.parts : 1;
-    const int begin = int(int64_t(tiles.lines) * at.part / parts), end = int(int64_t(tiles.lines) * (at.part + 1) / parts);
-    const int64_t of_row = int64_t(tiles.lines) * (halves::kLineBytes / 2);
+    int begin = 0, end = depth;
+    if (at.part >= 0) {  // in whole blocks of tokens, as a class's unit changes with them
+        const int units = (depth + kBlockLines - 1) / kBlockLines;
+        begin = int(int64_t(units) * at.part / tiles.parts) * kBlockLines;
+        end = min(depth, int(int64_t(units) * (at.part + 1) / tiles.parts) * kBlockLines);
+    }
+    const int64_t of_tile = int64_t(lines) * halves::kTile * (halves::kLineBytes / 2);
     halves::Tile tile;
     tile.clear();
-    tile.accumulate(a + at.m * halves::kTile * of_row, b + at.n * halves::kTile * of_row, tiles.lines, begin, end, lds);
-    if (at.split) {
-        const int rest = (int(blockIdx.x) - tiles.whole) % tiles.rest;
-        if (!tile.join(at.part, parts, partial + int64_t(rest) * parts * halves::Tile::kValues * halves::kThreads, &g_parts_done[rest],
-                       last))
-            return;
+    if constexpr (Of::kUnits) {
+        // A thread's two columns of the tile, which are classes, and the exponents of their units.
+        const uint32_t* const most = of.class_most + int64_t(at.n) * halves::kTile + 64 * (threadIdx.x / 64 % 4) + threadIdx.x % 32;
+        const uint32_t top = of.most_share[0];
+        const auto unit = [&](int s, int column) { return class_exponent(most[s / kBlockLines * of.whole_classes + 32 * column], top); };
+        int now[2], next[2];  // the sums end in units of one
+#pragma unroll
+        for (int j = 0; j < 2; ++j) now[j] = begin < end ? unit(begin, j) : 0;
+        tile.accumulate<kBlockLines>(
+            a + at.m * of_tile, b + at.n * of_tile, lines, begin, end, lds,
+            [&](int s) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) next[j] = s + kBlockLines < end ? unit(s + kBlockLines, j) : 0;
+            },
+            [&](int) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int by = next[j] - now[j];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) tile.acc[r][j][i] = __builtin_amdgcn_ldexpf(tile.acc[r][j][i], by);
+                    now[j] = next[j];
+                }
+            });
+    } else {
+        tile.accumulate<0>(a + at.m * of_tile, b + at.n * of_tile, lines, begin, end, lds, [](int) {}, [](int) {});
     }
-    epilogue(tile, at.m, at.n);
+    if (at.part >= 0)
+        tile.store_part(partial + int64_t(at.rest * tiles.parts + at.part) * halves::Tile::kValues * halves::kThreads);
+    else if constexpr (Of::kElementwise)
+        tile.each4([&](int r, int c, float(&v)[4]) { of.store(at.m, at.n, r, c, v); });
+    else
+        of(tile, at.m, at.n);
+}
+
+// The split tiles of a product: a workgroup each, or, of results that are stored value by value, one for four values of every
+// thread.
+template <class Of>
+__global__ __launch_bounds__(halves::kThreads) void join_kernel(int places, const float* __restrict__ partial, Of of) {
+    if (of.idle()) return;
+    const halves::Tiles tiles = halves::tiles_of(of.rows_a(), of.rows_b(), of.depth(), places);
+    constexpr int kShares = Of::kElementwise ? halves::Tile::kValues / 4 : 1;
+    for (int u = blockIdx.x; u < tiles.rest * kShares; u += gridDim.x) {
+        const int rest = u / kShares;
+        const halves::Place at = halves::tile_at(tiles, tiles.whole + rest);
+        const float* const from = partial + int64_t(rest * tiles.parts) * halves::Tile::kValues * halves::kThreads;
+        if constexpr (Of::kElementwise) {
+            halves::Tile::each_part(from, tiles.parts, u % kShares, [&](int r, int c, const float(&v)[4]) { of.store(at.m, at.n, r, c, v); });
+        } else {
+            halves::Tile tile;
+            tile.clear();
+            tile.load_parts(from, tiles.parts);
+            of(tile, at.m, at.n);
+        }
+    }
 }
 
 void run(int status) {
@@ -636,109 +806,122 @@ void gradient(Device& d, const Call& c, const float* shares, bool one_share, flo
     }
 }
 
-template <class Epilogue>
-void packed_product(Device& d, const half* a, const half* b, int64_t rows_a, int64_t rows_b, int64_t lines, const Epilogue& epilogue) {
-    const halves::Tiles tiles = halves::tiles_of(rows_a, rows_b, lines, d.cu_count);
-    if (tiles.rest > kMostSplit) fail(VC_HIP_ERR_RUNTIME, "linear_cross_entropy: more split tiles than counters");
-    Scratch partial(tiles.rest ? size_t(tiles.rest) * tiles.parts * halves::Tile::kValues * halves::kThreads * sizeof(float) : 4);
-    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<Epilogue>),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, halves::Tile::kLds);
-    check_hip(allowed, "hipFuncSetAttribute");
-    launch(product_kernel<Epilogue>, dim3(unsigned(tiles.blocks())), dim3(halves::kThreads), uint32_t(halves::Tile::kLds), d.stream, a, b,
-           tiles, partial.as<float>(), epilogue);
-    after_launch("linear_cross_entropy product");
-}
-
 int64_t whole_tiles(int64_t n) { return (n + halves::kTile - 1) / halves::kTile * halves::kTile; }
 int64_t lines_of(int64_t n) { return (n + halves::kSlice - 1) / halves::kSlice; }
 // A packed matrix of `rows` rows of `depth` values.
 size_t packed_bytes(int64_t rows, int64_t depth) { return size_t(whole_tiles(rows)) * size_t(lines_of(depth)) * halves::kLineBytes; }
 
-template <class Source>
-void pack(Device& d, const Source& from, half* by_row, half* by_column) {
-    const int64_t down = (by_row ? whole_tiles(from.rows) : lines_of(from.rows) * 32) / kPackRows;
-    const int64_t across = whole_tiles(from.columns) / kPackColumns;
-    launch(pack_kernel<Source>, grid_2d(size_t(down * across)), dim3(kPackThreads), 0, d.stream, from, by_row, int(lines_of(from.columns)),
-           by_column, int(lines_of(from.rows)), int(across));
+// A product of at most these rows; partial: room for one split tile a CU.
+template <class Of>
+void product_of(Device& d, const half* a, const half* b, int64_t rows_a, int64_t rows_b, int64_t lines, float* partial, const Of& of) {
+    const int64_t blocks = halves::most_blocks(rows_a, rows_b, d.cu_count);
+    if (blocks > int64_t(1) << 22) fail(VC_HIP_ERR_OVERFLOW, "linear_cross_entropy: too many tiles");
+    static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<Of>),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, halves::Tile::kLds);
+    check_hip(allowed, "hipFuncSetAttribute");
+    launch(product_kernel<Of>, dim3(unsigned(blocks)), dim3(halves::kThreads), uint32_t(halves::Tile::kLds), d.stream, a, b, int(lines),
+           d.cu_count, partial, of);
+    after_launch("linear_cross_entropy product");
+    launch(join_kernel<Of>, dim3(unsigned(d.cu_count) * (Of::kElementwise ? 4u : 1u)), dim3(halves::kThreads), 0, d.stream, d.cu_count,
+           static_cast<const float*>(partial), of);
+    after_launch("linear_cross_entropy join");
+}
+
+void pack(Device& d, const float* values, const Piece& of, int64_t rows, int64_t columns, const uint32_t* row_most,
+          const uint32_t* column_most, half* by_row, half* by_column) {
+    const int64_t down = (by_row ? whole_tiles(rows) : lines_of(rows) * 32) / kPackRows, across = whole_tiles(columns) / kPackColumns;
+    launch(pack_kernel, grid_2d(size_t(down * across)), dim3(kPackThreads), 0, d.stream, values, of, rows, columns, row_most, column_most,
+           by_row, int(lines_of(columns)), by_column, int(lines_of(rows)), int(down), int(across));
     after_launch("linear_cross_entropy pack");
 }
 
 void largest(Device& d, const float* values, const float* targets, size_t rows, size_t columns, size_t classes, uint32_t* row_most,
-             uint32_t* column_most) {
+             uint32_t* column_most, float* cleared) {
     const size_t down = (rows + kMostRows - 1) / kMostRows, across = (columns + kMostColumns - 1) / kMostColumns;
     launch(most_kernel, grid_2d(down * across), dim3(256), 0, d.stream, values, targets, int64_t(rows), int64_t(columns),
-           int64_t(classes), int(across), row_most, column_most);
+           int64_t(classes), int(across), row_most, column_most, cleared);
     after_launch("linear_cross_entropy largest");
 }
 
-// The packed route. losses or, of a gradient, any output may be null; a call without gradients has no shares.
-void packed(Device& d, const Call& c, const float* shares, bool one_share, float* losses, float* grad_x, float* grad_weight,
+void count(Device& d, const Call& c, const float* shares, int* counted, float* share, int* place, uint32_t* most, float* losses) {
+    launch(count_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, c.targets, shares, int64_t(c.rows), int64_t(c.classes), counted, share,
+           place, most, losses);
+    after_launch("linear_cross_entropy count");
+}
+
+// The packed route. shares: of each row, or null for those of the mean, which goes to share[0]. losses and, of a gradient, any
+// output may be null.
+//
+// A piece's logits and their packed gradients take 4 bytes each a value: 2 GiB and 2 GiB at most, of 288.
+void packed(Device& d, const Call& c, const float* shares, float* share, float* losses, float* grad_x, float* grad_weight,
             float* grad_bias) {
     const bool gradient = grad_x || grad_weight || grad_bias;
     const int64_t width = int64_t(c.width), classes = int64_t(c.classes), rows = int64_t(c.rows);
-    const int64_t most_rows = gradient ? std::max<int64_t>(1, (int64_t(1) << 28) / classes / halves::kTile) * halves::kTile : 65536;
-    const int64_t pieces = (rows + most_rows - 1) / most_rows;
-    const int64_t piece = std::min(most_rows, whole_tiles((rows + pieces - 1) / pieces));
-    const int64_t parts = 2 * whole_tiles(classes) / halves::kTile;
-    const int64_t groups = (piece + kGroupTokens - 1) / kGroupTokens;
+    const int64_t fitting = gradient ? std::max<int64_t>(1, (int64_t(1) << 29) / classes / halves::kTile) * halves::kTile : 65536;
+    const int64_t most_rows = std::min<int64_t>(fitting, 65536), pieces = (rows + most_rows - 1) / most_rows;
+    const int64_t piece = whole_tiles((rows + pieces - 1) / pieces);
+    const int64_t whole_classes = whole_tiles(classes), parts = 2 * whole_classes / halves::kTile, blocks = piece / kBlockTokens;
 
-    // The largest magnitudes: of W's rows and columns, of x's rows and columns, of a piece's classes.
-    const int64_t n_width = whole_tiles(width), n_classes = whole_tiles(classes), n_rows = whole_tiles(rows);
-    const int64_t n_most = 2 * n_width + n_classes + n_rows + (gradient ? pieces * n_classes : 0);
-    Scratch most(size_t(n_most) * sizeof(uint32_t));
+    // The largest magnitudes: of W's rows and columns, of x's rows and columns, of the shares.
+    const int64_t n_most = 2 * width + whole_classes + rows + 1;
+    Scratch most(size_t(n_most) * sizeof(uint32_t)), numbers(size_t(rows + 1) * sizeof(int));
     run(vc_hip_fill(most.as<float>(), size_t(n_most), 0.0f));
-    uint32_t *const w_rows = most.as<uint32_t>(), *const x_columns = w_rows + n_width, *const w_columns = x_columns + n_width;
-    uint32_t *const x_rows = w_columns + n_classes, *const z_classes = x_rows + n_rows;
-    largest(d, c.weight, nullptr, c.width, c.classes, c.classes, grad_x ? w_rows : nullptr, w_columns);
-    largest(d, c.x, c.targets, c.rows, c.width, c.classes, x_rows, grad_weight ? x_columns : nullptr);
+    uint32_t *const w_columns = most.as<uint32_t>(), *const w_rows = w_columns + whole_classes, *const x_columns = w_rows + width;
+    uint32_t *const x_rows = x_columns + width, *const most_share = x_rows + rows;
+    int *const counted = numbers.as<int>(), *const place = counted + 1;
+    count(d, c, shares, counted, share, place, gradient ? most_share : nullptr, losses);
+    largest(d, c.weight, nullptr, c.width, c.classes, c.classes, grad_x ? w_rows : nullptr, w_columns, nullptr);
+    largest(d, c.x, c.targets, c.rows, c.width, c.classes, x_rows, grad_weight ? x_columns : nullptr, grad_x);
+
+    Scratch of_class(size_t(2 * whole_classes) * sizeof(float));
+    int* const exponents = of_class.as<int>();
+    float* const bias = of_class.as<float>() + whole_classes;
+    launch(classes_kernel, dim3(unsigned(whole_classes / 256)), dim3(256), 0, d.stream, c.bias, w_columns, exponents, bias, classes,
+           whole_classes);
+    after_launch("linear_cross_entropy classes");
 
     Scratch wt(packed_bytes(classes, width)), w(grad_x ? packed_bytes(width, classes) : 4);
-    pack(d, Plain{c.weight, nullptr, width, classes, classes, w_rows, w_columns}, grad_x ? w.as<half>() : nullptr, wt.as<half>());
+    pack(d, c.weight, Piece{}, width, classes, w_rows, w_columns, grad_x ? w.as<half>() : nullptr, wt.as<half>());
 
     Scratch x(packed_bytes(piece, width)), xt(grad_weight ? packed_bytes(width, piece) : 4);
-    Scratch logits(gradient ? size_t(classes * piece) * sizeof(float) : 4);
-    Scratch zt(grad_weight ? packed_bytes(classes, piece) : 4), z(grad_x ? packed_bytes(piece, classes) : 4);
-    Scratch statistics(size_t(2 * parts + 1) * size_t(piece) * sizeof(float)), tokens(size_t(piece) * sizeof(Token));
-    Scratch sums(grad_bias ? size_t(pieces * groups * classes) * sizeof(double) : 4);
-    float *const part_most = statistics.as<float>(), *const part_sum = part_most + parts * piece, *const at_target = part_sum + parts * piece;
-    int64_t sum_rows = 0;
+    Scratch logits(gradient ? size_t(whole_classes * piece) * sizeof(float) : 4), z(grad_x ? packed_bytes(piece, classes) : 4);
+    Scratch statistics(size_t(2 * parts + 2) * size_t(piece) * sizeof(float)), tokens(size_t(piece) * sizeof(Token));
+    Scratch class_most(gradient ? size_t(blocks * whole_classes) * sizeof(uint32_t) : 4);
+    Scratch sums(grad_bias ? size_t(pieces * blocks * classes) * sizeof(double) : 4);
+    Scratch partial(size_t(d.cu_count) * halves::Tile::kValues * halves::kThreads * sizeof(float));
+    float *const part_most = statistics.as<float>(), *const part_sum = part_most + parts * piece;
+    float *const at_target = part_sum + parts * piece, *const own_shares = at_target + piece;
 
-    for (int64_t p = 0, first = 0; p < pieces && first < rows; ++p, first += piece) {
-        const int64_t n = std::min(piece, rows - first);
-        const float *const targets = c.targets + first, *const own_shares = one_share ? shares : shares + first;
-        uint32_t* const class_most = z_classes + p * n_classes;
-        pack(d, Plain{c.x + first * width, targets, n, width, classes, x_rows + first, x_columns}, x.as<half>(),
-             grad_weight ? xt.as<half>() : nullptr);
-        packed_product(d, wt.as<half>(), x.as<half>(), classes, n, lines_of(width),
-                       Logits{w_columns, x_rows + first, c.bias, targets, gradient ? logits.as<float>() : nullptr, part_most, part_sum,
-                              at_target, classes, n, piece});
-        launch(token_kernel, dim3(unsigned((n + 63) / 64)), dim3(256), 0, d.stream, part_most, part_sum, at_target, targets, int(parts),
-               piece, n, classes, gradient ? tokens.as<Token>() : nullptr, losses ? losses + first : nullptr);
+    for (int64_t p = 0; p < pieces; ++p) {
+        const Piece of{counted, place, p * piece, piece};
+        pack(d, c.x, of, piece, width, x_rows, x_columns, x.as<half>(), grad_weight ? xt.as<half>() : nullptr);
+        const auto z_of = [&](auto store) {
+            product_of(d, wt.as<half>(), x.as<half>(), classes, piece, lines_of(width), partial.as<float>(),
+                       Logits<store()>{of, exponents, x_rows, bias, c.targets, logits.as<float>(), part_most, part_sum, at_target, classes,
+                                       piece, int(lines_of(width))});
+        };
+        gradient ? z_of(std::true_type{}) : z_of(std::false_type{});
+        launch(token_kernel, dim3(unsigned(piece / 64)), dim3(64 * kTokenWaves), 0, d.stream, of, part_most, part_sum, at_target, c.targets,
+               int(parts), piece, classes, shares ? shares : share, !shares, gradient ? tokens.as<Token>() : nullptr, own_shares, losses);
         after_launch("linear_cross_entropy tokens");
         if (!gradient) continue;
-        const Gradients from{logits.as<float>(), piece, tokens.as<Token>(), own_shares, one_share, classes, n, class_most};
-        const int64_t own_groups = (n + kGroupTokens - 1) / kGroupTokens;
-        if (grad_weight || grad_bias) {
-            const dim3 grid = grid_2d(size_t(own_groups * ((classes + kGroupClasses - 1) / kGroupClasses)));
-            if (grad_bias)
-                launch(class_most_kernel<true>, grid, dim3(64), 0, d.stream, from, class_most, sums.as<double>() + sum_rows * classes,
-                       int(own_groups));
-            else
-                launch(class_most_kernel<false>, grid, dim3(64), 0, d.stream, from, class_most, nullptr, int(own_groups));
-            after_launch("linear_cross_entropy classes");
-            sum_rows += own_groups;
-        }
-        if (grad_x || grad_weight) pack(d, from, grad_weight ? zt.as<half>() : nullptr, grad_x ? z.as<half>() : nullptr);
+        const auto gradients = grad_bias ? gradients_kernel<true> : gradients_kernel<false>;
+        launch(gradients, grid_2d(size_t(blocks * lines_of(classes))), dim3(256), 0, d.stream, logits.as<float>(), piece, of,
+               tokens.as<Token>(), own_shares, most_share, classes, whole_classes, class_most.as<uint32_t>(),
+               grad_x ? z.as<half>() : nullptr, int(lines_of(classes)), sums.as<double>() + (grad_bias ? p * blocks * classes : 0),
+               int(blocks));
+        after_launch("linear_cross_entropy gradients");
         if (grad_x)
-            packed_product(d, z.as<half>(), w.as<half>(), n, width, lines_of(classes),
-                           InputGradient{tokens.as<Token>(), w_rows, own_shares, one_share, grad_x + first * width, n, width});
+            product_of(d, z.as<half>(), w.as<half>(), piece, width, lines_of(classes), partial.as<float>(),
+                       InputGradient{of, tokens.as<Token>(), w_rows, own_shares, grad_x, width, int(lines_of(classes))});
         if (grad_weight)
-            packed_product(d, xt.as<half>(), zt.as<half>(), width, classes, lines_of(n),
-                           WeightGradient{x_columns, class_most, grad_weight, width, classes, p > 0});
+            product_of(d, xt.as<half>(), logits.as<half>(), width, classes, piece / halves::kSlice, partial.as<float>(),
+                       WeightGradient{of, x_columns, class_most.as<uint32_t>(), most_share, grad_weight, width, classes, whole_classes,
+                                      p > 0});
     }
     if (grad_bias) {
         launch(red::column_partials_kernel, dim3(unsigned((classes + 63) / 64)), dim3(64 * red::kCombineWaves), 0, d.stream,
-               sums.as<double>(), sum_rows, classes, grad_bias);
+               sums.as<double>(), pieces * blocks, classes, grad_bias);
         after_launch("linear_cross_entropy bias");
     }
 }
@@ -748,10 +931,6 @@ bool takes_packed(const Call& c) {
            c.width < (size_t(1) << 21);
 }
 
-void count(Device& d, const Call& c, float* share) {
-    launch(count_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, c.targets, int64_t(c.rows), int64_t(c.classes), share);
-    after_launch("linear_cross_entropy count");
-}
 void mean_of(Device& d, const Call& c, const float* losses, const float* share, float* mean) {
     launch(mean_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, losses, int64_t(c.rows), share, mean);
     after_launch("linear_cross_entropy mean");
@@ -782,13 +961,14 @@ int vc_hip_linear_xent_forward(const float* x, const float* weight, const float*
             own = std::make_unique<Scratch>(rows * sizeof(float));
             losses = own->as<float>();
         }
-        if (takes_packed(c)) packed(d, c, nullptr, true, losses, nullptr, nullptr, nullptr);
-        else forward(d, c, losses);
-        if (mean) {
-            Scratch share(sizeof(float));
-            count(d, c, share.as<float>());
-            mean_of(d, c, losses, share.as<float>(), mean);
+        Scratch share(sizeof(float));
+        if (takes_packed(c)) {
+            packed(d, c, nullptr, share.as<float>(), losses, nullptr, nullptr, nullptr);
+        } else {
+            forward(d, c, losses);
+            if (mean) count(d, c, nullptr, nullptr, share.as<float>(), nullptr, nullptr, nullptr);
         }
+        if (mean) mean_of(d, c, losses, share.as<float>(), mean);
         p.done();
     });
 }
@@ -811,10 +991,13 @@ int vc_hip_linear_xent_gradient(const float* x, const float* weight, const float
         Profiled p("linear_cross_entropy_gradient", products * (1.0 + (grad_x != nullptr) + (grad_weight != nullptr)),
                    8.0 * double(width) * double(rows + classes));
         Scratch share(sizeof(float)), losses(mean ? rows * sizeof(float) : 4);
-        if (!shares) count(d, c, share.as<float>());
-        const auto route = takes_packed(c) ? packed : gradient;
-        route(d, c, shares ? shares : share.as<float>(), !shares, mean ? losses.as<float>() : nullptr, grad_x, grad_weight,
-              grad_bias);
+        float* const each = mean ? losses.as<float>() : nullptr;
+        if (takes_packed(c)) {
+            packed(d, c, shares, share.as<float>(), each, grad_x, grad_weight, grad_bias);
+        } else {
+            if (!shares) count(d, c, nullptr, nullptr, share.as<float>(), nullptr, nullptr, nullptr);
+            gradient(d, c, shares ? shares : share.as<float>(), !shares, each, grad_x, grad_weight, grad_bias);
+        }
         if (mean) mean_of(d, c, losses.as<float>(), share.as<float>(), mean);
         p.done();
     });
