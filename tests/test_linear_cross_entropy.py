@@ -79,14 +79,15 @@ def run(x, w, t, b, device, reduction="mean", dy=None, host=False):
 
 SIZES = [(1, 1, 1), (1, 1, 2), (3, 5, 2), (1, 64, 10), (7, 64, 10), (64, 16, 256), (65, 33, 129), (33, 130, 257), (130, 96, 1000),
          (257, 128, 2049), (64, 511, 4099), (5, 300, 20001)]
-# Products of 2^28 multiplications and more, on either side of whole tiles and lines.
-LARGE = [(1000, 96, 3001), (129, 515, 5003), (2049, 64, 2500), (40, 700, 12000), (700, 1030, 400), (256, 1024, 1024)]
-SIZES += LARGE
+# Larger ones of either side of whole tiles and lines, products that are packed (a fifth of the rows left out), and rows in more
+# pieces than one of either route.
+LARGE = [(1000, 96, 3001), (40, 700, 12000), (700, 1030, 400), (256, 1024, 1024), (999, 515, 10007), (2049, 1030, 1537),
+         (513, 1030, 6007), (4099, 515, 2051), (257, 2050, 8200), (70000, 64, 515)]
+CASES = [(*s, "cpu") for s in SIZES + LARGE[:3]] + [pytest.param(*s, "hip", marks=pytest.mark.gpu) for s in SIZES + LARGE]
 
 
-@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("bias", [True, False])
-@pytest.mark.parametrize("rows,width,classes", SIZES)
+@pytest.mark.parametrize("rows,width,classes,device", CASES)
 def test_mean(rows, width, classes, bias, device):
     x, w, t, b = problem(rows, width, classes, bias=bias)
     loss, dx, dw, db = run(x, w, t, b, device, host=rows % 2 == 0)
@@ -100,8 +101,7 @@ def test_mean(rows, width, classes, bias, device):
     assert (dx[t < 0] == 0).all()
 
 
-@pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("rows,width,classes", SIZES)
+@pytest.mark.parametrize("rows,width,classes,device", CASES)
 def test_none(rows, width, classes, device):
     x, w, t, b = problem(rows, width, classes, seed=1)
     dy = np.random.default_rng(rows).standard_normal(rows).astype(np.float32)
@@ -114,7 +114,7 @@ def test_none(rows, width, classes, device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("reduction", ["mean", "none"])
-@pytest.mark.parametrize("rows,width,classes", [(9, 20, 30), (300, 64, 3000)])
+@pytest.mark.parametrize("rows,width,classes", [(9, 20, 30), (300, 64, 3000), (900, 516, 10008)])
 def test_left_out_rows_may_hold_anything(rows, width, classes, reduction, device):
     x, w, t, b = problem(rows, width, classes, seed=2, left_out=0.5)
     t[0] = -1
@@ -129,11 +129,59 @@ def test_left_out_rows_may_hold_anything(rows, width, classes, reduction, device
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("rows,width,classes", [(5, 6, 7), (260, 64, 2100)])
+@pytest.mark.parametrize("rows,width,classes", [(5, 6, 7), (260, 64, 2100), (900, 516, 10008)])
 def test_no_row_counts(rows, width, classes, device):
     x, w, t, b = problem(rows, width, classes)
     loss, dx, dw, db = run(x, w, np.full(rows, -1), b, device)
     assert loss == 0 and (dx == 0).all() and (dw == 0).all() and (db == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows,width,classes", [(300, 70, 90), (1100, 300, 9000)])
+def test_the_largest_value_of_a_row_may_be_anywhere(rows, width, classes, device):
+    """Rows of x and columns of the weight whose values are a thousandth of one of them, at every place of a row in turn."""
+    x, w, t, b = problem(rows, width, classes, seed=3)
+    x *= np.float32(1e-3)
+    w *= np.float32(1e-3)
+    x[np.arange(rows), np.arange(rows) % width] = 3.7
+    w[(5 * np.arange(classes) + 3) % width, np.arange(classes)] = -1.9
+    dy = np.random.default_rng(rows).random(rows).astype(np.float32)
+    loss, dx, dw, db = run(x, w, t, b, device, "none", dy)
+    want, off = exact(x, w, t, b, dy.astype(np.float64))
+    for got, name in ((loss, "loss"), (dx, "dx"), (dw, "dw"), (db, "db")):
+        close(got, want[name], off[name])
+
+
+@pytest.mark.parametrize("rows,device", [(3, "cpu"), (9, "cpu"), pytest.param(3, "hip", marks=pytest.mark.gpu),
+                                         pytest.param(33, "hip", marks=pytest.mark.gpu)])
+def test_two_million_classes(rows, device):
+    """More than the packed operands' offsets reach, and more logits than a piece of the other route holds; sums of millions
+    of small products beside a large one."""
+    x, w, t, b = problem(rows, 2, 2 ** 21 + 3, bias=False)
+    loss, dx, dw, _ = run(x, w, t, b, device)
+    number = (t >= 0).sum()
+    want, off = exact(x, w, t, b, 1 / number)
+    close(loss, want["loss"].sum() / number, off["loss"].sum() / number + 4 * UNIT * want["loss"].sum() / number)
+    close(dx, want["dx"], off["dx"])
+    close(dw, want["dw"], off["dw"])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9, 16, 17])
+@pytest.mark.parametrize("width,classes", [(1, 1), (15, 127), (17, 129), (130, 128), (257, 1001)])
+def test_scores_of_a_few_rows(rows, width, classes, device):
+    """Without gradients, and of rows some of which are left out."""
+    x, w, t, b = problem(rows, width, classes)
+    t[0] = classes - 1
+    tensors = [vc.Tensor(v, device=device) for v in (x, w)]
+    bias = vc.Tensor(b, device=device)
+    want, off = exact(x, w, t, b, 1.0)
+    each = vc.linear_cross_entropy(*tensors, t, bias=bias, reduction="none")
+    assert not each.requires_grad
+    close(each.numpy(), want["loss"], off["loss"])
+    number = (t >= 0).sum()
+    mean = vc.linear_cross_entropy(*tensors, t, bias=bias).item()
+    close(mean, want["loss"].sum() / number, off["loss"].sum() / number + 4 * UNIT * want["loss"].sum() / number)
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -146,11 +194,11 @@ def test_numbers_that_are_no_class(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("rows,classes", [(6, 50), (300, 2500)])
-def test_classes_without_a_chance(rows, classes, device):
+@pytest.mark.parametrize("rows,width,classes", [(6, 24, 50), (300, 24, 2500), (1100, 300, 9000)])
+def test_classes_without_a_chance(rows, width, classes, device):
     """A bias of minus infinity, and the type's lowest value, take a class out; a target among them loses everything."""
     for lowest in (-np.inf, np.finfo(np.float32).min):
-        x, w, t, b = problem(rows, 24, classes, left_out=0)
+        x, w, t, b = problem(rows, width, classes, left_out=0)
         out = np.arange(0, classes, 3)
         t = np.where(t % 3 == 0, (t + 1) % classes, t)
         t = np.where(t % 3 == 0, 1, t)
@@ -169,18 +217,18 @@ def test_classes_without_a_chance(rows, classes, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("classes", [40, 3000])
-def test_sure_rows_keep_their_small_gradients(classes, device):
+@pytest.mark.parametrize("rows,width,classes", [(70, 16, 40), (70, 16, 3000), (1100, 300, 9000)])
+def test_sure_rows_keep_their_small_gradients(rows, width, classes, device):
     """A target of probability 1 - 1e-9: one minus a float32 share would leave nothing of the gradient."""
     rng = np.random.default_rng(4)
-    x = rng.standard_normal((70, 16)).astype(np.float32)
-    w = np.zeros((16, classes), np.float32)
-    t = rng.integers(0, classes, 70)
+    x = rng.standard_normal((rows, width)).astype(np.float32)
+    w = np.zeros((width, classes), np.float32)
+    t = rng.integers(0, classes, rows)
     b = np.full(classes, -20.0, np.float32)
     b[5] = 8.0
     t[:] = 5
     loss, dx, dw, db = run(x, w, t, b, device)
-    want, off = exact(x, w, t, b, 1 / 70)
+    want, off = exact(x, w, t, b, 1 / rows)
     assert 0 < -want["db"][5] < 1e-7
     close(dw, want["dw"], off["dw"])
     close(db, want["db"], off["db"])
@@ -188,9 +236,9 @@ def test_sure_rows_keep_their_small_gradients(classes, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("rows,classes", [(4, 30), (260, 2100)])
-def test_a_row_of_nan_gives_nan(rows, classes, device):
-    x, w, t, b = problem(rows, 16, classes, left_out=0)
+@pytest.mark.parametrize("rows,width,classes", [(4, 16, 30), (19, 16, 30), (260, 16, 2100), (1100, 300, 9000)])
+def test_a_row_of_nan_gives_nan(rows, width, classes, device):
+    x, w, t, b = problem(rows, width, classes, left_out=0)
     x[1, 3] = np.nan
     each = vc.linear_cross_entropy(vc.Tensor(x, device=device), vc.Tensor(w, device=device), t, reduction="none").numpy()
     assert np.isnan(each[1]) and np.isfinite(np.delete(each, 1)).all()
@@ -199,9 +247,9 @@ def test_a_row_of_nan_gives_nan(rows, classes, device):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("wanted", ["x", "weight", "bias"])
 @pytest.mark.parametrize("reduction", ["mean", "none"])
-@pytest.mark.parametrize("rows,classes", [(12, 37), (270, 2300)])
-def test_one_gradient_alone(rows, classes, reduction, wanted, device):
-    x, w, t, b = problem(rows, 40, classes)
+@pytest.mark.parametrize("rows,width,classes", [(12, 40, 37), (270, 40, 2300), (1500, 1026, 10010)])
+def test_one_gradient_alone(rows, width, classes, reduction, wanted, device):
+    x, w, t, b = problem(rows, width, classes)
     leaf = lambda v, name: vc.Tensor(v, requires_grad=name == wanted, device=device)
     tensors = {"x": leaf(x, "x"), "weight": leaf(w, "weight"), "bias": leaf(b, "bias")}
     loss = vc.linear_cross_entropy(tensors["x"], tensors["weight"], t, bias=tensors["bias"], reduction=reduction)
@@ -280,7 +328,7 @@ def test_the_same_as_the_logits_loss(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("rows,width,classes", [(40, 50, 60), (300, 200, 2222)])
+@pytest.mark.parametrize("rows,width,classes", [(40, 50, 60), (300, 200, 2222), (900, 516, 10008)])
 def test_repeats_are_equal(rows, width, classes, device):
     x, w, t, b = problem(rows, width, classes)
     runs = [run(x, w, t, b, device) for _ in range(3)]

@@ -139,7 +139,11 @@ float linear_xent_mean(const float* losses, std::size_t rows, float share) {
 void linear_xent(const LinearLoss& call, const float* shares, bool one_share, float* losses, float* grad_x, float* grad_weight,
                  float* grad_bias) {
     const std::size_t width = call.width, classes = call.classes;
-    const std::size_t piece = std::max<std::size_t>(1, std::min(call.rows, (std::size_t{1} << 22) / classes));
+    // Eight rows or more: matmul adds the products of fewer than four one by one, and of millions of classes' in float32 the
+    // small ones are lost.
+    const std::size_t fitting = std::max<std::size_t>(8, (std::size_t{1} << 22) / classes);
+    const std::size_t pieces = std::max<std::size_t>(1, (call.rows + fitting - 1) / fitting);
+    const std::size_t piece = std::max<std::size_t>(1, (call.rows + pieces - 1) / pieces);
     const bool gradient = grad_x || grad_weight || grad_bias;
     std::vector<float> z(piece * classes), counted(grad_weight ? piece * width : 0);
     std::vector<float> part(grad_weight && call.rows > piece ? width * classes : 0);
@@ -172,7 +176,18 @@ void linear_xent(const LinearLoss& call, const float* shares, bool one_share, fl
             }
         });
         if (!gradient) continue;
-        if (grad_x) matmul(z.data(), call.weight, grad_x + first * width, n, classes, width, false, true);
+        if (grad_x && n >= 4) {
+            matmul(z.data(), call.weight, grad_x + first * width, n, classes, width, false, true);
+        } else if (grad_x) {
+            parallel_for(n * width, row_grain(classes), [&](std::size_t begin, std::size_t end) {
+                for (std::size_t i = begin; i < end; ++i) {
+                    const float *row = z.data() + i / width * classes, *weight = call.weight + i % width * classes;
+                    double sum = 0.0;
+                    for (std::size_t c = 0; c < classes; ++c) sum += static_cast<double>(row[c]) * weight[c];
+                    grad_x[first * width + i] = static_cast<float>(sum);
+                }
+            });
+        }
         if (grad_weight) {
             // Left out rows as zeros, whatever x holds there.
             for (std::size_t r = 0; r < n; ++r) {

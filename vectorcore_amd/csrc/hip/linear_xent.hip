@@ -16,7 +16,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <memory>
 #include <string>
 #include <type_traits>
 
@@ -25,7 +24,10 @@ namespace {
 
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr float kLowest = -__builtin_huge_valf();
+constexpr float kLowest = -__builtin_huge_valf(), kLog2e = 1.44269504f;
+
+// Off by roundings of x and one of the result, as the argument itself is.
+__device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // The class a target names, or -1.
 __device__ inline int64_t class_of(float target, int64_t classes) {
@@ -115,78 +117,171 @@ __global__ __launch_bounds__(kCountThreads) void mean_kernel(const float* __rest
     if (threadIdx.x == 0) mean[0] = float(s * double(share[0]));
 }
 
-// A copy of x whose left out rows are zeros: zero times what they hold would not be zero for an infinity or a NaN.
-__global__ __launch_bounds__(256) void counted_rows_kernel(const float* __restrict__ x, const float* __restrict__ targets,
-                                                           float* __restrict__ out, int64_t rows, int64_t width,
-                                                           int64_t classes) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const bool counted = class_of(targets[r], classes) >= 0;
-        for (int64_t c = threadIdx.x; c < width; c += 256) out[r * width + c] = counted ? x[r * width + c] : 0.0f;
-    }
-}
-
-constexpr int kRowThreads = 256;
-
+template <int Threads>
 __device__ inline float workgroup_max(float v, float* lds) {
     const int lane = red::lane_id();
-    const auto larger = [](float a, float b) { return fmaxf(a, b); };
-    v = larger(v, red::partner<0>(v, lane));
-    v = larger(v, red::partner<1>(v, lane));
-    v = larger(v, red::partner<2>(v, lane));
-    v = larger(v, red::partner<3>(v, lane));
-    v = larger(v, red::partner<4>(v, lane));
-    v = larger(v, red::partner<5>(v, lane));
+    v = fmaxf(v, red::partner<0>(v, lane));
+    v = fmaxf(v, red::partner<1>(v, lane));
+    v = fmaxf(v, red::partner<2>(v, lane));
+    v = fmaxf(v, red::partner<3>(v, lane));
+    v = fmaxf(v, red::partner<4>(v, lane));
+    v = fmaxf(v, red::partner<5>(v, lane));
     if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
     __syncthreads();
     float m = lds[0];
-    for (int w = 1; w < kRowThreads / 64; ++w) m = fmaxf(m, lds[w]);
+    for (int w = 1; w < Threads / 64; ++w) m = fmaxf(m, lds[w]);
     return m;
 }
 
-// A workgroup a row: its loss from the logits z (without the bias), and, where Gradient, z becomes dz.
-template <bool Gradient>
-__global__ __launch_bounds__(kRowThreads) void logits_kernel(float* __restrict__ z, const float* __restrict__ bias,
-                                                             const float* __restrict__ targets, const float* __restrict__ shares,
-                                                             bool one_share, int64_t rows, int64_t classes,
-                                                             float* __restrict__ losses) {
-    __shared__ double sums[kRowThreads / 64];
-    __shared__ float most[kRowThreads / 64];
+// What the rows' kernel makes beside dz. losses, x and mean: each may be null.
+struct RowOutputs {
+    float* losses;    // of each row
+    const float* x;   // [rows, width], of which counted_x gets a copy whose left out rows are zeros: zero times what they hold
+    float* counted_x; // would not be zero for an infinity or a NaN
+    int64_t width;
+    float* mean;      // the mean loss of all rows
+    double* partial;  // one of each workgroup
+};
+
+// Rows that each workgroup counts by itself: a launch less, but rows times rows reads. (Train steps of 1024 rows, 256 x 1000: 46 us,
+// 53 with a launch that counts; of 4096, 128 x 128: 51 and 41.)
+constexpr int kCountedHere = 1024;
+
+// A workgroup a row: its loss from the logits z (without the bias), and, where Gradient, z becomes dz. Held: the row, of at most
+// 4 Threads Held values, is read once and stays in registers; 0: read for the maximum, the sum and the gradient.
+// shares: of each row, or of all (one_share), or null: one over the number of rows that count, which each workgroup finds itself.
+template <int Threads, int Held, bool Gradient>
+__global__ __launch_bounds__(Threads) void logits_kernel(float* __restrict__ z, const float* __restrict__ bias,
+                                                         const float* __restrict__ targets, const float* __restrict__ shares,
+                                                         bool one_share, int64_t rows, int64_t classes, RowOutputs out) {
+    __shared__ double sums[Threads / 64];
+    __shared__ float most[Threads / 64];
     __shared__ double total_of_row;
+    float one = 0.0f;
+    if (!shares && (Gradient || out.mean)) {
+        double n = 0.0;
+        for (int64_t r = threadIdx.x; r < rows; r += Threads) n += class_of(targets[r], classes) >= 0 ? 1.0 : 0.0;
+        n = red::block_sum(n, sums);
+        if (threadIdx.x == 0) total_of_row = n;
+        __syncthreads();
+        n = total_of_row;
+        one = n > 0.0 ? float(1.0 / n) : 0.0f;
+    } else if (shares && one_share) {
+        one = shares[0];
+    }
+    double lost = 0.0;  // in thread 0
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         __syncthreads();
         float* const row = z + r * classes;
         const int64_t target = class_of(targets[r], classes);
+        if (Gradient && out.x)
+            for (int64_t c = threadIdx.x; c < out.width; c += Threads)
+                out.counted_x[r * out.width + c] = target >= 0 ? out.x[r * out.width + c] : 0.0f;
         if (target < 0) {
-            if (losses && threadIdx.x == 0) losses[r] = 0.0f;
+            if (out.losses && threadIdx.x == 0) out.losses[r] = 0.0f;
             if constexpr (Gradient)
-                for (int64_t c = threadIdx.x; c < classes; c += kRowThreads) row[c] = 0.0f;
+                for (int64_t c = threadIdx.x; c < classes; c += Threads) row[c] = 0.0f;
             continue;
         }
         const auto value = [&](int64_t c) { return bias ? row[c] + bias[c] : row[c]; };
+        const float at = value(target);
+        // f(class, logit), four logits at a time; what f makes of them is written back if `keep`.
+        const auto each = [&](auto&& f, bool keep = false) {
+            for (int64_t c = 4 * int64_t(threadIdx.x); c < classes; c += 4 * Threads) {
+                if (c + 3 < classes) {
+                    f4u x = *reinterpret_cast<const f4u*>(row + c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float y = bias ? x[e] + bias[c + e] : x[e];
+                        f(c + e, y);
+                        x[e] = y;
+                    }
+                    if (keep) *reinterpret_cast<f4u*>(row + c) = x;
+                } else {
+                    for (int64_t l = c; l < classes; ++l) {
+                        float y = value(l);
+                        f(l, y);
+                        if (keep) row[l] = y;
+                    }
+                }
+            }
+        };
+        f4u v[Held > 0 ? Held : 1];
         float m = kLowest;
-        for (int64_t c = threadIdx.x; c < classes; c += kRowThreads) m = fmaxf(m, value(c));
-        m = workgroup_max(m, most);
+        if constexpr (Held > 0) {
+#pragma unroll
+            for (int u = 0; u < Held; ++u) {
+                const int64_t c = 4 * int64_t(threadIdx.x) + 4 * Threads * u;
+                if (c + 3 < classes) {
+                    v[u] = *reinterpret_cast<const f4u*>(row + c);
+                    if (bias) {
+                        const f4u more = *reinterpret_cast<const f4u*>(bias + c);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[u][e] += more[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[u][e] = c + e < classes ? value(c + e) : kLowest;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < Held; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m = fmaxf(m, v[u][e]);
+        } else {
+            each([&](int64_t, float& x) { m = fmaxf(m, x); });
+        }
+        m = workgroup_max<Threads>(m, most);
         double s = 0.0;
-        for (int64_t c = threadIdx.x; c < classes; c += kRowThreads) s += double(expf(value(c) - m));
+        if constexpr (Held > 0) {
+#pragma unroll
+            for (int u = 0; u < Held; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool there = 4 * int64_t(threadIdx.x) + 4 * Threads * u + e < classes;
+                    v[u][e] = there ? exp_of(v[u][e] - m) : 0.0f;
+                    s += double(v[u][e]);
+                }
+        } else {
+            each([&](int64_t, float& x) { s += double(exp_of(x - m)); });
+        }
         s = red::block_sum(s, sums);
         if (threadIdx.x == 0) total_of_row = s;
-        __syncthreads();
+        __syncthreads();  // and every thread has read the target's logit
         s = total_of_row;
-        const float at = value(target) - m;
-        if (losses && threadIdx.x == 0) losses[r] = float(log(s) - double(at));
+        const double loss = log(s) - double(at - m);
+        if (threadIdx.x == 0) {
+            if (out.losses) out.losses[r] = float(loss);
+            lost += loss;
+        }
         if constexpr (Gradient) {
-            const float share = one_share ? shares[0] : shares[r], scale = float(double(share) / s);
-            const double own = double(expf(at));
-            __syncthreads();  // every thread has read the target's logit
-            for (int64_t c = threadIdx.x; c < classes; c += kRowThreads) {
-                const float e = expf(value(c) - m);
-                // The others' sum in double: one minus a share near one would leave no bits.
-                row[c] = c == target ? float(-double(share) * ((s - own) / s)) : e * scale;
+            const float share = !shares || one_share ? one : shares[r], scale = float(double(share) / s);
+            // The others' sum in double: one minus a share near one would leave no bits.
+            const float own = float(-double(share) * ((s - double(exp_of(at - m))) / s));
+            if constexpr (Held > 0) {
+#pragma unroll
+                for (int u = 0; u < Held; ++u) {
+                    const int64_t c = 4 * int64_t(threadIdx.x) + 4 * Threads * u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[u][e] = c + e == target ? own : v[u][e] * scale;
+                    if (c + 3 < classes) {
+                        *reinterpret_cast<f4u*>(row + c) = v[u];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < classes) row[c + e] = v[u][e];
+                    }
+                }
+            } else {
+                each([&](int64_t c, float& x) { x = c == target ? own : exp_of(x - m) * scale; }, true);
             }
         }
     }
+    if (!out.mean || threadIdx.x >= 64) return;
+    if (!red::count_in(lost, out.partial)) return;
+    const double total = red::finish_partials(out.partial);
+    if (threadIdx.x == 0) out.mean[0] = float(total * double(one));
 }
-
 
 // ---- large products: packed halves -----------------------------------------------------
 //
@@ -206,9 +301,6 @@ using halves::h8;
 
 constexpr int kPackThreads = 256, kPackRows = 32, kPackColumns = 128;
 constexpr int kBlockTokens = 256, kBlockLines = kBlockTokens / halves::kSlice;
-constexpr float kLog2e = 1.44269504f;
-
-__device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // A piece of the rows that count: rows place[first] .. of the call, as many as there are, at most `most`.
 struct Piece {
@@ -325,7 +417,8 @@ __global__ __launch_bounds__(256) void most_kernel(const float* __restrict__ val
         uint32_t row = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            uint32_t bits = __builtin_bit_cast(uint32_t, v[j][e]) & 0x7FFFFFFFu;
+            const float value = v[j][e];  // a bit cast of a vector's element itself takes the first one
+            uint32_t bits = __builtin_bit_cast(uint32_t, value) & 0x7FFFFFFFu;
             bits = bits < 0x7F800000u ? bits : 0u;
             most[e] = max(most[e], bits);
             row = max(row, bits);
@@ -739,6 +832,119 @@ __global__ __launch_bounds__(halves::kThreads) void join_kernel(int places, cons
     }
 }
 
+// ---- a few rows without gradients: the weights are read once -----------------------------
+//
+// Bound by reading W. A workgroup takes 128 classes, its wavefronts 16 features in turn, with their loads of 512 bytes in flight;
+// what its rows' logits come to there is left as in the packed route, and joined by a second launch.
+
+constexpr int kRowThreads = 256, kFewMost = 16, kFewWaves = 8, kFewClasses = 128, kFewLoads = 16;
+
+template <int Rows>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const float* __restrict__ x, const float* __restrict__ weight,
+                                                                  const float* __restrict__ bias, const float* __restrict__ targets,
+                                                                  int rows, int64_t width, int64_t classes, float* __restrict__ most,
+                                                                  float* __restrict__ sum, float* __restrict__ at_target) {
+    __shared__ float part[kFewWaves][Rows][kFewClasses];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t v0 = int64_t(blockIdx.x) * kFewClasses, v = v0 + 2 * lane;
+    // A pair past the end is read from the last two classes (or the only one twice) and never used.
+    const int64_t first = min(v, classes - 1), second = min(v + 1, classes - 1);
+    const bool pair = second == first + 1;
+    float acc[Rows][2] = {};
+    const auto add = [&](int64_t k, float a, float b) {
+#pragma unroll
+        for (int r = 0; r < Rows; ++r) {
+            const float own = x[int64_t(min(r, rows - 1)) * width + k];
+            acc[r][0] = __builtin_fmaf(own, a, acc[r][0]);
+            acc[r][1] = __builtin_fmaf(own, b, acc[r][1]);
+        }
+    };
+    typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
+    for (int64_t k = kFewLoads * wave; k < width; k += kFewLoads * kFewWaves) {
+        if (k + kFewLoads <= width) {
+            f2u w[kFewLoads];
+#pragma unroll
+            for (int u = 0; u < kFewLoads; ++u) {
+                const float* const at = weight + (k + u) * classes;
+                if (pair) w[u] = *reinterpret_cast<const f2u*>(at + first);
+                else w[u] = f2u{at[first], at[second]};
+            }
+#pragma unroll
+            for (int u = 0; u < kFewLoads; ++u) add(k + u, w[u][0], w[u][1]);
+        } else {
+            for (int64_t l = k; l < width; ++l) add(l, weight[l * classes + first], weight[l * classes + second]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        part[wave][r][2 * lane] = acc[r][0];
+        part[wave][r][2 * lane + 1] = acc[r][1];
+    }
+    __syncthreads();
+    for (int r = wave; r < rows; r += kFewWaves) {
+        const int64_t target = class_of(targets[r], classes);
+        float z[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = lane + 64 * i;
+            z[i] = part[0][r][c];
+#pragma unroll
+            for (int w = 1; w < kFewWaves; ++w) z[i] += part[w][r][c];
+            const bool there = v0 + c < classes;
+            if (bias && there) z[i] += bias[v0 + c];
+            if (!there) z[i] = kLowest;
+            if (there && v0 + c == target) at_target[r] = z[i];
+        }
+        float top = z[0] > kLowest ? z[0] : kLowest;
+        top = z[1] > top ? z[1] : top;
+        const auto larger = [](float a, float b) { return b > a ? b : a; };
+        top = larger(top, red::partner<0>(top, lane));
+        top = larger(top, red::partner<1>(top, lane));
+        top = larger(top, red::partner<2>(top, lane));
+        top = larger(top, red::partner<3>(top, lane));
+        top = larger(top, red::partner<4>(top, lane));
+        top = larger(top, red::partner<5>(top, lane));
+        const float over = top == kLowest ? 0.0f : top;
+        float others = v0 + lane == target ? 0.0f : exp_of(z[0] - over);
+        others += v0 + lane + 64 == target ? 0.0f : exp_of(z[1] - over);
+        others += red::partner<0>(others, lane);
+        others += red::partner<1>(others, lane);
+        others += red::partner<2>(others, lane);
+        others += red::partner<3>(others, lane);
+        others += red::partner<4>(others, lane);
+        others += red::partner<5>(others, lane);
+        if (lane == 0) {
+            most[int64_t(r) * gridDim.x + blockIdx.x] = top;
+            sum[int64_t(r) * gridDim.x + blockIdx.x] = others;
+        }
+    }
+}
+
+// A workgroup a row.
+__global__ __launch_bounds__(kRowThreads) void few_join_kernel(const float* __restrict__ most, const float* __restrict__ sum,
+                                                               const float* __restrict__ at_target, const float* __restrict__ targets,
+                                                               int parts, int64_t classes, float* __restrict__ losses) {
+    __shared__ float tops[kRowThreads / 64];
+    __shared__ double sums[kRowThreads / 64];
+    const int64_t r = blockIdx.x;
+    if (class_of(targets[r], classes) < 0) {
+        if (threadIdx.x == 0) losses[r] = 0.0f;
+        return;
+    }
+    float top = kLowest;
+    for (int p = threadIdx.x; p < parts; p += kRowThreads) top = fmaxf(top, most[r * parts + p]);
+    top = workgroup_max<kRowThreads>(top, tops);
+    double others = 0.0;
+    for (int p = threadIdx.x; p < parts; p += kRowThreads) {
+        const float m = most[r * parts + p];
+        others += double(sum[r * parts + p]) * (m == top ? 1.0 : double(exp_of(m - top)));
+    }
+    others = red::block_sum(others, sums);
+    if (threadIdx.x != 0) return;
+    const float at = at_target[r] - top;
+    losses[r] = float(log(others + double(expf(at))) - double(at));
+}
+
 void run(int status) {
     if (status != VC_HIP_OK) fail(status, vc_hip_last_error());
 }
@@ -756,46 +962,69 @@ void check_call(const char* op, const Call& c) {
     if (c.rows && (!c.x || !c.weight || !c.targets)) fail(VC_HIP_ERR_INVALID_ARGUMENT, name + ": null pointer");
 }
 
-// Logits of a piece: 2^28 of them, 1 GiB.
-size_t rows_of_piece(const Call& c) { return std::max<size_t>(1, std::min(c.rows, (size_t(1) << 28) / c.classes)); }
+// Logits of a piece: 2^26 of them, 256 MiB.
+size_t rows_of_piece(const Call& c) { return std::max<size_t>(1, std::min(c.rows, (size_t(1) << 26) / c.classes)); }
 
 void product(const float* a, const float* b, float* c, size_t m, size_t k, size_t n, bool trans_a, bool trans_b) {
     const size_t none = 0;
     run(vc_hip_matmul(a, b, c, m, k, n, &none, &none, 1, trans_a, trans_b));
 }
 
-void forward(Device& d, const Call& c, float* losses) {
-    const size_t piece = rows_of_piece(c);
-    Scratch logits(piece * c.classes * sizeof(float));
-    for (size_t r = 0; r < c.rows; r += piece) {
-        const size_t n = std::min(piece, c.rows - r);
-        product(c.x + r * c.width, c.weight, logits.as<float>(), n, c.width, c.classes, false, false);
-        launch(logits_kernel<false>, dim3(grid_1d(n, 1, 16u * unsigned(d.cu_count))), dim3(kRowThreads), 0, d.stream,
-               logits.as<float>(), c.bias, c.targets + r, nullptr, false, int64_t(n), int64_t(c.classes), losses + r);
-        after_launch("linear_cross_entropy rows");
-    }
+// Rows of a piece in whole. out's pointers are the piece's.
+template <bool Gradient>
+void rows_of(Device& d, float* z, const Call& c, const float* targets, const float* shares, bool one_share, size_t n, const RowOutputs& out) {
+    // One workgroup a row is at most what the finishing count takes.
+    const dim3 grid(unsigned(std::min<size_t>(n, std::min<size_t>(red::kMaxFinishBlocks, 16 * size_t(d.cu_count)))));
+    const auto go = [&](auto kernel, int threads) {
+        launch(kernel, grid, dim3(unsigned(threads)), 0, d.stream, z, c.bias, targets, shares, one_share, int64_t(n), int64_t(c.classes), out);
+    };
+    if (c.classes <= 256) go(logits_kernel<64, 1, Gradient>, 64);
+    else if (c.classes <= 1024) go(logits_kernel<256, 1, Gradient>, 256);
+    else if (c.classes <= 4096) go(logits_kernel<256, 4, Gradient>, 256);
+    else if (c.classes <= 8192) go(logits_kernel<1024, 2, Gradient>, 1024);
+    else go(logits_kernel<1024, 0, Gradient>, 1024);
+    after_launch("linear_cross_entropy rows");
 }
 
-void gradient(Device& d, const Call& c, const float* shares, bool one_share, float* losses, float* grad_x, float* grad_weight,
-              float* grad_bias) {
+void count(Device& d, const Call& c, const float* shares, int* counted, float* share, int* place, uint32_t* most, float* losses) {
+    launch(count_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, c.targets, shares, int64_t(c.rows), int64_t(c.classes), counted, share,
+           place, most, losses);
+    after_launch("linear_cross_entropy count");
+}
+void mean_of(Device& d, const Call& c, const float* losses, const float* share, float* mean) {
+    launch(mean_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, losses, int64_t(c.rows), share, mean);
+    after_launch("linear_cross_entropy mean");
+}
+
+// The route of float32 products: logits, rows, and the gradients' two products. losses or mean, or neither, and any gradient.
+// shares: of each row, or null for those of the mean.
+void direct(Device& d, const Call& c, const float* shares, float* losses, float* mean, float* grad_x, float* grad_weight,
+            float* grad_bias) {
+    const bool gradient = grad_x || grad_weight || grad_bias;
     const size_t piece = rows_of_piece(c), pieces = (c.rows + piece - 1) / piece;
-    Scratch logits(piece * c.classes * sizeof(float));
-    Scratch rows(grad_weight ? piece * c.width * sizeof(float) : 4);
-    Scratch more(pieces > 1 ? std::max(grad_weight ? c.width * c.classes : 0, c.classes) * sizeof(float) : 4);
+    const bool counted_here = pieces == 1 && c.rows <= kCountedHere, added_here = mean && pieces == 1;
+    Scratch share(sizeof(float)), own_losses(mean && !added_here ? c.rows * sizeof(float) : 4);
+    Scratch partial(added_here ? red::kMaxFinishBlocks * sizeof(double) : 4);
+    const bool count_first = !shares && (gradient || mean) && !counted_here;
+    if (count_first) count(d, c, nullptr, nullptr, share.as<float>(), nullptr, nullptr, nullptr);
+    if (mean && !added_here) losses = own_losses.as<float>();
+    Scratch logits(piece * c.classes * sizeof(float)), rows(grad_weight ? piece * c.width * sizeof(float) : 4);
+    Scratch more(pieces > 1 && gradient ? std::max(grad_weight ? c.width * c.classes : 0, c.classes) * sizeof(float) : 4);
     for (size_t r = 0; r < c.rows; r += piece) {
         const size_t n = std::min(piece, c.rows - r);
         const float* const x = c.x + r * c.width;
         float* const z = logits.as<float>();
         product(x, c.weight, z, n, c.width, c.classes, false, false);
-        launch(logits_kernel<true>, dim3(grid_1d(n, 1, 16u * unsigned(d.cu_count))), dim3(kRowThreads), 0, d.stream, z, c.bias,
-               c.targets + r, one_share ? shares : shares + r, one_share, int64_t(n), int64_t(c.classes),
-               losses ? losses + r : nullptr);
-        after_launch("linear_cross_entropy rows");
+        const RowOutputs out{losses ? losses + r : nullptr, grad_weight ? x : nullptr, rows.as<float>(), int64_t(c.width),
+                             added_here ? mean : nullptr, partial.as<double>()};
+        const float* const own = shares ? shares + r : count_first ? share.as<float>() : nullptr;
+        if (!gradient) {
+            rows_of<false>(d, z, c, c.targets + r, own, !shares, n, out);
+            continue;
+        }
+        rows_of<true>(d, z, c, c.targets + r, own, !shares, n, out);
         if (grad_x) product(z, c.weight, grad_x + r * c.width, n, c.classes, c.width, false, true);
         if (grad_weight) {
-            launch(counted_rows_kernel, dim3(grid_1d(n, 1, 16u * unsigned(d.cu_count))), dim3(256), 0, d.stream, x, c.targets + r,
-                   rows.as<float>(), int64_t(n), int64_t(c.width), int64_t(c.classes));
-            after_launch("linear_cross_entropy counted rows");
             product(rows.as<float>(), z, r ? more.as<float>() : grad_weight, c.width, n, c.classes, true, false);
             if (r) run(vc_hip_axpy(grad_weight, more.as<float>(), c.width * c.classes, 1.0f));
         }
@@ -804,6 +1033,7 @@ void gradient(Device& d, const Call& c, const float* shares, bool one_share, flo
             if (r) run(vc_hip_axpy(grad_bias, more.as<float>(), c.classes, 1.0f));
         }
     }
+    if (mean && !added_here) mean_of(d, c, losses, share.as<float>(), mean);
 }
 
 int64_t whole_tiles(int64_t n) { return (n + halves::kTile - 1) / halves::kTile * halves::kTile; }
@@ -841,12 +1071,6 @@ void largest(Device& d, const float* values, const float* targets, size_t rows, 
     launch(most_kernel, grid_2d(down * across), dim3(256), 0, d.stream, values, targets, int64_t(rows), int64_t(columns),
            int64_t(classes), int(across), row_most, column_most, cleared);
     after_launch("linear_cross_entropy largest");
-}
-
-void count(Device& d, const Call& c, const float* shares, int* counted, float* share, int* place, uint32_t* most, float* losses) {
-    launch(count_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, c.targets, shares, int64_t(c.rows), int64_t(c.classes), counted, share,
-           place, most, losses);
-    after_launch("linear_cross_entropy count");
 }
 
 // The packed route. shares: of each row, or null for those of the mean, which goes to share[0]. losses and, of a gradient, any
@@ -926,14 +1150,38 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
     }
 }
 
-bool takes_packed(const Call& c) {
-    return double(c.rows) * double(c.width) * double(c.classes) >= double(1 << 28) && c.classes < (size_t(1) << 21) &&
-           c.width < (size_t(1) << 21);
+void few_rows(Device& d, const Call& c, float* losses) {
+    const size_t parts = (c.classes + kFewClasses - 1) / kFewClasses;
+    Scratch statistics((2 * parts + 1) * c.rows * sizeof(float));
+    float *const most = statistics.as<float>(), *const sum = most + parts * c.rows, *const at_target = sum + parts * c.rows;
+    const auto kernel = c.rows == 1   ? few_rows_kernel<1>
+                        : c.rows == 2 ? few_rows_kernel<2>
+                        : c.rows <= 4 ? few_rows_kernel<4>
+                        : c.rows <= 8 ? few_rows_kernel<8>
+                                      : few_rows_kernel<16>;
+    launch(kernel, dim3(unsigned(parts)), dim3(64 * kFewWaves), 0, d.stream, c.x, c.weight, c.bias, c.targets, int(c.rows),
+           int64_t(c.width), int64_t(c.classes), most, sum, at_target);
+    after_launch("linear_cross_entropy few rows");
+    launch(few_join_kernel, dim3(unsigned(c.rows)), dim3(kRowThreads), 0, d.stream, most, sum, at_target, c.targets, int(parts),
+           int64_t(c.classes), losses);
+    after_launch("linear_cross_entropy few rows");
 }
 
-void mean_of(Device& d, const Call& c, const float* losses, const float* share, float* mean) {
-    launch(mean_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, losses, int64_t(c.rows), share, mean);
-    after_launch("linear_cross_entropy mean");
+bool takes_few(const Call& c) { return c.rows <= kFewMost; }
+
+// Whether packing pays: by estimates of both routes' times in us, for `products` products of the call's sizes (one, or up to three
+// with gradients). Measured (estimated), direct and packed, in us: losses alone of 128 rows, 1024 x 50000: 164 (144), 224 (223);
+// of 256: 265 (279), 226 (223); 999, 515 x 10007: 152 (181), 91 (87); 4096, 256 x 1000: 40 (36), 64 (54). Train steps of 128 rows,
+// 1024 x 50000: 463 (423), 594 (590); of 256: 773 (827), 636 (610); 2048, 1024 x 1024: 154 (152), 173 (186); 16384, 256 x 1000:
+// 285 (333), 243 (271).
+bool takes_packed(const Call& c, int products) {
+    if (c.classes >= (size_t(1) << 21) || c.width >= (size_t(1) << 21)) return false;  // a load's offset has 31 bits
+    const double n = double(c.rows), weights = double(c.width) * double(c.classes), logits = n * double(c.classes);
+    const bool gradient = products > 1, aligned = c.width % 4 == 0 && c.classes % 4 == 0;
+    const double direct = (gradient ? 20.0 : 10.0) + 2e-6 * products * n * weights / (aligned ? 105.0 : 66.0) + 1.5e-6 * products * logits;
+    const double tiles = double(whole_tiles(int64_t(c.rows))) * double(whole_tiles(int64_t(c.classes))) * double(c.width);
+    const double packing = (gradient ? 4.2e-6 : 2.0e-6) * (weights + n * double(c.width));
+    return direct > (gradient ? 130.0 : 45.0) + packing + 2e-6 * products * tiles / 350.0 + (gradient ? 3.0e-6 : 0.0) * logits;
 }
 
 }  // namespace
@@ -956,19 +1204,19 @@ int vc_hip_linear_xent_forward(const float* x, const float* weight, const float*
         if (!losses && !mean) return;
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy", products, 4.0 * double(width) * double(rows + classes));
-        std::unique_ptr<Scratch> own;
-        if (!losses) {
-            own = std::make_unique<Scratch>(rows * sizeof(float));
-            losses = own->as<float>();
-        }
-        Scratch share(sizeof(float));
-        if (takes_packed(c)) {
-            packed(d, c, nullptr, share.as<float>(), losses, nullptr, nullptr, nullptr);
+        if (!takes_few(c) && !takes_packed(c, 1)) {
+            direct(d, c, nullptr, losses, mean, nullptr, nullptr, nullptr);
         } else {
-            forward(d, c, losses);
-            if (mean) count(d, c, nullptr, nullptr, share.as<float>(), nullptr, nullptr, nullptr);
+            Scratch own(losses ? 4 : rows * sizeof(float)), share(sizeof(float));
+            if (!losses) losses = own.as<float>();
+            if (takes_few(c)) {
+                few_rows(d, c, losses);
+                if (mean) count(d, c, nullptr, nullptr, share.as<float>(), nullptr, nullptr, nullptr);
+            } else {
+                packed(d, c, nullptr, share.as<float>(), losses, nullptr, nullptr, nullptr);
+            }
+            if (mean) mean_of(d, c, losses, share.as<float>(), mean);
         }
-        if (mean) mean_of(d, c, losses, share.as<float>(), mean);
         p.done();
     });
 }
@@ -990,15 +1238,13 @@ int vc_hip_linear_xent_gradient(const float* x, const float* weight, const float
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy_gradient", products * (1.0 + (grad_x != nullptr) + (grad_weight != nullptr)),
                    8.0 * double(width) * double(rows + classes));
-        Scratch share(sizeof(float)), losses(mean ? rows * sizeof(float) : 4);
-        float* const each = mean ? losses.as<float>() : nullptr;
-        if (takes_packed(c)) {
-            packed(d, c, shares, share.as<float>(), each, grad_x, grad_weight, grad_bias);
+        if (takes_packed(c, 1 + (grad_x != nullptr) + (grad_weight != nullptr))) {
+            Scratch share(sizeof(float)), losses(mean ? rows * sizeof(float) : 4);
+            packed(d, c, shares, share.as<float>(), mean ? losses.as<float>() : nullptr, grad_x, grad_weight, grad_bias);
+            if (mean) mean_of(d, c, losses.as<float>(), share.as<float>(), mean);
         } else {
-            if (!shares) count(d, c, nullptr, nullptr, share.as<float>(), nullptr, nullptr, nullptr);
-            gradient(d, c, shares ? shares : share.as<float>(), !shares, each, grad_x, grad_weight, grad_bias);
+            direct(d, c, shares, nullptr, mean, grad_x, grad_weight, grad_bias);
         }
-        if (mean) mean_of(d, c, losses.as<float>(), share.as<float>(), mean);
         p.done();
     });
 }
