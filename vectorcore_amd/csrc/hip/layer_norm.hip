@@ -186,14 +186,34 @@ __global__ __launch_bounds__(kThreadsOf<G>) void rows_backward_kernel(
     const float n = float(width);
     f4 w[NV], dw[Columns ? NV : 1] = {}, db[Columns ? NV : 1] = {};
     if (weight) load<G>(weight, width, t, 0.0f, w);
-    for (int64_t first = int64_t(blockIdx.x) * kGroups; first < rows; first += int64_t(gridDim.x) * kGroups) {
+    // The next row is on its way while a row is made, where few workgroups share a CU and there are registers for it.
+    constexpr bool kAhead = Columns && G == 256;
+    const int64_t step = int64_t(gridDim.x) * kGroups;
+    f4 next_x[kAhead ? NV : 1], next_d[kAhead ? NV : 1];
+    RowStats next_stats{};
+    const auto fetch = [&](int64_t first, f4(&xs)[NV], f4(&ds)[NV], RowStats& st) {
+        const int64_t at = min(first + threadIdx.x / G, rows - 1);
+        load<G>(x + at * width, width, t, 0.0f, xs);
+        load<G>(grad + at * width, width, t, 0.0f, ds);
+        st = stats[at];
+    };
+    if constexpr (kAhead) fetch(int64_t(blockIdx.x) * kGroups, next_x, next_d, next_stats);
+    for (int64_t first = int64_t(blockIdx.x) * kGroups; first < rows; first += step) {
         const int64_t r = first + threadIdx.x / G;
         const bool there = r < rows;
-        const int64_t at = there ? r : rows - 1;
         f4 h[NV], d[NV];
-        load<G>(x + at * width, width, t, 0.0f, h);
-        load<G>(grad + at * width, width, t, 0.0f, d);
-        const RowStats st = stats[at];
+        RowStats st;
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
+                h[u] = next_x[u];
+                d[u] = next_d[u];
+            }
+            st = next_stats;
+            fetch(first + step, next_x, next_d, next_stats);
+        } else {
+            fetch(first, h, d, st);
+        }
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int u = 0; u < NV; ++u)
@@ -339,28 +359,32 @@ __global__ __launch_bounds__(256) void wide_columns_kernel(const float* __restri
 
 // ---- the partial rows -----------------------------------------------------------------
 
-constexpr int kFinishWaves = 16;
+constexpr int kFinishThreads = 1024, kFinishColumns = 32, kFinishGroups = kFinishThreads / kFinishColumns, kFinishLoads = 16;
 
-// Column c of 2 width: dw, then db. Wave w adds the parts w, w + 16, ... of 64 columns, then the waves are added in order.
-__global__ __launch_bounds__(64 * kFinishWaves) void finish_kernel(const float* __restrict__ sums, int parts, int64_t width,
-                                                                   float* __restrict__ dw, float* __restrict__ db) {
-    __shared__ double waves[kFinishWaves][64];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t c = int64_t(blockIdx.x) * 64 + lane;
+// Column c of 2 width: dw, then db. Group g of a workgroup adds the parts g, g + 32, ... of its 32 columns, 16 loads in flight,
+// then the groups are added in order.
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(const float* __restrict__ sums, int parts, int64_t width,
+                                                                float* __restrict__ dw, float* __restrict__ db) {
+    __shared__ double groups[kFinishGroups][kFinishColumns];
+    const int lane = threadIdx.x % kFinishColumns, group = threadIdx.x / kFinishColumns;
+    const int64_t c = int64_t(blockIdx.x) * kFinishColumns + lane;
     double total = 0.0;
     if (c < 2 * width) {
-        for (int p = wave; p < parts; p += 8 * kFinishWaves) {
-            float v[8];
+        for (int p = group; p < parts; p += kFinishLoads * kFinishGroups) {
+            float v[kFinishLoads];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = p + u * kFinishWaves < parts ? sums[int64_t(p + u * kFinishWaves) * 2 * width + c] : 0.0f;
+            for (int u = 0; u < kFinishLoads; ++u) {
+                const int at = p + u * kFinishGroups;
+                v[u] = at < parts ? sums[int64_t(at) * 2 * width + c] : 0.0f;
+            }
 #pragma unroll
-            for (int u = 0; u < 8; ++u) total += double(v[u]);
+            for (int u = 0; u < kFinishLoads; ++u) total += double(v[u]);
         }
     }
-    waves[wave][lane] = total;
+    groups[group][lane] = total;
     __syncthreads();
-    if (wave != 0 || c >= 2 * width) return;
-    for (int w = 1; w < kFinishWaves; ++w) total += waves[w][lane];
+    if (group != 0 || c >= 2 * width) return;
+    for (int g = 1; g < kFinishGroups; ++g) total += groups[g][lane];
     float* const out = c < width ? dw : db;
     if (out) out[c < width ? c : c - width] = float(total);
 }
@@ -479,7 +503,7 @@ int vc_hip_layer_norm_backward(const float* grad, const float* x, const float* w
         }
         after_launch("layer_norm_backward");
         if (columns) {
-            launch(finish_kernel, dim3(unsigned((2 * width + 63) / 64)), dim3(64 * kFinishWaves), 0, d.stream, sums->as<float>(),
+            launch(finish_kernel, dim3(unsigned((2 * width + kFinishColumns - 1) / kFinishColumns)), dim3(kFinishThreads), 0, d.stream, sums->as<float>(),
                    int(parts), int64_t(width), grad_weight, grad_bias);
             after_launch("layer_norm_backward columns");
         }

@@ -39,11 +39,15 @@ __device__ inline int64_t class_of(float target, int64_t classes) {
 constexpr int kCountThreads = 1024, kCountRows = 4;  // rows of a thread and turn
 
 // The rows that count: how many (counted), one over it or zero (share), and which, in order (place, or null), for the packed
-// route with the largest finite magnitude of their shares (most, or null). losses: zeros for the others, or null.
+// route with the largest finite magnitude of their shares (most, or null). losses: zeros for the others, or null. cleared: n_cleared
+// words of zeros, or null.
 __global__ __launch_bounds__(kCountThreads) void count_kernel(const float* __restrict__ targets, const float* __restrict__ shares,
                                                               int64_t rows, int64_t classes, int* __restrict__ counted,
                                                               float* __restrict__ share, int* __restrict__ place,
-                                                              uint32_t* __restrict__ most, float* __restrict__ losses) {
+                                                              uint32_t* __restrict__ most, float* __restrict__ losses,
+                                                              uint32_t* __restrict__ cleared, int64_t n_cleared) {
+    if (cleared)
+        for (int64_t i = threadIdx.x; i < n_cleared; i += kCountThreads) cleared[i] = 0u;
     __shared__ int of_wave[kCountThreads / 64];
     __shared__ uint32_t most_of_wave[kCountThreads / 64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
@@ -312,12 +316,15 @@ struct Piece {
 
 // Packs a matrix of floats [rows, columns] by its rows (along columns, row_lines a row) and by its columns (along rows,
 // column_lines a column); either may be null. of.place: the matrix's rows are the piece's; else `rows` of them in order. The
-// largest magnitudes are those of the whole matrix's rows and columns. A workgroup takes 32 rows and 128 columns, past the
-// ends zeros.
+// largest magnitudes are those of the whole matrix's rows and columns. exponents, filled: or null; of each column its exponent,
+// and bias (or zero), minus infinity for the columns that fill the last tile. A workgroup takes 32 rows and 128 columns, past
+// the ends zeros.
 __global__ __launch_bounds__(kPackThreads) void pack_kernel(const float* __restrict__ values, Piece of, int64_t rows, int64_t columns,
                                                             const uint32_t* __restrict__ row_most,
                                                             const uint32_t* __restrict__ column_most, half* __restrict__ by_row,
-                                                            int row_lines, half* __restrict__ by_column, int column_lines, int down, int across) {
+                                                            int row_lines, half* __restrict__ by_column, int column_lines, int down, int across,
+                                                            const float* __restrict__ bias, int* __restrict__ exponents,
+                                                            float* __restrict__ filled) {
     __shared__ float tile[kPackRows][kPackColumns + 4];
     const int64_t block = block_id();
     const int64_t row0 = block / across * kPackRows, column0 = block % across * kPackColumns;
@@ -325,6 +332,11 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(const float* __restr
     if (of.place) {
         rows = of.tokens();
         if (row0 >= (rows + halves::kTile - 1) / halves::kTile * halves::kTile) return;
+    }
+    if (exponents && row0 == 0 && threadIdx.x < kPackColumns) {
+        const int64_t v = column0 + threadIdx.x;
+        exponents[v] = v < columns ? halves::exponent_of(column_most[v]) : 0;
+        filled[v] = v >= columns ? kLowest : bias ? bias[v] : 0.0f;
     }
     // Sixteen threads read 512 neighbouring bytes of a row.
     const int c = 8 * (threadIdx.x % 16);
@@ -556,16 +568,6 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
 }
 
 // ---- the products -----------------------------------------------------------------------
-
-// Of each class the exponent of W's column, and the bias or zero, or minus infinity for the classes that fill the last tile.
-__global__ __launch_bounds__(256) void classes_kernel(const float* __restrict__ bias, const uint32_t* __restrict__ most,
-                                                      int* __restrict__ exponents, float* __restrict__ out, int64_t classes,
-                                                      int64_t whole_classes) {
-    const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (v >= whole_classes) return;
-    exponents[v] = v < classes ? halves::exponent_of(most[v]) : 0;
-    out[v] = v >= classes ? kLowest : bias ? bias[v] : 0.0f;
-}
 
 // z^T: scaled back, with the bias, stored for a gradient (Store); and of each 128 classes of a token the maximum, the sum of the
 // exponentials over it but the target's, and the target's logit. exponents, bias and out reach to the end of the last tile.
@@ -986,9 +988,10 @@ void rows_of(Device& d, float* z, const Call& c, const float* targets, const flo
     after_launch("linear_cross_entropy rows");
 }
 
-void count(Device& d, const Call& c, const float* shares, int* counted, float* share, int* place, uint32_t* most, float* losses) {
+void count(Device& d, const Call& c, const float* shares, int* counted, float* share, int* place, uint32_t* most, float* losses,
+           uint32_t* cleared = nullptr, int64_t n_cleared = 0) {
     launch(count_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, c.targets, shares, int64_t(c.rows), int64_t(c.classes), counted, share,
-           place, most, losses);
+           place, most, losses, cleared, n_cleared);
     after_launch("linear_cross_entropy count");
 }
 void mean_of(Device& d, const Call& c, const float* losses, const float* share, float* mean) {
@@ -1058,10 +1061,11 @@ void product_of(Device& d, const half* a, const half* b, int64_t rows_a, int64_t
 }
 
 void pack(Device& d, const float* values, const Piece& of, int64_t rows, int64_t columns, const uint32_t* row_most,
-          const uint32_t* column_most, half* by_row, half* by_column) {
+          const uint32_t* column_most, half* by_row, half* by_column, const float* bias = nullptr, int* exponents = nullptr,
+          float* filled = nullptr) {
     const int64_t down = (by_row ? whole_tiles(rows) : lines_of(rows) * 32) / kPackRows, across = whole_tiles(columns) / kPackColumns;
     launch(pack_kernel, grid_2d(size_t(down * across)), dim3(kPackThreads), 0, d.stream, values, of, rows, columns, row_most, column_most,
-           by_row, int(lines_of(columns)), by_column, int(lines_of(rows)), int(down), int(across));
+           by_row, int(lines_of(columns)), by_column, int(lines_of(rows)), int(down), int(across), bias, exponents, filled);
     after_launch("linear_cross_entropy pack");
 }
 
@@ -1087,25 +1091,22 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
     const int64_t whole_classes = whole_tiles(classes), parts = 2 * whole_classes / halves::kTile, blocks = piece / kBlockTokens;
 
     // The largest magnitudes: of W's rows and columns, of x's rows and columns, of the shares.
-    const int64_t n_most = 2 * width + whole_classes + rows + 1;
-    Scratch most(size_t(n_most) * sizeof(uint32_t)), numbers(size_t(rows + 1) * sizeof(int));
-    run(vc_hip_fill(most.as<float>(), size_t(n_most), 0.0f));
+    const int64_t n_most = 2 * width + whole_classes + rows;
+    Scratch most(size_t(n_most + 1) * sizeof(uint32_t)), numbers(size_t(rows + 1) * sizeof(int));
     uint32_t *const w_columns = most.as<uint32_t>(), *const w_rows = w_columns + whole_classes, *const x_columns = w_rows + width;
     uint32_t *const x_rows = x_columns + width, *const most_share = x_rows + rows;
     int *const counted = numbers.as<int>(), *const place = counted + 1;
-    count(d, c, shares, counted, share, place, gradient ? most_share : nullptr, losses);
+    count(d, c, shares, counted, share, place, gradient ? most_share : nullptr, losses, most.as<uint32_t>(), n_most);
     largest(d, c.weight, nullptr, c.width, c.classes, c.classes, grad_x ? w_rows : nullptr, w_columns, nullptr);
     largest(d, c.x, c.targets, c.rows, c.width, c.classes, x_rows, grad_weight ? x_columns : nullptr, grad_x);
 
     Scratch of_class(size_t(2 * whole_classes) * sizeof(float));
     int* const exponents = of_class.as<int>();
     float* const bias = of_class.as<float>() + whole_classes;
-    launch(classes_kernel, dim3(unsigned(whole_classes / 256)), dim3(256), 0, d.stream, c.bias, w_columns, exponents, bias, classes,
-           whole_classes);
-    after_launch("linear_cross_entropy classes");
 
     Scratch wt(packed_bytes(classes, width)), w(grad_x ? packed_bytes(width, classes) : 4);
-    pack(d, c.weight, Piece{}, width, classes, w_rows, w_columns, grad_x ? w.as<half>() : nullptr, wt.as<half>());
+    pack(d, c.weight, Piece{}, width, classes, w_rows, w_columns, grad_x ? w.as<half>() : nullptr, wt.as<half>(), c.bias,
+         exponents, bias);
 
     Scratch x(packed_bytes(piece, width)), xt(grad_weight ? packed_bytes(width, piece) : 4);
     Scratch logits(gradient ? size_t(whole_classes * piece) * sizeof(float) : 4), z(grad_x ? packed_bytes(piece, classes) : 4);
