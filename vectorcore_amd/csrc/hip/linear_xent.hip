@@ -402,25 +402,25 @@ __global__ __launch_bounds__(256) void most_kernel(const float* __restrict__ val
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int64_t c = column0 + 4 * lane;
     constexpr int kRows = kMostRows / 4;  // of a wavefront
+    const int64_t first = row0 + kRows * wave, own = first + lane;
+    const bool inside = lane < kRows && own < rows;
+    const uint64_t there = __ballot(inside), counted = __ballot(inside && (!targets || class_of(targets[own], classes) >= 0));
     f4u v[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-        const int64_t r = row0 + kRows * wave + j;
+        const float* const at = values + (first + j) * columns + c;
         v[j] = f4u{0.0f, 0.0f, 0.0f, 0.0f};
-        if (r >= rows) continue;
-        if (targets && class_of(targets[r], classes) < 0) {
-            if (cleared) {
+        if (counted >> j & 1) {
+            if (c + 4 <= columns) {
+                v[j] = *reinterpret_cast<const f4u*>(at);
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c + e < columns) cleared[r * columns + c + e] = 0.0f;
+                for (int e = 0; e < 4; ++e) v[j][e] = c + e < columns ? at[e] : 0.0f;
             }
-            continue;
-        }
-        if (c + 4 <= columns) {
-            v[j] = *reinterpret_cast<const f4u*>(values + r * columns + c);
-        } else {
+        } else if (cleared && (there >> j & 1)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[j][e] = c + e < columns ? values[r * columns + c + e] : 0.0f;
+            for (int e = 0; e < 4; ++e)
+                if (c + e < columns) cleared[(first + j) * columns + c + e] = 0.0f;
         }
     }
     uint32_t most[4] = {0, 0, 0, 0}, of_row = 0;  // lane j: of the wavefront's row j
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(256) void most_kernel(const float* __restrict__ val
             of_row = lane == j ? row : of_row;
         }
     }
-    if (of_row) atomicMax(&row_most[row0 + kRows * wave + lane], of_row);  // a row past the end has none
+    if (of_row) atomicMax(&row_most[own], of_row);  // a row past the end has none
     if (!column_most) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) of_column[wave][4 * lane + e] = most[e];
@@ -465,9 +465,11 @@ struct Token {
 };
 
 // The exponent of a class's gradients in a block of tokens: that of the largest, but no unit is smaller than 2^-82 of the one
-// that the largest of all could have, so that sums of larger units, 2^44 at most, stay finite in it.
+// that the largest of all could have, so that sums of larger units, 2^44 at most, stay finite in it. A block without any has the
+// smallest, in which no sum loses bits.
 __device__ inline int class_exponent(uint32_t most, uint32_t most_share) {
-    return min(halves::exponent_of(most), halves::exponent_of(most_share) + 82);
+    const int smallest = halves::exponent_of(most_share) + 82;
+    return most == 0 ? smallest : min(halves::exponent_of(most), smallest);
 }
 
 constexpr int kGradientStride = kBlockTokens + 2;  // four threads that read eight classes of a token each meet different banks
@@ -1055,6 +1057,7 @@ void product_of(Device& d, const half* a, const half* b, int64_t rows_a, int64_t
     launch(product_kernel<Of>, dim3(unsigned(blocks)), dim3(halves::kThreads), uint32_t(halves::Tile::kLds), d.stream, a, b, int(lines),
            d.cu_count, partial, of);
     after_launch("linear_cross_entropy product");
+    if (lines < halves::kLeastSplit) return;
     launch(join_kernel<Of>, dim3(unsigned(d.cu_count) * (Of::kElementwise ? 4u : 1u)), dim3(halves::kThreads), 0, d.stream, d.cu_count,
            static_cast<const float*>(partial), of);
     after_launch("linear_cross_entropy join");
