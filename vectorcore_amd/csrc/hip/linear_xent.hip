@@ -314,29 +314,51 @@ struct Piece {
     __device__ inline int64_t row(int64_t t) const { return place[first + t]; }
 };
 
-// Packs a matrix of floats [rows, columns] by its rows (along columns, row_lines a row) and by its columns (along rows,
+// A matrix of floats [rows, columns], packed by its rows (along columns, row_lines a row) and by its columns (along rows,
 // column_lines a column); either may be null. of.place: the matrix's rows are the piece's; else `rows` of them in order. The
 // largest magnitudes are those of the whole matrix's rows and columns. exponents, filled: or null; of each column its exponent,
 // and bias (or zero), minus infinity for the columns that fill the last tile. A workgroup takes 32 rows and 128 columns, past
 // the ends zeros.
-__global__ __launch_bounds__(kPackThreads) void pack_kernel(const float* __restrict__ values, Piece of, int64_t rows, int64_t columns,
-                                                            const uint32_t* __restrict__ row_most,
-                                                            const uint32_t* __restrict__ column_most, half* __restrict__ by_row,
-                                                            int row_lines, half* __restrict__ by_column, int column_lines, int down, int across,
-                                                            const float* __restrict__ bias, int* __restrict__ exponents,
-                                                            float* __restrict__ filled) {
+struct Packing {
+    const float* values;
+    Piece of;
+    int64_t rows, columns;
+    const uint32_t *row_most, *column_most;
+    half *by_row, *by_column;
+    int row_lines, column_lines, down, across;
+    const float* bias;
+    int* exponents;
+    float* filled;
+    size_t blocks() const { return size_t(down) * size_t(across); }
+};
+
+// Of two matrices in one launch, or of one (the second has no blocks).
+__global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing two) {
     __shared__ float tile[kPackRows][kPackColumns + 4];
-    const int64_t block = block_id();
+    int64_t block = block_id();
+    const int64_t in_one = int64_t(one.down) * one.across;
+    const bool first_one = block < in_one;
+    if (!first_one) block -= in_one;
+    const Packing p = first_one ? one : two;
+    const int down = p.down, across = p.across, row_lines = p.row_lines, column_lines = p.column_lines;
+    if (across == 0) return;
     const int64_t row0 = block / across * kPackRows, column0 = block % across * kPackColumns;
     if (block / across >= down) return;
+    const Piece of = p.of;
+    int64_t rows = p.rows;
+    const int64_t columns = p.columns;
+    const float* __restrict__ values = p.values;
+    const uint32_t *const row_most = p.row_most, *const column_most = p.column_most;
+    half* __restrict__ by_row = p.by_row;
+    half* __restrict__ by_column = p.by_column;
     if (of.place) {
         rows = of.tokens();
         if (row0 >= (rows + halves::kTile - 1) / halves::kTile * halves::kTile) return;
     }
-    if (exponents && row0 == 0 && threadIdx.x < kPackColumns) {
+    if (p.exponents && row0 == 0 && threadIdx.x < kPackColumns) {
         const int64_t v = column0 + threadIdx.x;
-        exponents[v] = v < columns ? halves::exponent_of(column_most[v]) : 0;
-        filled[v] = v >= columns ? kLowest : bias ? bias[v] : 0.0f;
+        p.exponents[v] = v < columns ? halves::exponent_of(column_most[v]) : 0;
+        p.filled[v] = v >= columns ? kLowest : p.bias ? p.bias[v] : 0.0f;
     }
     // Sixteen threads read 512 neighbouring bytes of a row.
     const int c = 8 * (threadIdx.x % 16);
@@ -392,13 +414,29 @@ constexpr int kMostRows = 64, kMostColumns = 256;
 // The largest finite magnitudes of a matrix's rows and columns, as bits, into arrays of zeros: bits of positive floats are
 // ordered as the floats are, so the order of the atomics does not matter. Rows that targets (or null) leave out have no part;
 // cleared (or null) gets zeros for them. A workgroup takes 64 rows and 256 columns.
-__global__ __launch_bounds__(256) void most_kernel(const float* __restrict__ values, const float* __restrict__ targets,
-                                                   int64_t rows, int64_t columns, int64_t classes, int across,
-                                                   uint32_t* __restrict__ row_most, uint32_t* __restrict__ column_most,
-                                                   float* __restrict__ cleared) {
+struct Largest {
+    const float *values, *targets;
+    int64_t rows, columns;
+    int down, across;
+    uint32_t *row_most, *column_most;
+    float* cleared;
+    size_t blocks() const { return size_t(down) * size_t(across); }
+};
+
+// Of two matrices in one launch.
+__global__ __launch_bounds__(256) void most_kernel(Largest one, Largest two, int64_t classes) {
     __shared__ uint32_t of_column[4][kMostColumns];
-    const int64_t block = block_id();
-    const int64_t row0 = block / across * kMostRows, column0 = block % across * kMostColumns;
+    int64_t block = block_id();
+    const int64_t in_one = int64_t(one.down) * one.across;
+    const bool first_one = block < in_one;
+    if (!first_one) block -= in_one;
+    const Largest p = first_one ? one : two;
+    if (block / p.across >= p.down) return;
+    const int64_t rows = p.rows, columns = p.columns;
+    const int64_t row0 = block / p.across * kMostRows, column0 = block % p.across * kMostColumns;
+    const float *__restrict__ values = p.values, *__restrict__ targets = p.targets;
+    uint32_t *const row_most = p.row_most, *const column_most = p.column_most;
+    float* __restrict__ cleared = p.cleared;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int64_t c = column0 + 4 * lane;
     constexpr int kRows = kMostRows / 4;  // of a wavefront
@@ -1063,21 +1101,21 @@ void product_of(Device& d, const half* a, const half* b, int64_t rows_a, int64_t
     after_launch("linear_cross_entropy join");
 }
 
-void pack(Device& d, const float* values, const Piece& of, int64_t rows, int64_t columns, const uint32_t* row_most,
-          const uint32_t* column_most, half* by_row, half* by_column, const float* bias = nullptr, int* exponents = nullptr,
-          float* filled = nullptr) {
+Packing packing(const float* values, const Piece& of, int64_t rows, int64_t columns, const uint32_t* row_most,
+                const uint32_t* column_most, half* by_row, half* by_column) {
     const int64_t down = (by_row ? whole_tiles(rows) : lines_of(rows) * 32) / kPackRows, across = whole_tiles(columns) / kPackColumns;
-    launch(pack_kernel, grid_2d(size_t(down * across)), dim3(kPackThreads), 0, d.stream, values, of, rows, columns, row_most, column_most,
-           by_row, int(lines_of(columns)), by_column, int(lines_of(rows)), int(down), int(across), bias, exponents, filled);
+    return Packing{values, of, rows, columns, row_most, column_most, by_row, by_column, int(lines_of(columns)), int(lines_of(rows)),
+                   int(down), int(across), nullptr, nullptr, nullptr};
+}
+void pack(Device& d, const Packing& one, const Packing& two) {
+    launch(pack_kernel, grid_2d(one.blocks() + two.blocks()), dim3(kPackThreads), 0, d.stream, one, two);
     after_launch("linear_cross_entropy pack");
 }
 
-void largest(Device& d, const float* values, const float* targets, size_t rows, size_t columns, size_t classes, uint32_t* row_most,
-             uint32_t* column_most, float* cleared) {
-    const size_t down = (rows + kMostRows - 1) / kMostRows, across = (columns + kMostColumns - 1) / kMostColumns;
-    launch(most_kernel, grid_2d(down * across), dim3(256), 0, d.stream, values, targets, int64_t(rows), int64_t(columns),
-           int64_t(classes), int(across), row_most, column_most, cleared);
-    after_launch("linear_cross_entropy largest");
+Largest largest(const float* values, const float* targets, size_t rows, size_t columns, uint32_t* row_most, uint32_t* column_most,
+                float* cleared) {
+    return Largest{values, targets, int64_t(rows), int64_t(columns), int((rows + kMostRows - 1) / kMostRows),
+                   int((columns + kMostColumns - 1) / kMostColumns), row_most, column_most, cleared};
 }
 
 // The packed route. shares: of each row, or null for those of the mean, which goes to share[0]. losses and, of a gradient, any
@@ -1100,16 +1138,19 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
     uint32_t *const x_rows = x_columns + width, *const most_share = x_rows + rows;
     int *const counted = numbers.as<int>(), *const place = counted + 1;
     count(d, c, shares, counted, share, place, gradient ? most_share : nullptr, losses, most.as<uint32_t>(), n_most);
-    largest(d, c.weight, nullptr, c.width, c.classes, c.classes, grad_x ? w_rows : nullptr, w_columns, nullptr);
-    largest(d, c.x, c.targets, c.rows, c.width, c.classes, x_rows, grad_weight ? x_columns : nullptr, grad_x);
-
+    const Largest of_w = largest(c.weight, nullptr, c.width, c.classes, grad_x ? w_rows : nullptr, w_columns, nullptr);
+    const Largest of_x = largest(c.x, c.targets, c.rows, c.width, x_rows, grad_weight ? x_columns : nullptr, grad_x);
+    launch(most_kernel, grid_2d(of_w.blocks() + of_x.blocks()), dim3(256), 0, d.stream, of_w, of_x, classes);
+    after_launch("linear_cross_entropy largest");
     Scratch of_class(size_t(2 * whole_classes) * sizeof(float));
     int* const exponents = of_class.as<int>();
     float* const bias = of_class.as<float>() + whole_classes;
 
     Scratch wt(packed_bytes(classes, width)), w(grad_x ? packed_bytes(width, classes) : 4);
-    pack(d, c.weight, Piece{}, width, classes, w_rows, w_columns, grad_x ? w.as<half>() : nullptr, wt.as<half>(), c.bias,
-         exponents, bias);
+    Packing of_weight = packing(c.weight, Piece{}, width, classes, w_rows, w_columns, grad_x ? w.as<half>() : nullptr, wt.as<half>());
+    of_weight.bias = c.bias;
+    of_weight.exponents = exponents;
+    of_weight.filled = bias;
 
     Scratch x(packed_bytes(piece, width)), xt(grad_weight ? packed_bytes(width, piece) : 4);
     Scratch logits(gradient ? size_t(whole_classes * piece) * sizeof(float) : 4), z(grad_x ? packed_bytes(piece, classes) : 4);
@@ -1122,7 +1163,8 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
 
     for (int64_t p = 0; p < pieces; ++p) {
         const Piece of{counted, place, p * piece, piece};
-        pack(d, c.x, of, piece, width, x_rows, x_columns, x.as<half>(), grad_weight ? xt.as<half>() : nullptr);
+        const Packing of_rows = packing(c.x, of, piece, width, x_rows, x_columns, x.as<half>(), grad_weight ? xt.as<half>() : nullptr);
+        pack(d, of_rows, p == 0 ? of_weight : Packing{});
         const auto z_of = [&](auto store) {
             product_of(d, wt.as<half>(), x.as<half>(), classes, piece, lines_of(width), partial.as<float>(),
                        Logits<store()>{of, exponents, x_rows, bias, c.targets, logits.as<float>(), part_most, part_sum, at_target, classes,
