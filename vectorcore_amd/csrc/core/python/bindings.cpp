@@ -71,6 +71,15 @@ std::vector<std::size_t> targets_from(const py::object& obj) {
 // Integer targets with -1 for rows that are left out, of one dimension.
 std::vector<std::int64_t> signed_targets_from(const py::object& obj) {
     if (!py::isinstance<py::array>(obj)) return py::cast<std::vector<std::int64_t>>(obj);
+    const char kind = py::cast<py::array>(obj).dtype().kind();
+    if (kind != 'i' && kind != 'u')
+        throw std::invalid_argument("linear_cross_entropy expects an array of integers as targets; a Tensor takes floats");
+    if (kind == 'u') {
+        auto arr = py::array_t<std::uint64_t, py::array::c_style | py::array::forcecast>::ensure(obj);
+        for (py::ssize_t i = 0; i < arr.size(); ++i)
+            if (arr.data()[i] > static_cast<std::uint64_t>(INT64_MAX))
+                throw std::out_of_range("target class " + std::to_string(arr.data()[i]) + " is out of range");
+    }
     auto arr = py::array_t<std::int64_t, py::array::c_style | py::array::forcecast>::ensure(obj);
     if (!arr || arr.ndim() != 1) throw std::invalid_argument("linear_cross_entropy expects targets of shape [rows]");
     return {arr.data(), arr.data() + arr.size()};

@@ -84,8 +84,8 @@ struct Tile {
         load_one<At + 24576>(rs, off, 3 * step, lds);
     }
 
-    // acc += the products of lines [begin, end) of 256 rows of each operand; a, b: their first rows; lines: of a row, fewer
-    // than 2^16 (a load's offset has 31 bits). lds: kLds bytes. Row r's chunk c lies in slot c ^ (r / 2 % 8) of its 128 bytes:
+    // acc += the products of lines [begin, end) of 256 rows of each operand; a, b: their first rows; lines: of a row, at
+    // most 2^16 (a load's offset has 31 bits). lds: kLds bytes. Row r's chunk c lies in slot c ^ (r / 2 % 8) of its 128 bytes:
     // the rows of a fragment then meet different banks.
     // Run lines at a time (0: all), from a multiple of that many, before(s) and after(s) around those from s.
     template <int Run, class Before, class After>
