@@ -9,7 +9,8 @@
 // Bound by HBM (8 bytes an element, 12 with a residual): ten rounds of two 32 x 32
 // products make four words, about 20 instructions an element at a quarter rate or
 // better. A thread makes the words of four neighbours, which it loads and stores
-// as one 16-byte access.
+// as one 16-byte access, of four such groups in flight. 8192 x 4096: 52 us (5.2
+// TB/s), 85 us with a residual (4.7; a copy of 1 GiB reaches 5.1). 256 x 256: 3.3.
 #include "vc_hip_internal.hpp"
 
 #include <cmath>

@@ -15,6 +15,11 @@
 // A row's mean is kept as a float and what the float is off by: x - m would
 // otherwise lose the bits of a row that lies far from zero. The statistics are
 // sums of at most 64 values a lane, then a tree.
+//
+// Measured: 8192 rows of 4096, forward 47 us (5.7 TB/s), backward 79 us (5.1) and
+// 8 us for the partial rows; 262144 rows of 64 without a weight 24 and 33 us (5.7
+// and 6.1; a copy of 1 GiB reaches 5.1, these partly stay in the last cache);
+// 999 rows of 515 4.5 us, and 5.7 and 5.8; one row of 4096 3.5 us.
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"
 
@@ -186,7 +191,8 @@ __global__ __launch_bounds__(kThreadsOf<G>) void rows_backward_kernel(
     const float n = float(width);
     f4 w[NV], dw[Columns ? NV : 1] = {}, db[Columns ? NV : 1] = {};
     if (weight) load<G>(weight, width, t, 0.0f, w);
-    // The next row is on its way while a row is made, where few workgroups share a CU and there are registers for it.
+    // The next row is on its way while a row is made, where few workgroups share a CU and there are registers for it (8192 rows
+    // of 4096: 116 us without, 79 with).
     constexpr bool kAhead = Columns && G == 256;
     const int64_t step = int64_t(gridDim.x) * kGroups;
     f4 next_x[kAhead ? NV : 1], next_d[kAhead ? NV : 1];
@@ -362,7 +368,8 @@ __global__ __launch_bounds__(256) void wide_columns_kernel(const float* __restri
 constexpr int kFinishThreads = 1024, kFinishColumns = 32, kFinishGroups = kFinishThreads / kFinishColumns, kFinishLoads = 16;
 
 // Column c of 2 width: dw, then db. Group g of a workgroup adds the parts g, g + 32, ... of its 32 columns, 16 loads in flight,
-// then the groups are added in order.
+// then the groups are added in order. Bound by those loads' latency where rows are short: 512 parts of 4096 columns 8 us, of 515
+// 5.8.
 __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const float* __restrict__ sums, int parts, int64_t width,
                                                                 float* __restrict__ dw, float* __restrict__ db) {
     __shared__ double groups[kFinishGroups][kFinishColumns];

@@ -9,7 +9,16 @@
 // upstream gradient, or one over the number of rows that count (the mean loss).
 //
 // Rows are taken in pieces: the logits of a piece live in a workspace until
-// their gradients are used.
+// their gradients are used. Three routes, by sizes alone:
+// - up to 16 rows without gradients read W once and keep no logits; bound by HBM
+//   (1 row, 1024 x 50000: 37 us of 205 MB, 5.5 TB/s, and 4 us to join);
+// - small or thin calls take float32 products and a kernel of the rows; bound by
+//   launches (256 rows, 256 x 10 with gradients: 25 us in five);
+// - others take packed products, bound by matrix instructions: 8192 rows, 1024 x
+//   50000, of which 7373 count, with gradients 6.8 ms: 2.05 (the logits, 369
+//   TFLOP/s), 1.83 and 1.94 (their gradients' products), 1.01 (the gradients, 4.4
+//   GB at 4.4 TB/s), 0.3 for all others. 1536 rows that count without: 0.55 ms,
+//   of which the logits 0.48.
 #include "halves_product.hpp"
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"
@@ -1216,10 +1225,10 @@ void few_rows(Device& d, const Call& c, float* losses) {
 bool takes_few(const Call& c) { return c.rows <= kFewMost; }
 
 // Whether packing pays: by estimates of both routes' times in us, for `products` products of the call's sizes (one, or up to three
-// with gradients). Measured (estimated), direct and packed, in us: losses alone of 128 rows, 1024 x 50000: 164 (144), 224 (223);
-// of 256: 265 (279), 226 (223); 999, 515 x 10007: 152 (181), 91 (87); 4096, 256 x 1000: 40 (36), 64 (54). Train steps of 128 rows,
-// 1024 x 50000: 463 (423), 594 (590); of 256: 773 (827), 636 (610); 2048, 1024 x 1024: 154 (152), 173 (186); 16384, 256 x 1000:
-// 285 (333), 243 (271).
+// with gradients). Measured (estimated), direct and packed, in us: losses alone of 128 rows, 1024 x 50000: 177 (144), 221 (219);
+// of 256: 284 (279), 220 (219); 999, 515 x 10007: 158 (181), 75 (83); 4096, 256 x 1000: 41 (36), 48 (50); 2048, 512 x 2048: 53
+// (57), 59 (57). Train steps of 128 rows, 1024 x 50000: 462 (423), 576 (560); of 256: 771 (827), 628 (580); 2048, 1024 x 1024: 152
+// (152), 158 (156); 2048, 512 x 2048: 149 (162), 146 (158); 16384, 256 x 1000: 275 (333), 236 (241).
 bool takes_packed(const Call& c, int products) {
     if (c.classes >= (size_t(1) << 21) || c.width >= (size_t(1) << 21)) return false;  // a load's offset has 31 bits
     const double n = double(c.rows), weights = double(c.width) * double(c.classes), logits = n * double(c.classes);
@@ -1227,7 +1236,7 @@ bool takes_packed(const Call& c, int products) {
     const double direct = (gradient ? 20.0 : 10.0) + 2e-6 * products * n * weights / (aligned ? 105.0 : 66.0) + 1.5e-6 * products * logits;
     const double tiles = double(whole_tiles(int64_t(c.rows))) * double(whole_tiles(int64_t(c.classes))) * double(c.width);
     const double packing = (gradient ? 4.2e-6 : 2.0e-6) * (weights + n * double(c.width));
-    return direct > (gradient ? 130.0 : 45.0) + packing + 2e-6 * products * tiles / 350.0 + (gradient ? 3.0e-6 : 0.0) * logits;
+    return direct > (gradient ? 100.0 : 41.0) + packing + 2e-6 * products * tiles / 350.0 + (gradient ? 3.0e-6 : 0.0) * logits;
 }
 
 }  // namespace
