@@ -188,26 +188,26 @@ struct Tile {
                 to += 16 * kThreads;
             }
     }
-    // The sum of all parts, in their order, of a cleared tile; four parts' loads of 16 values in flight.
-    __device__ inline void load_parts(const float* partial, int parts) {
+    // The sum of all parts, in their order, of a thread's values in column block b; four parts' loads of 16 values in flight.
+    static __device__ inline void load_parts(const float* partial, int parts, int thread, int b, f16v (&sum)[4][1]) {
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+        for (int a = 0; a < 4; ++a) {
+            const float* from = partial + (2 * a + b) * 16 * kThreads + thread;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const float* from = partial + (2 * a + b) * 16 * kThreads + threadIdx.x;
-                for (int p = 0; p < parts; p += 4) {
-                    float v[4][16];
+            for (int i = 0; i < 16; ++i) sum[a][0][i] = 0.0f;
+            for (int p = 0; p < parts; p += 4) {
+                float v[4][16];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 4; ++q)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            v[q][i] = p + q < parts ? from[(int64_t(p + q) * kValues + i) * kThreads] : 0.0f;
+                    for (int i = 0; i < 16; ++i)
+                        v[q][i] = p + q < parts ? from[(int64_t(p + q) * kValues + i) * kThreads] : 0.0f;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 4; ++q)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[a][b][i] += v[q][i];
-                }
+                    for (int i = 0; i < 16; ++i) sum[a][0][i] += v[q][i];
             }
+        }
     }
     // The same for four values alone: group q of 32 of a thread, f(row, column, v).
     template <class F>

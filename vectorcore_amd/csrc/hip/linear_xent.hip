@@ -161,7 +161,9 @@ struct RowOutputs {
 constexpr int kCountedHere = 1024;
 
 // A workgroup a row: its loss from the logits z (without the bias), and, where Gradient, z becomes dz. Held: the row, of at most
-// 4 Threads Held values, is read once and stays in registers; 0: read for the maximum, the sum and the gradient.
+// 4 Threads Held values, is read once and stays in registers; 0: read for the maximum, the sum and the gradient. Bound by the
+// loads' latency: 468 rows of 26655 with gradients 35 us (of 100 MB; 57 with one load of a thread in flight), 19 rows of 52907
+// 21 (47); 256 rows of 10, one wavefront each, 8.6.
 // shares: of each row, or of all (one_share), or null: one over the number of rows that count, which each workgroup finds itself.
 template <int Threads, int Held, bool Gradient>
 __global__ __launch_bounds__(Threads) void logits_kernel(float* __restrict__ z, const float* __restrict__ bias,
@@ -198,23 +200,36 @@ __global__ __launch_bounds__(Threads) void logits_kernel(float* __restrict__ z, 
         }
         const auto value = [&](int64_t c) { return bias ? row[c] + bias[c] : row[c]; };
         const float at = value(target);
-        // f(class, logit), four logits at a time; what f makes of them is written back if `keep`.
+        // f(class, logit), four loads of four logits in flight; what f makes of them is written back if `keep`.
         const auto each = [&](auto&& f, bool keep = false) {
-            for (int64_t c = 4 * int64_t(threadIdx.x); c < classes; c += 4 * Threads) {
-                if (c + 3 < classes) {
-                    f4u x = *reinterpret_cast<const f4u*>(row + c);
+            constexpr int kLoads = 4;
+            for (int64_t c0 = 4 * int64_t(threadIdx.x); c0 < classes; c0 += 4 * Threads * kLoads) {
+                f4u x[kLoads], more[kLoads];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float y = bias ? x[e] + bias[c + e] : x[e];
-                        f(c + e, y);
-                        x[e] = y;
+                for (int u = 0; u < kLoads; ++u) {
+                    const int64_t c = c0 + 4 * Threads * u;
+                    if (c + 3 < classes) {
+                        x[u] = *reinterpret_cast<const f4u*>(row + c);
+                        if (bias) more[u] = *reinterpret_cast<const f4u*>(bias + c);
                     }
-                    if (keep) *reinterpret_cast<f4u*>(row + c) = x;
-                } else {
-                    for (int64_t l = c; l < classes; ++l) {
-                        float y = value(l);
-                        f(l, y);
-                        if (keep) row[l] = y;
+                }
+#pragma unroll
+                for (int u = 0; u < kLoads; ++u) {
+                    const int64_t c = c0 + 4 * Threads * u;
+                    if (c + 3 < classes) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float y = bias ? x[u][e] + more[u][e] : x[u][e];
+                            f(c + e, y);
+                            x[u][e] = y;
+                        }
+                        if (keep) *reinterpret_cast<f4u*>(row + c) = x[u];
+                    } else {
+                        for (int64_t l = c; l < classes; ++l) {
+                            float y = value(l);
+                            f(l, y);
+                            if (keep) row[l] = y;
+                        }
                     }
                 }
             }
@@ -634,15 +649,17 @@ struct Logits {
     __device__ inline int64_t rows_b() const { return piece.tokens(); }
     __device__ inline int depth() const { return lines; }
     __device__ inline bool idle() const { return false; }
-    __device__ inline void operator()(halves::Tile& tile, int m, int n) const {
-        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-        const int64_t v0 = int64_t(m) * halves::kTile, t0 = int64_t(n) * halves::kTile + 64 * (wave % 4) + lane % 32;
+    // Of wave `wave` of a tile: its blocks of 32 columns from block `first`.
+    template <int Blocks>
+    __device__ inline void operator()(const halves::f16v (&acc)[4][Blocks], int m, int n, int wave, int first) const {
+        const int lane = threadIdx.x % 64, column = 64 * (wave % 4) + 32 * first + lane % 32;
+        const int64_t v0 = int64_t(m) * halves::kTile, t0 = int64_t(n) * halves::kTile + column;
         const int64_t tokens = piece.tokens();
         const int row0 = 128 * (wave / 4) + 4 * (lane / 32);
-        float top[2], others[2];
-        int e_token[2], target[2];  // the target's row in this tile
+        float top[Blocks], others[Blocks];
+        int e_token[Blocks], target[Blocks];  // the target's row in this tile
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < Blocks; ++b) {
             top[b] = kLowest;
             others[b] = 0.0f;
             const int64_t t = t0 + 32 * b;
@@ -656,7 +673,7 @@ struct Logits {
         // A row of the tile is a scalar offset: 256 rows of at most 2^16 floats stay within a buffer's 31 bits.
         const __amdgpu_buffer_rsrc_t rows =
             __builtin_amdgcn_make_buffer_rsrc(out + v0 * stride + int64_t(n) * halves::kTile, short(0), 0x7FFFFFFE, 0x00020000);
-        const uint32_t row_bytes = uint32_t(stride) * 4u, at = uint32_t(row0) * row_bytes + uint32_t(64 * (wave % 4) + lane % 32) * 4u;
+        const uint32_t row_bytes = uint32_t(stride) * 4u, at = uint32_t(row0) * row_bytes + uint32_t(column) * 4u;
 #pragma unroll
         for (int a = 0; a < 4; ++a) {       // 32 rows of the tile, 16 of this thread's, at a time:
             asm volatile("" ::: "memory");  // the exponents of all do not fit the registers
@@ -675,13 +692,13 @@ struct Logits {
                 for (int i = 0; i < 4; ++i) add[4 * g + i] = more[i];
             }
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < Blocks; ++b) {
                 int own = target[b] - row0 - r0;  // the target's among these rows, if it is
                 float z[16], high = top[b], found = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int r = 8 * (i / 4) + i % 4;
-                    z[i] = __builtin_amdgcn_ldexpf(tile.acc[a][b][i], -(e[i] + e_token[b])) + add[i];
+                    z[i] = __builtin_amdgcn_ldexpf(acc[a][b][i], -(e[i] + e_token[b])) + add[i];
                     if constexpr (Store)
                         __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, z[i]), rows, at + 128u * b,
                                                               uint32_t(r0 + r) * row_bytes, 0);
@@ -701,7 +718,7 @@ struct Logits {
             }
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < Blocks; ++b) {
             const int64_t t = t0 + 32 * b;
             const float both = fmaxf(top[b], red::partner<5>(top[b], lane));
             float mine = top[b] == both ? others[b] : others[b] * exp_of(top[b] - both);
@@ -858,27 +875,31 @@ __global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* _
     else if constexpr (Of::kElementwise)
         tile.each4([&](int r, int c, float(&v)[4]) { of.store(at.m, at.n, r, c, v); });
     else
-        of(tile, at.m, at.n);
+        of(tile.acc, at.m, at.n, int(threadIdx.x / 64), 0);
 }
 
-// The split tiles of a product: a workgroup each, or, of results that are stored value by value, one for four values of every
-// thread.
+// The split tiles of a product: a workgroup for four values of every thread, of results that are stored value by value, or for one
+// of the two blocks of 32 columns of two waves. (48 tiles of five parts of the logits: 20 us, 35 with a workgroup for a tile.)
 template <class Of>
-__global__ __launch_bounds__(halves::kThreads) void join_kernel(int places, const float* __restrict__ partial, Of of) {
+constexpr int kJoinThreads = Of::kElementwise ? halves::kThreads : 128;
+template <class Of>
+constexpr int kJoinShares = Of::kElementwise ? halves::Tile::kValues / 4 : 2 * halves::kThreads / kJoinThreads<Of>;
+
+template <class Of>
+__global__ __launch_bounds__(kJoinThreads<Of>) void join_kernel(int places, const float* __restrict__ partial, Of of) {
     if (of.idle()) return;
     const halves::Tiles tiles = halves::tiles_of(of.rows_a(), of.rows_b(), of.depth(), places);
-    constexpr int kShares = Of::kElementwise ? halves::Tile::kValues / 4 : 1;
-    for (int u = blockIdx.x; u < tiles.rest * kShares; u += gridDim.x) {
-        const int rest = u / kShares;
+    for (int u = blockIdx.x; u < tiles.rest * kJoinShares<Of>; u += gridDim.x) {
+        const int rest = u / kJoinShares<Of>, share = u % kJoinShares<Of>;
         const halves::Place at = halves::tile_at(tiles, tiles.whole + rest);
         const float* const from = partial + int64_t(rest * tiles.parts) * halves::Tile::kValues * halves::kThreads;
         if constexpr (Of::kElementwise) {
-            halves::Tile::each_part(from, tiles.parts, u % kShares, [&](int r, int c, const float(&v)[4]) { of.store(at.m, at.n, r, c, v); });
+            halves::Tile::each_part(from, tiles.parts, share, [&](int r, int c, const float(&v)[4]) { of.store(at.m, at.n, r, c, v); });
         } else {
-            halves::Tile tile;
-            tile.clear();
-            tile.load_parts(from, tiles.parts);
-            of(tile, at.m, at.n);
+            const int thread = share / 2 * kJoinThreads<Of> + int(threadIdx.x);
+            halves::f16v acc[4][1];
+            halves::Tile::load_parts(from, tiles.parts, thread, share % 2, acc);
+            of(acc, at.m, at.n, thread / 64, share % 2);
         }
     }
 }
@@ -1105,7 +1126,7 @@ void product_of(Device& d, const half* a, const half* b, int64_t rows_a, int64_t
            d.cu_count, partial, of);
     after_launch("linear_cross_entropy product");
     if (lines < halves::kLeastSplit) return;
-    launch(join_kernel<Of>, dim3(unsigned(d.cu_count) * (Of::kElementwise ? 4u : 1u)), dim3(halves::kThreads), 0, d.stream, d.cu_count,
+    launch(join_kernel<Of>, dim3(unsigned(d.cu_count) * (Of::kElementwise ? 4u : 8u)), dim3(kJoinThreads<Of>), 0, d.stream, d.cu_count,
            static_cast<const float*>(partial), of);
     after_launch("linear_cross_entropy join");
 }
