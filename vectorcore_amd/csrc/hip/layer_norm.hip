@@ -510,8 +510,8 @@ int vc_hip_layer_norm_backward(const float* grad, const float* x, const float* w
         }
         after_launch("layer_norm_backward");
         if (columns) {
-            launch(finish_kernel, dim3(unsigned((2 * width + kFinishColumns - 1) / kFinishColumns)), dim3(kFinishThreads), 0, d.stream, sums->as<float>(),
-                   int(parts), int64_t(width), grad_weight, grad_bias);
+            launch(finish_kernel, dim3(unsigned((2 * width + kFinishColumns - 1) / kFinishColumns)), dim3(kFinishThreads), 0, d.stream,
+                   sums->as<float>(), int(parts), int64_t(width), grad_weight, grad_bias);
             after_launch("layer_norm_backward columns");
         }
         p.done();
