@@ -59,7 +59,7 @@ __device__ inline void wait_loads() {
 
 // A tile of 256 x 256 by eight waves, wave w rows 128 (w / 4) .. and columns 64 (w % 4) .. in 32 x 32 blocks. Two waves a SIMD
 // and one workgroup a CU: a 16-deep step of a wave reads 12 KiB of LDS for 24 instructions, and a slice of 32 k (64 KiB of
-// loads) takes 3072 cycles, which covers the loads of the next.
+// loads) takes about 3000 cycles, which covers the loads of the next.
 struct Tile {
     static constexpr int kStage = 2 * kTile * kLineBytes, kLds = 2 * kStage, kValues = 128;
     f16v acc[4][2];

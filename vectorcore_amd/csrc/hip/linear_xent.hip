@@ -1249,15 +1249,19 @@ bool takes_few(const Call& c) { return c.rows <= kFewMost; }
 // with gradients). Measured (estimated), direct and packed, in us: losses alone of 128 rows, 1024 x 50000: 177 (144), 221 (219);
 // of 256: 284 (279), 220 (219); 999, 515 x 10007: 158 (181), 75 (83); 4096, 256 x 1000: 41 (36), 48 (50); 2048, 512 x 2048: 53
 // (57), 59 (57). Train steps of 128 rows, 1024 x 50000: 462 (423), 576 (560); of 256: 771 (827), 628 (580); 2048, 1024 x 1024: 152
-// (152), 158 (156); 2048, 512 x 2048: 149 (162), 146 (158); 16384, 256 x 1000: 275 (333), 236 (241).
-bool takes_packed(const Call& c, int products) {
+// (152), 158 (156); 3145, 18 x 25838: 505 (519), 656 (613), with a bias, a tenth of the rows left out, 658 (673), 588 (613); 4096,
+// 96 x 10000: 386 (429), 375 (374); 16384, 256 x 1000: 275 (333), 236 (241).
+bool takes_packed(const Call& c, int products, bool grad_bias) {
     if (c.classes >= (size_t(1) << 21) || c.width >= (size_t(1) << 21)) return false;  // a load's offset has 31 bits
     const double n = double(c.rows), weights = double(c.width) * double(c.classes), logits = n * double(c.classes);
     const bool gradient = products > 1, aligned = c.width % 4 == 0 && c.classes % 4 == 0;
-    const double direct = (gradient ? 20.0 : 10.0) + 2e-6 * products * n * weights / (aligned ? 105.0 : 66.0) + 1.5e-6 * products * logits;
-    const double tiles = double(whole_tiles(int64_t(c.rows))) * double(whole_tiles(int64_t(c.classes))) * double(c.width);
+    const double direct = (gradient ? 20.0 : 10.0) + 2e-6 * products * n * weights / (aligned ? 105.0 : 66.0) +
+                          (1.5e-6 * products + (grad_bias ? 1.9e-6 : 0.0)) * logits;
+    // The features are a depth of whole lines in the logits, and whole tiles in the gradients' products.
+    const double features = 32.0 * double(lines_of(int64_t(c.width))) + (products - 1) * double(whole_tiles(int64_t(c.width)));
+    const double tiles = double(whole_tiles(int64_t(c.rows))) * double(whole_tiles(int64_t(c.classes))) * features;
     const double packing = (gradient ? 4.2e-6 : 2.0e-6) * (weights + n * double(c.width));
-    return direct > (gradient ? 100.0 : 41.0) + packing + 2e-6 * products * tiles / 350.0 + (gradient ? 3.0e-6 : 0.0) * logits;
+    return direct > (gradient ? 100.0 : 41.0) + packing + 2e-6 * tiles / 350.0 + (gradient ? 3.0e-6 : 0.0) * logits;
 }
 
 }  // namespace
@@ -1280,7 +1284,7 @@ int vc_hip_linear_xent_forward(const float* x, const float* weight, const float*
         if (!losses && !mean) return;
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy", products, 4.0 * double(width) * double(rows + classes));
-        if (!takes_few(c) && !takes_packed(c, 1)) {
+        if (!takes_few(c) && !takes_packed(c, 1, false)) {
             direct(d, c, nullptr, losses, mean, nullptr, nullptr, nullptr);
         } else {
             Scratch own(losses ? 4 : rows * sizeof(float)), share(sizeof(float));
@@ -1314,7 +1318,7 @@ int vc_hip_linear_xent_gradient(const float* x, const float* weight, const float
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy_gradient", products * (1.0 + (grad_x != nullptr) + (grad_weight != nullptr)),
                    8.0 * double(width) * double(rows + classes));
-        if (takes_packed(c, 1 + (grad_x != nullptr) + (grad_weight != nullptr))) {
+        if (takes_packed(c, 1 + (grad_x != nullptr) + (grad_weight != nullptr), grad_bias != nullptr)) {
             Scratch share(sizeof(float)), losses(mean ? rows * sizeof(float) : 4);
             packed(d, c, shares, share.as<float>(), mean ? losses.as<float>() : nullptr, grad_x, grad_weight, grad_bias);
             if (mean) mean_of(d, c, losses.as<float>(), share.as<float>(), mean);
