@@ -1069,18 +1069,19 @@ void mean_of(Device& d, const Call& c, const float* losses, const float* share, 
     after_launch("linear_cross_entropy mean");
 }
 
-// The route of float32 products: logits, rows, and the gradients' two products. losses or mean, or neither, and any gradient.
+// The route of float32 products: logits, rows, and the gradients' two products. losses, mean and the gradients: any of them.
 // shares: of each row, or null for those of the mean.
 void direct(Device& d, const Call& c, const float* shares, float* losses, float* mean, float* grad_x, float* grad_weight,
             float* grad_bias) {
     const bool gradient = grad_x || grad_weight || grad_bias;
     const size_t piece = rows_of_piece(c), pieces = (c.rows + piece - 1) / piece;
     const bool counted_here = pieces == 1 && c.rows <= kCountedHere, added_here = mean && pieces == 1;
-    Scratch share(sizeof(float)), own_losses(mean && !added_here ? c.rows * sizeof(float) : 4);
+    const bool own_losses = mean && !added_here && !losses;  // the mean adds up the rows' losses, which the caller may want too
+    Scratch share(sizeof(float)), losses_of_mean(own_losses ? c.rows * sizeof(float) : 4);
     Scratch partial(added_here ? red::kMaxFinishBlocks * sizeof(double) : 4);
     const bool count_first = !shares && (gradient || mean) && !counted_here;
     if (count_first) count(d, c, nullptr, nullptr, share.as<float>(), nullptr, nullptr, nullptr);
-    if (mean && !added_here) losses = own_losses.as<float>();
+    if (own_losses) losses = losses_of_mean.as<float>();
     Scratch logits(piece * c.classes * sizeof(float)), rows(grad_weight ? piece * c.width * sizeof(float) : 4);
     Scratch more(pieces > 1 && gradient ? std::max(grad_weight ? c.width * c.classes : 0, c.classes) * sizeof(float) : 4);
     for (size_t r = 0; r < c.rows; r += piece) {
