@@ -53,10 +53,13 @@ void layer_norm_forward(const float* x, const float* weight, const float* bias, 
             for (std::size_t c = 0; c < width; ++c) sum += row[c];
             const double mean = sum / static_cast<double>(width);
             for (std::size_t c = 0; c < width; ++c) squares += (row[c] - mean) * (row[c] - mean);
-            const float near = static_cast<float>(mean), rest = static_cast<float>(mean - near);
-            const float scale = static_cast<float>(1.0 / std::sqrt(squares / static_cast<double>(width) + eps));
+            const double deviation = std::sqrt(squares / static_cast<double>(width) + eps);
+            const float factor = deviation >= 0x1p100 ? 0x1p-100F : deviation > 0.0 && deviation < 0x1p-100 ? 0x1p100F : 1.0F;
+            const double centre = mean * factor;
+            const float near = static_cast<float>(centre), rest = static_cast<float>(centre - near);
+            const float scale = static_cast<float>(1.0 / (deviation * factor));
             for (std::size_t c = 0; c < width; ++c) {
-                float h = (row[c] - near - rest) * scale;
+                float h = (row[c] * factor - near - rest) * scale;
                 if (weight) h *= weight[c];
                 if (bias) h += bias[c];
                 y[r * width + c] = h;
@@ -65,7 +68,7 @@ void layer_norm_forward(const float* x, const float* weight, const float* bias, 
                 stats[4 * r] = near;
                 stats[4 * r + 1] = rest;
                 stats[4 * r + 2] = scale;
-                stats[4 * r + 3] = 0.0F;
+                stats[4 * r + 3] = factor;
             }
         }
     });
@@ -74,7 +77,7 @@ void layer_norm_forward(const float* x, const float* weight, const float* bias, 
 void layer_norm_backward(const float* grad, const float* x, const float* weight, const float* stats, std::size_t rows,
                          std::size_t width, float* grad_x, float* grad_weight, float* grad_bias) {
     const auto normed = [&](std::size_t r, std::size_t c) {
-        return (x[r * width + c] - stats[4 * r] - stats[4 * r + 1]) * stats[4 * r + 2];
+        return (x[r * width + c] * stats[4 * r + 3] - stats[4 * r] - stats[4 * r + 1]) * stats[4 * r + 2];
     };
     if (grad_x) {
         parallel_for(rows, row_grain(width), [&](std::size_t begin, std::size_t end) {
@@ -88,7 +91,7 @@ void layer_norm_backward(const float* grad, const float* x, const float* weight,
                 const float m = static_cast<float>(first / static_cast<double>(width));
                 const float mh = static_cast<float>(second / static_cast<double>(width));
                 for (std::size_t c = 0; c < width; ++c)
-                    grad_x[r * width + c] = (of(c) - m - normed(r, c) * mh) * stats[4 * r + 2];
+                    grad_x[r * width + c] = (of(c) - m - normed(r, c) * mh) * stats[4 * r + 2] * stats[4 * r + 3];
             }
         });
     }

@@ -7,7 +7,8 @@
 
 namespace vectorcore::cpu {
 
-// stats: of each row its mean, what the float mean is off by, 1 / sqrt(variance + eps) and an unused word; or null.
+// stats: of each row times factor its mean, what the float mean is off by and 1 / deviation, then the factor: one, or the power
+// of two that brings a deviation past 2^100 or below 2^-100 to where its reciprocal is a normal float. Or null.
 void layer_norm_forward(const float* x, const float* weight, const float* bias, std::size_t rows, std::size_t width, float eps,
                         float* y, float* stats);
 // The outputs that are null are left out.
