@@ -1,5 +1,5 @@
-"""Layer normalisation of rows near the ends of float32's range, alike for rows of every length and on both
-devices."""
+"""Layer normalisation of rows near the ends of float32's range, alike for rows of every length and on both devices, and sums
+over very many rows."""
 
 import numpy as np
 import pytest
@@ -62,3 +62,20 @@ def test_one_row_does_not_change_another(device):
     x[4] *= np.float32(1e-36)
     y = vc.layer_norm(vc.Tensor(x, device=device)).numpy()
     np.testing.assert_array_equal(y[[0, 2, 3, 5]], alone[[0, 2, 3, 5]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width", [(2 ** 21 + 3, 500), (2 ** 19 + 1, 4000), (2 ** 24 + 5, 12)])
+def test_sums_over_many_equal_rows(rows, width):
+    """Equal terms, whose roundings do not cancel: of a float32 sum of n of them each addition may lose half a step of it, UNIT
+    n / 2 of the whole. Sixty-four are added so, the rest in double; and a product and a deviation's roundings for the weight."""
+    rng = np.random.default_rng(width)
+    row, d = rng.standard_normal(width).astype(np.float32), (1 + rng.random(width)).astype(np.float32)
+    ones = vc.Tensor(np.ones((rows, 1), np.float32), device="hip")
+    x, dy = (ones * vc.Tensor(v, device="hip") for v in (row, d))
+    w, b = (leaf(np.ones(width, np.float32), "hip") for _ in range(2))
+    vc.layer_norm(x, w, b).backward(dy)
+    h = row.astype(np.float64) - row.astype(np.float64).mean()
+    h /= np.sqrt((h * h).mean() + float(np.float32(1e-5)))
+    assert (np.abs(grad_of(b) / (rows * d.astype(np.float64)) - 1) <= 34 * UNIT).all()
+    assert (np.abs(grad_of(w) - rows * h * d) <= rows * d * UNIT * (42 * np.abs(h) + 8)).all()

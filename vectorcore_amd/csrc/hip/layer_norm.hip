@@ -11,6 +11,8 @@
 // made of it, and the backward collects dw and db on the way: a thread holds the
 // same columns of every row of its workgroup, each workgroup leaves one partial
 // row of either sum, and a second launch adds those in a fixed order, in double.
+// The thread's own sums are float32, of at most 64 rows: of many more of one sign
+// the late ones would lose their bits (1e-5 of a sum of 2^21 equal ones).
 //
 // A row's mean is kept as a float and what the float is off by: x - m would
 // otherwise lose the bits of a row that lies far from zero. All of a row's sums
@@ -267,10 +269,10 @@ __global__ __launch_bounds__(kThreadsOf<G>) void rows_backward_kernel(
                     *reinterpret_cast<f4*>(columns + threadIdx.x / G * kMost + 4 * t + 4 * G * u) = which ? db[u] : dw[u];
                 __syncthreads();
                 for (int c = threadIdx.x; c < width; c += Shape<G, NV>::kThreads) {
-                    float total = 0.0f;
+                    double total = 0.0;
 #pragma unroll
-                    for (int g = 0; g < kGroups; ++g) total += columns[g * kMost + c];
-                    out[which * width + c] = total;
+                    for (int g = 0; g < kGroups; ++g) total += double(columns[g * kMost + c]);
+                    out[which * width + c] = float(total);
                 }
             }
         }
@@ -399,6 +401,8 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const float* __r
     if (out) out[c < width ? c : c - width] = float(total);
 }
 
+constexpr size_t kMostAdded = 64;  // rows of a thread's float32 sums
+
 // f(G, NV) for the least shape that holds a row; false where none does.
 template <class F>
 bool with_shape(size_t width, F&& f) {
@@ -489,7 +493,9 @@ int vc_hip_layer_norm_backward(const float* grad, const float* x, const float* w
             using S = Shape<g(), nv()>;
             if constexpr (S::kHoldsSums) {
                 if (columns) {
-                    const unsigned grid = grid_1d(rows, S::kGroups, 2u * unsigned(d.cu_count));
+                    const size_t least = (rows + kMostAdded * S::kGroups - 1) / (kMostAdded * S::kGroups);
+                    if (least > kMostBlocks * 256 / S::kThreads) fail(VC_HIP_ERR_OVERFLOW, "layer_norm_backward: too many rows");
+                    const unsigned grid = grid_1d(rows, S::kGroups, std::max(unsigned(least), 2u * unsigned(d.cu_count)));
                     launch(rows_backward_kernel<g(), nv(), true>, dim3(grid), dim3(S::kThreads), 0, d.stream, grad, x, weight, st,
                            grad_x, scratch(grid), int64_t(rows), int(width));
                     collected = true;
