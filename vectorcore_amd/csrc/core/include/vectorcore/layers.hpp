@@ -32,7 +32,10 @@ enum class Reduction { Mean, None };
 // is a class number as a float; a row whose target is no class number (padding,
 // -1) is left out. Mean: the mean loss of the rows that count, zero if none does;
 // its gradients are computed with it. None: the loss of each row, zero for one
-// that is left out; the gradients compute the logits again.
+// that is left out; the gradients compute the logits again. Large calls on the
+// GPU compute products from two half-precision parts of each value, 22 bits of it,
+// and take longer (by two thirds) where rows of x or W hold values that are too
+// unlike each other for that, say a feature of raw size, and get three parts.
 Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& targets, const std::optional<Tensor>& bias = {},
                             Reduction reduction = Reduction::Mean);
 // The same with host targets, as cross_entropy takes them; -1 leaves a row out.

@@ -220,7 +220,8 @@ PYBIND11_MODULE(_vectorcore, m) {
         "Softmax cross entropy of x @ weight + bias, whose [rows, classes] logits are never kept. targets: class numbers, as "
         "integers or as a Tensor of floats on x's device; -1 (in a Tensor anything that is no class number) leaves a row out. "
         "reduction 'mean': over the rows that count, zero if none does, its gradients computed with it; 'none': the loss of "
-        "each row, zero for one left out.");
+        "each row, zero for one left out. Large calls on the GPU multiply 22 bits of each value, or all 24 in two thirds more "
+        "time where rows of x or weight hold values too unlike each other for that.");
     m.def("softmax", [](const Tensor& t, std::int64_t axis) { return t.softmax(axis); }, py::arg("value"),
           py::arg("axis") = -1);
     m.def("log_softmax", [](const Tensor& t, std::int64_t axis) { return t.log_softmax(axis); }, py::arg("value"),

@@ -3,10 +3,11 @@
 //
 // A value is scaled by a power of two of its row and split, x 2^e = x1 + x2, with
 // half-precision parts. e brings the row's largest magnitude to 2^13 .. 2^14, so a
-// value keeps 22 bits or an error of 2^-39 of the largest, whichever is more. Of
+// value keeps 22 bits or an error of 2^-38 of the largest, whichever is more. Of
 // the four products of two values' parts x2 y2 (2^-22 of the largest) is left out.
 // Three instructions of 32 cycles take the place of eight of 64 of the float32
-// matrix instruction.
+// matrix instruction. For operands whose rows hold values that are finite and not
+// too unlike each other; for others thirds_product.hpp.
 //
 // 32 neighbouring values of a row are one 128-byte line, their first parts, then
 // their second ones: four threads that hold eight values each then write 64

@@ -8,6 +8,9 @@
 // every gradient are zero, whatever x holds there. The share of a row is its
 // upstream gradient, or one over the number of rows that count (the mean loss).
 //
+// All of them keep float32's precision: an error is one of a few roundings of the
+// terms of the sum that it is in, whatever the operands' other values.
+//
 // Rows are taken in pieces: the logits of a piece live in a workspace until
 // their gradients are used. Three routes, by sizes alone:
 // - up to 16 rows without gradients read W once and keep no logits; bound by HBM
@@ -15,12 +18,14 @@
 // - small or thin calls take float32 products and a kernel of the rows; bound by
 //   launches (256 rows, 256 x 10 with gradients: 25 us in five);
 // - others take packed products, bound by matrix instructions: 8192 rows, 1024 x
-//   50000, of which 7373 count, with gradients 6.8 ms: 2.05 (the logits, 369
-//   TFLOP/s), 1.83 and 1.94 (their gradients' products), 1.01 (the gradients, 4.4
-//   GB at 4.4 TB/s), 0.3 for all others. 1536 rows that count without: 0.55 ms,
-//   of which the logits 0.48.
+//   50000, of which 7373 count, with gradients 6.9 ms: 2.05 (the logits, 369
+//   TFLOP/s), 1.87 and 1.94 (their gradients' products), 1.01 (the gradients, 4.4
+//   GB at 4.4 TB/s), 0.3 for all others. 1536 rows that count without: 0.56 ms,
+//   of which the logits 0.48. Where the operands' rows hold values too unlike for
+//   two half-precision parts, three parts: 11.6 and 0.89 ms.
 #include "halves_product.hpp"
 #include "reduce_common.hpp"
+#include "thirds_product.hpp"
 #include "vc_hip_internal.hpp"
 
 #include <algorithm>
@@ -49,14 +54,17 @@ constexpr int kCountThreads = 1024, kCountRows = 4;  // rows of a thread and tur
 
 // The rows that count: how many (counted), one over it or zero (share), and which, in order (place, or null), for the packed
 // route with the largest finite magnitude of their shares (most, or null). losses: zeros for the others, or null. cleared: n_cleared
-// words of zeros, or null.
+// words of zeros, by the workgroups behind the first.
 __global__ __launch_bounds__(kCountThreads) void count_kernel(const float* __restrict__ targets, const float* __restrict__ shares,
                                                               int64_t rows, int64_t classes, int* __restrict__ counted,
                                                               float* __restrict__ share, int* __restrict__ place,
                                                               uint32_t* __restrict__ most, float* __restrict__ losses,
                                                               uint32_t* __restrict__ cleared, int64_t n_cleared) {
-    if (cleared)
-        for (int64_t i = threadIdx.x; i < n_cleared; i += kCountThreads) cleared[i] = 0u;
+    if (blockIdx.x > 0) {
+        const int64_t step = int64_t(gridDim.x - 1) * kCountThreads;
+        for (int64_t i = int64_t(blockIdx.x - 1) * kCountThreads + threadIdx.x; i < n_cleared; i += step) cleared[i] = 0u;
+        return;
+    }
     __shared__ int of_wave[kCountThreads / 64];
     __shared__ uint32_t most_of_wave[kCountThreads / 64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
@@ -327,6 +335,36 @@ __global__ __launch_bounds__(Threads) void logits_kernel(float* __restrict__ z, 
 using halves::half;
 using halves::h8;
 
+// How far the rows of the packed operands hold values unlike each other, in sixteenths of a bit: the most by which a row's largest
+// exponent lies above the mean of its values' (zeros aside), for the rows of x and the columns of W (along the features), the
+// rows of W (along the classes) and the columns of x (along the tokens). Also the largest exponents of x and W, and whether
+// either holds an infinity or a NaN.
+//
+// Two half-precision parts keep 22 bits of a value or 2^-38 of its row's largest, X. The latter's share of a sum of n products is
+// at most 2^-37 n X Y; the sum of the products' magnitudes is at least n times the product of both rows' geometric means, so that
+// share is below 2^-22 of it where both rows' largest lie less than 15 bits above them (13 of the exponents, each of which leaves
+// a bit open). Or it is below 2^-24, what an exponential rounds by in any case, where n X Y <= 2^13. In the gradients' products the
+// other operand is the logits' gradients, whose lost parts are likewise 2^-38 of a token's, or class's, largest times the sum of the
+// row: ten bits keep that below 2^-22 of the row's mean for 2^17 classes and tokens. Other calls take three bfloat16 parts
+// (thirds_product.hpp), which keep every value's 24 bits: a feature of 1e9 whose weights are 1e-9 costs time, not the logits.
+struct Unlike {
+    int x_rows, w_columns, w_rows, x_columns, x_most, w_most, not_finite;
+    // width_bits: of the next power of two.
+    __device__ inline bool thirds(int width_bits) const {
+        const bool alike = x_rows + w_columns <= 13 * 16, small = x_most + w_most - 2 * kExponents + width_bits <= 13;
+        return not_finite || !(alike || small) || w_rows > 10 * 16 || x_columns > 10 * 16;
+    }
+    static constexpr int kExponents = 149;  // of a finite value's exponent, for positive numbers
+};
+__device__ inline int exponent_over(float finite) { return __builtin_amdgcn_frexp_expf(finite) + Unlike::kExponents; }
+
+// Which form the packed operands of a call have.
+struct Form {
+    const Unlike* unlike;
+    int width_bits;
+    __device__ inline bool thirds() const { return unlike->thirds(width_bits); }
+};
+
 constexpr int kPackThreads = 256, kPackRows = 32, kPackColumns = 128;
 constexpr int kBlockTokens = 256, kBlockLines = kBlockTokens / halves::kSlice;
 
@@ -357,7 +395,7 @@ struct Packing {
 };
 
 // Of two matrices in one launch, or of one (the second has no blocks).
-__global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing two) {
+__global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing two, Form form) {
     __shared__ float tile[kPackRows][kPackColumns + 4];
     int64_t block = block_id();
     const int64_t in_one = int64_t(one.down) * one.across;
@@ -384,6 +422,7 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing
         p.exponents[v] = v < columns ? halves::exponent_of(column_most[v]) : 0;
         p.filled[v] = v >= columns ? kLowest : p.bias ? p.bias[v] : 0.0f;
     }
+    const bool thirds = form.thirds();
     // Sixteen threads read 512 neighbouring bytes of a row.
     const int c = 8 * (threadIdx.x % 16);
     const int64_t column = column0 + c;
@@ -407,7 +446,7 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) tile[r][c + i] = v[i];
-        if (by_row && column / 32 < row_lines) {
+        if (!thirds && by_row && column / 32 < row_lines) {
             h8 first, second;
             halves::split8(v, there ? halves::exponent_of(row_most[row]) : 0, first, second);
             half* const to = by_row + ((row0 + r) * row_lines + column / 32) * 64 + column % 32;
@@ -415,9 +454,35 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing
             *reinterpret_cast<h8*>(to + 32) = second;
         }
     }
-    if (!by_column) return;
+    if (!by_column && !thirds) return;
     __syncthreads();
     const int64_t line = row0 / 32;
+    if (thirds) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r = threadIdx.x % 32, g = threadIdx.x / 32 + 8 * j;
+            if (by_row && (column0 + 8 * g) / 32 < row_lines) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = tile[r][8 * g + i];
+                const bool there = row0 + r < rows;
+                const int64_t row = there && of.place ? of.row(row0 + r) : row0 + r;
+                thirds::store8(by_row, row_lines, row0 + r, column0 / 8 + g, v, there ? halves::exponent_of(row_most[row]) : 0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int at = threadIdx.x % 128, g = threadIdx.x / 128 + 2 * j;
+            if (by_column && line < column_lines) {
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = tile[8 * g + i][at];
+                thirds::store8(by_column, column_lines, column0 + at, row0 / 8 + g, v,
+                               column0 + at < columns ? halves::exponent_of(column_most[column0 + at]) : 0);
+            }
+        }
+        return;
+    }
     if (line >= column_lines) return;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -433,23 +498,46 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing
     }
 }
 
-constexpr int kMostRows = 64, kMostColumns = 256;
+constexpr int kMostRows = 64, kMostColumns = 256, kCountShift = 36;
+constexpr size_t kMostCounted = size_t(1) << 27;  // values of a row or column: their exponents' sum stays below 2^36
 
-// The largest finite magnitudes of a matrix's rows and columns, as bits, into arrays of zeros: bits of positive floats are
-// ordered as the floats are, so the order of the atomics does not matter. Rows that targets (or null) leave out have no part;
-// cleared (or null) gets zeros for them. A workgroup takes 64 rows and 256 columns.
+// The largest finite magnitudes of a matrix's rows and columns, as bits, and how many finite values are no zeros, times 2^36, plus
+// their exponents' sum, into arrays of zeros: bits of positive floats are ordered as the floats are, and whole numbers are added,
+// so the order of the atomics does not matter. Rows that targets (or null) leave out have no part; cleared (or null) gets zeros for
+// them. A workgroup takes 64 rows and 256 columns.
 struct Largest {
     const float *values, *targets;
     int64_t rows, columns;
     int down, across;
     uint32_t *row_most, *column_most;
+    unsigned long long *row_sum, *column_sum;
     float* cleared;
     size_t blocks() const { return size_t(down) * size_t(across); }
 };
 
+// Over the wavefront, for 2^(Step + 1) rows at a time of which every lane holds a part: lane l gets row l % 16 of sixteen. Each
+// exchange leaves a lane and its partner half of the rows each.
+template <int Step, int N, class Op>
+__device__ inline uint32_t lanes_rows(const uint32_t (&part)[N], int lane, Op op) {
+    static_assert(N == 2 << Step);
+    const bool upper = lane >> Step & 1;
+    uint32_t kept[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const uint32_t mine = upper ? part[N / 2 + i] : part[i], other = upper ? part[i] : part[N / 2 + i];
+        kept[i] = op(mine, red::partner<Step>(other, lane));
+    }
+    if constexpr (Step > 0) {
+        return lanes_rows<Step - 1>(kept, lane, op);
+    } else {
+        uint32_t all = op(kept[0], red::partner<4>(kept[0], lane));
+        return op(all, red::partner<5>(all, lane));
+    }
+}
+
 // Of two matrices in one launch.
-__global__ __launch_bounds__(256) void most_kernel(Largest one, Largest two, int64_t classes) {
-    __shared__ uint32_t of_column[4][kMostColumns];
+__global__ __launch_bounds__(256) void most_kernel(Largest one, Largest two, int64_t classes, Unlike* __restrict__ unlike) {
+    __shared__ uint32_t of_column[4][kMostColumns], sum_of_column[4][kMostColumns];
     int64_t block = block_id();
     const int64_t in_one = int64_t(one.down) * one.across;
     const bool first_one = block < in_one;
@@ -459,7 +547,7 @@ __global__ __launch_bounds__(256) void most_kernel(Largest one, Largest two, int
     const int64_t rows = p.rows, columns = p.columns;
     const int64_t row0 = block / p.across * kMostRows, column0 = block % p.across * kMostColumns;
     const float *__restrict__ values = p.values, *__restrict__ targets = p.targets;
-    uint32_t *const row_most = p.row_most, *const column_most = p.column_most;
+    uint32_t* const column_most = p.column_most;
     float* __restrict__ cleared = p.cleared;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int64_t c = column0 + 4 * lane;
@@ -485,38 +573,97 @@ __global__ __launch_bounds__(256) void most_kernel(Largest one, Largest two, int
                 if (c + e < columns) cleared[(first + j) * columns + c + e] = 0.0f;
         }
     }
-    uint32_t most[4] = {0, 0, 0, 0}, of_row = 0;  // lane j: of the wavefront's row j
+    // Sums of at most 256 values: their number times 2^20 and their exponents'.
+    uint32_t most[4] = {0, 0, 0, 0}, sums[4] = {0, 0, 0, 0}, row_most[kRows], row_sums[kRows];
+    bool not_finite = false;
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-        uint32_t row = 0;
+        row_most[j] = row_sums[j] = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float value = v[j][e];  // a bit cast of a vector's element itself takes the first one
             uint32_t bits = __builtin_bit_cast(uint32_t, value) & 0x7FFFFFFFu;
+            not_finite |= bits >= 0x7F800000u;
             bits = bits < 0x7F800000u ? bits : 0u;
+            const uint32_t exponent = bits ? (1u << 20) + uint32_t(exponent_over(value)) : 0u;
             most[e] = max(most[e], bits);
-            row = max(row, bits);
+            sums[e] += exponent;
+            row_most[j] = max(row_most[j], bits);
+            row_sums[j] += exponent;
         }
-        if (row_most) {
-            row = max(row, red::partner<0>(row, lane));
-            row = max(row, red::partner<1>(row, lane));
-            row = max(row, red::partner<2>(row, lane));
-            row = max(row, red::partner<3>(row, lane));
-            row = max(row, red::partner<4>(row, lane));
-            row = max(row, red::partner<5>(row, lane));
-            of_row = lane == j ? row : of_row;
-        }
+        asm volatile("" : "+v"(row_most[j]), "+v"(row_sums[j]));  // a row at a time: what is made of all of them needs more registers
+#pragma unroll
+        for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(most[e]), "+v"(sums[e]));
     }
-    if (of_row) atomicMax(&row_most[own], of_row);  // a row past the end has none
+    uint32_t of_row = 0, sum_of_row = 0;
+    if (p.row_most) {  // lane j of the first sixteen: of the wavefront's row j
+        of_row = lanes_rows<3>(row_most, lane, [](uint32_t a, uint32_t b) { return max(a, b); });
+        sum_of_row = lanes_rows<3>(row_sums, lane, [](uint32_t a, uint32_t b) { return a + b; });
+        if (lane >= kRows) of_row = 0;
+    }
+    if (__ballot(not_finite) && lane == 0) unlike->not_finite = 1;  // whoever writes it, and whenever, it is one
+    const auto add = [](uint32_t* most, unsigned long long* sums, uint32_t largest, uint32_t sum) {
+        if (!largest) return;
+        atomicMax(most, largest);
+        atomicAdd(sums, (unsigned long long)(sum >> 20) << kCountShift | (sum & 0xFFFFFu));
+    };
+    add(&p.row_most[own], &p.row_sum[own], of_row, sum_of_row);  // a row past the end has none
     if (!column_most) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) of_column[wave][4 * lane + e] = most[e];
+    for (int e = 0; e < 4; ++e) {
+        of_column[wave][4 * lane + e] = most[e];
+        sum_of_column[wave][4 * lane + e] = sums[e];
+    }
     __syncthreads();
     const int64_t column = column0 + threadIdx.x;
-    uint32_t all = of_column[0][threadIdx.x];
+    uint32_t all = of_column[0][threadIdx.x], sum = sum_of_column[0][threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) all = max(all, of_column[w][threadIdx.x]);
-    if (column < columns && all) atomicMax(&column_most[column], all);
+    for (int w = 1; w < 4; ++w) {
+        all = max(all, of_column[w][threadIdx.x]);
+        sum += sum_of_column[w][threadIdx.x];
+    }
+    if (column < columns) add(&column_most[column], &p.column_sum[column], all, sum);
+}
+
+// The most unlike rows, of maxima and sums in the order W's columns (whole_classes of them), W's rows (width), x's columns
+// (width), x's rows; what most_kernel was not asked for is zeros.
+__global__ __launch_bounds__(256) void unlike_kernel(const uint32_t* __restrict__ most, const unsigned long long* __restrict__ sums,
+                                                     int64_t whole_classes, int64_t width, int64_t rows, Unlike* __restrict__ unlike) {
+    int gaps[4] = {0, 0, 0, 0}, high[4] = {0, 0, 0, 0};
+    const int64_t n = whole_classes + 2 * width + rows;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+        const unsigned long long of = sums[i];
+        const uint64_t values = of >> kCountShift, sum = of & ((1ull << kCountShift) - 1);
+        if (!values) continue;
+        const int exponent = exponent_over(__builtin_bit_cast(float, most[i]));
+        const int gap = int(((uint64_t(exponent) * values - sum) * 16 + values - 1) / values);
+        const int group = i < whole_classes ? 0 : i < whole_classes + width ? 1 : i < whole_classes + 2 * width ? 2 : 3;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            gaps[g] = group == g ? max(gaps[g], gap) : gaps[g];
+            high[g] = group == g ? max(high[g], exponent) : high[g];
+        }
+    }
+    __shared__ int of_wave[4][6];
+    const int lane = threadIdx.x % 64;
+    const int found[6] = {gaps[0], gaps[1], gaps[2], gaps[3], high[0], high[3]};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        int v = found[i];
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) v = max(v, __shfl_xor(v, d, 64));
+        if (lane == 0) of_wave[threadIdx.x / 64][i] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 6) return;
+    int* const to[6] = {&unlike->w_columns, &unlike->w_rows, &unlike->x_columns, &unlike->x_rows, &unlike->w_most, &unlike->x_most};
+    int v = 0;
+    for (int w = 0; w < 4; ++w) v = max(v, of_wave[w][threadIdx.x]);
+    int* at = to[0];
+#pragma unroll
+    for (int i = 1; i < 6; ++i) at = int(threadIdx.x) == i ? to[i] : at;
+    // Most workgroups find nothing more: a look costs less than the atomic.
+    if (v > __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(at, v);
 }
 
 // What a token's gradients are made of, from its logits' statistics.
@@ -537,15 +684,16 @@ __device__ inline int class_exponent(uint32_t most, uint32_t most_share) {
 constexpr int kGradientStride = kBlockTokens + 2;  // four threads that read eight classes of a token each meet different banks
 
 // The gradients dz^T of a piece from its logits z^T [classes, stride]: times the tokens' shares, packed along the tokens, in
-// their place; and for shares of one packed along the classes (by_token, or null). most [blocks][whole classes]: the largest of
+// their place (three parts: into by_class, in the unit of the largest share); and for shares of one packed along the classes
+// (by_token, or null). most [blocks][whole classes]: the largest of
 // each class, as bits. Sums: of each class, into sums [blocks][classes]. A workgroup takes 32 classes and a block of tokens;
 // four lanes of a wavefront read a line of the logits, and then write it.
 template <bool Sums>
 __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t stride, Piece piece, const Token* __restrict__ tokens,
                                                         const float* __restrict__ shares, const uint32_t* __restrict__ most_share,
                                                         int64_t classes, int64_t whole_classes, uint32_t* __restrict__ most,
-                                                        half* __restrict__ by_token, int lines, double* __restrict__ sums,
-                                                        int blocks) {
+                                                        half* __restrict__ by_token, half* __restrict__ by_class, int lines,
+                                                        double* __restrict__ sums, int blocks, Form form) {
     __shared__ float tile[32][kGradientStride];
     const int64_t id = block_id(), block = id % blocks, v0 = id / blocks * 32;
     if (v0 >= classes) return;
@@ -572,6 +720,7 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
         share[i] = t0 + c + i < n ? shares[t0 + c + i] : 0.0f;
     }
     const uint32_t top = most_share[0];
+    const bool thirds = form.thirds();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int r = threadIdx.x / 32 + 8 * j;
@@ -604,11 +753,15 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
             sum += red::partner<4>(sum, lane);
         }
         if (!there) continue;
-        h8 first, second;
-        halves::split8(d, class_exponent(high, top), first, second);
-        half* const to = reinterpret_cast<half*>(at - c % 32 + 8 * j * stride) + c % 32;
-        *reinterpret_cast<h8*>(to) = first;
-        *reinterpret_cast<h8*>(to + 32) = second;
+        if (thirds) {
+            thirds::store8(by_class, int(stride / halves::kSlice), v, (t0 + c) / 8, d, halves::exponent_of(top));
+        } else {
+            h8 first, second;
+            halves::split8(d, class_exponent(high, top), first, second);
+            half* const to = reinterpret_cast<half*>(at - c % 32 + 8 * j * stride) + c % 32;
+            *reinterpret_cast<h8*>(to) = first;
+            *reinterpret_cast<h8*>(to + 32) = second;
+        }
         if (threadIdx.x % 32 == 0) {
             most[block * whole_classes + v] = high;
             if constexpr (Sums) sums[block * classes + v] = sum;
@@ -618,11 +771,16 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int t = threadIdx.x / 4 + 64 * j, g = threadIdx.x % 4;
+        // Three parts of neighbouring tokens lie next to each other, of two parts those of neighbouring classes.
+        const int t = thirds ? int(threadIdx.x) : threadIdx.x / 4 + 64 * j, g = thirds ? j : threadIdx.x % 4;
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = tile[8 * g + i][t];
         const uint32_t others = t0 + t < n ? __builtin_bit_cast(uint32_t, tokens[t0 + t].others) : 0u;
+        if (thirds) {
+            thirds::store8(by_token, lines, t0 + t, v0 / 8 + g, v, halves::exponent_of(others));
+            continue;
+        }
         h8 first, second;
         halves::split8(v, halves::exponent_of(others), first, second);
         half* const to = by_token + ((t0 + t) * lines + v0 / 32) * 64 + 8 * g;
@@ -823,10 +981,12 @@ struct WeightGradient {
     }
 };
 
-// lines: a row's of either operand, of which depth() are multiplied. The parts of split tiles go to partial, for join_kernel.
+// lines: a row's of either operand, of which depth() are multiplied; b_thirds: b in three parts. The parts of split tiles go to
+// partial, for join_kernel.
 template <class Of>
-__global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* __restrict__ a, const half* __restrict__ b, int lines,
-                                                                   int places, float* __restrict__ partial, Of of) {
+__global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* __restrict__ a, const half* __restrict__ b,
+                                                                   const half* __restrict__ b_thirds, int lines, int places,
+                                                                   float* __restrict__ partial, Of of, Form form) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
     if (of.idle()) return;
     const int depth = of.depth();
@@ -842,7 +1002,20 @@ __global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* _
     const int64_t of_tile = int64_t(lines) * halves::kTile * (halves::kLineBytes / 2);
     halves::Tile tile;
     tile.clear();
-    if constexpr (Of::kUnits) {
+    if (form.thirds()) {
+        const int64_t bytes = thirds::tile_bytes(lines);
+        thirds::accumulate(tile, reinterpret_cast<const char*>(a) + at.m * bytes, reinterpret_cast<const char*>(b_thirds) + at.n * bytes,
+                           begin, end, lds);
+        if constexpr (Of::kUnits) {
+            const int by = -halves::exponent_of(of.most_share[0]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) tile.acc[r][j][i] = __builtin_amdgcn_ldexpf(tile.acc[r][j][i], by);
+        }
+    } else if constexpr (Of::kUnits) {
         // A thread's two columns of the tile, which are classes, and the exponents of their units.
         const uint32_t* const most = of.class_most + int64_t(at.n) * halves::kTile + 64 * (threadIdx.x / 64 % 4) + threadIdx.x % 32;
         const uint32_t top = of.most_share[0];
@@ -1060,8 +1233,9 @@ void rows_of(Device& d, float* z, const Call& c, const float* targets, const flo
 
 void count(Device& d, const Call& c, const float* shares, int* counted, float* share, int* place, uint32_t* most, float* losses,
            uint32_t* cleared = nullptr, int64_t n_cleared = 0) {
-    launch(count_kernel, dim3(1), dim3(kCountThreads), 0, d.stream, c.targets, shares, int64_t(c.rows), int64_t(c.classes), counted, share,
-           place, most, losses, cleared, n_cleared);
+    const unsigned clearing = n_cleared > 0 ? grid_1d(size_t(n_cleared), kCountThreads, 64) : 0;
+    launch(count_kernel, dim3(1 + clearing), dim3(kCountThreads), 0, d.stream, c.targets, shares, int64_t(c.rows), int64_t(c.classes),
+           counted, share, place, most, losses, cleared, n_cleared);
     after_launch("linear_cross_entropy count");
 }
 void mean_of(Device& d, const Call& c, const float* losses, const float* share, float* mean) {
@@ -1112,19 +1286,23 @@ void direct(Device& d, const Call& c, const float* shares, float* losses, float*
 
 int64_t whole_tiles(int64_t n) { return (n + halves::kTile - 1) / halves::kTile * halves::kTile; }
 int64_t lines_of(int64_t n) { return (n + halves::kSlice - 1) / halves::kSlice; }
-// A packed matrix of `rows` rows of `depth` values.
-size_t packed_bytes(int64_t rows, int64_t depth) { return size_t(whole_tiles(rows)) * size_t(lines_of(depth)) * halves::kLineBytes; }
+// A packed matrix of `rows` rows of `depth` values, in the larger of both forms: three parts.
+size_t packed_bytes(int64_t rows, int64_t depth) {
+    return size_t(whole_tiles(rows) / halves::kTile) * size_t(thirds::tile_bytes(int(lines_of(depth))));
+}
 
 // A product of at most these rows; partial: room for one split tile a CU.
 template <class Of>
-void product_of(Device& d, const half* a, const half* b, int64_t rows_a, int64_t rows_b, int64_t lines, float* partial, const Of& of) {
+void product_of(Device& d, const half* a, const half* b, const half* b_thirds, int64_t rows_a, int64_t rows_b, int64_t lines,
+                float* partial, const Of& of, const Form& form) {
+    constexpr int kLds = std::max(halves::Tile::kLds, thirds::kLds);
     const int64_t blocks = halves::most_blocks(rows_a, rows_b, d.cu_count);
     if (blocks > int64_t(1) << 22) fail(VC_HIP_ERR_OVERFLOW, "linear_cross_entropy: too many tiles");
     static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<Of>),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, halves::Tile::kLds);
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     check_hip(allowed, "hipFuncSetAttribute");
-    launch(product_kernel<Of>, dim3(unsigned(blocks)), dim3(halves::kThreads), uint32_t(halves::Tile::kLds), d.stream, a, b, int(lines),
-           d.cu_count, partial, of);
+    launch(product_kernel<Of>, dim3(unsigned(blocks)), dim3(halves::kThreads), uint32_t(kLds), d.stream, a, b, b_thirds, int(lines),
+           d.cu_count, partial, of, form);
     after_launch("linear_cross_entropy product");
     if (lines < halves::kLeastSplit) return;
     launch(join_kernel<Of>, dim3(unsigned(d.cu_count) * (Of::kElementwise ? 4u : 8u)), dim3(kJoinThreads<Of>), 0, d.stream, d.cu_count,
@@ -1138,21 +1316,23 @@ Packing packing(const float* values, const Piece& of, int64_t rows, int64_t colu
     return Packing{values, of, rows, columns, row_most, column_most, by_row, by_column, int(lines_of(columns)), int(lines_of(rows)),
                    int(down), int(across), nullptr, nullptr, nullptr};
 }
-void pack(Device& d, const Packing& one, const Packing& two) {
-    launch(pack_kernel, grid_2d(one.blocks() + two.blocks()), dim3(kPackThreads), 0, d.stream, one, two);
+void pack(Device& d, const Packing& one, const Packing& two, const Form& form) {
+    launch(pack_kernel, grid_2d(one.blocks() + two.blocks()), dim3(kPackThreads), 0, d.stream, one, two, form);
     after_launch("linear_cross_entropy pack");
 }
 
-Largest largest(const float* values, const float* targets, size_t rows, size_t columns, uint32_t* row_most, uint32_t* column_most,
-                float* cleared) {
+// sums - most: of the arrays' sums and maxima, which lie in the same order.
+Largest largest(const float* values, const float* targets, size_t rows, size_t columns, uint32_t* most, unsigned long long* sums,
+                uint32_t* row_most, uint32_t* column_most, float* cleared) {
+    const auto sums_of = [&](uint32_t* of) { return of ? sums + (of - most) : nullptr; };
     return Largest{values, targets, int64_t(rows), int64_t(columns), int((rows + kMostRows - 1) / kMostRows),
-                   int((columns + kMostColumns - 1) / kMostColumns), row_most, column_most, cleared};
+                   int((columns + kMostColumns - 1) / kMostColumns), row_most, column_most, sums_of(row_most), sums_of(column_most), cleared};
 }
 
 // The packed route. shares: of each row, or null for those of the mean, which goes to share[0]. losses and, of a gradient, any
 // output may be null.
 //
-// A piece's logits and their packed gradients take 4 bytes each a value: 2 GiB and 2 GiB at most, of 288.
+// A piece's logits take 4 bytes a value, their packed gradients 6 and 6: 2 GiB and 6 GiB at most, of 288.
 void packed(Device& d, const Call& c, const float* shares, float* share, float* losses, float* grad_x, float* grad_weight,
             float* grad_bias) {
     const bool gradient = grad_x || grad_weight || grad_bias;
@@ -1162,17 +1342,30 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
     const int64_t piece = whole_tiles((rows + pieces - 1) / pieces);
     const int64_t whole_classes = whole_tiles(classes), parts = 2 * whole_classes / halves::kTile, blocks = piece / kBlockTokens;
 
-    // The largest magnitudes: of W's rows and columns, of x's rows and columns, of the shares.
-    const int64_t n_most = 2 * width + whole_classes + rows;
-    Scratch most(size_t(n_most + 1) * sizeof(uint32_t)), numbers(size_t(rows + 1) * sizeof(int));
-    uint32_t *const w_columns = most.as<uint32_t>(), *const w_rows = w_columns + whole_classes, *const x_columns = w_rows + width;
+    // Of W's rows and columns and x's rows and columns the sums of exponents and the largest magnitudes, behind what they come to,
+    // and the largest of the shares.
+    const int64_t n_most = 2 * width + whole_classes + rows, cleared = 8 + 3 * n_most;  // words
+    static_assert(sizeof(Unlike) <= 8 * sizeof(uint32_t));
+    Scratch most(size_t(cleared + 1) * sizeof(uint32_t)), numbers(size_t(rows + 1) * sizeof(int));
+    Unlike* const unlike = most.as<Unlike>();
+    auto* const exponent_sums = reinterpret_cast<unsigned long long*>(most.as<uint32_t>() + 8);
+    uint32_t* const maxima = most.as<uint32_t>() + 8 + 2 * n_most;
+    uint32_t *const w_columns = maxima, *const w_rows = w_columns + whole_classes, *const x_columns = w_rows + width;
     uint32_t *const x_rows = x_columns + width, *const most_share = x_rows + rows;
     int *const counted = numbers.as<int>(), *const place = counted + 1;
-    count(d, c, shares, counted, share, place, gradient ? most_share : nullptr, losses, most.as<uint32_t>(), n_most);
-    const Largest of_w = largest(c.weight, nullptr, c.width, c.classes, grad_x ? w_rows : nullptr, w_columns, nullptr);
-    const Largest of_x = largest(c.x, c.targets, c.rows, c.width, x_rows, grad_weight ? x_columns : nullptr, grad_x);
-    launch(most_kernel, grid_2d(of_w.blocks() + of_x.blocks()), dim3(256), 0, d.stream, of_w, of_x, classes);
+    count(d, c, shares, counted, share, place, gradient ? most_share : nullptr, losses, most.as<uint32_t>(), cleared);
+    const Largest of_w = largest(c.weight, nullptr, c.width, c.classes, maxima, exponent_sums, grad_x ? w_rows : nullptr, w_columns,
+                                 nullptr);
+    const Largest of_x = largest(c.x, c.targets, c.rows, c.width, maxima, exponent_sums, x_rows, grad_weight ? x_columns : nullptr,
+                                 grad_x);
+    launch(most_kernel, grid_2d(of_w.blocks() + of_x.blocks()), dim3(256), 0, d.stream, of_w, of_x, classes, unlike);
     after_launch("linear_cross_entropy largest");
+    launch(unlike_kernel, dim3(grid_1d(size_t(n_most), 256, 256)), dim3(256), 0, d.stream, static_cast<const uint32_t*>(maxima),
+           static_cast<const unsigned long long*>(exponent_sums), whole_classes, width, rows, unlike);
+    after_launch("linear_cross_entropy unlike");
+    int width_bits = 0;
+    while ((int64_t(1) << width_bits) < width) ++width_bits;
+    const Form form{unlike, width_bits};
     Scratch of_class(size_t(2 * whole_classes) * sizeof(float));
     int* const exponents = of_class.as<int>();
     float* const bias = of_class.as<float>() + whole_classes;
@@ -1185,6 +1378,7 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
 
     Scratch x(packed_bytes(piece, width)), xt(grad_weight ? packed_bytes(width, piece) : 4);
     Scratch logits(gradient ? size_t(whole_classes * piece) * sizeof(float) : 4), z(grad_x ? packed_bytes(piece, classes) : 4);
+    Scratch zt(gradient ? packed_bytes(classes, piece) : 4);
     Scratch statistics(size_t(2 * parts + 2) * size_t(piece) * sizeof(float)), tokens(size_t(piece) * sizeof(Token));
     Scratch class_most(gradient ? size_t(blocks * whole_classes) * sizeof(uint32_t) : 4);
     Scratch sums(grad_bias ? size_t(pieces * blocks * classes) * sizeof(double) : 4);
@@ -1195,11 +1389,12 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
     for (int64_t p = 0; p < pieces; ++p) {
         const Piece of{counted, place, p * piece, piece};
         const Packing of_rows = packing(c.x, of, piece, width, x_rows, x_columns, x.as<half>(), grad_weight ? xt.as<half>() : nullptr);
-        pack(d, of_rows, p == 0 ? of_weight : Packing{});
+        pack(d, of_rows, p == 0 ? of_weight : Packing{}, form);
         const auto z_of = [&](auto store) {
-            product_of(d, wt.as<half>(), x.as<half>(), classes, piece, lines_of(width), partial.as<float>(),
+            product_of(d, wt.as<half>(), x.as<half>(), x.as<half>(), classes, piece, lines_of(width), partial.as<float>(),
                        Logits<store()>{of, exponents, x_rows, bias, c.targets, logits.as<float>(), part_most, part_sum, at_target, classes,
-                                       piece, int(lines_of(width))});
+                                       piece, int(lines_of(width))},
+                       form);
         };
         gradient ? z_of(std::true_type{}) : z_of(std::false_type{});
         launch(token_kernel, dim3(unsigned(piece / 64)), dim3(64 * kTokenWaves), 0, d.stream, of, part_most, part_sum, at_target, c.targets,
@@ -1209,16 +1404,17 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
         const auto gradients = grad_bias ? gradients_kernel<true> : gradients_kernel<false>;
         launch(gradients, grid_2d(size_t(blocks * lines_of(classes))), dim3(256), 0, d.stream, logits.as<float>(), piece, of,
                tokens.as<Token>(), own_shares, most_share, classes, whole_classes, class_most.as<uint32_t>(),
-               grad_x ? z.as<half>() : nullptr, int(lines_of(classes)), sums.as<double>() + (grad_bias ? p * blocks * classes : 0),
-               int(blocks));
+               grad_x ? z.as<half>() : nullptr, zt.as<half>(), int(lines_of(classes)),
+               sums.as<double>() + (grad_bias ? p * blocks * classes : 0), int(blocks), form);
         after_launch("linear_cross_entropy gradients");
         if (grad_x)
-            product_of(d, z.as<half>(), w.as<half>(), piece, width, lines_of(classes), partial.as<float>(),
-                       InputGradient{of, tokens.as<Token>(), w_rows, own_shares, grad_x, width, int(lines_of(classes))});
+            product_of(d, z.as<half>(), w.as<half>(), w.as<half>(), piece, width, lines_of(classes), partial.as<float>(),
+                       InputGradient{of, tokens.as<Token>(), w_rows, own_shares, grad_x, width, int(lines_of(classes))}, form);
         if (grad_weight)
-            product_of(d, xt.as<half>(), logits.as<half>(), width, classes, piece / halves::kSlice, partial.as<float>(),
+            product_of(d, xt.as<half>(), logits.as<half>(), zt.as<half>(), width, classes, piece / halves::kSlice, partial.as<float>(),
                        WeightGradient{of, x_columns, class_most.as<uint32_t>(), most_share, grad_weight, width, classes, whole_classes,
-                                      p > 0});
+                                      p > 0},
+                       form);
     }
     if (grad_bias) {
         launch(red::column_partials_kernel, dim3(unsigned((classes + 63) / 64)), dim3(64 * red::kCombineWaves), 0, d.stream,
@@ -1254,6 +1450,7 @@ bool takes_few(const Call& c) { return c.rows <= kFewMost; }
 // 96 x 10000: 386 (429), 375 (374); 16384, 256 x 1000: 275 (333), 236 (241).
 bool takes_packed(const Call& c, int products, bool grad_bias) {
     if (c.classes >= (size_t(1) << 21) || c.width >= (size_t(1) << 21)) return false;  // a load's offset has 31 bits
+    if (c.rows >= kMostCounted) return false;
     const double n = double(c.rows), weights = double(c.width) * double(c.classes), logits = n * double(c.classes);
     const bool gradient = products > 1, aligned = c.width % 4 == 0 && c.classes % 4 == 0;
     const double direct = (gradient ? 20.0 : 10.0) + 2e-6 * products * n * weights / (aligned ? 105.0 : 66.0) +
