@@ -137,3 +137,13 @@ def test_upstream_gradients_of_any_size(rows, width, classes, scale, device):
     x, w, t, b = raw(rows, width, classes, 1e9)
     dy = (scale * np.random.default_rng(rows).random(rows)).astype(np.float32)
     check(x, w, t, b, device, dy=dy)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows,width,classes", SIZES)
+def test_left_out_rows_beside_an_infinite_weight(rows, width, classes, device):
+    """Their gradient is zero, where a product of zeros and the weight would be NaN."""
+    x, w, t, b = problem(rows, width, classes, seed=10, left_out=0.5)
+    w[3, 5], t[0] = -np.inf, -1
+    _, dx, _, _ = run(x, w, t, b, device, "none", np.ones(rows, np.float32))
+    assert (dx[t < 0] == 0).all()
