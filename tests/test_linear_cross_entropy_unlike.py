@@ -140,6 +140,58 @@ def test_upstream_gradients_of_any_size(rows, width, classes, scale, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows,width,classes", SIZES + [(513, 1030, 6007)])
+def test_a_weight_of_minus_infinity(rows, width, classes, device):
+    """A constant feature whose weights of minus infinity take every third class out. That feature's own gradient is a sum of
+    zeros times infinities, NaN; everything else is as without those classes."""
+    if device == "cpu" and rows > 1000:
+        rows, width, classes = 40, 100, 700
+    x, w, t, b = problem(rows, width, classes, seed=8)
+    x[:, 2] = 0.5
+    out = np.arange(0, classes, 3)
+    w[2, out] = -np.inf
+    t = np.where(t % 3 == 0, 1, t)
+    keep = np.setdiff1d(np.arange(classes), out)
+    want, off = exact(x, w[:, keep], np.where(t >= 0, np.searchsorted(keep, t), -1), b[keep], 1.0)
+    each = vc.linear_cross_entropy(*(vc.Tensor(v, device=device) for v in (x, w)), t, bias=vc.Tensor(b, device=device), reduction="none")
+    close(each.numpy(), want["loss"], off["loss"])
+    loss, dx, dw, db = run(x, w, t, b, device, "none", np.ones(rows, np.float32))
+    close(loss, want["loss"], off["loss"])
+    counts = t >= 0
+    assert np.isnan(dx[counts, 2]).all() and (dx[~counts] == 0).all()
+    others = np.delete(np.arange(width), 2)
+    close(dx[:, others], want["dx"][:, others], off["dx"][:, others])
+    close(dw[:, keep], want["dw"], off["dw"])
+    close(db[keep], want["db"], off["db"])
+    assert (dw[:, out] == 0).all() and (db[out] == 0).all()
+    t[0] = 0  # a class without a chance
+    each = vc.linear_cross_entropy(*(vc.Tensor(v, device=device) for v in (x, w)), t, bias=vc.Tensor(b, device=device),
+                                   reduction="none").numpy()
+    assert np.isposinf(each[0]) and np.isfinite(each[1:]).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows,width,classes", SIZES)
+def test_infinite_logits_are_nan_in_their_rows_alone(rows, width, classes, device):
+    """A logit of plus infinity has no loss; a row's infinity is its own."""
+    x, w, t, b = problem(rows, width, classes, seed=9, left_out=0)
+    scores = lambda x, w: vc.linear_cross_entropy(*(vc.Tensor(v, device=device) for v in (x, w)), t, reduction="none").numpy()
+    clean = exact(x, w, t, None, 1.0)
+    dirty = x.copy()
+    dirty[1, 4], dirty[3, 0] = np.inf, -np.inf
+    each = scores(dirty, w)
+    assert np.isnan(each[[1, 3]]).all()
+    close(np.delete(each, [1, 3]), np.delete(clean[0]["loss"], [1, 3]), np.delete(clean[1]["loss"], [1, 3]))
+    above = x[:, 6] > 0
+    w[6, 3] = np.inf
+    t[t == 3] = 4
+    each, keep = scores(x, w), np.delete(np.arange(classes), 3)
+    want, off = exact(x, w[:, keep], np.searchsorted(keep, t), None, 1.0)
+    assert np.isnan(each[above]).all()  # plus infinity; minus infinity below zero
+    close(each[~above], want["loss"][~above], off["loss"][~above])
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("rows,width,classes", SIZES)
 def test_left_out_rows_beside_an_infinite_weight(rows, width, classes, device):
     """Their gradient is zero, where a product of zeros and the weight would be NaN."""

@@ -803,6 +803,9 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
 
 // z^T: scaled back, with the bias, stored for a gradient (Store); and of each 128 classes of a token the maximum, the sum of the
 // exponentials over it but the target's, and the target's logit. exponents, bias and out reach to the end of the last tile.
+//
+// A sum that holds an infinity or a NaN is lost to the parts (infinity minus infinity): it is made again value by value, so a
+// class whose weight is minus infinity has no chance, as in the other routes.
 template <bool Store>
 struct Logits {
     static constexpr bool kElementwise = false, kUnits = false;
@@ -813,16 +816,40 @@ struct Logits {
     float *out, *most, *sum, *at_target;
     int64_t classes, stride;
     int lines;
+    const float *x, *weight;
+    int64_t width;
+    Form form;
     __device__ inline int64_t rows_a() const { return classes; }
     __device__ inline int64_t rows_b() const { return piece.tokens(); }
     __device__ inline int depth() const { return lines; }
     __device__ inline bool idle() const { return false; }
+    // Class v's logit of token t, without the bias.
+    __device__ inline float again(int64_t v, int64_t t) const {
+        const float *const row = x + piece.row(t) * width, *column = weight + v;
+        float s = 0.0f;
+        int64_t k = 0;
+        for (; k + 8 <= width && s == s; k += 8) {
+            float a[8], b[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[i] = row[k + i];
+                b[i] = column[(k + i) * classes];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s = __builtin_fmaf(a[i], b[i], s);
+        }
+        if (s != s) return s;
+        for (; k < width; ++k) s = __builtin_fmaf(row[k], column[k * classes], s);
+        return s;
+    }
+    static __device__ inline bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
     // Of wave `wave` of a tile: its blocks of 32 columns from block `first`.
     template <int Blocks>
     __device__ inline void operator()(const halves::f16v (&acc)[4][Blocks], int m, int n, int wave, int first) const {
         const int lane = threadIdx.x % 64, column = 64 * (wave % 4) + 32 * first + lane % 32;
         const int64_t v0 = int64_t(m) * halves::kTile, t0 = int64_t(n) * halves::kTile + column;
         const int64_t tokens = piece.tokens();
+        const bool thirds = form.thirds();
         const int row0 = 128 * (wave / 4) + 4 * (lane / 32);
         float top[Blocks], others[Blocks];
         int e_token[Blocks], target[Blocks];  // the target's row in this tile
@@ -864,9 +891,31 @@ struct Logits {
                 int own = target[b] - row0 - r0;  // the target's among these rows, if it is
                 float z[16], high = top[b], found = 0.0f;
 #pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] = __builtin_amdgcn_ldexpf(acc[a][b][i], -(e[i] + e_token[b])) + add[i];
+                if (thirds) {
+                    bool lost = false;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) lost |= !finite(acc[a][b][i]);
+                    if (lost) {
+#pragma unroll 1
+                        for (int l = 0; l < 16; ++l) {
+                            float sum = 0.0f, more = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                sum = l == i ? acc[a][b][i] : sum;
+                                more = l == i ? add[i] : more;
+                            }
+                            if (finite(sum)) continue;
+                            const int64_t v = v0 + row0 + r0 + 8 * (l / 4) + l % 4, t = t0 + 32 * b;
+                            const float logit = (v < classes && t < tokens ? again(v, t) : 0.0f) + more;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) z[i] = l == i ? logit : z[i];
+                        }
+                    }
+                }
+#pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int r = 8 * (i / 4) + i % 4;
-                    z[i] = __builtin_amdgcn_ldexpf(acc[a][b][i], -(e[i] + e_token[b])) + add[i];
                     if constexpr (Store)
                         __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, z[i]), rows, at + 128u * b,
                                                               uint32_t(r0 + r) * row_bytes, 0);
@@ -1408,7 +1457,7 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
         const auto z_of = [&](auto store) {
             product_of(d, wt.as<half>(), x.as<half>(), x.as<half>(), classes, piece, lines_of(width), partial.as<float>(),
                        Logits<store()>{of, exponents, x_rows, bias, c.targets, logits.as<float>(), part_most, part_sum, at_target, classes,
-                                       piece, int(lines_of(width))},
+                                       piece, int(lines_of(width)), c.x, c.weight, width, form},
                        form);
         };
         gradient ? z_of(std::true_type{}) : z_of(std::false_type{});
