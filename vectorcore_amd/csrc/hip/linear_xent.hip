@@ -694,7 +694,7 @@ __device__ inline int class_exponent(uint32_t most, uint32_t most_share) {
 constexpr int kGradientStride = kBlockTokens + 2;  // four threads that read eight classes of a token each meet different banks
 
 // The gradients dz^T of a piece from its logits z^T [classes, stride]: times the tokens' shares, packed along the tokens, in
-// their place (three parts: into by_class, in the unit of the largest share); and for shares of one packed along the classes
+// their place (three parts: into by_class, or null, in the unit of the largest share); and for shares of one packed along the classes
 // (by_token, or null). most [blocks][whole classes]: the largest of
 // each class, as bits. Sums: of each class, into sums [blocks][classes]. A workgroup takes 32 classes and a block of tokens;
 // four lanes of a wavefront read a line of the logits, and then write it.
@@ -764,7 +764,7 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
         }
         if (!there) continue;
         if (thirds) {
-            thirds::store8(by_class, int(stride / halves::kSlice), v, (t0 + c) / 8, d, halves::exponent_of(top));
+            if (by_class) thirds::store8(by_class, int(stride / halves::kSlice), v, (t0 + c) / 8, d, halves::exponent_of(top));
         } else {
             h8 first, second;
             halves::split8(d, class_exponent(high, top), first, second);
@@ -986,6 +986,24 @@ __global__ __launch_bounds__(64 * kTokenWaves) void token_kernel(Piece piece, co
     if (!out) return;
     out[t] = Token{top, float(1.0 / total), float(others / total), int(class_of(targets[row], classes))};
     own_shares[t] = shares[one_share ? 0 : row];
+}
+
+// total[c] = what the pieces before left there, but for the first one, plus the piece's blocks; out: of the last one, or null.
+__global__ __launch_bounds__(64 * red::kCombineWaves) void bias_kernel(const double* __restrict__ sums, int64_t blocks, int64_t classes,
+                                                                       bool first, double* __restrict__ total, float* __restrict__ out) {
+    __shared__ double of_wave[red::kCombineWaves][64];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int64_t c = int64_t(blockIdx.x) * 64 + lane;
+    double acc[1] = {0.0};
+    if (c < classes) red::combine_waves<1>(sums, blocks, classes, c, wave, 0, acc);
+    of_wave[wave][lane] = acc[0];
+    __syncthreads();
+    if (wave != 0 || c >= classes) return;
+    double sum = of_wave[0][lane];
+    for (int w = 1; w < red::kCombineWaves; ++w) sum += of_wave[w][lane];
+    if (!first) sum += total[c];
+    if (out) out[c] = float(sum);
+    else total[c] = sum;
 }
 
 // dx [rows, width], times the tokens' shares.
@@ -1396,15 +1414,16 @@ Largest largest(const float* values, const float* targets, size_t rows, size_t c
 // The packed route. shares: of each row, or null for those of the mean, which goes to share[0]. losses and, of a gradient, any
 // output may be null.
 //
-// A piece's logits take 4 bytes a value, their packed gradients 6 and 6: 2 GiB and 6 GiB at most, of 288.
+// A piece's logits take 4 bytes a value, their packed gradients 6 for each of x and W: 2 GiB and 6 GiB at most, of 288.
 void packed(Device& d, const Call& c, const float* shares, float* share, float* losses, float* grad_x, float* grad_weight,
             float* grad_bias) {
     const bool gradient = grad_x || grad_weight || grad_bias;
     const int64_t width = int64_t(c.width), classes = int64_t(c.classes), rows = int64_t(c.rows);
-    const int64_t fitting = gradient ? std::max<int64_t>(1, (int64_t(1) << 29) / classes / halves::kTile) * halves::kTile : 65536;
+    const int64_t whole_classes = whole_tiles(classes);
+    const int64_t fitting = gradient ? (int64_t(1) << 29) / whole_classes / halves::kTile * halves::kTile : 65536;  // classes < 2^21
     const int64_t most_rows = std::min<int64_t>(fitting, 65536), pieces = (rows + most_rows - 1) / most_rows;
     const int64_t piece = whole_tiles((rows + pieces - 1) / pieces);
-    const int64_t whole_classes = whole_tiles(classes), parts = 2 * whole_classes / halves::kTile, blocks = piece / kBlockTokens;
+    const int64_t parts = 2 * whole_classes / halves::kTile, blocks = piece / kBlockTokens;
 
     // Of W's rows and columns and x's rows and columns the sums of exponents and the largest magnitudes, behind what they come to,
     // and the largest of the shares.
@@ -1442,10 +1461,11 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
 
     Scratch x(packed_bytes(piece, width)), xt(grad_weight ? packed_bytes(width, piece) : 4);
     Scratch logits(gradient ? size_t(whole_classes * piece) * sizeof(float) : 4), z(grad_x ? packed_bytes(piece, classes) : 4);
-    Scratch zt(gradient ? packed_bytes(classes, piece) : 4);
+    Scratch zt(grad_weight ? packed_bytes(classes, piece) : 4);
     Scratch statistics(size_t(2 * parts + 2) * size_t(piece) * sizeof(float)), tokens(size_t(piece) * sizeof(Token));
     Scratch class_most(gradient ? size_t(blocks * whole_classes) * sizeof(uint32_t) : 4);
-    Scratch sums(grad_bias ? size_t(pieces * blocks * classes) * sizeof(double) : 4);
+    Scratch sums(grad_bias ? size_t((blocks + 1) * classes) * sizeof(double) : 4);
+    double* const bias_total = sums.as<double>() + blocks * classes;
     Scratch partial(size_t(d.cu_count) * halves::Tile::kValues * halves::kThreads * sizeof(float));
     float *const part_most = statistics.as<float>(), *const part_sum = part_most + parts * piece;
     float *const at_target = part_sum + parts * piece, *const own_shares = at_target + piece;
@@ -1468,9 +1488,14 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
         const auto gradients = grad_bias ? gradients_kernel<true> : gradients_kernel<false>;
         launch(gradients, grid_2d(size_t(blocks * lines_of(classes))), dim3(256), 0, d.stream, logits.as<float>(), piece, of,
                tokens.as<Token>(), own_shares, most_share, classes, whole_classes, class_most.as<uint32_t>(),
-               grad_x ? z.as<half>() : nullptr, zt.as<half>(), int(lines_of(classes)),
-               sums.as<double>() + (grad_bias ? p * blocks * classes : 0), int(blocks), form);
+               grad_x ? z.as<half>() : nullptr, grad_weight ? zt.as<half>() : nullptr, int(lines_of(classes)),
+               sums.as<double>(), int(blocks), form);
         after_launch("linear_cross_entropy gradients");
+        if (grad_bias) {
+            launch(bias_kernel, dim3(unsigned((classes + 63) / 64)), dim3(64 * red::kCombineWaves), 0, d.stream,
+                   static_cast<const double*>(sums.as<double>()), blocks, classes, p == 0, bias_total, p + 1 == pieces ? grad_bias : nullptr);
+            after_launch("linear_cross_entropy bias");
+        }
         if (grad_x)
             product_of(d, z.as<half>(), w.as<half>(), w.as<half>(), piece, width, lines_of(classes), partial.as<float>(),
                        InputGradient{of, tokens.as<Token>(), w_rows, own_shares, grad_x, width, int(lines_of(classes))}, form);
@@ -1479,11 +1504,6 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
                        WeightGradient{of, x_columns, class_most.as<uint32_t>(), most_share, grad_weight, width, classes, whole_classes,
                                       p > 0},
                        form);
-    }
-    if (grad_bias) {
-        launch(red::column_partials_kernel, dim3(unsigned((classes + 63) / 64)), dim3(64 * red::kCombineWaves), 0, d.stream,
-               sums.as<double>(), pieces * blocks, classes, grad_bias);
-        after_launch("linear_cross_entropy bias");
     }
 }
 
