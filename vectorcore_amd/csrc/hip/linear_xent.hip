@@ -13,8 +13,9 @@
 //
 // Rows are taken in pieces: the logits of a piece live in a workspace until
 // their gradients are used. Three routes, by sizes alone:
-// - up to 16 rows without gradients read W once and keep no logits; bound by HBM
-//   (1 row, 1024 x 50000: 37 us of 205 MB, 5.5 TB/s, and 4 us to join);
+// - up to 16 rows of many classes without gradients read W once and keep no
+//   logits; bound by HBM (1 row, 1024 x 50000: 37 us of 205 MB, 5.5 TB/s, and 4 us
+//   to join);
 // - small or thin calls take float32 products and a kernel of the rows; bound by
 //   launches (256 rows, 256 x 10 with gradients: 25 us in five);
 // - others take packed products, bound by matrix instructions: 8192 rows, 1024 x
@@ -1160,6 +1161,7 @@ __global__ __launch_bounds__(kJoinThreads<Of>) void join_kernel(int places, cons
 // what its rows' logits come to there is left as in the packed route, and joined by a second launch.
 
 constexpr int kRowThreads = 256, kFewMost = 16, kFewWaves = 8, kFewClasses = 128, kFewLoads = 16;
+constexpr int kFewFeatures = kFewWaves * kFewLoads;  // of a workgroup's turn
 
 template <int Rows>
 __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const float* __restrict__ x, const float* __restrict__ weight,
@@ -1182,7 +1184,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const float* _
         }
     };
     typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
-    for (int64_t k = kFewLoads * wave; k < width; k += kFewLoads * kFewWaves) {
+    for (int64_t k = kFewLoads * wave; k < width; k += kFewFeatures) {
         if (k + kFewLoads <= width) {
             f2u w[kFewLoads];
 #pragma unroll
@@ -1524,7 +1526,18 @@ void few_rows(Device& d, const Call& c, float* losses) {
     after_launch("linear_cross_entropy few rows");
 }
 
-bool takes_few(const Call& c) { return c.rows <= kFewMost; }
+// Whether reading the weight once for a few rows pays, by estimates of this route's time and that of float32 products in us. A
+// workgroup walks all features of its 128 classes, 128 features in 1.6 us or more, so few classes leave most CUs idle for long.
+// Measured, this route and products: 1 row, 1024 x 50000: 39, 56 us; 1024 x 16000: 16, 21; 1024 x 4000: 18, 13; 4096 x 10: 51, 10;
+// 65536 x 10: 740, 19. 8 rows, 1024 x 50000: 44, 57; 512 x 16000: 15.7, 16.0; 128 x 400: 8.9, 9.7; 2048 x 1000: 41, 11. 16 rows,
+// 512 x 50000: 37, 39; 1024 x 50000: 62, 57; 16 x 128: 9.8, 8.2.
+bool takes_few(const Device& d, const Call& c) {
+    if (c.rows > kFewMost) return false;
+    const double rows = double(c.rows), bytes = 4.0 * double(c.width) * double(c.classes);
+    const double groups = double((c.classes + kFewClasses - 1) / kFewClasses), turns = double((c.width + kFewFeatures - 1) / kFewFeatures);
+    const double few = 5.5 + std::max(bytes / 5.5e6, turns * (1.6 + 0.009 * rows * rows) * std::max(1.0, groups / double(d.cu_count)));
+    return few < 0.9 * (9.0 + bytes / 5.0e6 + 1.2e-4 * double(c.classes));
+}
 
 // Whether packing pays: by estimates of both routes' times in us, for `products` products of the call's sizes (one, or up to three
 // with gradients). Measured (estimated), direct and packed, in us: losses alone of 128 rows, 1024 x 50000: 177 (144), 221 (219);
@@ -1566,12 +1579,13 @@ int vc_hip_linear_xent_forward(const float* x, const float* weight, const float*
         if (!losses && !mean) return;
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy", products, 4.0 * double(width) * double(rows + classes));
-        if (!takes_few(c) && !takes_packed(c, 1, false)) {
+        const bool few = takes_few(d, c);
+        if (!few && !takes_packed(c, 1, false)) {
             direct(d, c, nullptr, losses, mean, nullptr, nullptr, nullptr);
         } else {
             Scratch own(losses ? 4 : rows * sizeof(float)), share(sizeof(float));
             if (!losses) losses = own.as<float>();
-            if (takes_few(c)) {
+            if (few) {
                 few_rows(d, c, losses);
                 if (mean) count(d, c, nullptr, nullptr, share.as<float>(), nullptr, nullptr, nullptr);
             } else {
