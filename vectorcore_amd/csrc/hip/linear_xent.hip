@@ -637,44 +637,43 @@ __global__ __launch_bounds__(256) void most_kernel(Largest one, Largest two, int
 }
 
 // The most unlike rows, of maxima and sums in the order W's columns (whole_classes of them), W's rows (width), x's columns
-// (width), x's rows; what most_kernel was not asked for is zeros.
+// (width), x's rows, which are blockIdx.y in this order; what most_kernel was not asked for is zeros.
 __global__ __launch_bounds__(256) void unlike_kernel(const uint32_t* __restrict__ most, const unsigned long long* __restrict__ sums,
                                                      int64_t whole_classes, int64_t width, int64_t rows, Unlike* __restrict__ unlike) {
-    int gaps[4] = {0, 0, 0, 0}, high[4] = {0, 0, 0, 0};
-    const int64_t n = whole_classes + 2 * width + rows;
+    __shared__ int of_wave[4][2];
+    const int group = blockIdx.y, lane = threadIdx.x % 64;
+    const int64_t first = group == 0 ? 0 : whole_classes + (group - 1) * width, n = group == 0 ? whole_classes : group == 3 ? rows : width;
+    if (int64_t(blockIdx.x) * 256 >= n) return;
+    int found[2] = {0, 0};  // the gap, the exponent
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
-        const unsigned long long of = sums[i];
-        const uint64_t values = of >> kCountShift, sum = of & ((1ull << kCountShift) - 1);
-        if (!values) continue;
-        const int exponent = exponent_over(__builtin_bit_cast(float, most[i]));
-        const int gap = int(((uint64_t(exponent) * values - sum) * 16 + values - 1) / values);
-        const int group = i < whole_classes ? 0 : i < whole_classes + width ? 1 : i < whole_classes + 2 * width ? 2 : 3;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            gaps[g] = group == g ? max(gaps[g], gap) : gaps[g];
-            high[g] = group == g ? max(high[g], exponent) : high[g];
-        }
+        const unsigned long long of = sums[first + i];
+        const float values = float(of >> kCountShift);
+        if (values == 0.0f) continue;
+        const int exponent = exponent_over(__builtin_bit_cast(float, most[first + i]));
+        // The mean is off by 2^-14 at most, a sixteenth is the unit.
+        const float mean = float(of & ((1ull << kCountShift) - 1)) / values;
+        found[0] = max(found[0], int(ceilf((float(exponent) - mean) * 16.0f + 0.01f)));
+        found[1] = max(found[1], exponent);
     }
-    __shared__ int of_wave[4][6];
-    const int lane = threadIdx.x % 64;
-    const int found[6] = {gaps[0], gaps[1], gaps[2], gaps[3], high[0], high[3]};
 #pragma unroll
-    for (int i = 0; i < 6; ++i) {
+    for (int i = 0; i < 2; ++i) {
         int v = found[i];
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) v = max(v, __shfl_xor(v, d, 64));
+        v = max(v, red::partner<0>(v, lane));
+        v = max(v, red::partner<1>(v, lane));
+        v = max(v, red::partner<2>(v, lane));
+        v = max(v, red::partner<3>(v, lane));
+        v = max(v, red::partner<4>(v, lane));
+        v = max(v, red::partner<5>(v, lane));
         if (lane == 0) of_wave[threadIdx.x / 64][i] = v;
     }
     __syncthreads();
-    if (threadIdx.x >= 6) return;
-    int* const to[6] = {&unlike->w_columns, &unlike->w_rows, &unlike->x_columns, &unlike->x_rows, &unlike->w_most, &unlike->x_most};
-    int v = 0;
-    for (int w = 0; w < 4; ++w) v = max(v, of_wave[w][threadIdx.x]);
-    int* at = to[0];
-#pragma unroll
-    for (int i = 1; i < 6; ++i) at = int(threadIdx.x) == i ? to[i] : at;
+    if (threadIdx.x >= 2) return;
+    int* const gap = group == 0 ? &unlike->w_columns : group == 1 ? &unlike->w_rows : group == 2 ? &unlike->x_columns : &unlike->x_rows;
+    int* const to = threadIdx.x == 0 ? gap : group == 0 ? &unlike->w_most : group == 3 ? &unlike->x_most : nullptr;
+    if (!to) return;
+    const int v = max(max(of_wave[0][threadIdx.x], of_wave[1][threadIdx.x]), max(of_wave[2][threadIdx.x], of_wave[3][threadIdx.x]));
     // Most workgroups find nothing more: a look costs less than the atomic.
-    if (v > __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(at, v);
+    if (v > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(to, v);
 }
 
 // What a token's gradients are made of, from its logits' statistics.
@@ -1445,7 +1444,7 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
                                  grad_x);
     launch(most_kernel, grid_2d(of_w.blocks() + of_x.blocks()), dim3(256), 0, d.stream, of_w, of_x, classes, unlike);
     after_launch("linear_cross_entropy largest");
-    launch(unlike_kernel, dim3(grid_1d(size_t(n_most), 256, 256)), dim3(256), 0, d.stream, static_cast<const uint32_t*>(maxima),
+    launch(unlike_kernel, dim3(grid_1d(size_t(std::max({whole_classes, width, rows})), 256, 256), 4), dim3(256), 0, d.stream, static_cast<const uint32_t*>(maxima),
            static_cast<const unsigned long long*>(exponent_sums), whole_classes, width, rows, unlike);
     after_launch("linear_cross_entropy unlike");
     int width_bits = 0;
@@ -1540,23 +1539,25 @@ bool takes_few(const Device& d, const Call& c) {
 }
 
 // Whether packing pays: by estimates of both routes' times in us, for `products` products of the call's sizes (one, or up to three
-// with gradients). Measured (estimated), direct and packed, in us: losses alone of 128 rows, 1024 x 50000: 177 (144), 221 (219);
-// of 256: 284 (279), 220 (219); 999, 515 x 10007: 158 (181), 75 (83); 4096, 256 x 1000: 41 (36), 48 (50); 2048, 512 x 2048: 53
-// (57), 59 (57). Train steps of 128 rows, 1024 x 50000: 462 (423), 576 (560); of 256: 771 (827), 628 (580); 2048, 1024 x 1024: 152
-// (152), 158 (156); 3145, 18 x 25838: 505 (519), 656 (613), with a bias, a tenth of the rows left out, 658 (673), 588 (613); 4096,
-// 96 x 10000: 386 (429), 375 (374); 16384, 256 x 1000: 275 (333), 236 (241).
-bool takes_packed(const Call& c, int products, bool grad_bias) {
+// with gradients; the bias's gradient alone takes one). Measured (estimated), direct and packed, in us: losses alone of 128 rows,
+// 1024 x 50000: 163 (144), 235 (224); of 256: 259 (279), 232 (224); 999, 515 x 10007: 162 (181), 78 (90); 4096, 256 x 1000: 43 (36),
+// 50 (55); 2048, 512 x 2048: 57 (57), 61 (63). Train steps of 128 rows, 1024 x 50000: 460 (423), 592 (556); of 256: 773 (827), 628
+// (576); 2048, 1024 x 1024: 162 (152), 148 (152); 3145, 18 x 25838: 489 (519), 637 (610), with a bias, a tenth of the rows left out,
+// 659 (673), 595 (610); 4096, 96 x 10000: 386 (429), 365 (370); 16384, 256 x 1000: 283 (333), 237 (238). The gradient of x alone, 256
+// rows, 1024 x 50000: 522 (558), 446 (418); of the weight alone, 4096, 96 x 10000: 283 (293), 220 (264); of the bias alone, 4096, 96
+// x 10000: 246 (234), 157 (160); 2048, 512 x 2048: 78 (75), 82 (84); 8192, 1024 x 5000: 885 (958), 386 (406).
+bool takes_packed(const Call& c, bool gradient, int products, bool grad_bias) {
     if (c.classes >= (size_t(1) << 21) || c.width >= (size_t(1) << 21)) return false;  // a load's offset has 31 bits
     if (c.rows >= kMostCounted) return false;
     const double n = double(c.rows), weights = double(c.width) * double(c.classes), logits = n * double(c.classes);
-    const bool gradient = products > 1, aligned = c.width % 4 == 0 && c.classes % 4 == 0;
+    const bool aligned = c.width % 4 == 0 && c.classes % 4 == 0;
     const double direct = (gradient ? 20.0 : 10.0) + 2e-6 * products * n * weights / (aligned ? 105.0 : 66.0) +
                           (1.5e-6 * products + (grad_bias ? 1.9e-6 : 0.0)) * logits;
     // The features are a depth of whole lines in the logits, and whole tiles in the gradients' products.
     const double features = 32.0 * double(lines_of(int64_t(c.width))) + (products - 1) * double(whole_tiles(int64_t(c.width)));
     const double tiles = double(whole_tiles(int64_t(c.rows))) * double(whole_tiles(int64_t(c.classes))) * features;
-    const double packing = (gradient ? 4.2e-6 : 2.0e-6) * (weights + n * double(c.width));
-    return direct > (gradient ? 100.0 : 41.0) + packing + 2e-6 * tiles / 350.0 + (gradient ? 3.0e-6 : 0.0) * logits;
+    const double packing = (0.9e-6 + 1.1e-6 * products) * (weights + n * double(c.width));
+    return direct > (gradient ? 42.0 + 18.0 * products + (1.2e-6 + 0.6e-6 * products) * logits : 46.0) + packing + 2e-6 * tiles / 350.0;
 }
 
 }  // namespace
@@ -1580,7 +1581,7 @@ int vc_hip_linear_xent_forward(const float* x, const float* weight, const float*
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy", products, 4.0 * double(width) * double(rows + classes));
         const bool few = takes_few(d, c);
-        if (!few && !takes_packed(c, 1, false)) {
+        if (!few && !takes_packed(c, false, 1, false)) {
             direct(d, c, nullptr, losses, mean, nullptr, nullptr, nullptr);
         } else {
             Scratch own(losses ? 4 : rows * sizeof(float)), share(sizeof(float));
@@ -1614,7 +1615,8 @@ int vc_hip_linear_xent_gradient(const float* x, const float* weight, const float
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy_gradient", products * (1.0 + (grad_x != nullptr) + (grad_weight != nullptr)),
                    8.0 * double(width) * double(rows + classes));
-        if (takes_packed(c, 1 + (grad_x != nullptr) + (grad_weight != nullptr), grad_bias != nullptr)) {
+        const bool gradient = grad_x || grad_weight || grad_bias;
+        if (takes_packed(c, gradient, 1 + (grad_x != nullptr) + (grad_weight != nullptr), grad_bias != nullptr)) {
             Scratch share(sizeof(float)), losses(mean ? rows * sizeof(float) : 4);
             packed(d, c, shares, share.as<float>(), mean ? losses.as<float>() : nullptr, grad_x, grad_weight, grad_bias);
             if (mean) mean_of(d, c, losses.as<float>(), share.as<float>(), mean);
