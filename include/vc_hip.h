@@ -527,7 +527,8 @@ int vc_hip_dropout(const float* x, const float* residual, size_t count, double p
 int vc_hip_linear_xent_forward(const float* x, const float* weight, const float* bias, const float* targets, size_t rows,
                                size_t width, size_t classes, float* losses, float* mean);
 /* The gradients of sum_t shares[t] loss_t; each may be NULL. shares NULL: those of the mean loss, which then goes to
- * mean (or NULL). A row that is left out has a gradient of zero and no part in the others. */
+ * mean (or NULL). A row that is left out has a gradient of zero and no part in the others, whatever it holds; where a
+ * feature has an infinite weight, that feature's gradient may be zero times infinity, NaN, of any row. */
 int vc_hip_linear_xent_gradient(const float* x, const float* weight, const float* bias, const float* targets,
                                 const float* shares, size_t rows, size_t width, size_t classes, float* mean,
                                 float* grad_x, float* grad_weight, float* grad_bias);

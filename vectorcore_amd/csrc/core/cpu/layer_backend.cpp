@@ -191,10 +191,6 @@ void linear_xent(const LinearLoss& call, const float* shares, bool one_share, fl
                 }
             });
         }
-        if (grad_x)  // zero times an infinity of the weight is not zero
-            for (std::size_t r = 0; r < n; ++r)
-                if (class_of(call.targets[first + r], classes) == classes)
-                    std::fill_n(grad_x + (first + r) * width, width, 0.0F);
         if (grad_weight) {
             // Left out rows as zeros, whatever x holds there.
             for (std::size_t r = 0; r < n; ++r) {

@@ -139,16 +139,6 @@ __global__ __launch_bounds__(kCountThreads) void mean_kernel(const float* __rest
     if (threadIdx.x == 0) mean[0] = float(s * double(share[0]));
 }
 
-// Zeros for the rows that are left out: of a product zero times an infinity of the weight would not be. (256 rows of 256: 1.9 us.)
-__global__ __launch_bounds__(256) void clear_rows_kernel(const float* __restrict__ targets, int64_t rows, int64_t classes, int64_t width,
-                                                         float* __restrict__ out) {
-    const int64_t step = int64_t(gridDim.x) * 4;
-    for (int64_t r = int64_t(blockIdx.x) * 4 + threadIdx.x / 64; r < rows; r += step) {
-        if (class_of(targets[r], classes) >= 0) continue;
-        for (int64_t c = threadIdx.x % 64; c < width; c += 64) out[r * width + c] = 0.0f;
-    }
-}
-
 template <int Threads>
 __device__ inline float workgroup_max(float v, float* lds) {
     const int lane = red::lane_id();
@@ -1349,12 +1339,7 @@ void direct(Device& d, const Call& c, const float* shares, float* losses, float*
             continue;
         }
         rows_of<true>(d, z, c, c.targets + r, own, !shares, n, out);
-        if (grad_x) {
-            product(z, c.weight, grad_x + r * c.width, n, c.classes, c.width, false, true);
-            launch(clear_rows_kernel, dim3(grid_1d(n, 4, 8u * unsigned(d.cu_count))), dim3(256), 0, d.stream, c.targets + r, int64_t(n),
-                   int64_t(c.classes), int64_t(c.width), grad_x + r * c.width);
-            after_launch("linear_cross_entropy left out");
-        }
+        if (grad_x) product(z, c.weight, grad_x + r * c.width, n, c.classes, c.width, false, true);
         if (grad_weight) {
             product(rows.as<float>(), z, r ? more.as<float>() : grad_weight, c.width, n, c.classes, true, false);
             if (r) run(vc_hip_axpy(grad_weight, more.as<float>(), c.width * c.classes, 1.0f));
