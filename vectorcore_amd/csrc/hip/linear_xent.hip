@@ -1525,12 +1525,13 @@ bool takes_few(const Device& d, const Call& c) {
 
 // Whether packing pays: by estimates of both routes' times in us, for `products` products of the call's sizes (one, or up to three
 // with gradients; the bias's gradient alone takes one). Measured (estimated), direct and packed, in us: losses alone of 128 rows,
-// 1024 x 50000: 163 (144), 235 (224); of 256: 259 (279), 232 (224); 999, 515 x 10007: 162 (181), 78 (90); 4096, 256 x 1000: 43 (36),
-// 50 (55); 2048, 512 x 2048: 57 (57), 61 (63). Train steps of 128 rows, 1024 x 50000: 460 (423), 592 (556); of 256: 773 (827), 628
-// (576); 2048, 1024 x 1024: 162 (152), 148 (152); 3145, 18 x 25838: 489 (519), 637 (610), with a bias, a tenth of the rows left out,
-// 659 (673), 595 (610); 4096, 96 x 10000: 386 (429), 365 (370); 16384, 256 x 1000: 283 (333), 237 (238). The gradient of x alone, 256
-// rows, 1024 x 50000: 522 (558), 446 (418); of the weight alone, 4096, 96 x 10000: 283 (293), 220 (264); of the bias alone, 4096, 96
-// x 10000: 246 (234), 157 (160); 2048, 512 x 2048: 78 (75), 82 (84); 8192, 1024 x 5000: 885 (958), 386 (406).
+// 1024 x 50000: 163 (144), 235 (219); of 256: 259 (279), 232 (219); 999, 515 x 10007: 162 (181), 78 (85); 4096, 256 x 1000: 43 (36),
+// 50 (50); 2048, 512 x 2048: 57 (57), 61 (58). Train steps of 128 rows, 1024 x 50000: 460 (423), 592 (560); of 256: 773 (827), 628
+// (580); 2048, 1024 x 1024: 162 (152), 148 (156); 2135, 1719 x 466: 163 (154), 201 (158); 3145, 18 x 25838: 489 (519), 637 (614),
+// with a bias, a tenth of the rows left out, 659 (673), 595 (614); 4096, 96 x 10000: 386 (429), 365 (374); 16384, 256 x 1000: 283
+// (333), 237 (242). The gradient of x alone, 256 rows, 1024 x 50000: 522 (558), 446 (422); of the weight alone, 4096, 96 x 10000: 283
+// (293), 220 (268); of the bias alone, 4096, 96 x 10000: 246 (234), 157 (164); 2048, 512 x 2048: 78 (75), 82 (88); 8192, 1024 x 5000:
+// 885 (958), 386 (410).
 bool takes_packed(const Call& c, bool gradient, int products, bool grad_bias) {
     if (c.classes >= (size_t(1) << 21) || c.width >= (size_t(1) << 21)) return false;  // a load's offset has 31 bits
     if (c.rows >= kMostCounted) return false;
@@ -1542,7 +1543,8 @@ bool takes_packed(const Call& c, bool gradient, int products, bool grad_bias) {
     const double features = 32.0 * double(lines_of(int64_t(c.width))) + (products - 1) * double(whole_tiles(int64_t(c.width)));
     const double tiles = double(whole_tiles(int64_t(c.rows))) * double(whole_tiles(int64_t(c.classes))) * features;
     const double packing = (0.9e-6 + 1.1e-6 * products) * (weights + n * double(c.width));
-    return direct > (gradient ? 42.0 + 18.0 * products + (1.2e-6 + 0.6e-6 * products) * logits : 46.0) + packing + 2e-6 * tiles / 350.0;
+    const double others = gradient ? 46.0 + 18.0 * products + (1.2e-6 + 0.6e-6 * products) * logits : 41.0;
+    return direct > others + packing + 2e-6 * tiles / 350.0;
 }
 
 }  // namespace
