@@ -54,6 +54,24 @@ def test_upstream_gradients_whose_sums_no_float_holds(width, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("eps", [1e-5, 1e-30])
+@pytest.mark.parametrize("width", WIDTHS + [1000, 3000])
+def test_equal_values_of_any_size_are_zeros(width, eps, device):
+    """Their mean is exact, so that nothing but eps is left of the variance, and the gradient is one over its root."""
+    values = np.float32([1e7, -1.2345678e8, 3e20, -1.1e38, 3.3e38, 1e-7, 1e-25, -1e-38, 0])
+    x = np.repeat(values[:, None], width, 1)
+    dy = np.random.default_rng(width).standard_normal(x.shape).astype(np.float32)
+    tx = leaf(x, device)
+    y = vc.layer_norm(tx, eps=eps)
+    y.backward(vc.Tensor(dy, device=device))
+    assert (y.numpy() == 0).all()
+    d = dy - dy.astype(np.float64).mean(1, keepdims=True)
+    root = np.sqrt(float(np.float32(eps)))
+    # The mean of dy by sums of at most 32 roundings of the mean magnitude, and roundings of the difference and the products.
+    assert (np.abs(grad_of(tx) - d / root) <= UNIT / root * (8 * np.abs(d) + 40 * np.abs(dy).mean(1, keepdims=True))).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_one_row_does_not_change_another(device):
     rng = np.random.default_rng(1)
     x = rng.standard_normal((6, 300)).astype(np.float32)
