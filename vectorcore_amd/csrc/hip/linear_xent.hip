@@ -9,7 +9,8 @@
 // upstream gradient, or one over the number of rows that count (the mean loss).
 //
 // All of them keep float32's precision: an error is one of a few roundings of the
-// terms of the sum that it is in, whatever the operands' other values.
+// terms of the sum that it is in, whatever the operands' other values; packed, the
+// gradients of a class do so down to 2^-82 of the largest upstream gradient.
 //
 // Rows are taken in pieces: the logits of a piece live in a workspace until
 // their gradients are used. Three routes, by sizes alone:
@@ -341,13 +342,14 @@ using halves::h8;
 // rows of W (along the classes) and the columns of x (along the tokens). Also the largest exponents of x and W, and whether
 // either holds an infinity or a NaN.
 //
-// Two half-precision parts keep 22 bits of a value or 2^-38 of its row's largest, X. The latter's share of a sum of n products is
-// at most 2^-37 n X Y; the sum of the products' magnitudes is at least n times the product of both rows' geometric means, so that
-// share is below 2^-22 of it where both rows' largest lie less than 15 bits above them (13 of the exponents, each of which leaves
-// a bit open). Or it is below 2^-24, what an exponential rounds by in any case, where n X Y <= 2^13. In the gradients' products the
-// other operand is the logits' gradients, whose lost parts are likewise 2^-38 of a token's, or class's, largest times the sum of the
-// row: ten bits keep that below 2^-22 of the row's mean for 2^17 classes and tokens. Other calls take three bfloat16 parts
-// (thirds_product.hpp), which keep every value's 24 bits: a feature of 1e9 whose weights are 1e-9 costs time, not the logits.
+// Two half-precision parts keep 22 bits of a value or 2^-38 of its row's largest. The latter takes 2^-37 n X Y at most from a sum of
+// n products, X and Y being both rows' largest. The sum of the products' magnitudes is at least n times the product of both rows'
+// geometric means: where the largest lie 15 bits above those together (13 by the exponents, each of which leaves a bit open), less
+// than 2^-22 of the sum's own terms is lost. Or n X Y <= 2^13: then it is 2^-24, what an exponential rounds by in any case. In the
+// products of the logits' gradients that operand loses 2^-38 of a token's (of W: a class's) largest gradient at every class (token),
+// for 2^17 of them 2^-21 of it times the other row's mean, and ten bits keep what the other row loses below 2^-26 of its mean.
+// Calls beyond take three bfloat16 parts (thirds_product.hpp), which keep every value's 24 bits: a feature of 1e9 whose weights are
+// 1e-9 costs time, not the logits.
 struct Unlike {
     int x_rows, w_columns, w_rows, x_columns, x_most, w_most, not_finite;
     // width_bits: of the next power of two.
