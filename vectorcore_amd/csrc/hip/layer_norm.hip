@@ -19,12 +19,14 @@
 // double, which also holds any row's. The squares' sum is float32, of at most 16
 // values a lane, then a tree; rows whose largest value is past 2^50 or below 2^-40
 // are scaled by a power of two for it, so rows of any length have the cpu's range.
-// (Both sums in double took 53 us of 8192 rows of 4096, and 22 of 1269 of 8558.)
+// (Both sums in double took 53 us of 8192 rows of 4096, for 49.)
 //
-// Measured: 8192 rows of 4096, forward 47 us (5.7 TB/s), backward 79 us (5.1) and
+// Measured: 8192 rows of 4096, forward 49 us (5.5 TB/s), backward 77 us (5.2) and
 // 8 us for the partial rows; 262144 rows of 64 without a weight 24 and 33 us (5.7
 // and 6.1; a copy of 1 GiB reaches 5.1, these partly stay in the last cache);
-// 999 rows of 515 4.5 us, and 5.7 and 5.8; one row of 4096 3.5 us.
+// 999 rows of 515 4.6 us, and 5.7 and 5.4; one row of 4096 3.7 us. 4000 rows of
+// 10000 68 us, and 106 and 25; 2048 of 16384 59 us, and 87 and 83 (x and dy again
+// for the columns) and 7; 1024 of 32768 115 us, and 116, 72 and 10.
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"
 

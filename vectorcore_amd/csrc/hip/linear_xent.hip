@@ -20,10 +20,10 @@
 // - small or thin calls take float32 products and a kernel of the rows; bound by
 //   launches (256 rows, 256 x 10 with gradients: 25 us in five);
 // - others take packed products, bound by matrix instructions: 8192 rows, 1024 x
-//   50000, of which 7373 count, with gradients 6.9 ms: 2.05 (the logits, 369
-//   TFLOP/s), 1.87 and 1.94 (their gradients' products), 1.01 (the gradients, 4.4
+//   50000, of which 7373 count, with gradients 6.8 ms: 2.05 (the logits, 369
+//   TFLOP/s), 1.81 and 1.90 (their gradients' products), 0.99 (the gradients, 4.4
 //   GB at 4.4 TB/s), 0.3 for all others. 1536 rows that count without: 0.56 ms,
-//   of which the logits 0.48. Where the operands' rows hold values too unlike for
+//   of which the logits 0.47. Where the operands' rows hold values too unlike for
 //   two half-precision parts, three parts: 11.6 and 0.89 ms.
 #include "halves_product.hpp"
 #include "reduce_common.hpp"
@@ -380,7 +380,7 @@ struct Piece {
 };
 
 // A matrix of floats [rows, columns], packed by its rows (along columns, row_lines a row) and by its columns (along rows,
-// column_lines a column); either may be null. of.place: the matrix's rows are the piece's; else `rows` of them in order. The
+// column_lines a column); either may be without memory. of.place: the matrix's rows are the piece's; else `rows` of them in order. The
 // largest magnitudes are those of the whole matrix's rows and columns. exponents, filled: or null; of each column its exponent,
 // and bias (or zero), minus infinity for the columns that fill the last tile. A workgroup takes 32 rows and 128 columns, past
 // the ends zeros.
@@ -389,7 +389,7 @@ struct Packing {
     Piece of;
     int64_t rows, columns;
     const uint32_t *row_most, *column_most;
-    half *by_row, *by_column;
+    thirds::Operand by_row, by_column;
     int row_lines, column_lines, down, across;
     const float* bias;
     int* exponents;
@@ -414,8 +414,8 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing
     const int64_t columns = p.columns;
     const float* __restrict__ values = p.values;
     const uint32_t *const row_most = p.row_most, *const column_most = p.column_most;
-    half* __restrict__ by_row = p.by_row;
-    half* __restrict__ by_column = p.by_column;
+    half* __restrict__ by_row = p.by_row.first;
+    half* __restrict__ by_column = p.by_column.first;
     if (of.place) {
         rows = of.tokens();
         if (row0 >= (rows + halves::kTile - 1) / halves::kTile * halves::kTile) return;
@@ -470,7 +470,7 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing
                 for (int i = 0; i < 8; ++i) v[i] = tile[r][8 * g + i];
                 const bool there = row0 + r < rows;
                 const int64_t row = there && of.place ? of.row(row0 + r) : row0 + r;
-                thirds::store8(by_row, row_lines, row0 + r, column0 / 8 + g, v, there ? halves::exponent_of(row_most[row]) : 0);
+                thirds::store8(p.by_row, row_lines, row0 + r, column0 / 8 + g, v, there ? halves::exponent_of(row_most[row]) : 0);
             }
         }
 #pragma unroll
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(Packing one, Packing
                 float v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = tile[8 * g + i][at];
-                thirds::store8(by_column, column_lines, column0 + at, row0 / 8 + g, v,
+                thirds::store8(p.by_column, column_lines, column0 + at, row0 / 8 + g, v,
                                column0 + at < columns ? halves::exponent_of(column_most[column0 + at]) : 0);
             }
         }
@@ -686,15 +686,15 @@ __device__ inline int class_exponent(uint32_t most, uint32_t most_share) {
 constexpr int kGradientStride = kBlockTokens + 2;  // four threads that read eight classes of a token each meet different banks
 
 // The gradients dz^T of a piece from its logits z^T [classes, stride]: times the tokens' shares, packed along the tokens, in
-// their place (three parts: into by_class, or null, in the unit of the largest share); and for shares of one packed along the classes
-// (by_token, or null). most [blocks][whole classes]: the largest of
+// their place (three parts: into by_class, in the unit of the largest share); and for shares of one packed along the classes, by_token.
+// Either may be without memory. most [blocks][whole classes]: the largest of
 // each class, as bits. Sums: of each class, into sums [blocks][classes]. A workgroup takes 32 classes and a block of tokens;
 // four lanes of a wavefront read a line of the logits, and then write it.
 template <bool Sums>
 __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t stride, Piece piece, const Token* __restrict__ tokens,
                                                         const float* __restrict__ shares, const uint32_t* __restrict__ most_share,
                                                         int64_t classes, int64_t whole_classes, uint32_t* __restrict__ most,
-                                                        half* __restrict__ by_token, half* __restrict__ by_class, int lines,
+                                                        thirds::Operand by_token, thirds::Operand by_class, int lines,
                                                         double* __restrict__ sums, int blocks, Form form) {
     __shared__ float tile[32][kGradientStride];
     const int64_t id = block_id(), block = id % blocks, v0 = id / blocks * 32;
@@ -756,7 +756,7 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
         }
         if (!there) continue;
         if (thirds) {
-            if (by_class) thirds::store8(by_class, int(stride / halves::kSlice), v, (t0 + c) / 8, d, halves::exponent_of(top));
+            if (by_class.first) thirds::store8(by_class, int(stride / halves::kSlice), v, (t0 + c) / 8, d, halves::exponent_of(top));
         } else {
             h8 first, second;
             halves::split8(d, class_exponent(high, top), first, second);
@@ -769,7 +769,7 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
             if constexpr (Sums) sums[block * classes + v] = sum;
         }
     }
-    if (!by_token) return;
+    if (!by_token.first) return;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -785,7 +785,7 @@ __global__ __launch_bounds__(256) void gradients_kernel(float* logits, int64_t s
         }
         h8 first, second;
         halves::split8(v, halves::exponent_of(others), first, second);
-        half* const to = by_token + ((t0 + t) * lines + v0 / 32) * 64 + 8 * g;
+        half* const to = by_token.first + ((t0 + t) * lines + v0 / 32) * 64 + 8 * g;
         *reinterpret_cast<h8*>(to) = first;
         *reinterpret_cast<h8*>(to + 32) = second;
     }
@@ -834,14 +834,41 @@ struct Logits {
         for (; k < width; ++k) s = __builtin_fmaf(row[k], column[k * classes], s);
         return s;
     }
-    static __device__ inline bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
+    // Sums of three parts that are lost, again, in place: of finite values none is, and again() gives an infinity or a NaN, which
+    // no scale changes. Apart from the rest, whose registers it would take (253, 203).
+    template <int Blocks>
+    __device__ inline void restore(halves::f16v (&acc)[4][Blocks], int m, int n, int wave, int first) const {
+        const auto finite = [](float v) { return fabsf(v) < __builtin_huge_valf(); };
+        const int lane = threadIdx.x % 64;
+        const int64_t v0 = int64_t(m) * halves::kTile + 128 * (wave / 4) + 4 * (lane / 32);
+        const int64_t t0 = int64_t(n) * halves::kTile + 64 * (wave % 4) + 32 * first + lane % 32, tokens = piece.tokens();
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int b = 0; b < Blocks; ++b) {
+                bool lost = false;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) lost |= !finite(acc[a][b][i]);
+                if (!lost) continue;
+#pragma unroll 1
+                for (int l = 0; l < 16; ++l) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum = l == i ? acc[a][b][i] : sum;
+                    if (finite(sum)) continue;
+                    const int64_t v = v0 + 32 * a + 8 * (l / 4) + l % 4, t = t0 + 32 * b;
+                    sum = v < classes && t < tokens ? again(v, t) : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[a][b][i] = l == i ? sum : acc[a][b][i];
+                }
+            }
+    }
     // Of wave `wave` of a tile: its blocks of 32 columns from block `first`.
     template <int Blocks>
     __device__ inline void operator()(const halves::f16v (&acc)[4][Blocks], int m, int n, int wave, int first) const {
         const int lane = threadIdx.x % 64, column = 64 * (wave % 4) + 32 * first + lane % 32;
         const int64_t v0 = int64_t(m) * halves::kTile, t0 = int64_t(n) * halves::kTile + column;
         const int64_t tokens = piece.tokens();
-        const bool thirds = form.thirds();
         const int row0 = 128 * (wave / 4) + 4 * (lane / 32);
         float top[Blocks], others[Blocks];
         int e_token[Blocks], target[Blocks];  // the target's row in this tile
@@ -883,31 +910,9 @@ struct Logits {
                 int own = target[b] - row0 - r0;  // the target's among these rows, if it is
                 float z[16], high = top[b], found = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) z[i] = __builtin_amdgcn_ldexpf(acc[a][b][i], -(e[i] + e_token[b])) + add[i];
-                if (thirds) {
-                    bool lost = false;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) lost |= !finite(acc[a][b][i]);
-                    if (lost) {
-#pragma unroll 1
-                        for (int l = 0; l < 16; ++l) {
-                            float sum = 0.0f, more = 0.0f;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                sum = l == i ? acc[a][b][i] : sum;
-                                more = l == i ? add[i] : more;
-                            }
-                            if (finite(sum)) continue;
-                            const int64_t v = v0 + row0 + r0 + 8 * (l / 4) + l % 4, t = t0 + 32 * b;
-                            const float logit = (v < classes && t < tokens ? again(v, t) : 0.0f) + more;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) z[i] = l == i ? logit : z[i];
-                        }
-                    }
-                }
-#pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int r = 8 * (i / 4) + i % 4;
+                    z[i] = __builtin_amdgcn_ldexpf(acc[a][b][i], -(e[i] + e_token[b])) + add[i];
                     if constexpr (Store)
                         __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, z[i]), rows, at + 128u * b,
                                                               uint32_t(r0 + r) * row_bytes, 0);
@@ -1050,11 +1055,11 @@ struct WeightGradient {
     }
 };
 
-// lines: a row's of either operand, of which depth() are multiplied; b_thirds: b in three parts. The parts of split tiles go to
-// partial, for join_kernel.
+// lines: a row's of either operand, of which depth() are multiplied; b_thirds: b, if that is in three parts. The parts of split tiles
+// go to partial, for join_kernel.
 template <class Of>
-__global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* __restrict__ a, const half* __restrict__ b,
-                                                                   const half* __restrict__ b_thirds, int lines, int places,
+__global__ __launch_bounds__(halves::kThreads) void product_kernel(thirds::Operand a, const half* __restrict__ b,
+                                                                   thirds::Operand b_thirds, int lines, int places,
                                                                    float* __restrict__ partial, Of of, Form form) {
     extern __shared__ __attribute__((aligned(128))) char lds[];
     if (of.idle()) return;
@@ -1072,9 +1077,9 @@ __global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* _
     halves::Tile tile;
     tile.clear();
     if (form.thirds()) {
-        const int64_t bytes = thirds::tile_bytes(lines);
-        thirds::accumulate(tile, reinterpret_cast<const char*>(a) + at.m * bytes, reinterpret_cast<const char*>(b_thirds) + at.n * bytes,
-                           begin, end, lds);
+        thirds::accumulate(tile, thirds::tile_of(a, at.m, lines), thirds::tile_of(b_thirds, at.n, lines), begin, end, lds);
+        if constexpr (!Of::kElementwise)
+            if (at.part < 0) of.restore(tile.acc, at.m, at.n, int(threadIdx.x / 64), 0);
         if constexpr (Of::kUnits) {
             const int by = -halves::exponent_of(of.most_share[0]);
 #pragma unroll
@@ -1093,7 +1098,7 @@ __global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* _
 #pragma unroll
         for (int j = 0; j < 2; ++j) now[j] = begin < end ? unit(begin, j) : 0;
         tile.accumulate<kBlockLines>(
-            a + at.m * of_tile, b + at.n * of_tile, lines, begin, end, lds,
+            a.first + at.m * of_tile, b + at.n * of_tile, lines, begin, end, lds,
             [&](int s) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) next[j] = s + kBlockLines < end ? unit(s + kBlockLines, j) : 0;
@@ -1110,7 +1115,7 @@ __global__ __launch_bounds__(halves::kThreads) void product_kernel(const half* _
                 }
             });
     } else {
-        tile.accumulate<0>(a + at.m * of_tile, b + at.n * of_tile, lines, begin, end, lds, [](int) {}, [](int) {});
+        tile.accumulate<0>(a.first + at.m * of_tile, b + at.n * of_tile, lines, begin, end, lds, [](int) {}, [](int) {});
     }
     if (at.part >= 0)
         tile.store_part(partial + int64_t(at.rest * tiles.parts + at.part) * halves::Tile::kValues * halves::kThreads);
@@ -1141,6 +1146,7 @@ __global__ __launch_bounds__(kJoinThreads<Of>) void join_kernel(int places, cons
             const int thread = share / 2 * kJoinThreads<Of> + int(threadIdx.x);
             halves::f16v acc[4][1];
             halves::Tile::load_parts(from, tiles.parts, thread, share % 2, acc);
+            if (of.form.thirds()) of.restore(acc, at.m, at.n, thread / 64, share % 2);
             of(acc, at.m, at.n, thread / 64, share % 2);
         }
     }
@@ -1356,15 +1362,23 @@ void direct(Device& d, const Call& c, const float* shares, float* losses, float*
 
 int64_t whole_tiles(int64_t n) { return (n + halves::kTile - 1) / halves::kTile * halves::kTile; }
 int64_t lines_of(int64_t n) { return (n + halves::kSlice - 1) / halves::kSlice; }
-// A packed matrix of `rows` rows of `depth` values, in the larger of both forms: three parts.
-size_t packed_bytes(int64_t rows, int64_t depth) {
-    return size_t(whole_tiles(rows) / halves::kTile) * size_t(thirds::tile_bytes(int(lines_of(depth))));
-}
+// Memory of a packed matrix of `rows` rows of `depth` values, if it is wanted. The third parts lie apart, so that two parts lie as
+// if there were none (in one buffer of 1.5 times the size, 256 rows, 1024 x 50000 took 6 us more to pack and 11 to multiply).
+struct Packed {
+    Scratch first, third;
+    bool wanted;
+    static size_t third_bytes(int64_t rows, int64_t depth) {
+        return size_t(whole_tiles(rows) / halves::kTile) * size_t(thirds::third_bytes(int(lines_of(depth))));
+    }
+    Packed(int64_t rows, int64_t depth, bool want)
+        : first(want ? 2 * third_bytes(rows, depth) : 4), third(want ? third_bytes(rows, depth) : 4), wanted(want) {}
+    thirds::Operand operand() const { return wanted ? thirds::Operand{first.as<half>(), third.as<half>()} : thirds::Operand{nullptr, nullptr}; }
+};
 
 // A product of at most these rows; partial: room for one split tile a CU.
 template <class Of>
-void product_of(Device& d, const half* a, const half* b, const half* b_thirds, int64_t rows_a, int64_t rows_b, int64_t lines,
-                float* partial, const Of& of, const Form& form) {
+void product_of(Device& d, const thirds::Operand& a, const half* b, const thirds::Operand& b_thirds, int64_t rows_a, int64_t rows_b,
+                int64_t lines, float* partial, const Of& of, const Form& form) {
     constexpr int kLds = std::max(halves::Tile::kLds, thirds::kLds);
     const int64_t blocks = halves::most_blocks(rows_a, rows_b, d.cu_count);
     if (blocks > int64_t(1) << 22) fail(VC_HIP_ERR_OVERFLOW, "linear_cross_entropy: too many tiles");
@@ -1381,8 +1395,8 @@ void product_of(Device& d, const half* a, const half* b, const half* b_thirds, i
 }
 
 Packing packing(const float* values, const Piece& of, int64_t rows, int64_t columns, const uint32_t* row_most,
-                const uint32_t* column_most, half* by_row, half* by_column) {
-    const int64_t down = (by_row ? whole_tiles(rows) : lines_of(rows) * 32) / kPackRows, across = whole_tiles(columns) / kPackColumns;
+                const uint32_t* column_most, const thirds::Operand& by_row, const thirds::Operand& by_column) {
+    const int64_t down = (by_row.first ? whole_tiles(rows) : lines_of(rows) * 32) / kPackRows, across = whole_tiles(columns) / kPackColumns;
     return Packing{values, of, rows, columns, row_most, column_most, by_row, by_column, int(lines_of(columns)), int(lines_of(rows)),
                    int(down), int(across), nullptr, nullptr, nullptr};
 }
@@ -1441,15 +1455,15 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
     int* const exponents = of_class.as<int>();
     float* const bias = of_class.as<float>() + whole_classes;
 
-    Scratch wt(packed_bytes(classes, width)), w(grad_x ? packed_bytes(width, classes) : 4);
-    Packing of_weight = packing(c.weight, Piece{}, width, classes, w_rows, w_columns, grad_x ? w.as<half>() : nullptr, wt.as<half>());
+    const Packed wt(classes, width, true), w(width, classes, grad_x);
+    Packing of_weight = packing(c.weight, Piece{}, width, classes, w_rows, w_columns, w.operand(), wt.operand());
     of_weight.bias = c.bias;
     of_weight.exponents = exponents;
     of_weight.filled = bias;
 
-    Scratch x(packed_bytes(piece, width)), xt(grad_weight ? packed_bytes(width, piece) : 4);
-    Scratch logits(gradient ? size_t(whole_classes * piece) * sizeof(float) : 4), z(grad_x ? packed_bytes(piece, classes) : 4);
-    Scratch zt(grad_weight ? packed_bytes(classes, piece) : 4);
+    const Packed x(piece, width, true), xt(width, piece, grad_weight), z(piece, classes, grad_x);
+    const Packed zt(classes, piece, grad_weight);  // three parts: two take the place of the logits
+    Scratch logits(gradient ? size_t(whole_classes * piece) * sizeof(float) : 4);
     Scratch statistics(size_t(2 * parts + 2) * size_t(piece) * sizeof(float)), tokens(size_t(piece) * sizeof(Token));
     Scratch class_most(gradient ? size_t(blocks * whole_classes) * sizeof(uint32_t) : 4);
     Scratch sums(grad_bias ? size_t((blocks + 1) * classes) * sizeof(double) : 4);
@@ -1460,10 +1474,10 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
 
     for (int64_t p = 0; p < pieces; ++p) {
         const Piece of{counted, place, p * piece, piece};
-        const Packing of_rows = packing(c.x, of, piece, width, x_rows, x_columns, x.as<half>(), grad_weight ? xt.as<half>() : nullptr);
+        const Packing of_rows = packing(c.x, of, piece, width, x_rows, x_columns, x.operand(), xt.operand());
         pack(d, of_rows, p == 0 ? of_weight : Packing{}, form);
         const auto z_of = [&](auto store) {
-            product_of(d, wt.as<half>(), x.as<half>(), x.as<half>(), classes, piece, lines_of(width), partial.as<float>(),
+            product_of(d, wt.operand(), x.operand().first, x.operand(), classes, piece, lines_of(width), partial.as<float>(),
                        Logits<store()>{of, exponents, x_rows, bias, c.targets, logits.as<float>(), part_most, part_sum, at_target, classes,
                                        piece, int(lines_of(width)), c.x, c.weight, width, form},
                        form);
@@ -1476,7 +1490,7 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
         const auto gradients = grad_bias ? gradients_kernel<true> : gradients_kernel<false>;
         launch(gradients, grid_2d(size_t(blocks * lines_of(classes))), dim3(256), 0, d.stream, logits.as<float>(), piece, of,
                tokens.as<Token>(), own_shares, most_share, classes, whole_classes, class_most.as<uint32_t>(),
-               grad_x ? z.as<half>() : nullptr, grad_weight ? zt.as<half>() : nullptr, int(lines_of(classes)),
+               z.operand(), zt.operand(), int(lines_of(classes)),
                sums.as<double>(), int(blocks), form);
         after_launch("linear_cross_entropy gradients");
         if (grad_bias) {
@@ -1485,10 +1499,10 @@ void packed(Device& d, const Call& c, const float* shares, float* share, float* 
             after_launch("linear_cross_entropy bias");
         }
         if (grad_x)
-            product_of(d, z.as<half>(), w.as<half>(), w.as<half>(), piece, width, lines_of(classes), partial.as<float>(),
+            product_of(d, z.operand(), w.operand().first, w.operand(), piece, width, lines_of(classes), partial.as<float>(),
                        InputGradient{of, tokens.as<Token>(), w_rows, own_shares, grad_x, width, int(lines_of(classes))}, form);
         if (grad_weight)
-            product_of(d, xt.as<half>(), logits.as<half>(), zt.as<half>(), width, classes, piece / halves::kSlice, partial.as<float>(),
+            product_of(d, xt.operand(), logits.as<half>(), zt.operand(), width, classes, piece / halves::kSlice, partial.as<float>(),
                        WeightGradient{of, x_columns, class_most.as<uint32_t>(), most_share, grad_weight, width, classes, whole_classes,
                                       p > 0},
                        form);
@@ -1525,28 +1539,41 @@ bool takes_few(const Device& d, const Call& c) {
     return few < 0.9 * (9.0 + bytes / 5.0e6 + 1.2e-4 * double(c.classes));
 }
 
-// Whether packing pays: by estimates of both routes' times in us, for `products` products of the call's sizes (one, or up to three
-// with gradients; the bias's gradient alone takes one). Measured (estimated), direct and packed, in us: losses alone of 128 rows,
-// 1024 x 50000: 163 (144), 235 (219); of 256: 259 (279), 232 (219); 999, 515 x 10007: 162 (181), 78 (85); 4096, 256 x 1000: 43 (36),
-// 50 (50); 2048, 512 x 2048: 57 (57), 61 (58). Train steps of 128 rows, 1024 x 50000: 460 (423), 592 (560); of 256: 773 (827), 628
-// (580); 2048, 1024 x 1024: 162 (152), 148 (156); 2135, 1719 x 466: 163 (154), 201 (158); 3145, 18 x 25838: 489 (519), 637 (614),
-// with a bias, a tenth of the rows left out, 659 (673), 595 (614); 4096, 96 x 10000: 386 (429), 365 (374); 16384, 256 x 1000: 283
-// (333), 237 (242). The gradient of x alone, 256 rows, 1024 x 50000: 522 (558), 446 (422); of the weight alone, 4096, 96 x 10000: 283
-// (293), 220 (268); of the bias alone, 4096, 96 x 10000: 246 (234), 157 (164); 2048, 512 x 2048: 78 (75), 82 (88); 8192, 1024 x 5000:
-// 885 (958), 386 (410).
-bool takes_packed(const Call& c, bool gradient, int products, bool grad_bias) {
+// A packed product's time in us, of `tiles` tiles of `lines` lines on `places` CUs, by what tiles_of makes of it.
+double product_time(int64_t tiles, int64_t lines, int64_t places) {
+    const int64_t rest = tiles % places;
+    const double line = 2.5;
+    double time = 4.0 + line * double(lines) * double(tiles / places);
+    if (rest == 0) return time;
+    const int64_t parts = lines >= halves::kLeastSplit ? std::min(places / rest, lines / 8) : 1;
+    const bool split = parts > 1 && 50 * lines * (parts - 1) > parts * (100 + 2 * rest * parts);
+    return time + line * double(lines) / double(split ? parts : 1) + (split ? 16.0 : 0.0);
+}
+
+// Whether packing pays: by estimates of both routes' times in us, for the gradients that are wanted. Measured (estimated), direct
+// and packed, in us: losses alone of 128 rows, 1024 x 50000: 163 (144), 220 (217); of 256: 259 (279), 222 (217); 999, 515 x 10007:
+// 162 (181), 79 (88); 4096, 256 x 1000: 43 (36), 51 (57); 2135, 1719 x 466: 51 (63), 81 (81). Train steps of 128 rows, 1024 x 50000:
+// 460 (423), 567 (490); of 256: 773 (827), 612 (553); 2048, 1024 x 1024: 162 (152), 149 (183); 2135, 1719 x 466: 163 (180), 202
+// (189); 1590, 1518 x 1016: 211 (250), 166 (185); 3145, 18 x 25838: 489 (519), 629 (626), with a bias, a tenth of the rows left out,
+// 659 (673), 592 (626); 4096, 96 x 10000: 386 (429), 366 (364); 16384, 256 x 1000: 283 (333), 234 (224). The gradient of x alone, 256
+// rows, 1024 x 50000: 522 (558), 424 (398); of the weight alone, 4096, 96 x 10000: 283 (293), 226 (257); of the bias alone, 4096, 96
+// x 10000: 246 (234), 157 (145); 2048, 512 x 2048: 78 (75), 82 (91); 8192, 1024 x 5000: 885 (958), 384 (363).
+bool takes_packed(const Device& d, const Call& c, bool of_x, bool of_weight, bool of_bias) {
     if (c.classes >= (size_t(1) << 21) || c.width >= (size_t(1) << 21)) return false;  // a load's offset has 31 bits
     if (c.rows >= kMostCounted) return false;
+    const bool gradient = of_x || of_weight || of_bias, aligned = c.width % 4 == 0 && c.classes % 4 == 0;
     const double n = double(c.rows), weights = double(c.width) * double(c.classes), logits = n * double(c.classes);
-    const bool aligned = c.width % 4 == 0 && c.classes % 4 == 0;
+    const double products = 1.0 + of_x + of_weight;
     const double direct = (gradient ? 20.0 : 10.0) + 2e-6 * products * n * weights / (aligned ? 105.0 : 66.0) +
-                          (1.5e-6 * products + (grad_bias ? 1.9e-6 : 0.0)) * logits;
-    // The features are a depth of whole lines in the logits, and whole tiles in the gradients' products.
-    const double features = 32.0 * double(lines_of(int64_t(c.width))) + (products - 1) * double(whole_tiles(int64_t(c.width)));
-    const double tiles = double(whole_tiles(int64_t(c.rows))) * double(whole_tiles(int64_t(c.classes))) * features;
-    const double packing = (0.9e-6 + 1.1e-6 * products) * (weights + n * double(c.width));
-    const double others = gradient ? 46.0 + 18.0 * products + (1.2e-6 + 0.6e-6 * products) * logits : 41.0;
-    return direct > others + packing + 2e-6 * tiles / 350.0;
+                          (1.5e-6 * products + (of_bias ? 1.9e-6 : 0.0)) * logits;
+    const int64_t rows = whole_tiles(int64_t(c.rows)) / halves::kTile, features = whole_tiles(int64_t(c.width)) / halves::kTile;
+    const int64_t classes = whole_tiles(int64_t(c.classes)) / halves::kTile;
+    double packed = 30.0 + (0.9e-6 + 1.1e-6 * products) * (weights + n * double(c.width)) +
+                    product_time(classes * rows, lines_of(int64_t(c.width)), d.cu_count);
+    if (gradient) packed += 4.0 * products + (1.2e-6 + 0.8e-6 * products) * logits;
+    if (of_x) packed += product_time(rows * features, lines_of(int64_t(c.classes)), d.cu_count);
+    if (of_weight) packed += product_time(features * classes, lines_of(int64_t(c.rows)), d.cu_count);
+    return direct > packed;
 }
 
 }  // namespace
@@ -1570,7 +1597,7 @@ int vc_hip_linear_xent_forward(const float* x, const float* weight, const float*
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy", products, 4.0 * double(width) * double(rows + classes));
         const bool few = takes_few(d, c);
-        if (!few && !takes_packed(c, false, 1, false)) {
+        if (!few && !takes_packed(d, c, false, false, false)) {
             direct(d, c, nullptr, losses, mean, nullptr, nullptr, nullptr);
         } else {
             Scratch own(losses ? 4 : rows * sizeof(float)), share(sizeof(float));
@@ -1604,8 +1631,7 @@ int vc_hip_linear_xent_gradient(const float* x, const float* weight, const float
         const double products = 2.0 * double(rows) * double(width) * double(classes);
         Profiled p("linear_cross_entropy_gradient", products * (1.0 + (grad_x != nullptr) + (grad_weight != nullptr)),
                    8.0 * double(width) * double(rows + classes));
-        const bool gradient = grad_x || grad_weight || grad_bias;
-        if (takes_packed(c, gradient, 1 + (grad_x != nullptr) + (grad_weight != nullptr), grad_bias != nullptr)) {
+        if (takes_packed(d, c, grad_x, grad_weight, grad_bias)) {
             Scratch share(sizeof(float)), losses(mean ? rows * sizeof(float) : 4);
             packed(d, c, shares, share.as<float>(), mean ? losses.as<float>() : nullptr, grad_x, grad_weight, grad_bias);
             if (mean) mean_of(d, c, losses.as<float>(), share.as<float>(), mean);

@@ -9,12 +9,13 @@
 // infinity or a NaN is an infinity or a NaN, and so is every sum that it is in.
 //
 // An operand is stored as the matrix instructions read it: of each 256 rows and 16
-// k one block of 24 KiB, [part][k / 8][row][8]. A slice of either operand is then
-// one run of memory, of which every wave loads 1 KiB at a time straight to LDS, and
-// a fragment is read without bank conflicts.
+// k one block of 16 KiB, [part][k / 8][row][8], of the first two parts, which take
+// the place of the two half parts, and one of 8 KiB of the third parts elsewhere. A
+// slice of either operand is then two runs of memory, of which every wave loads 1
+// KiB at a time straight to LDS, and a fragment is read without bank conflicts.
 //
-// Bound by the matrix instructions: 7373 x 1024 by 50000 long sums take 3.23 ms (234
-// TFLOP/s of float32 products, 1403 of bfloat16 ones), two half parts 1.83.
+// Bound by the matrix instructions: 7373 x 1024 by 50000 long sums take 3.25 ms (232
+// TFLOP/s of float32 products, 1393 of bfloat16 ones), two half parts 1.81.
 #pragma once
 
 #include "halves_product.hpp"
@@ -25,19 +26,26 @@ namespace thirds {
 using halves::kThreads;
 using halves::kTile;
 
-constexpr int kSlice = 16, kParts = 3, kBlock = kParts * 2 * kTile * 16;  // bytes of a block
-constexpr int kStages = 3, kLds = kStages * 2 * kBlock;
+constexpr int kSlice = 16, kParts = 3, kPart = 2 * kTile * 16;  // bytes of a part of a block
+constexpr int kStages = 3, kLds = kStages * 2 * kParts * kPart;
 
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f2v __attribute__((ext_vector_type(2)));
 
+// A packed operand: its first parts, which hold both half parts otherwise, and its third ones.
+struct Operand {
+    halves::half *first, *third;
+};
+
 // Of rows of `lines` times 32 k: the eight from 8 k8 of a row, scaled by 2^e.
-__device__ inline void store8(void* to, int lines, int64_t row, int64_t k8, const float (&v)[8], int e) {
+__device__ inline void store8(const Operand& to, int lines, int64_t row, int64_t k8, const float (&v)[8], int e) {
     f2v rest[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) rest[i] = f2v{__builtin_amdgcn_ldexpf(v[2 * i], e), __builtin_amdgcn_ldexpf(v[2 * i + 1], e)};
-    b8* const at = static_cast<b8*>(to) + (((row / kTile) * (2 * int64_t(lines)) + k8 / 2) * (2 * kParts) + k8 % 2) * kTile + row % kTile;
+    const int64_t block = (row / kTile) * (2 * int64_t(lines)) + k8 / 2, in = k8 % 2 * kTile + row % kTile;
+    b8* const first = reinterpret_cast<b8*>(to.first) + block * (4 * kTile) + in;
+    b8* const third = reinterpret_cast<b8*>(to.third) + block * (2 * kTile) + in;
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
         b8 out;
@@ -49,43 +57,47 @@ __device__ inline void store8(void* to, int lines, int64_t row, int64_t k8, cons
             rest[i][0] -= float(part[0]);
             rest[i][1] -= float(part[1]);
         }
-        at[2 * p * kTile] = out;
+        if (p < 2) first[2 * p * kTile] = out;
+        else *third = out;
     }
 }
 
-// Bytes of an operand's tile.
-__host__ __device__ inline int64_t tile_bytes(int lines) { return 2 * int64_t(lines) * kBlock; }
+// Bytes of the third parts of an operand's tile; its first two take twice that, as much as its half parts.
+__host__ __device__ inline int64_t third_bytes(int lines) { return 2 * int64_t(lines) * kPart; }
+__device__ inline Operand tile_of(const Operand& of, int64_t tile, int lines) {
+    return Operand{of.first + tile * third_bytes(lines), of.third + tile * third_bytes(lines) / 2};  // two bytes each
+}
 
-template <int Q>
-__device__ inline void load_block(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t lds) {
-    halves::Tile::load_one<Q>(rs, off, 0, lds);
-    halves::Tile::load_one<Q + 8192>(rs, off, 8192, lds);
-    halves::Tile::load_one<Q + 16384>(rs, off, 16384, lds);
+template <int At>
+__device__ inline void load_block(__amdgpu_buffer_rsrc_t first, __amdgpu_buffer_rsrc_t third, uint32_t off, uint32_t lds) {
+    halves::Tile::load_one<At>(first, off, 0, lds);
+    halves::Tile::load_one<At + kPart>(first, off, kPart, lds);
+    halves::Tile::load_one<At + 2 * kPart>(third, off, 0, lds);
 }
 
 // tile += the products of lines [begin, end) of a tile of either operand. lds: kLds bytes. Two slices are on their way while one
 // is multiplied: a slice takes about 3000 cycles, as one of the halves' does.
-__device__ inline void accumulate(halves::Tile& tile, const void* a, const void* b, int begin, int end, char* lds) {
+__device__ inline void accumulate(halves::Tile& tile, const Operand& a, const Operand& b, int begin, int end, char* lds) {
     if (end <= begin) return;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const uint32_t off = 1024u * uint32_t(wave) + 16u * uint32_t(lane);
     const uint32_t to =
         __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>((halves::lds_ptr_t)lds)) + 1024u * uint32_t(wave));
     const int first = 2 * begin, last = 2 * end - 1;
-    const auto from = [](const void* operand, int s) {
-        char* const at = const_cast<char*>(static_cast<const char*>(operand)) + int64_t(s) * kBlock;
-        return __builtin_amdgcn_make_buffer_rsrc(at, short(0), kBlock, 0x00020000);
+    const auto from = [](halves::half* parts, int64_t s, int bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(parts) + s * bytes, short(0), bytes, 0x00020000);
     };
+    constexpr int kOperand = kParts * kPart;  // bytes in a stage
     const auto request = [&](int s, int stage) {
-        const uint32_t dst = to + uint32_t(stage) * (2 * kBlock);
-        load_block<0>(from(a, s), off, dst);
-        load_block<kBlock>(from(b, s), off, dst);
+        const uint32_t dst = to + uint32_t(stage) * (2 * kOperand);
+        load_block<0>(from(a.first, s, 2 * kPart), from(a.third, s, kPart), off, dst);
+        load_block<kOperand>(from(b.first, s, 2 * kPart), from(b.third, s, kPart), off, dst);
     };
     const int at_a = lane / 32 * (kTile * 16) + (128 * (wave / 4) + lane % 32) * 16;
-    const int at_b = kBlock + lane / 32 * (kTile * 16) + (64 * (wave % 4) + lane % 32) * 16;
+    const int at_b = kOperand + lane / 32 * (kTile * 16) + (64 * (wave % 4) + lane % 32) * 16;
     constexpr int kA[6] = {0, 2, 1, 0, 1, 0}, kB[6] = {2, 0, 1, 1, 0, 0};  // the small products first
     const auto multiply = [&](int stage) {
-        const char* const at = lds + stage * (2 * kBlock);
+        const char* const at = lds + stage * (2 * kOperand);
         b8 y[2][kParts];
 #pragma unroll
         for (int q = 0; q < kParts; ++q)
