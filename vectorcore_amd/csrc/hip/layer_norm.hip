@@ -74,8 +74,9 @@ struct Shape {
     // Of 16 wavefronts 128 registers a thread do not hold four groups of x, dy, w, dw and db.
     static constexpr bool kHoldsSums = G < 1024 || NV < 4;
     // Wavefronts a SIMD that the registers have to leave room for, where a few more would take a workgroup's place (1269 rows of 8558
-    // forward: 17 us, 22 with one workgroup of 1024 threads on a CU).
-    static constexpr int kForwardWaves = G == 1024 && NV < 4 ? 8 : 1, kBackwardWaves = G == 64 && NV == 4 ? 4 : 1;
+    // forward: 18 us, 22 with one workgroup of 1024 threads on a CU; 8192 rows of 4096: 49 with six of 256, 54 with five).
+    static constexpr int kForwardWaves = G == 1024 && NV < 4 ? 8 : G == 256 && NV == 4 ? 6 : 1;
+    static constexpr int kBackwardWaves = G == 64 && NV == 4 ? 4 : 1;
 };
 
 struct Add {
@@ -171,9 +172,16 @@ __device__ inline void store(float* __restrict__ row, int width, int t, const f4
     }
 }
 
+// A value that all threads have, in scalar registers.
+__device__ inline double uniform(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(bits))), hi = uint32_t(__builtin_amdgcn_readfirstlane(int(bits >> 32)));
+    return __builtin_bit_cast(double, lo | hi << 32);
+}
+
 // The row's values, with zeros past its end, become x factor - mean - rest; the same for every thread of the group. root: of eps.
 template <int G, int NV>
-__device__ inline RowStats statistics(f4 (&v)[NV], int width, double one_nth, int t, float eps, float root, SumAndLargest<G>& first,
+__device__ inline RowStats statistics(f4 (&v)[NV], int width, double n, double one_nth, int t, float eps, float root, SumAndLargest<G>& first,
                                       Sums<G>& second) {
     double sum = 0.0;
     float most = root;
@@ -187,7 +195,9 @@ __device__ inline RowStats statistics(f4 (&v)[NV], int width, double one_nth, in
         asm volatile("" : "+v"(sum));  // the doubles of one group at a time: they take registers
     }
     first(sum, most);
-    const double mean = sum * one_nth;
+    // The quotient to its last bit, as a division: of equal values it is their value.
+    const double about = sum * one_nth;
+    const double mean = __builtin_fma(__builtin_fma(-about, n, sum), one_nth, about);
     const float factor = factor_of(most);
     const double centre = mean * double(factor);
     const float near = float(centre), rest = float(centre - double(near));
@@ -216,14 +226,14 @@ __global__ __launch_bounds__(kThreadsOf<G>, (Shape<G, NV>::kForwardWaves)) void 
     f4 w[NV], b[NV];
     if (weight) load<G>(weight, width, t, 0.0f, w);
     if (bias) load<G>(bias, width, t, 0.0f, b);
-    const double one_nth = 1.0 / double(width);
-    const float root = sqrtf(eps);
+    const double n = uniform(double(width)), one_nth = uniform(1.0 / double(width));
+    const float root = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sqrtf(eps))));
     for (int64_t first = int64_t(blockIdx.x) * kGroups; first < rows; first += int64_t(gridDim.x) * kGroups) {
         const int64_t r = first + threadIdx.x / G;
         const bool there = r < rows;  // the wavefront stays whole
         f4 v[NV];
         load<G>(x + (there ? r : rows - 1) * width, width, t, 0.0f, v);
-        const RowStats st = statistics<G>(v, width, one_nth, t, eps, root, first_sum, second_sum);
+        const RowStats st = statistics<G>(v, width, n, one_nth, t, eps, root, first_sum, second_sum);
 #pragma unroll
         for (int u = 0; u < NV; ++u)
 #pragma unroll
@@ -520,7 +530,10 @@ int vc_hip_layer_norm_forward(const float* x, const float* weight, const float* 
         Profiled p("layer_norm", 8.0 * count, 8.0 * count);
         const bool held = with_shape(width, [&](auto g, auto nv) {
             using S = Shape<g(), nv()>;
-            const unsigned grid = grid_1d(rows, S::kGroups, 16u * unsigned(d.cu_count));
+            // Two rows of a group or more, which share the weight's loads, and 16 workgroups a CU if there are as many: 4000 rows of
+            // 3500 20.5 us, 22.7 with one; 8192 rows of 4096 49 us, 55 with eight.
+            const size_t pairs = rows / S::kGroups / 2, cus = size_t(d.cu_count);
+            const unsigned grid = grid_1d(rows, S::kGroups, unsigned(std::clamp(pairs, 8 * cus, 16 * cus)));
             launch(rows_forward_kernel<g(), nv()>, dim3(grid), dim3(S::kThreads), 0, d.stream, x, weight, bias, y, st,
                    int64_t(rows), int(width), eps);
         });
