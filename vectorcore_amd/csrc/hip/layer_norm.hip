@@ -25,7 +25,7 @@
 // 8 us for the partial rows; 262144 rows of 64 without a weight 24 and 33 us (5.7
 // and 6.1; a copy of 1 GiB reaches 5.1, these partly stay in the last cache);
 // 999 rows of 515 4.6 us, and 5.7 and 5.4; one row of 4096 3.7 us. 4000 rows of
-// 10000 68 us, and 106 and 25; 2048 of 16384 59 us, and 87 and 83 (x and dy again
+// 10000 67 us, and 106 and 26; 2048 of 16384 59 us, and 87 and 83 (x and dy again
 // for the columns) and 7; 1024 of 32768 115 us, and 116, 72 and 10.
 #include "reduce_common.hpp"
 #include "vc_hip_internal.hpp"

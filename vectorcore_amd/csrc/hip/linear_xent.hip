@@ -20,11 +20,11 @@
 // - small or thin calls take float32 products and a kernel of the rows; bound by
 //   launches (256 rows, 256 x 10 with gradients: 25 us in five);
 // - others take packed products, bound by matrix instructions: 8192 rows, 1024 x
-//   50000, of which 7373 count, with gradients 6.8 ms: 2.05 (the logits, 369
+//   50000, of which 7373 count, with gradients 6.75 ms: 2.05 (the logits, 369
 //   TFLOP/s), 1.81 and 1.90 (their gradients' products), 0.99 (the gradients, 4.4
-//   GB at 4.4 TB/s), 0.3 for all others. 1536 rows that count without: 0.56 ms,
+//   GB at 4.4 TB/s), 0.3 for all others. 1536 rows that count without: 0.55 ms,
 //   of which the logits 0.47. Where the operands' rows hold values too unlike for
-//   two half-precision parts, three parts: 11.6 and 0.89 ms.
+//   two half-precision parts, three parts: 11.6 and 0.84 ms.
 #include "halves_product.hpp"
 #include "reduce_common.hpp"
 #include "thirds_product.hpp"
